@@ -506,7 +506,7 @@ int omt_pointwise(int op, int64_t n, const float* a, const float* b, float alpha
  * OMT_FOREACH_MAX_NUMEL each; host arrays) in one launch per 64 tensors: dtype OMT_DT_F32 adds fvalue, OMT_DT_I64 adds
  * ivalue. The optimizers' step counts and BatchNorm's batch counters. Replaces the reference's _foreach_* handling,
  * which loops the per-tensor add on the device (csrc/device.cpp:220-225). */
-enum { OMT_DT_F32 = 0, OMT_DT_I64 = 1 };
+enum { OMT_DT_F32 = 0, OMT_DT_I64 = 1, OMT_DT_BF16 = 2 };
 #define OMT_FOREACH_MAX_NUMEL (1 << 16)
 int omt_foreach_add_scalar(int count, void* const* ptrs, const int64_t* numels, int dtype, int64_t ivalue,
                            float fvalue, void* stream);
@@ -613,6 +613,63 @@ typedef struct omt_sgd_params {
 } omt_sgd_params;
 /* Replaces _fused_sgd_ (csrc/optim.cpp:12-28). */
 int omt_fused_sgd(const omt_sgd_params* params, const omt_sgd_tensor* tensors, int count, void* stream);
+
+/* ---- the feed-forward sublayer of a language model: norm, 8-bit matrix products, gated block ------------------------
+ *
+ * No counterpart in the reference. Rows are dense; types are OMT_DT_F32 or OMT_DT_BF16, sums and statistics float32.
+ * 8 bits: e4m3 values with a float32 scale for each block of 128 consecutive ones of a row ([rows][ceil(cols / 128)];
+ * the last block of a row may be shorter), scale = max(largest magnitude, 1e-30) / 448; for weights of 128 x 128
+ * ([ceil(rows / 128)][ceil(cols / 128)]). A block that holds an infinity or NaN stands for NaN throughout.
+ * Arrays need the alignment of their type only, except where a line below says 16 bytes. */
+
+/* h = x + residual (residual may be null: h = x, not written); y = h / sqrt(mean(h^2) + eps) * weight, written to y in
+ * x's type and / or to q and scale in 8 bits; rstd (may be null) gets 1 / sqrt(mean(h^2) + eps) of each row. The weight
+ * is of x's type or float32. dim is at most 32768 (else OMT_UNSUPPORTED). */
+int omt_rms_norm_fwd(int dtype, int weight_dtype, int64_t rows, int64_t dim, const void* x, const void* residual,
+                     const void* weight, float eps, void* y, void* h, float* rstd, void* q, float* scale, void* stream);
+size_t omt_rms_norm_bwd_workspace(int64_t rows, int64_t dim);
+/* gx: the gradient of x and of the residual, of gy through the norm plus gh (may be null) past it; gweight (may be
+ * null, then no workspace) in the weight's type. */
+int omt_rms_norm_bwd(int dtype, int weight_dtype, int64_t rows, int64_t dim, const void* gy, const void* gh,
+                     const void* h, const void* weight, const float* rstd, void* gx, void* gweight, void* workspace,
+                     size_t workspace_bytes, void* stream);
+/* x in 8 bits. pow2: scales are the next power of two from the scale above on, so that the values stood for are exact
+ * in bfloat16. */
+int omt_quantize_fp8(int dtype, int64_t rows, int64_t cols, const void* x, int pow2, void* q, float* scale,
+                     void* stream);
+int omt_quantize_fp8_weight(int dtype, int64_t rows, int64_t cols, const void* w, void* q, float* scale, void* stream);
+
+/* c[m][n] = sum over k of a[m][k] b[n][k], both in 8 bits with scales (a by 1 x 128, b by 128 x 128); c in out_dtype.
+ * a, b and the workspace on 16 bytes. */
+size_t omt_matmul_fp8_workspace(int64_t m, int64_t n, int64_t k);
+int omt_matmul_fp8(int64_t m, int64_t n, int64_t k, const void* a, const float* a_scale, const void* b,
+                   const float* b_scale, int out_dtype, void* c, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The gated feed-forward block's first half: g = x Wg^T, u = x Wu^T, h = act(g) * u, of x [m][k], weights [f][k].
+ * act: x * sigmoid(x); x * (1 + erf(x / sqrt 2)) / 2; max(x, 0). */
+enum { OMT_GLU_SILU = 0, OMT_GLU_GELU = 1, OMT_GLU_RELU = 2 };
+/* What a forward pass keeps for the backward: nothing; x, g and u in 8 bits (x with power-of-two scales, from
+ * omt_quantize_fp8); or g and u in x's type, and x itself. */
+enum { OMT_KEEP_NONE = 0, OMT_KEEP_FP8 = 1, OMT_KEEP_FULL = 2 };
+
+/* keep OMT_KEEP_FP8: x_q and x_scale, g and g_scale, u and u_scale are written; OMT_KEEP_FULL: g and u. x, the weights
+ * and the workspace on 16 bytes. */
+size_t omt_glu_fwd_workspace(int dtype, int64_t m, int64_t k, int64_t f);
+int omt_glu_fwd(int dtype, int64_t m, int64_t k, int64_t f, int act, int keep, const void* x, const void* w_gate,
+                const void* w_up, void* h, void* x_q, float* x_scale, void* g, float* g_scale, void* u, float* u_scale,
+                void* workspace, size_t workspace_bytes, void* stream);
+/* The gradients of x (gx), w_gate and w_up (each may be null) from gh, the gradient of h, and what the forward pass
+ * kept: OMT_KEEP_FP8 or, with x in x and no scales, OMT_KEEP_FULL. The workspace on 16 bytes. */
+size_t omt_glu_bwd_workspace(int dtype, int64_t m, int64_t k, int64_t f);
+int omt_glu_bwd(int dtype, int64_t m, int64_t k, int64_t f, int act, int keep, const void* gh, const void* x,
+                const float* x_scale, const void* g, const float* g_scale, const void* u, const float* u_scale,
+                const void* w_gate, const void* w_up, void* gx, void* gw_gate, void* gw_up, void* workspace,
+                size_t workspace_bytes, void* stream);
+/* omt_glu_fwd of operands in 8 bits (weights by 128 x 128), h in 8 bits. x, the weights and the workspace on 16 bytes. */
+size_t omt_glu_fp8_workspace(int64_t m, int64_t k, int64_t f);
+int omt_glu_fp8(int64_t m, int64_t k, int64_t f, int act, const void* x, const float* x_scale, const void* w_gate,
+                const float* gate_scale, const void* w_up, const float* up_scale, void* h_q, float* h_scale,
+                void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,503 @@
+// The feed-forward operators over their matrix products (ffn_gemm.h): which tiles and slices run, operands laid out for
+// them, the sums of slices, and the elementwise part of the gated block's backward.
+//
+//     forward    g = x Wg^T, u = x Wu^T, h = act(g) u
+//     backward   dg = gh u act'(g), du = gh act(g)
+//                gx = dg Wg + du Wu,  gWg = dg^T x,  gWu = du^T x
+//
+// The tiles read both operands along the reduction, 16 bytes at a time. So the backward lays out dg and du twice, by
+// rows (for gx, side by side as one reduction over both) and transposed (for the weights' gradients, one below the
+// other as one product), and x and the weights transposed: 64 x 64 blocks through LDS, read and written once, against
+// products that read them from every tile.
+#include <algorithm>
+
+#include "ffn_gemm.h"
+
+namespace omt {
+
+// ---- operands laid out for the tiles ------------------------------------------------------------------------------------
+
+// Rows copied to a pitch that is a multiple of 16 bytes, zeros past their end.
+template <class T>
+__global__ void __launch_bounds__(256) pad_rows_kernel(const T* __restrict__ src, int64_t rows, int64_t cols,
+                                                       int64_t pitch, T* __restrict__ dst) {
+  const int64_t total = rows * pitch, step = (int64_t)gridDim.x * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
+    const int64_t r = i / pitch, c = i - r * pitch;
+    dst[i] = c < cols ? src[r * cols + c] : T(0);
+  }
+}
+
+// A 64 x 64 block held in LDS (rows of 65 floats), its rows or its columns written as `lines` lines of T at dst, `width`
+// elements of each (a multiple of 16), `stride` elements apart.
+constexpr int kBlk = 64, kBlkPitch = 65;
+template <class T>
+__device__ __forceinline__ void write_block(const float* blk, bool columns, T* dst, int64_t stride, int64_t lines,
+                                            int64_t width) {
+  const int line = threadIdx.x >> 2, part = (threadIdx.x & 3) * 16;  // 16 consecutive elements of one line
+  if (line >= lines || part >= width) return;
+  f32x8 lo, hi;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    lo[e] = columns ? blk[(part + e) * kBlkPitch + line] : blk[line * kBlkPitch + part + e];
+    hi[e] = columns ? blk[(part + 8 + e) * kBlkPitch + line] : blk[line * kBlkPitch + part + 8 + e];
+  }
+  T* p = dst + line * stride + part;
+  store8<true>(p, 0, 16, lo);
+  store8<true>(p, 8, 16, hi);
+}
+
+// dst [cols][pitch], `width` of each row written (zeros from `rows` on) = src^T of src [rows][cols]; SRC float, __bf16, or e4m3 with its scales.
+template <class T, class S>
+__global__ void __launch_bounds__(256) transpose_kernel(const S* __restrict__ src, const float* __restrict__ scale,
+                                                        int64_t rows, int64_t cols, int64_t width, int64_t pitch,
+                                                        T* __restrict__ dst) {
+  __shared__ float blk[kBlk * kBlkPitch];
+  const int64_t r0 = (int64_t)blockIdx.y * kBlk, c0 = (int64_t)blockIdx.x * kBlk;
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t blocks = (cols + kFp8Block - 1) / kFp8Block;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = w * 16 + i;
+    float v = 0.f;
+    if (r0 + r < rows && c0 + l < cols) {
+      if constexpr (sizeof(S) == 1) v = fp8_value(src[(r0 + r) * cols + c0 + l]) * scale[(r0 + r) * blocks + c0 / kFp8Block];
+      else v = (float)src[(r0 + r) * cols + c0 + l];
+    }
+    blk[r * kBlkPitch + l] = v;
+  }
+  __syncthreads();
+  write_block(blk, true, dst + c0 * pitch + r0, pitch, cols - c0, width - r0);
+}
+
+struct GateArgs {
+  const void *gh, *g, *u;
+  const float *gs, *us;
+  int64_t m, f, half, mp;  // half: the distance of dg and du in a row of `rows_out` (2 * half elements)
+  int act;
+  void *rows_out, *cols_out;  // [m][2 * half] and [2 * f][mp]; either may be null
+};
+// dg and du of a 64 x 64 block of (row, column of f), laid out by rows and by columns
+template <class T, bool FP8>
+__global__ void __launch_bounds__(256) glu_gate_kernel(GateArgs a) {
+  __shared__ float dg[kBlk * kBlkPitch], du[kBlk * kBlkPitch];
+  const int64_t r0 = (int64_t)blockIdx.y * kBlk, c0 = (int64_t)blockIdx.x * kBlk;
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t blocks = (a.f + kFp8Block - 1) / kFp8Block;
+#pragma unroll 4
+  for (int i = 0; i < 16; ++i) {
+    const int r = w * 16 + i;
+    float vg = 0.f, vu = 0.f;
+    if (r0 + r < a.m && c0 + l < a.f) {
+      const int64_t at = (r0 + r) * a.f + c0 + l;
+      const float gh = (float)((const T*)a.gh)[at];
+      float g, u;
+      if constexpr (FP8) {
+        const int64_t b = (r0 + r) * blocks + c0 / kFp8Block;
+        g = fp8_value(((const uint8_t*)a.g)[at]) * a.gs[b];
+        u = fp8_value(((const uint8_t*)a.u)[at]) * a.us[b];
+      } else {
+        g = (float)((const T*)a.g)[at];
+        u = (float)((const T*)a.u)[at];
+      }
+      vg = gh * u * glu_act_grad(g, a.act);
+      vu = gh * glu_act(g, a.act);
+    }
+    dg[r * kBlkPitch + l] = vg;
+    du[r * kBlkPitch + l] = vu;
+  }
+  __syncthreads();
+  if (a.rows_out) {
+    T* p = (T*)a.rows_out + r0 * 2 * a.half + c0;
+    write_block(dg, false, p, 2 * a.half, a.m - r0, a.half - c0);
+    write_block(du, false, p + a.half, 2 * a.half, a.m - r0, a.half - c0);
+  }
+  if (a.cols_out) {
+    T* p = (T*)a.cols_out + c0 * a.mp + r0;
+    write_block(dg, true, p, a.mp, a.f - c0, a.mp - r0);
+    write_block(du, true, p + a.f * a.mp, a.mp, a.f - c0, a.mp - r0);
+  }
+}
+
+// ---- the sums of slices ---------------------------------------------------------------------------------------------------
+
+// out = the slices' sums, in slice order, in the output's type; rows from `split` on go to out2
+template <bool VEC>
+__global__ void __launch_bounds__(256) ffn_join_kernel(GemmArgs a) {
+  const int64_t vecs = (a.n + 7) / 8, total = a.m * vecs, step = (int64_t)gridDim.x * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
+    const int64_t m = i / vecs, c = (i - m * vecs) * 8;
+    f32x8 v = {};
+    for (int s = 0; s < a.slices; ++s) v += load8<VEC>(a.parts + ((int64_t)s * a.m + m) * a.n, c, a.n);
+    void* out = m < a.split ? a.out : a.out2;
+    const int64_t row = m < a.split ? m : m - a.split;
+    if (a.out_kind == kOutBf16) store8<VEC>((__bf16*)out + row * a.n, c, a.n, v);
+    else store8<VEC>((float*)out + row * a.n, c, a.n, v);
+  }
+}
+
+// The gated form's epilogue over the slices' sums: 16 lanes to a block of 128 outputs of a row.
+template <bool VEC>
+__global__ void __launch_bounds__(256) glu_join_kernel(GemmArgs a) {
+  const int64_t blocks = (a.n + kFp8Block - 1) / kFp8Block, vecs = blocks * 16;
+  const int64_t total = a.m * vecs, step = (int64_t)gridDim.x * 256;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
+    const int64_t m = i / vecs, c = (i - m * vecs) * 8;
+    f32x8 g = {}, u = {}, h;
+    for (int s = 0; s < a.slices; ++s) {
+      const float* row = a.parts + ((int64_t)s * a.m + m) * 2 * a.n;
+      g += load8<VEC>(row, c, a.n);
+      u += load8<VEC>(row + a.n, c, a.n);
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) h[e] = glu_act(g[e], a.act) * u[e];
+    const int64_t row = m * a.n;
+    const bool first = (threadIdx.x & 15) == 0;
+    auto in_8 = [&](f32x8 v, void* q, float* scale) {
+      const float s = block_scale(row16_max(abs_bits8(v)));
+      store_fp8x8<VEC>((uint8_t*)q + row, c, a.n, pack_fp8x8(v, 1.f / s));
+      if (first) scale[i / 16] = s;
+    };
+    auto in_type = [&](f32x8 v, void* p) {
+      if (a.out_kind == kOutBf16) store8<VEC>((__bf16*)p + row, c, a.n, v);
+      else store8<VEC>((float*)p + row, c, a.n, v);
+    };
+    if (a.out_kind == kOutFp8) in_8(h, a.out, a.out_scale);
+    else in_type(h, a.out);
+    if (a.keep == kKeepFp8) {
+      in_8(g, a.keep_g, a.keep_gs);
+      in_8(u, a.keep_u, a.keep_us);
+    } else if (a.keep == kKeepFull) {
+      in_type(g, a.keep_g);
+      in_type(u, a.keep_u);
+    }
+  }
+}
+
+// ---- host -------------------------------------------------------------------------------------------------------------------
+
+// The launch of a product of m rows by n (of each weight, if gated) with rows of row_bytes.
+struct GemmPlan {
+  int bm, gx, gy, steps, slices, slice_steps;
+  size_t parts_bytes;
+};
+static GemmPlan plan_gemm(int mode, bool glu, int64_t m, int64_t n, int64_t row_bytes) {
+  GemmPlan p{};
+  p.bm = m <= 16 ? 16 : 64;
+  p.gx = (int)cdiv(n, glu ? 128 : 256);
+  p.gy = (int)cdiv(m, p.bm);
+  p.steps = (int)cdiv(row_bytes, 128);
+  p.slices = 1;
+  p.slice_steps = p.steps;
+  if (p.slices > 1) p.parts_bytes = (size_t)p.slices * m * n * (glu ? 2 : 1) * sizeof(float);
+  return p;
+}
+static int run_gemm(int mode, bool glu, const GemmPlan& p, GemmArgs a, void* parts, hipStream_t stream) {
+  a.steps = p.steps, a.slices = p.slices, a.slice_steps = p.slice_steps, a.gx = p.gx, a.gy = p.gy;
+  a.parts = (float*)parts;
+  int e = mode == kF32 ? ffn_gemm_f32(a, glu, p.bm, stream)
+          : mode == kBf16 ? ffn_gemm_bf16(a, glu, p.bm, stream) : ffn_gemm_fp8(a, glu, p.bm, stream);
+  if (e || p.slices == 1) return e;
+  const bool vec = a.n % 8 == 0;
+  if (glu) {
+    const dim3 grid(grid1d(a.m * cdiv(a.n, kFp8Block) * 16, 256, 1 << 16));
+    if (vec) hipLaunchKernelGGL(glu_join_kernel<true>, grid, dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL(glu_join_kernel<false>, grid, dim3(256), 0, stream, a);
+    return launch_check("glu_join_kernel");
+  }
+  const dim3 grid(grid1d(a.m * cdiv(a.n, 8), 256, 1 << 16));
+  if (vec) hipLaunchKernelGGL(ffn_join_kernel<true>, grid, dim3(256), 0, stream, a);
+  else hipLaunchKernelGGL(ffn_join_kernel<false>, grid, dim3(256), 0, stream, a);
+  return launch_check("ffn_join_kernel");
+}
+
+// A workspace handed out in 256-byte steps; `base` null to count only.
+struct Space {
+  char* base;
+  size_t used = 0;
+  void* take(size_t bytes) {
+    if (!bytes) return nullptr;
+    void* p = base ? base + used : nullptr;
+    used += (bytes + 255) & ~(size_t)255;
+    return p;
+  }
+};
+
+static int64_t up(int64_t v, int64_t to) { return cdiv(v, to) * to; }
+static int elem_bytes(int mode) { return mode == kF32 ? 4 : mode == kBf16 ? 2 : 1; }
+
+// An operand's rows as the tiles read them: in place where every row starts on 16 bytes, else copied.
+struct Operand {
+  void* copy = nullptr;
+  int64_t pitch = 0;  // bytes
+};
+static Operand place_rows(Space& sp, int mode, int64_t rows, int64_t cols) {
+  const int64_t bytes = cols * elem_bytes(mode);
+  if (bytes % 16 == 0) return {nullptr, bytes};
+  return {sp.take((size_t)(rows * up(bytes, 16))), up(bytes, 16)};
+}
+static const void* lay_rows(const Operand& o, int mode, const void* src, int64_t rows, int64_t cols, hipStream_t stream,
+                            int* err) {
+  if (!o.copy || *err) return src;
+  const int64_t pitch = o.pitch / elem_bytes(mode);
+  const dim3 grid(grid1d(rows * pitch, 256, 1 << 16));
+  if (mode == kF32)
+    hipLaunchKernelGGL(pad_rows_kernel<float>, grid, dim3(256), 0, stream, (const float*)src, rows, cols, pitch, (float*)o.copy);
+  else if (mode == kBf16)
+    hipLaunchKernelGGL(pad_rows_kernel<uint16_t>, grid, dim3(256), 0, stream, (const uint16_t*)src, rows, cols, pitch,
+                       (uint16_t*)o.copy);
+  else
+    hipLaunchKernelGGL(pad_rows_kernel<uint8_t>, grid, dim3(256), 0, stream, (const uint8_t*)src, rows, cols, pitch,
+                       (uint8_t*)o.copy);
+  *err = launch_check("pad_rows_kernel");
+  return o.copy;
+}
+
+static bool on16(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if ((uintptr_t)p & 15) return false;
+  return true;
+}
+// Offsets within a tile's rows are 32-bit: 256 rows of at most 4 MiB.
+static int product_check(const char* fn, int64_t m, int64_t n, int64_t k) {
+  if (m < 0 || n < 1 || k < 1)
+    return fail(OMT_INVALID, "%s: %lld x %lld x %lld", fn, (long long)m, (long long)n, (long long)k);
+  constexpr int64_t kMost = 1 << 20, kRows = 1 << 30;
+  if (k > kMost || m > kRows || n > kMost)
+    return fail(OMT_UNSUPPORTED, "%s: %lld x %lld x %lld", fn, (long long)m, (long long)n, (long long)k);
+  return OMT_OK;
+}
+static int need_space(const char* fn, size_t need, const void* ws, size_t bytes) {
+  if (need && (!ws || bytes < need)) return fail(OMT_INVALID, "%s: workspace of %zu bytes, %zu needed", fn, bytes, need);
+  if (!on16({ws})) return fail(OMT_INVALID, "%s: the workspace is not on 16 bytes", fn);
+  return OMT_OK;
+}
+
+struct MatmulFp8 {
+  GemmPlan p;
+  Operand a, b;
+  void* parts;
+  MatmulFp8(Space& sp, int64_t m, int64_t n, int64_t k)
+      : p(plan_gemm(kFp8x, false, m, n, k)), a(place_rows(sp, kFp8x, m, k)), b(place_rows(sp, kFp8x, n, k)),
+        parts(sp.take(p.parts_bytes)) {}
+};
+struct GluFwd {
+  GemmPlan p;
+  Operand x, wg, wu;
+  void* parts;
+  GluFwd(Space& sp, int mode, int64_t m, int64_t k, int64_t f)
+      : p(plan_gemm(mode, true, m, f, k * elem_bytes(mode))), x(place_rows(sp, mode, m, k)),
+        wg(place_rows(sp, mode, f, k)), wu(place_rows(sp, mode, f, k)), parts(sp.take(p.parts_bytes)) {}
+};
+struct GluBwd {
+  int64_t half, mp;  // elements: dg and du of a row padded to `half` each; columns of m padded to mp
+  void *gate_rows, *gate_cols, *w_cols, *x_cols;
+  GemmPlan px, pw;
+  void *parts;
+  GluBwd(Space& sp, int mode, int64_t m, int64_t k, int64_t f) : half(up(f, kBlk)), mp(up(m, kBlk)) {
+    const int e = elem_bytes(mode);
+    gate_rows = sp.take((size_t)(m * 2 * half * e));
+    gate_cols = sp.take((size_t)(2 * f * mp * e));
+    w_cols = sp.take((size_t)(k * 2 * half * e));
+    x_cols = sp.take((size_t)(k * mp * e));
+    px = plan_gemm(mode, false, m, k, 2 * half * e);
+    pw = plan_gemm(mode, false, 2 * f, k, mp * e);
+    parts = sp.take(std::max(px.parts_bytes, pw.parts_bytes));
+  }
+};
+
+static int mode_of(int dtype) { return dtype == OMT_DT_F32 ? kF32 : kBf16; }
+static int glu_check(const char* fn, int dtype, int64_t m, int64_t k, int64_t f, int act) {
+  if (dtype != OMT_DT_F32 && dtype != OMT_DT_BF16) return fail(OMT_INVALID, "%s: dtype %d", fn, dtype);
+  if (act != OMT_GLU_SILU && act != OMT_GLU_GELU && act != OMT_GLU_RELU) return fail(OMT_INVALID, "%s: act %d", fn, act);
+  return product_check(fn, m, f, k);
+}
+
+// dst [cols][pitch] = src^T in elements of `mode`, rows padded to a multiple of 64
+template <class S>
+static int run_transpose(int mode, const S* src, const float* scale, int64_t rows, int64_t cols, int64_t pitch,
+                         void* dst, hipStream_t stream) {
+  const int64_t width = up(rows, kBlk);
+  const dim3 grid((unsigned)cdiv(cols, kBlk), (unsigned)cdiv(rows, kBlk));
+  if (mode == kF32)
+    hipLaunchKernelGGL((transpose_kernel<float, S>), grid, dim3(256), 0, stream, src, scale, rows, cols, width, pitch, (float*)dst);
+  else
+    hipLaunchKernelGGL((transpose_kernel<__bf16, S>), grid, dim3(256), 0, stream, src, scale, rows, cols, width, pitch, (__bf16*)dst);
+  return launch_check("transpose_kernel");
+}
+
+}  // namespace omt
+
+using namespace omt;
+
+OMT_EXPORT size_t omt_matmul_fp8_workspace(int64_t m, int64_t n, int64_t k) {
+  if (product_check("omt_matmul_fp8_workspace", m, n, k) || m == 0) return 0;
+  Space sp{nullptr};
+  MatmulFp8(sp, m, n, k);
+  return sp.used;
+}
+
+OMT_EXPORT int omt_matmul_fp8(int64_t m, int64_t n, int64_t k, const void* a, const float* a_scale, const void* b,
+                              const float* b_scale, int out_dtype, void* c, void* workspace, size_t workspace_bytes,
+                              void* stream) {
+  const char* fn = "omt_matmul_fp8";
+  if (out_dtype != OMT_DT_F32 && out_dtype != OMT_DT_BF16) return fail(OMT_INVALID, "%s: dtype %d", fn, out_dtype);
+  if (int e = product_check(fn, m, n, k)) return e;
+  if (m == 0) return OMT_OK;
+  if (!a || !a_scale || !b || !b_scale || !c) return fail(OMT_INVALID, "%s: null pointer", fn);
+  if (!on16({a, b, c})) return fail(OMT_INVALID, "%s: an operand is not on 16 bytes", fn);
+  if (int e = need_space(fn, omt_matmul_fp8_workspace(m, n, k), workspace, workspace_bytes)) return e;
+  Space sp{(char*)workspace};
+  const MatmulFp8 l(sp, m, n, k);
+  hipStream_t st = stream_of(stream);
+  int err = OMT_OK;
+  GemmArgs g{};
+  g.x = lay_rows(l.a, kFp8x, a, m, k, st, &err);
+  g.w = lay_rows(l.b, kFp8x, b, n, k, st, &err);
+  if (err) return err;
+  g.sx = a_scale, g.sw = b_scale;
+  g.xpitch = l.a.pitch, g.wpitch = l.b.pitch;
+  g.m = (int)m, g.n = (int)n, g.row_bytes = (int)l.a.pitch, g.blocks = (int)cdiv(k, kFp8Block);
+  g.out = c, g.split = (int)m, g.out_kind = out_dtype == OMT_DT_BF16 ? kOutBf16 : kOutF32;
+  return run_gemm(kFp8x, false, l.p, g, l.parts, st);
+}
+
+OMT_EXPORT size_t omt_glu_fwd_workspace(int dtype, int64_t m, int64_t k, int64_t f) {
+  if (glu_check("omt_glu_fwd_workspace", dtype, m, k, f, OMT_GLU_SILU) || m == 0) return 0;
+  Space sp{nullptr};
+  GluFwd(sp, mode_of(dtype), m, k, f);
+  return sp.used;
+}
+
+OMT_EXPORT int omt_glu_fwd(int dtype, int64_t m, int64_t k, int64_t f, int act, int keep, const void* x,
+                           const void* w_gate, const void* w_up, void* h, void* x_q, float* x_scale, void* g,
+                           float* g_scale, void* u, float* u_scale, void* workspace, size_t workspace_bytes,
+                           void* stream) {
+  const char* fn = "omt_glu_fwd";
+  if (int e = glu_check(fn, dtype, m, k, f, act)) return e;
+  if (keep != OMT_KEEP_NONE && keep != OMT_KEEP_FP8 && keep != OMT_KEEP_FULL) return fail(OMT_INVALID, "%s: keep %d", fn, keep);
+  if (m == 0) return OMT_OK;
+  if (!x || !w_gate || !w_up || !h || (keep != OMT_KEEP_NONE && (!g || !u)) ||
+      (keep == OMT_KEEP_FP8 && (!x_q || !x_scale || !g_scale || !u_scale)))
+    return fail(OMT_INVALID, "%s: null pointer", fn);
+  if (!on16({x, w_gate, w_up, h, g, u})) return fail(OMT_INVALID, "%s: an operand is not on 16 bytes", fn);
+  if (int e = need_space(fn, omt_glu_fwd_workspace(dtype, m, k, f), workspace, workspace_bytes)) return e;
+  const int mode = mode_of(dtype);
+  Space sp{(char*)workspace};
+  const GluFwd l(sp, mode, m, k, f);
+  hipStream_t st = stream_of(stream);
+  int err = OMT_OK;
+  if (keep == OMT_KEEP_FP8) err = omt_quantize_fp8(dtype, m, k, x, 1, x_q, x_scale, stream);
+  GemmArgs a{};
+  a.x = lay_rows(l.x, mode, x, m, k, st, &err);
+  a.w = lay_rows(l.wg, mode, w_gate, f, k, st, &err);
+  a.w_up = lay_rows(l.wu, mode, w_up, f, k, st, &err);
+  if (err) return err;
+  a.xpitch = l.x.pitch, a.wpitch = l.wg.pitch;
+  a.m = (int)m, a.n = (int)f, a.row_bytes = (int)l.x.pitch, a.split = (int)m;
+  a.out = h, a.out_kind = dtype == OMT_DT_BF16 ? kOutBf16 : kOutF32, a.act = act;
+  a.keep = keep == OMT_KEEP_FP8 ? kKeepFp8 : keep == OMT_KEEP_FULL ? kKeepFull : kKeepNone;
+  a.keep_g = g, a.keep_u = u, a.keep_gs = g_scale, a.keep_us = u_scale;
+  return run_gemm(mode, true, l.p, a, l.parts, st);
+}
+
+OMT_EXPORT size_t omt_glu_fp8_workspace(int64_t m, int64_t k, int64_t f) {
+  if (product_check("omt_glu_fp8_workspace", m, f, k) || m == 0) return 0;
+  Space sp{nullptr};
+  GluFwd(sp, kFp8x, m, k, f);
+  return sp.used;
+}
+
+OMT_EXPORT int omt_glu_fp8(int64_t m, int64_t k, int64_t f, int act, const void* x, const float* x_scale,
+                           const void* w_gate, const float* gate_scale, const void* w_up, const float* up_scale,
+                           void* h_q, float* h_scale, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "omt_glu_fp8";
+  if (int e = glu_check(fn, OMT_DT_F32, m, k, f, act)) return e;
+  if (m == 0) return OMT_OK;
+  if (!x || !x_scale || !w_gate || !gate_scale || !w_up || !up_scale || !h_q || !h_scale)
+    return fail(OMT_INVALID, "%s: null pointer", fn);
+  if (!on16({x, w_gate, w_up, h_q})) return fail(OMT_INVALID, "%s: an operand is not on 16 bytes", fn);
+  if (int e = need_space(fn, omt_glu_fp8_workspace(m, k, f), workspace, workspace_bytes)) return e;
+  Space sp{(char*)workspace};
+  const GluFwd l(sp, kFp8x, m, k, f);
+  hipStream_t st = stream_of(stream);
+  int err = OMT_OK;
+  GemmArgs a{};
+  a.x = lay_rows(l.x, kFp8x, x, m, k, st, &err);
+  a.w = lay_rows(l.wg, kFp8x, w_gate, f, k, st, &err);
+  a.w_up = lay_rows(l.wu, kFp8x, w_up, f, k, st, &err);
+  if (err) return err;
+  a.sx = x_scale, a.sw = gate_scale, a.sw_up = up_scale;
+  a.xpitch = l.x.pitch, a.wpitch = l.wg.pitch;
+  a.m = (int)m, a.n = (int)f, a.row_bytes = (int)l.x.pitch, a.blocks = (int)cdiv(k, kFp8Block), a.split = (int)m;
+  a.out = h_q, a.out_scale = h_scale, a.out_kind = kOutFp8, a.act = act, a.keep = kKeepNone;
+  return run_gemm(kFp8x, true, l.p, a, l.parts, st);
+}
+
+OMT_EXPORT size_t omt_glu_bwd_workspace(int dtype, int64_t m, int64_t k, int64_t f) {
+  if (glu_check("omt_glu_bwd_workspace", dtype, m, k, f, OMT_GLU_SILU)) return 0;
+  Space sp{nullptr};
+  GluBwd(sp, mode_of(dtype), std::max<int64_t>(m, 1), k, f);
+  return sp.used;
+}
+
+OMT_EXPORT int omt_glu_bwd(int dtype, int64_t m, int64_t k, int64_t f, int act, int keep, const void* gh, const void* x,
+                           const float* x_scale, const void* g, const float* g_scale, const void* u,
+                           const float* u_scale, const void* w_gate, const void* w_up, void* gx, void* gw_gate,
+                           void* gw_up, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* fn = "omt_glu_bwd";
+  if (int e = glu_check(fn, dtype, m, k, f, act)) return e;
+  if (keep != OMT_KEEP_FP8 && keep != OMT_KEEP_FULL) return fail(OMT_INVALID, "%s: keep %d", fn, keep);
+  if (!gw_gate != !gw_up) return fail(OMT_INVALID, "%s: one of the weights' gradients alone", fn);
+  const size_t e = dtype == OMT_DT_F32 ? 4 : 2;
+  if (m == 0) {  // no row: no gradient
+    if (!gw_gate) return OMT_OK;
+    if (int err = omt_memset_zero(gw_gate, (size_t)(f * k) * e, stream)) return err;
+    return omt_memset_zero(gw_up, (size_t)(f * k) * e, stream);
+  }
+  const bool fp8 = keep == OMT_KEEP_FP8;
+  if (!gh || !x || !g || !u || !w_gate || !w_up || (fp8 && (!x_scale || !g_scale || !u_scale)))
+    return fail(OMT_INVALID, "%s: null pointer", fn);
+  if (!on16({gx, gw_gate, gw_up})) return fail(OMT_INVALID, "%s: a gradient is not on 16 bytes", fn);
+  if (2 * f > 1 << 20 || cdiv(m, kBlk) > 65535 || m > 1 << 20)
+    return fail(OMT_UNSUPPORTED, "%s: %lld x %lld x %lld", fn, (long long)m, (long long)k, (long long)f);
+  if (int err = need_space(fn, omt_glu_bwd_workspace(dtype, m, k, f), workspace, workspace_bytes)) return err;
+  if (!gx && !gw_gate) return OMT_OK;
+  const int mode = mode_of(dtype), eb = elem_bytes(mode);
+  Space sp{(char*)workspace};
+  const GluBwd l(sp, mode, m, k, f);
+  hipStream_t st = stream_of(stream);
+
+  const GateArgs ga{gh, g, u, g_scale, u_scale, m, f, l.half, l.mp, act, gx ? l.gate_rows : nullptr,
+                    gw_gate ? l.gate_cols : nullptr};
+  const dim3 grid((unsigned)cdiv(f, kBlk), (unsigned)cdiv(m, kBlk));
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, ga); };
+  if (mode == kF32) fp8 ? go(glu_gate_kernel<float, true>) : go(glu_gate_kernel<float, false>);
+  else fp8 ? go(glu_gate_kernel<__bf16, true>) : go(glu_gate_kernel<__bf16, false>);
+  if (int err = launch_check("glu_gate_kernel")) return err;
+
+  auto transpose = [&](const void* src, int64_t rows, int64_t cols, int64_t pitch, void* dst) {
+    return mode == kF32 ? run_transpose(mode, (const float*)src, nullptr, rows, cols, pitch, dst, st)
+                        : run_transpose(mode, (const __bf16*)src, nullptr, rows, cols, pitch, dst, st);
+  };
+  if (gx) {  // [m][dg | du] by [k][Wg^T | Wu^T]
+    if (int err = transpose(w_gate, f, k, 2 * l.half, l.w_cols)) return err;
+    if (int err = transpose(w_up, f, k, 2 * l.half, (char*)l.w_cols + l.half * eb)) return err;
+    GemmArgs a{};
+    a.x = l.gate_rows, a.w = l.w_cols, a.xpitch = a.wpitch = 2 * l.half * eb;
+    a.m = (int)m, a.n = (int)k, a.row_bytes = (int)a.xpitch, a.split = (int)m;
+    a.out = gx, a.out_kind = mode == kF32 ? kOutF32 : kOutBf16;
+    if (int err = run_gemm(mode, false, l.px, a, l.parts, st)) return err;
+  }
+  if (gw_gate) {  // [dg^T over du^T] by [k][x^T]
+    int err = fp8 ? run_transpose(mode, (const uint8_t*)x, x_scale, m, k, l.mp, l.x_cols, st)
+                  : transpose(x, m, k, l.mp, l.x_cols);
+    if (err) return err;
+    GemmArgs a{};
+    a.x = l.gate_cols, a.w = l.x_cols, a.xpitch = a.wpitch = l.mp * eb;
+    a.m = (int)(2 * f), a.n = (int)k, a.row_bytes = (int)a.xpitch, a.split = (int)f;
+    a.out = gw_gate, a.out2 = gw_up, a.out_kind = mode == kF32 ? kOutF32 : kOutBf16;
+    if (err = run_gemm(mode, false, l.pw, a, l.parts, st); err) return err;
+  }
+  return OMT_OK;
+}

@@ -1,0 +1,382 @@
+// Matrix products of the feed-forward operators: out[m][n] = sum over k of x[m][k] w[n][k], both operands with the
+// reduction along their rows, in tiles of BM rows of x by 256 rows of w. The gated form takes 128 rows each of the gate's
+// and the up projection's weight, so that a workgroup holds both projections of its outputs, and a block of 128 of them.
+//
+// Every mode reads its operands the same way, 128 bytes of each row to a step: 32 floats, 64 bfloat16, 128 e4m3.
+// They go from memory to LDS without passing registers; within a row, 16-byte chunk c lies at c ^ (row & 7), so that
+// the 16 lanes that read one chunk of 16 rows touch every bank. NS stages are in flight, one workgroup barrier a step.
+// A lane's two chunks of a row (g and g + 4, g = lane / 16) feed the matrix cores in whatever order of k; the order is
+// the same for both operands, and a sum does not mind.
+#pragma once
+
+#include "block_fp8.h"
+#include "lds_dma.h"
+#include "tile_map.h"
+
+namespace omt {
+
+// kF32: v_mfma_f32_16x16x4_f32 on the floats themselves. kBf16: v_mfma_f32_16x16x32_bf16. kFp8x: e4m3 values taken to
+// bfloat16 (exact) for the same instruction; each step is one block of 128, whose sum is multiplied by the two scales.
+enum GemmMode { kF32, kBf16, kFp8x };
+enum GluKeep { kKeepNone, kKeepFp8, kKeepFull };
+enum OutKind { kOutF32, kOutBf16, kOutFp8 };
+
+// p, the same in every lane, in scalar registers
+template <class T>
+__device__ __forceinline__ const T* uniform(const T* p) {
+  const uint64_t b = (uint64_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((int)(uint32_t)b);  // an int: no sign into the upper half
+  const uint32_t hi = __builtin_amdgcn_readfirstlane((int)(uint32_t)(b >> 32));
+  return (const T*)((uint64_t)hi << 32 | lo);
+}
+
+struct GemmArgs {
+  const void *x, *w, *w_up;           // rows of xpitch / wpitch bytes on 16-byte boundaries; w_up: the gated form's
+  const float *sx, *sw, *sw_up;       // kFp8x: x's scales [m][blocks], w's [ceil(n / 128)][blocks]
+  int64_t xpitch, wpitch;
+  int m, n, row_bytes, steps, blocks; // n: rows of w (and of w_up); row_bytes: the reduction's length
+  int slices, slice_steps;            // steps of each slice of the reduction; more than one slice: sums go to parts
+  int gx, gy;                         // tiles
+  float* parts;                       // [slices][m][n], gated: [slices][m][2][n]
+  void *out, *out2;                   // rows of n; rows of x from split on go to out2
+  int split, out_kind;
+  // the gated form: out gets act(g) * u, in 8 bits with scales out_scale; keep: what the backward pass needs
+  int act, keep;
+  float* out_scale;
+  void *keep_g, *keep_u;
+  float *keep_gs, *keep_us;
+};
+
+__device__ __forceinline__ float glu_act(float g, int act) {
+  if (act == OMT_GLU_SILU) return g / (1.f + expf(-g));
+  if (act == OMT_GLU_GELU) return 0.5f * g * erfcf(-0.70710678118654752f * g);
+  return g < 0.f ? 0.f : g;  // NaN stays
+}
+__device__ __forceinline__ float glu_act_grad(float g, int act) {
+  if (act == OMT_GLU_SILU) {
+    const float p = 1.f / (1.f + expf(-g));
+    return p * (1.f + g * (1.f - p));
+  }
+  if (act == OMT_GLU_GELU)
+    return 0.5f * erfcf(-0.70710678118654752f * g) + 0.3989422804014327f * g * expf(-0.5f * g * g);
+  return g > 0.f ? 1.f : 0.f;
+}
+
+// four consecutive columns c.. of a row of `cols`, at p (the row's start)
+template <class T>
+__device__ __forceinline__ void store4(T* p, int c, int cols, bool vec, f32x4 v) {
+  if (vec) {
+    if (c < cols) {
+      if constexpr (sizeof(T) == 4) *(f32x4*)(p + c) = v;
+      else *(bf16x4*)(p + c) = __builtin_convertvector(v, bf16x4);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c + e < cols) p[c + e] = (T)v[e];
+  }
+}
+__device__ __forceinline__ void store4_any(void* p, int64_t row, int c, int cols, bool vec, int kind, f32x4 v) {
+  if (kind == kOutBf16) store4((__bf16*)p + row * cols, c, cols, vec, v);
+  else store4((float*)p + row * cols, c, cols, vec, v);
+}
+__device__ __forceinline__ void store4_fp8(void* p, int64_t row, int c, int cols, bool vec, f32x4 v, float inv) {
+  const uint32_t w = pack_fp8(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
+  uint8_t* q = (uint8_t*)p + row * cols;
+  if (vec) {
+    if (c < cols) *(uint32_t*)(q + c) = w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (c + e < cols) q[c + e] = (uint8_t)(w >> (8 * e));
+  }
+}
+
+template <int MODE, int BM, int NS>
+struct GemmTile {
+  static constexpr int WM = BM >= 128 ? 2 : 1;        // waves along the rows of x; 4 along the rows of w
+  static constexpr int NW = WM * 4, THREADS = NW * 64;
+  static constexpr int TI = BM / WM / 16, TJ = 4;      // a wave's 16 x 16 tiles
+  static constexpr int XI = BM / 8, DI = XI + 32;      // loads of 8 rows a step
+  static constexpr int DW = (DI + NW - 1) / NW;        // ... by each wave (some repeated, so that all waves' counts are one)
+  static constexpr bool SCALED = MODE == kFp8x;
+  static constexpr int SROWS = BM < 64 ? 64 : BM;
+  static constexpr int SI = SROWS / 64 + 4;            // loads of 64 scales a step
+  static constexpr int SW = SCALED ? (SI + NW - 1) / NW : 0;
+  static constexpr int LOADS = DW + SW;
+  static constexpr int STAGE = (BM + 256) * 128 + (SCALED ? (SROWS + 256) * 4 : 0);
+  static constexpr int LDS = NS * STAGE;
+};
+
+template <int MODE, bool GLU, int BM, int NS>
+__global__ void __launch_bounds__((GemmTile<MODE, BM, NS>::THREADS), (GemmTile<MODE, BM, NS>::NW / 4))
+ffn_gemm_kernel(GemmArgs a) {
+  using Tl = GemmTile<MODE, BM, NS>;
+  constexpr int TI = Tl::TI, TJ = Tl::TJ, NT = GLU ? 128 : 256;
+  static_assert(Tl::LDS >= 3 * 4 * BM * 4, "the epilogue's maxima lie where the stages were");
+  __shared__ __attribute__((aligned(128))) unsigned char lds[Tl::LDS];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 2, wn = wave & 3, r16 = lane & 15, g = lane >> 4;
+  const TileId id = xcd_tile(blockIdx.x, a.gx, a.gy, a.slices, 4);
+  const int m0 = id.y * BM, n0 = id.x * NT;
+  const int s0 = id.z * a.slice_steps, s1 = min(a.steps, s0 + a.slice_steps);
+
+  // where each of this wave's loads reads: a base that advances 128 bytes a step, and the lane's offset from it. Rows
+  // past the operand's last read as 0 (an offset out of the range that the load checks).
+  const uint32_t chunk16 = ((lane & 7) ^ (lane >> 3)) * 16;
+  const unsigned char* dbase[Tl::DW];
+  uint32_t doff[Tl::DW], ddst[Tl::DW];
+#pragma unroll
+  for (int t = 0; t < Tl::DW; ++t) {
+    const int slot = min(wave + Tl::NW * t, Tl::DI - 1);
+    ddst[t] = slot * 1024;
+    if (slot < Tl::XI) {
+      const int r = slot * 8 + (lane >> 3);
+      dbase[t] = (const unsigned char*)a.x + m0 * a.xpitch;
+      doff[t] = m0 + r < a.m ? (uint32_t)r * (uint32_t)a.xpitch + chunk16 : kOOB;
+    } else {
+      const int r8 = (slot - Tl::XI) * 8, r = (GLU ? r8 & 127 : r8) + (lane >> 3);
+      dbase[t] = (const unsigned char*)(GLU && r8 >= 128 ? a.w_up : a.w) + n0 * a.wpitch;
+      doff[t] = n0 + r < a.n ? (uint32_t)r * (uint32_t)a.wpitch + chunk16 : kOOB;
+    }
+  }
+  const float* sbase[Tl::SW + 1];
+  uint32_t soff[Tl::SW + 1], sdst[Tl::SW + 1];
+  if constexpr (Tl::SCALED) {
+#pragma unroll
+    for (int t = 0; t < Tl::SW; ++t) {
+      const int slot = min(wave + Tl::NW * t, Tl::SI - 1);
+      sdst[t] = (BM + 256) * 128 + slot * 256;
+      if (slot < Tl::SROWS / 64) {
+        const int r = slot * 64 + lane;
+        sbase[t] = a.sx + (int64_t)m0 * a.blocks;
+        soff[t] = m0 + r < a.m && r < BM ? (uint32_t)(r * a.blocks) * 4 : kOOB;
+      } else {
+        const int r64 = (slot - Tl::SROWS / 64) * 64, r = (GLU ? r64 & 127 : r64) + lane;
+        sbase[t] = (GLU && r64 >= 128 ? a.sw_up : a.sw) + (int64_t)(n0 >> 7) * a.blocks;
+        soff[t] = n0 + r < a.n ? (uint32_t)((r >> 7) * a.blocks) * 4 : kOOB;
+      }
+    }
+  }
+  const uint32_t lds0 = lds_addr((const float*)lds);
+  // Step s into stage `buf`. Past the slice's last step every lane's offset is out of range: the loads count, and read
+  // nothing.
+  auto issue = [&](int buf, int s) {
+    const uint32_t at = lds0 + buf * Tl::STAGE;
+    const uint32_t left = s < s1 ? (uint32_t)(a.row_bytes - s * 128) : 0u;
+    const bool in = chunk16 < left;
+#pragma unroll
+    for (int t = 0; t < Tl::DW; ++t)
+      lds_load_b128(rsrc_words(uniform(dbase[t] + (int64_t)s * 128), 0x7fffffffu),
+                    __builtin_amdgcn_readfirstlane(at + ddst[t]), in ? doff[t] : kOOB);
+    if constexpr (Tl::SCALED) {
+#pragma unroll
+      for (int t = 0; t < Tl::SW; ++t)
+        lds_load_b32(rsrc_words(uniform(sbase[t] + s), 0x7fffffffu),
+                     __builtin_amdgcn_readfirstlane(at + sdst[t]), left ? soff[t] : kOOB, 0);
+    }
+  };
+
+  f32x4 acc[TI][TJ] = {};
+  const uint32_t frag = r16 * 128 + ((g ^ (r16 & 7)) << 4);  // chunk g of row r16; chunk g + 4 lies at ^ 64
+  auto wrow = [&](int j) { return GLU ? (j >> 1) * 128 + wn * 32 + (j & 1) * 16 : wn * 64 + j * 16; };
+  const int xrow = wm * TI * 16;
+
+  auto compute = [&](int buf) {
+    const unsigned char* xs = lds + buf * Tl::STAGE + xrow * 128;
+    const unsigned char* ws = lds + buf * Tl::STAGE + BM * 128;
+    auto chunk = [](const unsigned char* p) { return *(const omt_u32x4*)p; };
+    if constexpr (MODE == kF32 || MODE == kBf16) {
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        omt_u32x4 wv[TJ];
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) wv[j] = chunk(ws + wrow(j) * 128 + (frag ^ (kk * 64)));
+#pragma unroll
+        for (int i = 0; i < TI; ++i) {
+          const omt_u32x4 xv = chunk(xs + i * 2048 + (frag ^ (kk * 64)));
+#pragma unroll
+          for (int j = 0; j < TJ; ++j) {
+            if constexpr (MODE == kBf16) {
+              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[j]),
+                                                                  __builtin_bit_cast(bf16x8, xv), acc[i][j], 0, 0, 0);
+            } else {
+              const f32x4 wf = __builtin_bit_cast(f32x4, wv[j]), xf = __builtin_bit_cast(f32x4, xv);
+#pragma unroll
+              for (int q = 0; q < 4; ++q)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(wf[q], xf[q], acc[i][j], 0, 0, 0);
+            }
+          }
+        }
+      }
+    } else {
+      const float* sx = (const float*)(lds + buf * Tl::STAGE + (BM + 256) * 128);
+      const float* sw = sx + Tl::SROWS;
+      auto widen = [](omt_u32x4 c, int half) {  // eight e4m3 values as bfloat16
+        bf16x8 v;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const auto lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[half * 2 + e], 1.f, false);
+          const auto hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[half * 2 + e], 1.f, true);
+          v[4 * e] = lo[0], v[4 * e + 1] = lo[1], v[4 * e + 2] = hi[0], v[4 * e + 3] = hi[1];
+        }
+        return v;
+      };
+      f32x4 part[TI][TJ] = {};
+#pragma unroll
+      for (int kk = 0; kk < 2; ++kk) {
+        omt_u32x4 wv[TJ];
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) wv[j] = chunk(ws + wrow(j) * 128 + (frag ^ (kk * 64)));
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          bf16x8 wb[TJ];
+#pragma unroll
+          for (int j = 0; j < TJ; ++j) wb[j] = widen(wv[j], half);
+#pragma unroll
+          for (int i = 0; i < TI; ++i) {
+            const bf16x8 xb = widen(chunk(xs + i * 2048 + (frag ^ (kk * 64))), half);
+#pragma unroll
+            for (int j = 0; j < TJ; ++j)
+              part[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[j], xb, part[i][j], 0, 0, 0);
+          }
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < TI; ++i)
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) acc[i][j] += part[i][j] * (sx[xrow + i * 16 + r16] * sw[wrow(j)]);
+    }
+  };
+
+#pragma unroll
+  for (int p = 0; p < NS - 1; ++p) issue(p, s0 + p);
+  int cur = 0, nxt = NS - 1;
+  for (int s = s0; s < s1; ++s) {
+    // this wave's loads of step s have landed, and its reads of the step before are done; past the barrier, every
+    // wave's, so that stage may be written again
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm(Tl::LOADS * (NS - 2)) & ~0xF00);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    issue(nxt, s + NS - 1);
+    compute(cur);
+    cur = cur + 1 == NS ? 0 : cur + 1;
+    nxt = nxt + 1 == NS ? 0 : nxt + 1;
+  }
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0) & ~0xF00);
+  asm volatile("" ::: "memory");
+  __syncthreads();
+
+  // a lane holds four consecutive columns (4 g ..) of one row (r16) of each 16 x 16 tile
+  const bool vec = (a.n & 3) == 0;
+  if (a.slices > 1) {
+    const int64_t width = GLU ? 2 * (int64_t)a.n : a.n;
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+      const int m = m0 + xrow + i * 16 + r16;
+      if (m >= a.m) continue;
+      float* row = a.parts + ((int64_t)id.z * a.m + m) * width;
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) {
+        const int r = wrow(j) + 4 * g;
+        if constexpr (GLU) store4(row + (r >= 128 ? a.n : 0), n0 + (r & 127), a.n, vec, acc[i][j]);
+        else store4(row, n0 + r, a.n, vec, acc[i][j]);
+      }
+    }
+    return;
+  }
+  if constexpr (!GLU) {
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+      const int m = m0 + xrow + i * 16 + r16;
+      if (m >= a.m) continue;
+#pragma unroll
+      for (int j = 0; j < TJ; ++j)
+        store4_any(m < a.split ? a.out : a.out2, m < a.split ? m : m - a.split, n0 + wrow(j) + 4 * g, a.n, vec,
+                   a.out_kind, acc[i][j]);
+    }
+  } else {
+    uint32_t* top = (uint32_t*)lds;  // [g, u, h][wave][row]: each wave's largest magnitudes of 32 columns
+    const bool keep8 = a.keep == kKeepFp8, out8 = a.out_kind == kOutFp8;
+    auto h4 = [&](f32x4 gv, f32x4 uv) {
+      f32x4 h;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) h[e] = glu_act(gv[e], a.act) * uv[e];
+      return h;
+    };
+    if (keep8 || out8) {
+#pragma unroll
+      for (int i = 0; i < TI; ++i) {
+        uint32_t b[3] = {0, 0, 0};
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          const f32x4 h = out8 ? h4(acc[i][jj], acc[i][jj + 2]) : f32x4{};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            b[0] = max_u32(b[0], abs_bits(acc[i][jj][e]));
+            b[1] = max_u32(b[1], abs_bits(acc[i][jj + 2][e]));
+            b[2] = max_u32(b[2], abs_bits(h[e]));
+          }
+        }
+#pragma unroll
+        for (int z = 0; z < 3; ++z) {
+          b[z] = max_u32(b[z], (uint32_t)__shfl_xor((int)b[z], 16));
+          b[z] = max_u32(b[z], (uint32_t)__shfl_xor((int)b[z], 32));
+          if (g == 0) top[(z * 4 + wn) * BM + xrow + i * 16 + r16] = b[z];
+        }
+      }
+      __syncthreads();
+    }
+    const int blocks = (a.n + kFp8Block - 1) / kFp8Block;
+#pragma unroll
+    for (int i = 0; i < TI; ++i) {
+      const int lr = xrow + i * 16 + r16, m = m0 + lr;
+      float s[3] = {1.f, 1.f, 1.f}, inv[3];
+      if (keep8 || out8) {
+#pragma unroll
+        for (int z = 0; z < 3; ++z) {
+          const uint32_t* p = top + z * 4 * BM + lr;
+          s[z] = block_scale(max_u32(max_u32(p[0], p[BM]), max_u32(p[2 * BM], p[3 * BM])));
+        }
+      }
+#pragma unroll
+      for (int z = 0; z < 3; ++z) inv[z] = 1.f / s[z];
+      if (m >= a.m) continue;
+      if (wn == 0 && g == 0) {
+        const int64_t at = (int64_t)m * blocks + (n0 >> 7);
+        if (keep8) a.keep_gs[at] = s[0], a.keep_us[at] = s[1];
+        if (out8) a.out_scale[at] = s[2];
+      }
+#pragma unroll
+      for (int jj = 0; jj < 2; ++jj) {
+        const int c = n0 + wrow(jj) + 4 * g;
+        const f32x4 gv = acc[i][jj], uv = acc[i][jj + 2], h = h4(gv, uv);
+        if (out8) store4_fp8(a.out, m, c, a.n, vec, h, inv[2]);
+        else store4_any(a.out, m, c, a.n, vec, a.out_kind, h);
+        if (keep8) {
+          store4_fp8(a.keep_g, m, c, a.n, vec, gv, inv[0]);
+          store4_fp8(a.keep_u, m, c, a.n, vec, uv, inv[1]);
+        } else if (a.keep == kKeepFull) {
+          store4_any(a.keep_g, m, c, a.n, vec, a.out_kind, gv);
+          store4_any(a.keep_u, m, c, a.n, vec, a.out_kind, uv);
+        }
+      }
+    }
+  }
+}
+
+template <int MODE, bool GLU, int BM, int NS>
+int launch_gemm(const GemmArgs& a, hipStream_t stream) {
+  hipLaunchKernelGGL((ffn_gemm_kernel<MODE, GLU, BM, NS>), dim3((unsigned)(a.gx * a.gy * a.slices)),
+                     dim3(GemmTile<MODE, BM, NS>::THREADS), 0, stream, a);
+  return launch_check("ffn_gemm_kernel");
+}
+
+// bm: 16 or 64 rows of x to a tile (a.gx, a.gy in those units)
+int ffn_gemm_f32(const GemmArgs& a, bool glu, int bm, hipStream_t stream);
+int ffn_gemm_bf16(const GemmArgs& a, bool glu, int bm, hipStream_t stream);
+int ffn_gemm_fp8(const GemmArgs& a, bool glu, int bm, hipStream_t stream);
+
+}  // namespace omt

@@ -20,7 +20,9 @@ TILE_SPLIT = 256  # OMT_TILE_SPLIT
 NOALLOC_SCRATCH_BYTES = 64 << 20  # OMT_NOALLOC_SCRATCH_BYTES
 (OMT_PW_ADD, OMT_PW_MUL, OMT_PW_RELU, OMT_PW_THRESHOLD_BWD, OMT_PW_HARDSWISH, OMT_PW_HARDSWISH_BWD, OMT_PW_HARDSIGMOID,
  OMT_PW_HARDSIGMOID_BWD, OMT_PW_SCALE, OMT_PW_FILL, OMT_PW_ADD_SCALAR) = range(11)
-OMT_DT_F32, OMT_DT_I64 = 0, 1
+OMT_DT_F32, OMT_DT_I64, OMT_DT_BF16 = 0, 1, 2
+OMT_GLU_SILU, OMT_GLU_GELU, OMT_GLU_RELU = 0, 1, 2
+OMT_KEEP_NONE, OMT_KEEP_FP8, OMT_KEEP_FULL = 0, 1, 2
 OMT_ACT_NONE, OMT_ACT_RELU, OMT_ACT_HARDSWISH = 0, 1, 2
 FOREACH_MAX_NUMEL = 1 << 16  # OMT_FOREACH_MAX_NUMEL
 
@@ -215,6 +217,19 @@ SIGNATURES = {
     "omt_adapool_bwd": (I32, [I64] * 5 + [VP, VP, VP]),
     "omt_fused_adam": (I32, [ctypes.POINTER(AdamParams), ctypes.POINTER(AdamTensor), I32, VP]),
     "omt_fused_sgd": (I32, [ctypes.POINTER(SgdParams), ctypes.POINTER(SgdTensor), I32, VP]),
+    "omt_rms_norm_fwd": (I32, [I32, I32, I64, I64, VP, VP, VP, F32, VP, VP, VP, VP, VP, VP]),
+    "omt_rms_norm_bwd_workspace": (SZ, [I64, I64]),
+    "omt_rms_norm_bwd": (I32, [I32, I32, I64, I64] + [VP] * 8 + [SZ, VP]),
+    "omt_quantize_fp8": (I32, [I32, I64, I64, VP, I32, VP, VP, VP]),
+    "omt_quantize_fp8_weight": (I32, [I32, I64, I64, VP, VP, VP, VP]),
+    "omt_matmul_fp8_workspace": (SZ, [I64, I64, I64]),
+    "omt_matmul_fp8": (I32, [I64, I64, I64, VP, VP, VP, VP, I32, VP, VP, SZ, VP]),
+    "omt_glu_fwd_workspace": (SZ, [I32, I64, I64, I64]),
+    "omt_glu_fwd": (I32, [I32, I64, I64, I64, I32, I32] + [VP] * 11 + [SZ, VP]),
+    "omt_glu_bwd_workspace": (SZ, [I32, I64, I64, I64]),
+    "omt_glu_bwd": (I32, [I32, I64, I64, I64, I32, I32] + [VP] * 13 + [SZ, VP]),
+    "omt_glu_fp8_workspace": (SZ, [I64, I64, I64]),
+    "omt_glu_fp8": (I32, [I64, I64, I64, I32] + [VP] * 9 + [SZ, VP]),
 }
 
 ABI_VERSION = 5
