@@ -176,21 +176,46 @@ __global__ void __launch_bounds__(256) glu_join_kernel(GemmArgs a) {
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
 
-// The launch of a product of m rows by n (of each weight, if gated) with rows of row_bytes.
+// The launch of a product of m rows by n (of each weight, if gated) with rows of row_bytes. Every choice of rows to a
+// tile and slices of the reduction is priced, in microseconds, and the cheapest taken: rounds of workgroups over the 256
+// CUs (two at a time of the tiles of 16 and 64 rows, whose stages leave room), each its steps and a fixed 1.5, but no
+// less than the operands' bytes at 5.5 TB/s; slices add the second launch and their sums' way to memory and back at
+// 4 TB/s. Measured steps (4096 x 4096 x 4096, all CUs busy), us; [mode][16, 64, 128, 256 rows]:
+constexpr float kStepUs[][4] = {
+    {1.3f, 4.0f, 3.83f, 7.46f},   // kF32
+    {0.45f, 1.12f, 0.96f, 1.75f}, // kBf16
+    {0.8f, 2.9f, 2.1f, 3.8f},     // kFp8x
+    {0.45f, 2.2f, 1.3f, 2.7f},    // kFp8
+    {0.8f, 2.3f, 1.52f, 2.86f},   // kSplit
+};
+constexpr int kBm[4] = {16, 64, 128, 256}, kResident[4] = {2, 2, 1, 1};
 struct GemmPlan {
   int bm, gx, gy, steps, slices, slice_steps;
+  float us;
   size_t parts_bytes;
 };
 static GemmPlan plan_gemm(int mode, bool glu, int64_t m, int64_t n, int64_t row_bytes) {
-  GemmPlan p{};
-  p.bm = m <= 16 ? 16 : 64;
-  p.gx = (int)cdiv(n, glu ? 128 : 256);
-  p.gy = (int)cdiv(m, p.bm);
-  p.steps = (int)cdiv(row_bytes, 128);
-  p.slices = 1;
-  p.slice_steps = p.steps;
-  if (p.slices > 1) p.parts_bytes = (size_t)p.slices * m * n * (glu ? 2 : 1) * sizeof(float);
-  return p;
+  const int64_t gx = cdiv(n, glu ? 128 : 256), steps = cdiv(row_bytes, 128), sums = m * n * (glu ? 2 : 1);
+  const float bytes_us = (float)(m + n * (glu ? 2 : 1)) * (float)row_bytes / 5.5e6f;
+  GemmPlan best{};
+  best.us = 1e30f;
+  for (int v = 0; v < 4; ++v) {
+    const int64_t gy = cdiv(m, kBm[v]);
+    if (v > 0 && m <= kBm[v - 1]) break;
+    for (int64_t s = 1; s <= 32 && s * 2 <= std::max<int64_t>(steps, 2); ++s) {
+      const int64_t per = cdiv(steps, s), slices = cdiv(steps, per);
+      if (slices != s) continue;
+      const float rounds = (float)cdiv(gx * gy * s, 256 * kResident[v]);
+      // a CU's second workgroup slows the first: one alone takes about half the step that two take
+      const float step = kStepUs[mode][v] * (kResident[v] == 2 && gx * gy * s <= 256 ? 0.6f : 1.f);
+      float us = std::max(rounds * (per * step + 1.5f), bytes_us);
+      if (s > 1) us += 4.f + 2.f * s * sums * 4 / 4e6f;
+      if (us < best.us) best = {kBm[v], (int)gx, (int)gy, (int)steps, (int)s, (int)per, us, 0};
+      if (gx * gy * s > 2048) break;
+    }
+  }
+  if (best.slices > 1) best.parts_bytes = (size_t)best.slices * sums * sizeof(float);
+  return best;
 }
 static int run_gemm(int mode, bool glu, const GemmPlan& p, GemmArgs a, void* parts, hipStream_t stream) {
   a.steps = p.steps, a.slices = p.slices, a.slice_steps = p.slice_steps, a.gx = p.gx, a.gy = p.gy;
@@ -357,7 +382,8 @@ OMT_EXPORT int omt_matmul_fp8(int64_t m, int64_t n, int64_t k, const void* a, co
   if (err) return err;
   g.sx = a_scale, g.sw = b_scale;
   g.xpitch = l.a.pitch, g.wpitch = l.b.pitch;
-  g.m = (int)m, g.n = (int)n, g.row_bytes = (int)l.a.pitch, g.blocks = (int)cdiv(k, kFp8Block);
+  g.m = (int)m, g.n = (int)n, g.row_bytes = (int)l.a.pitch;
+  g.sx_row = g.sw_row = (int)cdiv(k, kFp8Block), g.sx_step = g.sw_step = 1;
   g.out = c, g.split = (int)m, g.out_kind = out_dtype == OMT_DT_BF16 ? kOutBf16 : kOutF32;
   return run_gemm(kFp8x, false, l.p, g, l.parts, st);
 }
@@ -429,7 +455,8 @@ OMT_EXPORT int omt_glu_fp8(int64_t m, int64_t k, int64_t f, int act, const void*
   if (err) return err;
   a.sx = x_scale, a.sw = gate_scale, a.sw_up = up_scale;
   a.xpitch = l.x.pitch, a.wpitch = l.wg.pitch;
-  a.m = (int)m, a.n = (int)f, a.row_bytes = (int)l.x.pitch, a.blocks = (int)cdiv(k, kFp8Block), a.split = (int)m;
+  a.m = (int)m, a.n = (int)f, a.row_bytes = (int)l.x.pitch, a.split = (int)m;
+  a.sx_row = a.sw_row = (int)cdiv(k, kFp8Block), a.sx_step = a.sw_step = 1;
   a.out = h_q, a.out_scale = h_scale, a.out_kind = kOutFp8, a.act = act, a.keep = kKeepNone;
   return run_gemm(kFp8x, true, l.p, a, l.parts, st);
 }

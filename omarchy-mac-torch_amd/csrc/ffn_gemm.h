@@ -17,7 +17,7 @@ namespace omt {
 
 // kF32: v_mfma_f32_16x16x4_f32 on the floats themselves. kBf16: v_mfma_f32_16x16x32_bf16. kFp8x: e4m3 values taken to
 // bfloat16 (exact) for the same instruction; each step is one block of 128, whose sum is multiplied by the two scales.
-enum GemmMode { kF32, kBf16, kFp8x };
+enum GemmMode { kF32, kBf16, kFp8x, kFp8, kSplit };
 enum GluKeep { kKeepNone, kKeepFp8, kKeepFull };
 enum OutKind { kOutF32, kOutBf16, kOutFp8 };
 
@@ -32,9 +32,10 @@ __device__ __forceinline__ const T* uniform(const T* p) {
 
 struct GemmArgs {
   const void *x, *w, *w_up;           // rows of xpitch / wpitch bytes on 16-byte boundaries; w_up: the gated form's
-  const float *sx, *sw, *sw_up;       // kFp8x: x's scales [m][blocks], w's [ceil(n / 128)][blocks]
+  const float *sx, *sw, *sw_up;       // 8 bits: x's scales [m][blocks], w's [ceil(n / 128)][blocks]
+  int sx_row, sw_row, sx_step, sw_step;  // floats from a row's scale to the next row's, and to its next step's
   int64_t xpitch, wpitch;
-  int m, n, row_bytes, steps, blocks; // n: rows of w (and of w_up); row_bytes: the reduction's length
+  int m, n, row_bytes, steps;         // n: rows of w (and of w_up); row_bytes: the reduction's length
   int slices, slice_steps;            // steps of each slice of the reduction; more than one slice: sums go to parts
   int gx, gy;                         // tiles
   float* parts;                       // [slices][m][n], gated: [slices][m][2][n]
@@ -92,6 +93,19 @@ __device__ __forceinline__ void store4_fp8(void* p, int64_t row, int c, int cols
   }
 }
 
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+// eight e4m3 values as bfloat16
+__device__ __forceinline__ omt_u32x4 widen_fp8(uint32_t lo, uint32_t hi) {
+  return omt_u32x4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, 1.f, true)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, false)),
+                   __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, 1.f, true))};
+}
+__device__ __forceinline__ i32x8 join8(omt_u32x4 a, omt_u32x4 b) {
+  return i32x8{(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+}
+
 template <int MODE, int BM, int NS>
 struct GemmTile {
   static constexpr int WM = BM >= 128 ? 2 : 1;        // waves along the rows of x; 4 along the rows of w
@@ -99,7 +113,7 @@ struct GemmTile {
   static constexpr int TI = BM / WM / 16, TJ = 4;      // a wave's 16 x 16 tiles
   static constexpr int XI = BM / 8, DI = XI + 32;      // loads of 8 rows a step
   static constexpr int DW = (DI + NW - 1) / NW;        // ... by each wave (some repeated, so that all waves' counts are one)
-  static constexpr bool SCALED = MODE == kFp8x;
+  static constexpr bool SCALED = MODE != kF32 && MODE != kBf16;
   static constexpr int SROWS = BM < 64 ? 64 : BM;
   static constexpr int SI = SROWS / 64 + 4;            // loads of 64 scales a step
   static constexpr int SW = SCALED ? (SI + NW - 1) / NW : 0;
@@ -150,15 +164,17 @@ ffn_gemm_kernel(GemmArgs a) {
       sdst[t] = (BM + 256) * 128 + slot * 256;
       if (slot < Tl::SROWS / 64) {
         const int r = slot * 64 + lane;
-        sbase[t] = a.sx + (int64_t)m0 * a.blocks;
-        soff[t] = m0 + r < a.m && r < BM ? (uint32_t)(r * a.blocks) * 4 : kOOB;
+        sbase[t] = a.sx + (int64_t)m0 * a.sx_row;
+        soff[t] = m0 + r < a.m && r < BM ? (uint32_t)(r * a.sx_row) * 4 : kOOB;
       } else {
         const int r64 = (slot - Tl::SROWS / 64) * 64, r = (GLU ? r64 & 127 : r64) + lane;
-        sbase[t] = (GLU && r64 >= 128 ? a.sw_up : a.sw) + (int64_t)(n0 >> 7) * a.blocks;
-        soff[t] = n0 + r < a.n ? (uint32_t)((r >> 7) * a.blocks) * 4 : kOOB;
+        constexpr int kShift = MODE == kSplit ? 0 : 7;
+        sbase[t] = (GLU && r64 >= 128 ? a.sw_up : a.sw) + (int64_t)(n0 >> kShift) * a.sw_row;
+        soff[t] = n0 + r < a.n ? (uint32_t)((r >> kShift) * a.sw_row) * 4 : kOOB;
       }
     }
   }
+  auto slot_of_x = [&](int t) { return wave + Tl::NW * t < Tl::SROWS / 64; };
   const uint32_t lds0 = lds_addr((const float*)lds);
   // Step s into stage `buf`. Past the slice's last step every lane's offset is out of range: the loads count, and read
   // nothing.
@@ -173,7 +189,7 @@ ffn_gemm_kernel(GemmArgs a) {
     if constexpr (Tl::SCALED) {
 #pragma unroll
       for (int t = 0; t < Tl::SW; ++t)
-        lds_load_b32(rsrc_words(uniform(sbase[t] + s), 0x7fffffffu),
+        lds_load_b32(rsrc_words(uniform(sbase[t] + (slot_of_x(t) ? s * (int64_t)a.sx_step : s * (int64_t)a.sw_step)), 0x7fffffffu),
                      __builtin_amdgcn_readfirstlane(at + sdst[t]), left ? soff[t] : kOOB, 0);
     }
   };
@@ -211,42 +227,57 @@ ffn_gemm_kernel(GemmArgs a) {
         }
       }
     } else {
-      const float* sx = (const float*)(lds + buf * Tl::STAGE + (BM + 256) * 128);
-      const float* sw = sx + Tl::SROWS;
-      auto widen = [](omt_u32x4 c, int half) {  // eight e4m3 values as bfloat16
-        bf16x8 v;
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const auto lo = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[half * 2 + e], 1.f, false);
-          const auto hi = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c[half * 2 + e], 1.f, true);
-          v[4 * e] = lo[0], v[4 * e + 1] = lo[1], v[4 * e + 2] = hi[0], v[4 * e + 3] = hi[1];
+      // a block's sum, then times both scales, onto the sum of the blocks
+      const float* sx = (const float*)(lds + buf * Tl::STAGE + (BM + 256) * 128) + xrow + r16;
+      const float* sw = (const float*)(lds + buf * Tl::STAGE + (BM + 256) * 128) + Tl::SROWS;
+      constexpr int KQ = MODE == kFp8x ? 4 : 2;
+      auto fragments = [&](omt_u32x4* f, const unsigned char* row) {
+        const omt_u32x4 lo = chunk(row + frag), hi = chunk(row + (frag ^ 64));
+        if constexpr (MODE == kFp8x) {
+          f[0] = widen_fp8(lo[0], lo[1]), f[1] = widen_fp8(lo[2], lo[3]);
+          f[2] = widen_fp8(hi[0], hi[1]), f[3] = widen_fp8(hi[2], hi[3]);
+        } else {
+          f[0] = lo, f[1] = hi;
         }
-        return v;
       };
-      f32x4 part[TI][TJ] = {};
+      omt_u32x4 wv[TJ][KQ];
+      using Scale = std::conditional_t<MODE == kSplit, f32x4, float>;
+      Scale ws4[TJ];
 #pragma unroll
-      for (int kk = 0; kk < 2; ++kk) {
-        omt_u32x4 wv[TJ];
-#pragma unroll
-        for (int j = 0; j < TJ; ++j) wv[j] = chunk(ws + wrow(j) * 128 + (frag ^ (kk * 64)));
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          bf16x8 wb[TJ];
-#pragma unroll
-          for (int j = 0; j < TJ; ++j) wb[j] = widen(wv[j], half);
-#pragma unroll
-          for (int i = 0; i < TI; ++i) {
-            const bf16x8 xb = widen(chunk(xs + i * 2048 + (frag ^ (kk * 64))), half);
-#pragma unroll
-            for (int j = 0; j < TJ; ++j)
-              part[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[j], xb, part[i][j], 0, 0, 0);
-          }
-        }
+      for (int j = 0; j < TJ; ++j) {
+        fragments(wv[j], ws + wrow(j) * 128);
+        if constexpr (MODE == kSplit) ws4[j] = *(const f32x4*)(sw + wrow(j) + 4 * g);
+        else ws4[j] = sw[wrow(j)];  // one block of 128 rows
       }
 #pragma unroll
-      for (int i = 0; i < TI; ++i)
+      for (int i = 0; i < TI; ++i) {
+        omt_u32x4 xv[KQ];
+        fragments(xv, xs + i * 2048);
+        const float xscale = sx[i * 16];
+        f32x4 part[TJ] = {};
+        if constexpr (MODE == kFp8x) {
 #pragma unroll
-        for (int j = 0; j < TJ; ++j) acc[i][j] += part[i][j] * (sx[xrow + i * 16 + r16] * sw[wrow(j)]);
+          for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int j = 0; j < TJ; ++j)
+              part[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[j][q]),
+                                                                __builtin_bit_cast(bf16x8, xv[q]), part[j], 0, 0, 0);
+        } else if constexpr (MODE == kFp8) {
+#pragma unroll
+          for (int j = 0; j < TJ; ++j)
+            part[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join8(wv[j][0], wv[j][1]), join8(xv[0], xv[1]),
+                                                                       part[j], 0, 0, 0, 0, 0, 0);
+        } else {  // high by low, low by high, high by high
+#pragma unroll
+          for (int q = 0; q < 3; ++q)
+#pragma unroll
+            for (int j = 0; j < TJ; ++j)
+              part[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, wv[j][q == 1]),
+                                                               __builtin_bit_cast(f16x8, xv[q == 0]), part[j], 0, 0, 0);
+        }
+#pragma unroll
+        for (int j = 0; j < TJ; ++j) acc[i][j] += part[j] * (ws4[j] * xscale);
+      }
     }
   };
 
@@ -374,7 +405,18 @@ int launch_gemm(const GemmArgs& a, hipStream_t stream) {
   return launch_check("ffn_gemm_kernel");
 }
 
-// bm: 16 or 64 rows of x to a tile (a.gx, a.gy in those units)
+// bm rows of x to a tile: 16, 64, 128 or 256 (a.gx, a.gy in those units). Two stages: two workgroups of the small tiles
+// fit a CU's 160 KB together and hide each other's waits better than a third stage does (64 rows bf16, 4096 x 4096 x
+// 4096: 144 us with two, 226 with three and one workgroup); 128 rows gain 1-3% from a third where it fits.
+template <int MODE>
+int launch_gemm_of(const GemmArgs& a, bool glu, int bm, hipStream_t stream) {
+  switch (bm) {
+    case 16: return glu ? launch_gemm<MODE, true, 16, 2>(a, stream) : launch_gemm<MODE, false, 16, 2>(a, stream);
+    case 64: return glu ? launch_gemm<MODE, true, 64, 2>(a, stream) : launch_gemm<MODE, false, 64, 2>(a, stream);
+    case 128: return glu ? launch_gemm<MODE, true, 128, 3>(a, stream) : launch_gemm<MODE, false, 128, 3>(a, stream);
+    default: return glu ? launch_gemm<MODE, true, 256, 2>(a, stream) : launch_gemm<MODE, false, 256, 2>(a, stream);
+  }
+}
 int ffn_gemm_f32(const GemmArgs& a, bool glu, int bm, hipStream_t stream);
 int ffn_gemm_bf16(const GemmArgs& a, bool glu, int bm, hipStream_t stream);
 int ffn_gemm_fp8(const GemmArgs& a, bool glu, int bm, hipStream_t stream);
