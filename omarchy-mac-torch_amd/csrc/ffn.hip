@@ -28,32 +28,91 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const T* __restrict__ src
   }
 }
 
-// A 64 x 64 block held in LDS (rows of 65 floats), its rows or its columns written as `lines` lines of T at dst, `width`
-// elements of each (a multiple of 16), `stride` elements apart.
+// Where lines of an operand go: bfloat16 (kBf16), or float32 as two halves (kSplit). There the 32 elements that a step of
+// the tiles reads of a line are scaled by one power of two, so that the largest lies in [2^14, 2^15), and each is held as
+// the nearest float16 and the float16 nearest to what is left: 22 bits, or 2^-40 of the largest where that is more. 32
+// high halves, then the 32 low ones; the scales lie by step, then line. Where a group holds an infinity its scale is
+// infinite, with +-1 for the infinities and 0 for the rest; where it holds NaN, NaN.
+struct Lines {
+  char* p = nullptr;
+  int64_t pitch = 0;       // bytes
+  float* scale = nullptr;  // kSplit: [pitch / 128][scale_lines]
+  int64_t scale_lines = 0;
+};
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+
+// 16 elements (at: a multiple of 16) of a line; kSplit: threads 2i and 2i + 1 call it together for the two halves of 32
+template <int FMT>
+__device__ __forceinline__ void write16(const Lines& d, int64_t line, int64_t at, f32x8 lo, f32x8 hi) {
+  if constexpr (FMT == kBf16) {
+    __bf16* p = (__bf16*)(d.p + line * d.pitch) + at;
+    store8<true>(p, 0, 16, lo);
+    store8<true>(p, 8, 16, hi);
+  } else {
+    uint32_t b = max_u32(abs_bits8(lo), abs_bits8(hi));
+    b = max_u32(b, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)b, 0xB1, 0xF, 0xF, false));  // quad_perm [1,0,3,2]
+    float up, scale;
+    if (b < 0x7f800000u) {
+      const uint32_t e = max_u32(b >> 23, 15u);
+      up = __builtin_bit_cast(float, (268u - e) << 23);
+      scale = __builtin_bit_cast(float, (e - 14u) << 23);
+    } else {
+      up = 1.f;
+      scale = __builtin_bit_cast(float, b);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        lo[e] = abs_bits(lo[e]) == 0x7f800000u ? copysignf(1.f, lo[e]) : 0.f;
+        hi[e] = abs_bits(hi[e]) == 0x7f800000u ? copysignf(1.f, hi[e]) : 0.f;
+      }
+    }
+    char* p = d.p + line * d.pitch + (at >> 5) * 128 + (at & 31) * 2;
+    auto halves = [&](f32x8 v, char* to) {
+      v *= up;
+      const half8 h = __builtin_convertvector(v, half8);
+      *(half8*)to = h;
+      *(half8*)(to + 64) = __builtin_convertvector(v - __builtin_convertvector(h, f32x8), half8);
+    };
+    halves(lo, p);
+    halves(hi, p + 16);
+    if ((at & 31) == 0) d.scale[(at >> 5) * d.scale_lines + line] = scale;
+  }
+}
+
+// A 64 x 64 block held in LDS (rows of 65 floats): its rows, or its columns, as lines line0.. (below `lines`) of d, elements
+// at.. of each
 constexpr int kBlk = 64, kBlkPitch = 65;
-template <class T>
-__device__ __forceinline__ void write_block(const float* blk, bool columns, T* dst, int64_t stride, int64_t lines,
-                                            int64_t width) {
-  const int line = threadIdx.x >> 2, part = (threadIdx.x & 3) * 16;  // 16 consecutive elements of one line
-  if (line >= lines || part >= width) return;
+template <int FMT>
+__device__ __forceinline__ void write_block(const float* blk, bool columns, const Lines& d, int64_t line0, int64_t lines,
+                                            int64_t at) {
+  const int line = threadIdx.x >> 2, part = (threadIdx.x & 3) * 16;
+  if (line0 + line >= lines) return;  // all four threads of a line
   f32x8 lo, hi;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     lo[e] = columns ? blk[(part + e) * kBlkPitch + line] : blk[line * kBlkPitch + part + e];
     hi[e] = columns ? blk[(part + 8 + e) * kBlkPitch + line] : blk[line * kBlkPitch + part + 8 + e];
   }
-  T* p = dst + line * stride + part;
-  store8<true>(p, 0, 16, lo);
-  store8<true>(p, 8, 16, hi);
+  write16<FMT>(d, line0 + line, at + part, lo, hi);
 }
 
-// dst [cols][pitch], `width` of each row written (zeros from `rows` on) = src^T of src [rows][cols]; SRC float, __bf16, or e4m3 with its scales.
-template <class T, class S>
+// rows of floats as kSplit lines, zeros past their end up to a multiple of 64
+template <bool VEC>
+__global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ src, int64_t rows, int64_t cols,
+                                                         Lines d) {
+  const int64_t line = (int64_t)blockIdx.x * kBlk + (threadIdx.x >> 2);
+  const int64_t at = (int64_t)blockIdx.y * kBlk + (threadIdx.x & 3) * 16;
+  if (line >= rows) return;
+  const float* p = src + line * cols;
+  write16<kSplit>(d, line, at, load8<VEC>(p, at, cols), load8<VEC>(p, at + 8, cols));
+}
+
+// The columns of src [rows][cols] as lines of d, zeros from `rows` on up to a multiple of 64; S float, __bf16, or e4m3 with
+// its scales.
+template <int FMT, class S>
 __global__ void __launch_bounds__(256) transpose_kernel(const S* __restrict__ src, const float* __restrict__ scale,
-                                                        int64_t rows, int64_t cols, int64_t width, int64_t pitch,
-                                                        T* __restrict__ dst) {
+                                                        int64_t rows, int64_t cols, Lines d) {
   __shared__ float blk[kBlk * kBlkPitch];
-  const int64_t r0 = (int64_t)blockIdx.y * kBlk, c0 = (int64_t)blockIdx.x * kBlk;
+  const int64_t r0 = (int64_t)blockIdx.x * kBlk, c0 = (int64_t)blockIdx.y * kBlk;
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t blocks = (cols + kFp8Block - 1) / kFp8Block;
 #pragma unroll
@@ -67,21 +126,22 @@ __global__ void __launch_bounds__(256) transpose_kernel(const S* __restrict__ sr
     blk[r * kBlkPitch + l] = v;
   }
   __syncthreads();
-  write_block(blk, true, dst + c0 * pitch + r0, pitch, cols - c0, width - r0);
+  write_block<FMT>(blk, true, d, c0, cols, r0);
 }
 
 struct GateArgs {
   const void *gh, *g, *u;
   const float *gs, *us;
-  int64_t m, f, half, mp;  // half: the distance of dg and du in a row of `rows_out` (2 * half elements)
-  int act;
-  void *rows_out, *cols_out;  // [m][2 * half] and [2 * f][mp]; either may be null
+  int64_t m, f;
+  int act, by_rows, by_cols;
+  Lines g_rows, u_rows;  // m lines each: dg and du side by side
+  Lines g_cols, u_cols;  // f lines each: one below the other
 };
 // dg and du of a 64 x 64 block of (row, column of f), laid out by rows and by columns
-template <class T, bool FP8>
+template <int FMT, class T, bool FP8>
 __global__ void __launch_bounds__(256) glu_gate_kernel(GateArgs a) {
   __shared__ float dg[kBlk * kBlkPitch], du[kBlk * kBlkPitch];
-  const int64_t r0 = (int64_t)blockIdx.y * kBlk, c0 = (int64_t)blockIdx.x * kBlk;
+  const int64_t r0 = (int64_t)blockIdx.x * kBlk, c0 = (int64_t)blockIdx.y * kBlk;
   const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int64_t blocks = (a.f + kFp8Block - 1) / kFp8Block;
 #pragma unroll 4
@@ -107,15 +167,13 @@ __global__ void __launch_bounds__(256) glu_gate_kernel(GateArgs a) {
     du[r * kBlkPitch + l] = vu;
   }
   __syncthreads();
-  if (a.rows_out) {
-    T* p = (T*)a.rows_out + r0 * 2 * a.half + c0;
-    write_block(dg, false, p, 2 * a.half, a.m - r0, a.half - c0);
-    write_block(du, false, p + a.half, 2 * a.half, a.m - r0, a.half - c0);
+  if (a.by_rows) {
+    write_block<FMT>(dg, false, a.g_rows, r0, a.m, c0);
+    write_block<FMT>(du, false, a.u_rows, r0, a.m, c0);
   }
-  if (a.cols_out) {
-    T* p = (T*)a.cols_out + c0 * a.mp + r0;
-    write_block(dg, true, p, a.mp, a.f - c0, a.mp - r0);
-    write_block(du, true, p + a.f * a.mp, a.mp, a.f - c0, a.mp - r0);
+  if (a.by_cols) {
+    write_block<FMT>(dg, true, a.g_cols, c0, a.f, r0);
+    write_block<FMT>(du, true, a.u_cols, c0, a.f, r0);
   }
 }
 
@@ -221,6 +279,7 @@ static int run_gemm(int mode, bool glu, const GemmPlan& p, GemmArgs a, void* par
   a.steps = p.steps, a.slices = p.slices, a.slice_steps = p.slice_steps, a.gx = p.gx, a.gy = p.gy;
   a.parts = (float*)parts;
   int e = mode == kF32 ? ffn_gemm_f32(a, glu, p.bm, stream)
+          : mode == kSplit ? ffn_gemm_split(a, glu, p.bm, stream)
           : mode == kBf16 ? ffn_gemm_bf16(a, glu, p.bm, stream) : ffn_gemm_fp8(a, glu, p.bm, stream);
   if (e || p.slices == 1) return e;
   const bool vec = a.n % 8 == 0;
@@ -249,33 +308,64 @@ struct Space {
 };
 
 static int64_t up(int64_t v, int64_t to) { return cdiv(v, to) * to; }
-static int elem_bytes(int mode) { return mode == kF32 ? 4 : mode == kBf16 ? 2 : 1; }
+static int elem_bytes(int mode) { return mode == kF32 || mode == kSplit ? 4 : mode == kBf16 ? 2 : 1; }
 
-// An operand's rows as the tiles read them: in place where every row starts on 16 bytes, else copied.
-struct Operand {
-  void* copy = nullptr;
-  int64_t pitch = 0;  // bytes
-};
-static Operand place_rows(Space& sp, int mode, int64_t rows, int64_t cols) {
-  const int64_t bytes = cols * elem_bytes(mode);
-  if (bytes % 16 == 0) return {nullptr, bytes};
-  return {sp.take((size_t)(rows * up(bytes, 16))), up(bytes, 16)};
+// `lines` of n elements (a multiple of 64) in kBf16 or kSplit
+static Lines take_lines(Space& sp, int fmt, int64_t lines, int64_t n) {
+  Lines d;
+  d.pitch = n * elem_bytes(fmt);
+  d.p = (char*)sp.take((size_t)(lines * d.pitch));
+  if (fmt == kSplit) d.scale = (float*)sp.take((size_t)(n / 32 * lines) * sizeof(float)), d.scale_lines = lines;
+  return d;
 }
-static const void* lay_rows(const Operand& o, int mode, const void* src, int64_t rows, int64_t cols, hipStream_t stream,
-                            int* err) {
-  if (!o.copy || *err) return src;
-  const int64_t pitch = o.pitch / elem_bytes(mode);
+// the same from element `at` (a multiple of 64) and line `line` on
+static Lines from(Lines d, int fmt, int64_t line, int64_t at) {
+  d.p += line * d.pitch + at * elem_bytes(fmt);
+  if (d.scale) d.scale += at / 32 * d.scale_lines + line;
+  return d;
+}
+
+// An operand's rows as the tiles read them: in place where every row starts on 16 bytes, else copied; kSplit always copied.
+static Lines place_rows(Space& sp, int mode, int64_t rows, int64_t cols) {
+  if (mode == kSplit) return take_lines(sp, kSplit, rows, up(cols, kBlk));
+  Lines d;
+  const int64_t bytes = cols * elem_bytes(mode);
+  d.pitch = up(bytes, 16);
+  if (d.pitch != bytes) d.p = (char*)sp.take((size_t)(rows * d.pitch));
+  return d;
+}
+static int lay_rows(const Lines& d, int mode, const void* src, int64_t rows, int64_t cols, hipStream_t stream) {
+  if (mode == kSplit) {
+    const dim3 grid((unsigned)cdiv(rows, kBlk), (unsigned)cdiv(cols, kBlk));
+    if (cols % 8 == 0) hipLaunchKernelGGL(split_rows_kernel<true>, grid, dim3(256), 0, stream, (const float*)src, rows, cols, d);
+    else hipLaunchKernelGGL(split_rows_kernel<false>, grid, dim3(256), 0, stream, (const float*)src, rows, cols, d);
+    return launch_check("split_rows_kernel");
+  }
+  if (!d.p) return OMT_OK;
+  const int64_t pitch = d.pitch / elem_bytes(mode);
   const dim3 grid(grid1d(rows * pitch, 256, 1 << 16));
-  if (mode == kF32)
-    hipLaunchKernelGGL(pad_rows_kernel<float>, grid, dim3(256), 0, stream, (const float*)src, rows, cols, pitch, (float*)o.copy);
-  else if (mode == kBf16)
-    hipLaunchKernelGGL(pad_rows_kernel<uint16_t>, grid, dim3(256), 0, stream, (const uint16_t*)src, rows, cols, pitch,
-                       (uint16_t*)o.copy);
-  else
-    hipLaunchKernelGGL(pad_rows_kernel<uint8_t>, grid, dim3(256), 0, stream, (const uint8_t*)src, rows, cols, pitch,
-                       (uint8_t*)o.copy);
-  *err = launch_check("pad_rows_kernel");
-  return o.copy;
+  auto go = [&](auto zero) {
+    using T = decltype(zero);
+    hipLaunchKernelGGL(pad_rows_kernel<T>, grid, dim3(256), 0, stream, (const T*)src, rows, cols, pitch, (T*)d.p);
+  };
+  mode == kF32 ? go(uint32_t(0)) : mode == kBf16 ? go(uint16_t(0)) : go(uint8_t(0));
+  return launch_check("pad_rows_kernel");
+}
+// Lays out x [m][k] and the weights [n][k] (w_up may be null) and points a at them.
+static int lay_operands(GemmArgs& a, int mode, const Lines& x, const Lines& w, const Lines& w_up, const void* px,
+                        const void* pw, const void* pw_up, int64_t m, int64_t n, int64_t k, hipStream_t stream) {
+  if (int e = lay_rows(x, mode, px, m, k, stream)) return e;
+  if (int e = lay_rows(w, mode, pw, n, k, stream)) return e;
+  if (pw_up)
+    if (int e = lay_rows(w_up, mode, pw_up, n, k, stream)) return e;
+  a.x = x.p ? x.p : px, a.w = w.p ? w.p : pw, a.w_up = w_up.p ? w_up.p : pw_up;
+  a.xpitch = x.pitch, a.wpitch = w.pitch, a.row_bytes = (int)x.pitch;
+  a.m = (int)m, a.n = (int)n, a.split = (int)m;
+  if (mode == kSplit) {
+    a.sx = x.scale, a.sw = w.scale, a.sw_up = w_up.scale;
+    a.sx_row = a.sw_row = 1, a.sx_step = (int)x.scale_lines, a.sw_step = (int)w.scale_lines;
+  }
+  return OMT_OK;
 }
 
 static bool on16(std::initializer_list<const void*> ps) {
@@ -300,55 +390,70 @@ static int need_space(const char* fn, size_t need, const void* ws, size_t bytes)
 
 struct MatmulFp8 {
   GemmPlan p;
-  Operand a, b;
+  Lines a, b;
   void* parts;
   MatmulFp8(Space& sp, int64_t m, int64_t n, int64_t k)
       : p(plan_gemm(kFp8x, false, m, n, k)), a(place_rows(sp, kFp8x, m, k)), b(place_rows(sp, kFp8x, n, k)),
         parts(sp.take(p.parts_bytes)) {}
 };
+// float32: on fp32 MFMA as it is, or as halves on float16 MFMA, three products for one. Laying out the halves reads and
+// writes the operands once (4 TB/s, three launches); it is taken where the products win that back.
+static int glu_mode(int dtype, int64_t m, int64_t k, int64_t f) {
+  if (dtype == OMT_DT_BF16) return kBf16;
+  const float lay_us = 8.f * (float)(m + 2 * f) * (float)k / 4e6f + 9.f;
+  return plan_gemm(kSplit, true, m, f, up(k, kBlk) * 4).us + lay_us < plan_gemm(kF32, true, m, f, k * 4).us ? kSplit : kF32;
+}
 struct GluFwd {
   GemmPlan p;
-  Operand x, wg, wu;
+  Lines x, wg, wu;
   void* parts;
   GluFwd(Space& sp, int mode, int64_t m, int64_t k, int64_t f)
-      : p(plan_gemm(mode, true, m, f, k * elem_bytes(mode))), x(place_rows(sp, mode, m, k)),
-        wg(place_rows(sp, mode, f, k)), wu(place_rows(sp, mode, f, k)), parts(sp.take(p.parts_bytes)) {}
+      : x(place_rows(sp, mode, m, k)), wg(place_rows(sp, mode, f, k)), wu(place_rows(sp, mode, f, k)) {
+    p = plan_gemm(mode, true, m, f, x.pitch);
+    parts = sp.take(p.parts_bytes);
+  }
 };
 struct GluBwd {
   int64_t half, mp;  // elements: dg and du of a row padded to `half` each; columns of m padded to mp
-  void *gate_rows, *gate_cols, *w_cols, *x_cols;
+  Lines gate_rows, gate_cols, w_cols, x_cols;
   GemmPlan px, pw;
-  void *parts;
-  GluBwd(Space& sp, int mode, int64_t m, int64_t k, int64_t f) : half(up(f, kBlk)), mp(up(m, kBlk)) {
-    const int e = elem_bytes(mode);
-    gate_rows = sp.take((size_t)(m * 2 * half * e));
-    gate_cols = sp.take((size_t)(2 * f * mp * e));
-    w_cols = sp.take((size_t)(k * 2 * half * e));
-    x_cols = sp.take((size_t)(k * mp * e));
-    px = plan_gemm(mode, false, m, k, 2 * half * e);
-    pw = plan_gemm(mode, false, 2 * f, k, mp * e);
+  void* parts;
+  GluBwd(Space& sp, int mode, int64_t m, int64_t k, int64_t f)
+      : half(up(f, kBlk)), mp(up(m, kBlk)), gate_rows(take_lines(sp, mode, m, 2 * half)),
+        gate_cols(take_lines(sp, mode, 2 * f, mp)), w_cols(take_lines(sp, mode, k, 2 * half)),
+        x_cols(take_lines(sp, mode, k, mp)) {
+    px = plan_gemm(mode, false, m, k, gate_rows.pitch);
+    pw = plan_gemm(mode, false, 2 * f, k, gate_cols.pitch);
     parts = sp.take(std::max(px.parts_bytes, pw.parts_bytes));
   }
 };
 
-static int mode_of(int dtype) { return dtype == OMT_DT_F32 ? kF32 : kBf16; }
 static int glu_check(const char* fn, int dtype, int64_t m, int64_t k, int64_t f, int act) {
   if (dtype != OMT_DT_F32 && dtype != OMT_DT_BF16) return fail(OMT_INVALID, "%s: dtype %d", fn, dtype);
   if (act != OMT_GLU_SILU && act != OMT_GLU_GELU && act != OMT_GLU_RELU) return fail(OMT_INVALID, "%s: act %d", fn, act);
   return product_check(fn, m, f, k);
 }
 
-// dst [cols][pitch] = src^T in elements of `mode`, rows padded to a multiple of 64
+static int bwd_mode(int dtype) { return dtype == OMT_DT_F32 ? kSplit : kBf16; }
+
 template <class S>
-static int run_transpose(int mode, const S* src, const float* scale, int64_t rows, int64_t cols, int64_t pitch,
-                         void* dst, hipStream_t stream) {
-  const int64_t width = up(rows, kBlk);
-  const dim3 grid((unsigned)cdiv(cols, kBlk), (unsigned)cdiv(rows, kBlk));
-  if (mode == kF32)
-    hipLaunchKernelGGL((transpose_kernel<float, S>), grid, dim3(256), 0, stream, src, scale, rows, cols, width, pitch, (float*)dst);
+static int run_transpose(int mode, const S* src, const float* scale, int64_t rows, int64_t cols, const Lines& d,
+                         hipStream_t stream) {
+  const dim3 grid((unsigned)cdiv(rows, kBlk), (unsigned)cdiv(cols, kBlk));
+  if (mode == kSplit)
+    hipLaunchKernelGGL((transpose_kernel<kSplit, S>), grid, dim3(256), 0, stream, src, scale, rows, cols, d);
   else
-    hipLaunchKernelGGL((transpose_kernel<__bf16, S>), grid, dim3(256), 0, stream, src, scale, rows, cols, width, pitch, (__bf16*)dst);
+    hipLaunchKernelGGL((transpose_kernel<kBf16, S>), grid, dim3(256), 0, stream, src, scale, rows, cols, d);
   return launch_check("transpose_kernel");
+}
+// the product of operands laid out as lines: x's lines by w's
+static int run_lines(int mode, const GemmPlan& p, GemmArgs a, const Lines& x, const Lines& w, int64_t m, int64_t n,
+                     void* parts, hipStream_t stream) {
+  a.x = x.p, a.w = w.p, a.xpitch = a.wpitch = x.pitch, a.row_bytes = (int)x.pitch;
+  a.m = (int)m, a.n = (int)n;
+  a.sx = x.scale, a.sw = w.scale, a.sx_row = a.sw_row = 1;
+  a.sx_step = (int)x.scale_lines, a.sw_step = (int)w.scale_lines;
+  return run_gemm(mode, false, p, a, parts, stream);
 }
 
 }  // namespace omt
@@ -375,23 +480,18 @@ OMT_EXPORT int omt_matmul_fp8(int64_t m, int64_t n, int64_t k, const void* a, co
   Space sp{(char*)workspace};
   const MatmulFp8 l(sp, m, n, k);
   hipStream_t st = stream_of(stream);
-  int err = OMT_OK;
   GemmArgs g{};
-  g.x = lay_rows(l.a, kFp8x, a, m, k, st, &err);
-  g.w = lay_rows(l.b, kFp8x, b, n, k, st, &err);
-  if (err) return err;
+  if (int e = lay_operands(g, kFp8x, l.a, l.b, {}, a, b, nullptr, m, n, k, st)) return e;
   g.sx = a_scale, g.sw = b_scale;
-  g.xpitch = l.a.pitch, g.wpitch = l.b.pitch;
-  g.m = (int)m, g.n = (int)n, g.row_bytes = (int)l.a.pitch;
   g.sx_row = g.sw_row = (int)cdiv(k, kFp8Block), g.sx_step = g.sw_step = 1;
-  g.out = c, g.split = (int)m, g.out_kind = out_dtype == OMT_DT_BF16 ? kOutBf16 : kOutF32;
+  g.out = c, g.out_kind = out_dtype == OMT_DT_BF16 ? kOutBf16 : kOutF32;
   return run_gemm(kFp8x, false, l.p, g, l.parts, st);
 }
 
 OMT_EXPORT size_t omt_glu_fwd_workspace(int dtype, int64_t m, int64_t k, int64_t f) {
   if (glu_check("omt_glu_fwd_workspace", dtype, m, k, f, OMT_GLU_SILU) || m == 0) return 0;
   Space sp{nullptr};
-  GluFwd(sp, mode_of(dtype), m, k, f);
+  GluFwd(sp, glu_mode(dtype, m, k, f), m, k, f);
   return sp.used;
 }
 
@@ -408,19 +508,14 @@ OMT_EXPORT int omt_glu_fwd(int dtype, int64_t m, int64_t k, int64_t f, int act, 
     return fail(OMT_INVALID, "%s: null pointer", fn);
   if (!on16({x, w_gate, w_up, h, g, u})) return fail(OMT_INVALID, "%s: an operand is not on 16 bytes", fn);
   if (int e = need_space(fn, omt_glu_fwd_workspace(dtype, m, k, f), workspace, workspace_bytes)) return e;
-  const int mode = mode_of(dtype);
+  const int mode = glu_mode(dtype, m, k, f);
   Space sp{(char*)workspace};
   const GluFwd l(sp, mode, m, k, f);
   hipStream_t st = stream_of(stream);
-  int err = OMT_OK;
-  if (keep == OMT_KEEP_FP8) err = omt_quantize_fp8(dtype, m, k, x, 1, x_q, x_scale, stream);
+  if (keep == OMT_KEEP_FP8)
+    if (int e = omt_quantize_fp8(dtype, m, k, x, 1, x_q, x_scale, stream)) return e;
   GemmArgs a{};
-  a.x = lay_rows(l.x, mode, x, m, k, st, &err);
-  a.w = lay_rows(l.wg, mode, w_gate, f, k, st, &err);
-  a.w_up = lay_rows(l.wu, mode, w_up, f, k, st, &err);
-  if (err) return err;
-  a.xpitch = l.x.pitch, a.wpitch = l.wg.pitch;
-  a.m = (int)m, a.n = (int)f, a.row_bytes = (int)l.x.pitch, a.split = (int)m;
+  if (int e = lay_operands(a, mode, l.x, l.wg, l.wu, x, w_gate, w_up, m, f, k, st)) return e;
   a.out = h, a.out_kind = dtype == OMT_DT_BF16 ? kOutBf16 : kOutF32, a.act = act;
   a.keep = keep == OMT_KEEP_FP8 ? kKeepFp8 : keep == OMT_KEEP_FULL ? kKeepFull : kKeepNone;
   a.keep_g = g, a.keep_u = u, a.keep_gs = g_scale, a.keep_us = u_scale;
@@ -447,15 +542,9 @@ OMT_EXPORT int omt_glu_fp8(int64_t m, int64_t k, int64_t f, int act, const void*
   Space sp{(char*)workspace};
   const GluFwd l(sp, kFp8x, m, k, f);
   hipStream_t st = stream_of(stream);
-  int err = OMT_OK;
   GemmArgs a{};
-  a.x = lay_rows(l.x, kFp8x, x, m, k, st, &err);
-  a.w = lay_rows(l.wg, kFp8x, w_gate, f, k, st, &err);
-  a.w_up = lay_rows(l.wu, kFp8x, w_up, f, k, st, &err);
-  if (err) return err;
+  if (int e = lay_operands(a, kFp8x, l.x, l.wg, l.wu, x, w_gate, w_up, m, f, k, st)) return e;
   a.sx = x_scale, a.sw = gate_scale, a.sw_up = up_scale;
-  a.xpitch = l.x.pitch, a.wpitch = l.wg.pitch;
-  a.m = (int)m, a.n = (int)f, a.row_bytes = (int)l.x.pitch, a.split = (int)m;
   a.sx_row = a.sw_row = (int)cdiv(k, kFp8Block), a.sx_step = a.sw_step = 1;
   a.out = h_q, a.out_scale = h_scale, a.out_kind = kOutFp8, a.act = act, a.keep = kKeepNone;
   return run_gemm(kFp8x, true, l.p, a, l.parts, st);
@@ -464,7 +553,7 @@ OMT_EXPORT int omt_glu_fp8(int64_t m, int64_t k, int64_t f, int act, const void*
 OMT_EXPORT size_t omt_glu_bwd_workspace(int dtype, int64_t m, int64_t k, int64_t f) {
   if (glu_check("omt_glu_bwd_workspace", dtype, m, k, f, OMT_GLU_SILU)) return 0;
   Space sp{nullptr};
-  GluBwd(sp, mode_of(dtype), std::max<int64_t>(m, 1), k, f);
+  GluBwd(sp, bwd_mode(dtype), std::max<int64_t>(m, 1), k, f);
   return sp.used;
 }
 
@@ -486,45 +575,41 @@ OMT_EXPORT int omt_glu_bwd(int dtype, int64_t m, int64_t k, int64_t f, int act, 
   if (!gh || !x || !g || !u || !w_gate || !w_up || (fp8 && (!x_scale || !g_scale || !u_scale)))
     return fail(OMT_INVALID, "%s: null pointer", fn);
   if (!on16({gx, gw_gate, gw_up})) return fail(OMT_INVALID, "%s: a gradient is not on 16 bytes", fn);
-  if (2 * f > 1 << 20 || cdiv(m, kBlk) > 65535 || m > 1 << 20)
+  if (m > 1 << 20 || f > 1 << 18)
     return fail(OMT_UNSUPPORTED, "%s: %lld x %lld x %lld", fn, (long long)m, (long long)k, (long long)f);
   if (int err = need_space(fn, omt_glu_bwd_workspace(dtype, m, k, f), workspace, workspace_bytes)) return err;
   if (!gx && !gw_gate) return OMT_OK;
-  const int mode = mode_of(dtype), eb = elem_bytes(mode);
+  const int mode = bwd_mode(dtype), out_kind = dtype == OMT_DT_F32 ? kOutF32 : kOutBf16;
   Space sp{(char*)workspace};
   const GluBwd l(sp, mode, m, k, f);
   hipStream_t st = stream_of(stream);
 
-  const GateArgs ga{gh, g, u, g_scale, u_scale, m, f, l.half, l.mp, act, gx ? l.gate_rows : nullptr,
-                    gw_gate ? l.gate_cols : nullptr};
-  const dim3 grid((unsigned)cdiv(f, kBlk), (unsigned)cdiv(m, kBlk));
+  const GateArgs ga{gh, g, u, g_scale, u_scale, m, f, act, gx != nullptr, gw_gate != nullptr,
+                    l.gate_rows, from(l.gate_rows, mode, 0, l.half), l.gate_cols, from(l.gate_cols, mode, f, 0)};
+  const dim3 grid((unsigned)cdiv(m, kBlk), (unsigned)cdiv(f, kBlk));
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, ga); };
-  if (mode == kF32) fp8 ? go(glu_gate_kernel<float, true>) : go(glu_gate_kernel<float, false>);
-  else fp8 ? go(glu_gate_kernel<__bf16, true>) : go(glu_gate_kernel<__bf16, false>);
+  if (mode == kSplit) fp8 ? go(glu_gate_kernel<kSplit, float, true>) : go(glu_gate_kernel<kSplit, float, false>);
+  else fp8 ? go(glu_gate_kernel<kBf16, __bf16, true>) : go(glu_gate_kernel<kBf16, __bf16, false>);
   if (int err = launch_check("glu_gate_kernel")) return err;
 
-  auto transpose = [&](const void* src, int64_t rows, int64_t cols, int64_t pitch, void* dst) {
-    return mode == kF32 ? run_transpose(mode, (const float*)src, nullptr, rows, cols, pitch, dst, st)
-                        : run_transpose(mode, (const __bf16*)src, nullptr, rows, cols, pitch, dst, st);
+  auto transpose = [&](const void* src, int64_t rows, int64_t cols, const Lines& d) {
+    return dtype == OMT_DT_F32 ? run_transpose(mode, (const float*)src, nullptr, rows, cols, d, st)
+                               : run_transpose(mode, (const __bf16*)src, nullptr, rows, cols, d, st);
   };
   if (gx) {  // [m][dg | du] by [k][Wg^T | Wu^T]
-    if (int err = transpose(w_gate, f, k, 2 * l.half, l.w_cols)) return err;
-    if (int err = transpose(w_up, f, k, 2 * l.half, (char*)l.w_cols + l.half * eb)) return err;
+    if (int err = transpose(w_gate, f, k, l.w_cols)) return err;
+    if (int err = transpose(w_up, f, k, from(l.w_cols, mode, 0, l.half))) return err;
     GemmArgs a{};
-    a.x = l.gate_rows, a.w = l.w_cols, a.xpitch = a.wpitch = 2 * l.half * eb;
-    a.m = (int)m, a.n = (int)k, a.row_bytes = (int)a.xpitch, a.split = (int)m;
-    a.out = gx, a.out_kind = mode == kF32 ? kOutF32 : kOutBf16;
-    if (int err = run_gemm(mode, false, l.px, a, l.parts, st)) return err;
+    a.out = gx, a.split = (int)m, a.out_kind = out_kind;
+    if (int err = run_lines(mode, l.px, a, l.gate_rows, l.w_cols, m, k, l.parts, st)) return err;
   }
   if (gw_gate) {  // [dg^T over du^T] by [k][x^T]
-    int err = fp8 ? run_transpose(mode, (const uint8_t*)x, x_scale, m, k, l.mp, l.x_cols, st)
-                  : transpose(x, m, k, l.mp, l.x_cols);
-    if (err) return err;
+    if (int err = fp8 ? run_transpose(mode, (const uint8_t*)x, x_scale, m, k, l.x_cols, st)
+                      : transpose(x, m, k, l.x_cols))
+      return err;
     GemmArgs a{};
-    a.x = l.gate_cols, a.w = l.x_cols, a.xpitch = a.wpitch = l.mp * eb;
-    a.m = (int)(2 * f), a.n = (int)k, a.row_bytes = (int)a.xpitch, a.split = (int)f;
-    a.out = gw_gate, a.out2 = gw_up, a.out_kind = mode == kF32 ? kOutF32 : kOutBf16;
-    if (err = run_gemm(mode, false, l.pw, a, l.parts, st); err) return err;
+    a.out = gw_gate, a.out2 = gw_up, a.split = (int)f, a.out_kind = out_kind;
+    if (int err = run_lines(mode, l.pw, a, l.gate_cols, l.x_cols, 2 * f, k, l.parts, st)) return err;
   }
   return OMT_OK;
 }

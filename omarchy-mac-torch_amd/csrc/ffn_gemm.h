@@ -17,6 +17,9 @@ namespace omt {
 
 // kF32: v_mfma_f32_16x16x4_f32 on the floats themselves. kBf16: v_mfma_f32_16x16x32_bf16. kFp8x: e4m3 values taken to
 // bfloat16 (exact) for the same instruction; each step is one block of 128, whose sum is multiplied by the two scales.
+// kSplit: floats as two float16 halves of a scaled group of 32 (a step: 32 high halves, 32 low ones; scales by step and
+// row), three v_mfma_f32_16x16x32_f16: high by high, high by low, low by high. The product left out is 2^-22 of the
+// whole. kFp8: the e4m3 values on v_mfma_f32_16x16x128_f8f6f4.
 enum GemmMode { kF32, kBf16, kFp8x, kFp8, kSplit };
 enum GluKeep { kKeepNone, kKeepFp8, kKeepFull };
 enum OutKind { kOutF32, kOutBf16, kOutFp8 };
@@ -419,6 +422,7 @@ int launch_gemm_of(const GemmArgs& a, bool glu, int bm, hipStream_t stream) {
 }
 int ffn_gemm_f32(const GemmArgs& a, bool glu, int bm, hipStream_t stream);
 int ffn_gemm_bf16(const GemmArgs& a, bool glu, int bm, hipStream_t stream);
+int ffn_gemm_split(const GemmArgs& a, bool glu, int bm, hipStream_t stream);
 int ffn_gemm_fp8(const GemmArgs& a, bool glu, int bm, hipStream_t stream);
 
 }  // namespace omt

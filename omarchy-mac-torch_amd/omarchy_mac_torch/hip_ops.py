@@ -797,56 +797,21 @@ def fused_sgd(params, grads, momentum_buffers=None, lr=1e-3, momentum=0.0, dampe
 
 # ---- the feed-forward sublayer of a language model: norm, 8-bit matrix products, gated block ------------------------
 #
-# No counterpart in the reference. Tensors of float32 or bfloat16 with any leading dimensions. Held in 8 bits: a
+# No counterpart in the reference. Tensors of float32 or bfloat16 with any leading dimensions, on torch.cuda or on the
+# omarchy_mac_torch device (differentiable forms for the latter: omarchy_mac_torch.ffn). Held in 8 bits: a
 # torch.float8_e4m3fn tensor with float32 scales, one for each block of 128 along the last dimension (the last block may
-# be shorter), or of 128 x 128 for weights; scale = max(largest magnitude, 1e-30) / 448.
+# be shorter), or of 128 x 128 for weights; scale = max(largest magnitude, 1e-30) / 448. A block that holds an infinity or
+# NaN stands for NaN throughout. The checks, and the launches, are torch.ops.omt's (torch_ext/ffn.cpp).
 
-FP8 = torch.float8_e4m3fn
-_DT = {torch.float32: _lib.OMT_DT_F32, torch.bfloat16: _lib.OMT_DT_BF16}
 _GLU_ACTS = {"silu": _lib.OMT_GLU_SILU, "gelu": _lib.OMT_GLU_GELU, "relu": _lib.OMT_GLU_RELU}
 _KEEPS = {None: _lib.OMT_KEEP_NONE, "fp8": _lib.OMT_KEEP_FP8, "full": _lib.OMT_KEEP_FULL}
-_BLOCK = 128
 
 
-def _blocks(n):
-    return -(-n // _BLOCK)
-
-
-def _take(t, name, dtypes, shape=None, device=None):
-    """t, contiguous and on 16 bytes (a copy where it is not), after checking its type, shape and device."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in dtypes:
-        got = f"{t.dtype} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
-        raise TypeError(f"{name}: expected {' or '.join(str(d) for d in dtypes)} on the HIP device, got {got}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name}: on {t.device}, the other operands on {device}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"{name}: expected {tuple(shape)}, got {tuple(t.shape)}")
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
-
-
-def _rows_of(t, name):
-    if t.dim() < 1 or t.shape[-1] < 1:
-        raise ValueError(f"{name}: expected rows of at least one value, got {tuple(t.shape)}")
-    return t.numel() // t.shape[-1], t.shape[-1]
-
-
-def _take_fp8(q, s, name, device=None):
-    q = _take(q, name, (FP8,), device=device)
-    rows, cols = _rows_of(q, name)
-    return q, _take(s, f"{name}'s scales", (torch.float32,), (*q.shape[:-1], _blocks(cols)), q.device), rows, cols
-
-
-def _take_fp8_weight(q, s, name, cols, device):
-    q = _take(q, name, (FP8,), device=device)
-    if q.dim() != 2 or q.shape[0] < 1 or q.shape[1] != cols:
-        raise ValueError(f"{name}: expected [rows, {cols}], got {tuple(q.shape)}")
-    return q, _take(s, f"{name}'s scales", (torch.float32,), (_blocks(q.shape[0]), _blocks(cols)), device)
-
-
-def _new_fp8(shape, device):
-    return (torch.empty(shape, device=device, dtype=FP8),
-            torch.empty((*shape[:-1], _blocks(shape[-1])), device=device, dtype=torch.float32))
+def _ffn(name, *args):
+    try:
+        return getattr(torch.ops.omt, name).default(*args)
+    except NotImplementedError as e:
+        raise _lib.Unsupported(_lib.OMT_UNSUPPORTED, str(e)) from None
 
 
 def _glu_act(act):
@@ -855,95 +820,41 @@ def _glu_act(act):
     return _GLU_ACTS[act]
 
 
-def _norm_operands(x, weight, residual):
-    x = _take(x, "x", tuple(_DT))
-    rows, dim = _rows_of(x, "x")
-    weight = _take(weight, "weight", (x.dtype, torch.float32), (dim,), x.device)
-    if residual is not None:
-        residual = _take(residual, "residual", (x.dtype,), x.shape, x.device)
-    return x, weight, residual, rows, dim
-
-
 def rms_norm(x, weight, residual=None, eps=1e-6):
-    """h = x + residual, rounded to x's type; y = h / sqrt(mean(h^2) + eps) * weight over the last dimension. Returns
-    (y, h, rstd), rstd the float32 1 / sqrt(...) of each row; without a residual h is x. The weight is of x's type or
-    float32."""
-    x, weight, residual, rows, dim = _norm_operands(x, weight, residual)
-    y = torch.empty_like(x)
-    h = torch.empty_like(x) if residual is not None else x
-    rstd = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
-    check(L.omt_rms_norm_fwd(_DT[x.dtype], _DT[weight.dtype], rows, dim, _ptr(x), _ptr(residual), _ptr(weight), eps,
-                             _ptr(y), _ptr(h), _ptr(rstd), None, None, _stream(x.device)), "rms_norm")
-    return y, h, rstd
+    """h = x + residual, rounded to x's type; y = h / sqrt(mean(h^2) + eps) * weight over the last dimension (at most
+    32768). Returns (y, h, rstd), rstd the float32 1 / sqrt(...) of each row; without a residual h is x. The weight is of
+    x's type or float32."""
+    y, h, rstd = _ffn("rms_norm", x, weight, residual, eps)
+    return y, (x if residual is None else h), rstd
 
 
 def rms_norm_fp8(x, weight, residual=None, eps=1e-6):
     """rms_norm with y in 8 bits: returns (q, scale, h)."""
-    x, weight, residual, rows, dim = _norm_operands(x, weight, residual)
-    q, scale = _new_fp8(x.shape, x.device)
-    h = torch.empty_like(x) if residual is not None else x
-    check(L.omt_rms_norm_fwd(_DT[x.dtype], _DT[weight.dtype], rows, dim, _ptr(x), _ptr(residual), _ptr(weight), eps,
-                             None, _ptr(h), None, _ptr(q), _ptr(scale), _stream(x.device)), "rms_norm_fp8")
-    return q, scale, h
+    q, scale, h = _ffn("rms_norm_fp8", x, weight, residual, eps)
+    return q, scale, (x if residual is None else h)
 
 
 def rms_norm_backward(gy, h, weight, rstd, gh=None, weight_grad=True):
     """From gy, the gradient of rms_norm's y, and gh, the one that reaches h past the norm (none: zero): returns (the
     gradient of x, which is the residual's too; the weight's, or None)."""
-    h, weight, gh, rows, dim = _norm_operands(h, weight, gh)
-    gy = _take(gy, "gy", (h.dtype,), h.shape, h.device)
-    rstd = _take(rstd, "rstd", (torch.float32,), h.shape[:-1], h.device)
-    gx = torch.empty_like(h)
-    gw = torch.empty_like(weight) if weight_grad else None
-    ws, nb = _workspace(L.omt_rms_norm_bwd_workspace(rows, dim) if weight_grad else 0, h.device)
-    check(L.omt_rms_norm_bwd(_DT[h.dtype], _DT[weight.dtype], rows, dim, _ptr(gy), _ptr(gh), _ptr(h), _ptr(weight),
-                             _ptr(rstd), _ptr(gx), _ptr(gw), _ptr(ws), nb, _stream(h.device)), "rms_norm_backward")
-    return gx, gw
+    return _ffn("rms_norm_backward", gy, h, weight, rstd, gh, weight_grad)
 
 
 def quantize_fp8(x, pow2=False):
     """x in 8 bits: (q, scale). pow2: each scale is the next power of two from its block's largest magnitude / 448 on,
     so that q * scale is exact in bfloat16."""
-    x = _take(x, "x", tuple(_DT))
-    rows, cols = _rows_of(x, "x")
-    q, scale = _new_fp8(x.shape, x.device)
-    check(L.omt_quantize_fp8(_DT[x.dtype], rows, cols, _ptr(x), int(pow2), _ptr(q), _ptr(scale), _stream(x.device)),
-          "quantize_fp8")
-    return q, scale
+    return _ffn("quantize_fp8", x, pow2)
 
 
 def quantize_fp8_weight(w):
     """A weight [rows, cols] in 8 bits with a scale for each block of 128 x 128: (q, scale)."""
-    w = _take(w, "w", tuple(_DT))
-    if w.dim() != 2 or min(w.shape) < 1:
-        raise ValueError(f"w: expected a matrix, got {tuple(w.shape)}")
-    q = torch.empty_like(w, dtype=FP8)
-    scale = torch.empty((_blocks(w.shape[0]), _blocks(w.shape[1])), device=w.device, dtype=torch.float32)
-    check(L.omt_quantize_fp8_weight(_DT[w.dtype], *w.shape, _ptr(w), _ptr(q), _ptr(scale), _stream(w.device)),
-          "quantize_fp8_weight")
-    return q, scale
+    return _ffn("quantize_fp8_weight", w)
 
 
 def matmul_fp8(a, a_scale, b, b_scale, dtype=torch.bfloat16):
     """a b^T of operands held in 8 bits: a [..., k] with scales by blocks of 128 along k, b [n, k] with scales by
     128 x 128. Returns [..., n] of dtype (bfloat16 or float32)."""
-    if dtype not in _DT:
-        raise TypeError(f"dtype: expected bfloat16 or float32, got {dtype}")
-    a, a_scale, m, k = _take_fp8(a, a_scale, "a")
-    b, b_scale = _take_fp8_weight(b, b_scale, "b", k, a.device)
-    n = b.shape[0]
-    c = torch.empty((*a.shape[:-1], n), device=a.device, dtype=dtype)
-    ws, nb = _workspace(L.omt_matmul_fp8_workspace(m, n, k), a.device)
-    check(L.omt_matmul_fp8(m, n, k, _ptr(a), _ptr(a_scale), _ptr(b), _ptr(b_scale), _DT[dtype], _ptr(c), _ptr(ws), nb,
-                           _stream(a.device)), "matmul_fp8")
-    return c
-
-
-def _glu_weights(w_gate, w_up, dtype, k, device):
-    w_gate = _take(w_gate, "w_gate", (dtype,), device=device)
-    if w_gate.dim() != 2 or w_gate.shape[0] < 1 or w_gate.shape[1] != k:
-        raise ValueError(f"w_gate: expected [rows, {k}], got {tuple(w_gate.shape)}")
-    return w_gate, _take(w_up, "w_up", (dtype,), w_gate.shape, device)
+    return _ffn("matmul_fp8", a, a_scale, b, b_scale, dtype)
 
 
 def glu(x, w_gate, w_up, act="silu", checkpoint=None):
@@ -953,66 +864,20 @@ def glu(x, w_gate, w_up, act="silu", checkpoint=None):
     (x, None, g, None, u, None) in x's type."""
     if checkpoint not in _KEEPS:
         raise ValueError(f"checkpoint: expected None, 'fp8' or 'full', got {checkpoint!r}")
-    act = _glu_act(act)
-    x = _take(x, "x", tuple(_DT))
-    m, k = _rows_of(x, "x")
-    w_gate, w_up = _glu_weights(w_gate, w_up, x.dtype, k, x.device)
-    f, dt = w_gate.shape[0], _DT[x.dtype]
-    shape = (*x.shape[:-1], f)
-    h = torch.empty(shape, device=x.device, dtype=x.dtype)
-    kept = (None,) * 6
-    if checkpoint == "fp8":
-        kept = _new_fp8(x.shape, x.device) + _new_fp8(shape, x.device) + _new_fp8(shape, x.device)
-    elif checkpoint == "full":
-        kept = (x, None, torch.empty_like(h), None, torch.empty_like(h), None)
-    ws, nb = _workspace(L.omt_glu_fwd_workspace(dt, m, k, f), x.device)
-    check(L.omt_glu_fwd(dt, m, k, f, act, _KEEPS[checkpoint], _ptr(x), _ptr(w_gate), _ptr(w_up), _ptr(h),
-                        *[_ptr(t) for t in kept], _ptr(ws), nb, _stream(x.device)), "glu")
-    return h, kept if checkpoint else None
+    h, *kept = _ffn("glu", x, w_gate, w_up, _glu_act(act), _KEEPS[checkpoint])
+    if checkpoint == "full":
+        kept[0] = x
+    return h, tuple(kept) if checkpoint else None
 
 
 def glu_backward(gh, kept, w_gate, w_up, act="silu", input_grad=True, weight_grad=True):
     """The gradients of glu's x, w_gate and w_up from gh, the gradient of h, and what glu kept. A gradient that is not
     asked for is None."""
-    act = _glu_act(act)
     if len(kept) != 6:
         raise ValueError(f"kept: expected glu's six values, got {len(kept)}")
-    x, xs, g, gs, u, us = kept
-    gh = _take(gh, "gh", tuple(_DT))
-    m, f = _rows_of(gh, "gh")
-    if xs is not None:
-        (x, xs, mx, k), (g, gs, _, _), (u, us, _, _) = (
-            _take_fp8(x, xs, "x", gh.device), _take_fp8(g, gs, "g", gh.device), _take_fp8(u, us, "u", gh.device))
-    else:
-        x, g, u = (_take(t, name, (gh.dtype,), device=gh.device) for t, name in ((x, "x"), (g, "g"), (u, "u")))
-        mx, k = _rows_of(x, "x")
-    if g.shape != gh.shape or u.shape != gh.shape or x.shape[:-1] != gh.shape[:-1]:
-        raise ValueError(f"glu_backward: gh {tuple(gh.shape)}, x {tuple(x.shape)}, g {tuple(g.shape)}, "
-                         f"u {tuple(u.shape)} do not belong together")
-    w_gate, w_up = _glu_weights(w_gate, w_up, gh.dtype, k, gh.device)
-    if w_gate.shape[0] != f:
-        raise ValueError(f"w_gate: expected [{f}, {k}], got {tuple(w_gate.shape)}")
-    gx = torch.empty(x.shape, device=gh.device, dtype=gh.dtype) if input_grad else None
-    gwg, gwu = (torch.empty_like(w_gate), torch.empty_like(w_up)) if weight_grad else (None, None)
-    dt = _DT[gh.dtype]
-    ws, nb = _workspace(L.omt_glu_bwd_workspace(dt, m, k, f), gh.device)
-    check(L.omt_glu_bwd(dt, m, k, f, act, _lib.OMT_KEEP_FP8 if xs is not None else _lib.OMT_KEEP_FULL, _ptr(gh),
-                        _ptr(x), _ptr(xs), _ptr(g), _ptr(gs), _ptr(u), _ptr(us), _ptr(w_gate), _ptr(w_up), _ptr(gx),
-                        _ptr(gwg), _ptr(gwu), _ptr(ws), nb, _stream(gh.device)), "glu_backward")
-    return gx, gwg, gwu
+    return _ffn("glu_backward", gh, *kept, w_gate, w_up, _glu_act(act), input_grad, weight_grad)
 
 
 def glu_fp8(x, x_scale, w_gate, gate_scale, w_up, up_scale, act="silu"):
     """glu of operands held in 8 bits, for serving: returns h in 8 bits, (q, scale)."""
-    act = _glu_act(act)
-    x, x_scale, m, k = _take_fp8(x, x_scale, "x")
-    w_gate, gate_scale = _take_fp8_weight(w_gate, gate_scale, "w_gate", k, x.device)
-    w_up, up_scale = _take_fp8_weight(w_up, up_scale, "w_up", k, x.device)
-    f = w_gate.shape[0]
-    if w_up.shape[0] != f:
-        raise ValueError(f"w_up: expected {tuple(w_gate.shape)}, got {tuple(w_up.shape)}")
-    q, scale = _new_fp8((*x.shape[:-1], f), x.device)
-    ws, nb = _workspace(L.omt_glu_fp8_workspace(m, k, f), x.device)
-    check(L.omt_glu_fp8(m, k, f, act, _ptr(x), _ptr(x_scale), _ptr(w_gate), _ptr(gate_scale), _ptr(w_up),
-                        _ptr(up_scale), _ptr(q), _ptr(scale), _ptr(ws), nb, _stream(x.device)), "glu_fp8")
-    return q, scale
+    return _ffn("glu_fp8", x, x_scale, w_gate, gate_scale, w_up, up_scale, _glu_act(act))
