@@ -641,7 +641,7 @@ int omt_quantize_fp8_weight(int dtype, int64_t rows, int64_t cols, const void* w
 
 /* c[m][n] = sum over k of a[m][k] b[n][k], both in 8 bits with scales (a by 1 x 128, b by 128 x 128); c in out_dtype.
  * a, b and the workspace on 16 bytes. */
-size_t omt_matmul_fp8_workspace(int64_t m, int64_t n, int64_t k);
+size_t omt_matmul_fp8_workspace(int64_t m, int64_t n, int64_t k, int out_dtype);
 int omt_matmul_fp8(int64_t m, int64_t n, int64_t k, const void* a, const float* a_scale, const void* b,
                    const float* b_scale, int out_dtype, void* c, void* workspace, size_t workspace_bytes, void* stream);
 

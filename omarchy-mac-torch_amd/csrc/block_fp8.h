@@ -46,6 +46,27 @@ __device__ __forceinline__ f32x8 load8(const __bf16* p, int64_t c, int64_t cols)
   }
   return v;
 }
+// e4m3, without its scale
+__device__ __forceinline__ f32x8 widen_fp8x8(uint2 w) {
+  f32x8 v;
+  v[0] = __builtin_amdgcn_cvt_f32_fp8((int)w.x, 0), v[1] = __builtin_amdgcn_cvt_f32_fp8((int)w.x, 1);
+  v[2] = __builtin_amdgcn_cvt_f32_fp8((int)w.x, 2), v[3] = __builtin_amdgcn_cvt_f32_fp8((int)w.x, 3);
+  v[4] = __builtin_amdgcn_cvt_f32_fp8((int)w.y, 0), v[5] = __builtin_amdgcn_cvt_f32_fp8((int)w.y, 1);
+  v[6] = __builtin_amdgcn_cvt_f32_fp8((int)w.y, 2), v[7] = __builtin_amdgcn_cvt_f32_fp8((int)w.y, 3);
+  return v;
+}
+template <bool VEC>
+__device__ __forceinline__ f32x8 load8(const uint8_t* p, int64_t c, int64_t cols) {
+  uint2 w = make_uint2(0, 0);
+  if constexpr (VEC) {
+    if (c < cols) w = *(const uint2*)(p + c);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < cols) (e < 4 ? w.x : w.y) |= (uint32_t)p[c + e] << (8 * (e & 3));
+  }
+  return widen_fp8x8(w);
+}
 template <bool VEC>
 __device__ __forceinline__ void store8(float* p, int64_t c, int64_t cols, f32x8 v) {
   if constexpr (VEC) {
@@ -127,6 +148,5 @@ __device__ __forceinline__ void store_fp8x8(uint8_t* p, int64_t c, int64_t cols,
       if (c + e < cols) p[c + e] = (uint8_t)((e < 4 ? w.x : w.y) >> (8 * (e & 3)));
   }
 }
-__device__ __forceinline__ float fp8_value(uint8_t q) { return __builtin_amdgcn_cvt_f32_fp8((int)q, 0); }
 
 }  // namespace omt

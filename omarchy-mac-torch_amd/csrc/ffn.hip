@@ -41,92 +41,85 @@ struct Lines {
 };
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 
-// 16 elements (at: a multiple of 16) of a line; kSplit: threads 2i and 2i + 1 call it together for the two halves of 32
+// 8 elements (at: a multiple of 8) of a line; kSplit: the four threads of a quad call it together for a group of 32
 template <int FMT>
-__device__ __forceinline__ void write16(const Lines& d, int64_t line, int64_t at, f32x8 lo, f32x8 hi) {
+__device__ __forceinline__ void write8(const Lines& d, int64_t line, int64_t at, f32x8 v) {
   if constexpr (FMT == kBf16) {
-    __bf16* p = (__bf16*)(d.p + line * d.pitch) + at;
-    store8<true>(p, 0, 16, lo);
-    store8<true>(p, 8, 16, hi);
+    store8<true>((__bf16*)(d.p + line * d.pitch), at, d.pitch / 2, v);
   } else {
-    uint32_t b = max_u32(abs_bits8(lo), abs_bits8(hi));
+    uint32_t b = abs_bits8(v);
     b = max_u32(b, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)b, 0xB1, 0xF, 0xF, false));  // quad_perm [1,0,3,2]
-    float up, scale;
+    b = max_u32(b, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)b, 0x4E, 0xF, 0xF, false));  // quad_perm [2,3,0,1]
+    float scale;
     if (b < 0x7f800000u) {
       const uint32_t e = max_u32(b >> 23, 15u);
-      up = __builtin_bit_cast(float, (268u - e) << 23);
+      v *= __builtin_bit_cast(float, (268u - e) << 23);
       scale = __builtin_bit_cast(float, (e - 14u) << 23);
     } else {
-      up = 1.f;
       scale = __builtin_bit_cast(float, b);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        lo[e] = abs_bits(lo[e]) == 0x7f800000u ? copysignf(1.f, lo[e]) : 0.f;
-        hi[e] = abs_bits(hi[e]) == 0x7f800000u ? copysignf(1.f, hi[e]) : 0.f;
-      }
+      for (int e = 0; e < 8; ++e) v[e] = abs_bits(v[e]) == 0x7f800000u ? copysignf(1.f, v[e]) : 0.f;
     }
     char* p = d.p + line * d.pitch + (at >> 5) * 128 + (at & 31) * 2;
-    auto halves = [&](f32x8 v, char* to) {
-      v *= up;
-      const half8 h = __builtin_convertvector(v, half8);
-      *(half8*)to = h;
-      *(half8*)(to + 64) = __builtin_convertvector(v - __builtin_convertvector(h, f32x8), half8);
-    };
-    halves(lo, p);
-    halves(hi, p + 16);
+    const half8 h = __builtin_convertvector(v, half8);
+    *(half8*)p = h;
+    *(half8*)(p + 64) = __builtin_convertvector(v - __builtin_convertvector(h, f32x8), half8);
     if ((at & 31) == 0) d.scale[(at >> 5) * d.scale_lines + line] = scale;
   }
 }
 
-// A 64 x 64 block held in LDS (rows of 65 floats): its rows, or its columns, as lines line0.. (below `lines`) of d, elements
-// at.. of each
+// Blocks of 64 x 64 elements: thread t has eight consecutive ones of rows t / 8 and t / 8 + 32. Columns go through LDS, rows
+// of 65 floats: eight lanes of a row and eight rows write 64 banks, and lines read as columns do too.
 constexpr int kBlk = 64, kBlkPitch = 65;
-template <int FMT>
-__device__ __forceinline__ void write_block(const float* blk, bool columns, const Lines& d, int64_t line0, int64_t lines,
-                                            int64_t at) {
-  const int line = threadIdx.x >> 2, part = (threadIdx.x & 3) * 16;
-  if (line0 + line >= lines) return;  // all four threads of a line
-  f32x8 lo, hi;
+__device__ __forceinline__ void to_lds(float* blk, int row, int at, f32x8 v) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    lo[e] = columns ? blk[(part + e) * kBlkPitch + line] : blk[line * kBlkPitch + part + e];
-    hi[e] = columns ? blk[(part + 8 + e) * kBlkPitch + line] : blk[line * kBlkPitch + part + 8 + e];
+  for (int e = 0; e < 8; ++e) blk[row * kBlkPitch + at + e] = v[e];
+}
+// the block's columns as lines line0.. (below `lines`) of d, elements at.. of each
+template <int FMT>
+__device__ __forceinline__ void write_columns(const float* blk, const Lines& d, int64_t line0, int64_t lines, int64_t at) {
+  const int part = (threadIdx.x & 7) * 8;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int line = (threadIdx.x >> 3) + 32 * i;
+    if (line0 + line >= lines) break;  // all eight threads of a line
+    f32x8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = blk[(part + e) * kBlkPitch + line];
+    write8<FMT>(d, line0 + line, at + part, v);
   }
-  write16<FMT>(d, line0 + line, at + part, lo, hi);
 }
 
 // rows of floats as kSplit lines, zeros past their end up to a multiple of 64
 template <bool VEC>
 __global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ src, int64_t rows, int64_t cols,
                                                          Lines d) {
-  const int64_t line = (int64_t)blockIdx.x * kBlk + (threadIdx.x >> 2);
-  const int64_t at = (int64_t)blockIdx.y * kBlk + (threadIdx.x & 3) * 16;
-  if (line >= rows) return;
-  const float* p = src + line * cols;
-  write16<kSplit>(d, line, at, load8<VEC>(p, at, cols), load8<VEC>(p, at + 8, cols));
+  const int64_t line = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
+  const int64_t at = (int64_t)blockIdx.y * kBlk + (threadIdx.x & 7) * 8;
+  if (line < rows) write8<kSplit>(d, line, at, load8<VEC>(src + line * cols, at, cols));
 }
 
 // The columns of src [rows][cols] as lines of d, zeros from `rows` on up to a multiple of 64; S float, __bf16, or e4m3 with
 // its scales.
-template <int FMT, class S>
+template <int FMT, bool VEC, class S>
 __global__ void __launch_bounds__(256) transpose_kernel(const S* __restrict__ src, const float* __restrict__ scale,
                                                         int64_t rows, int64_t cols, Lines d) {
   __shared__ float blk[kBlk * kBlkPitch];
   const int64_t r0 = (int64_t)blockIdx.x * kBlk, c0 = (int64_t)blockIdx.y * kBlk;
-  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int part = (threadIdx.x & 7) * 8;
   const int64_t blocks = (cols + kFp8Block - 1) / kFp8Block;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int r = w * 16 + i;
-    float v = 0.f;
-    if (r0 + r < rows && c0 + l < cols) {
-      if constexpr (sizeof(S) == 1) v = fp8_value(src[(r0 + r) * cols + c0 + l]) * scale[(r0 + r) * blocks + c0 / kFp8Block];
-      else v = (float)src[(r0 + r) * cols + c0 + l];
+  for (int i = 0; i < 2; ++i) {
+    const int r = (threadIdx.x >> 3) + 32 * i;
+    f32x8 v = {};
+    if (r0 + r < rows) {
+      v = load8<VEC>(src + (r0 + r) * cols, c0 + part, cols);
+      if constexpr (sizeof(S) == 1) v *= scale[(r0 + r) * blocks + c0 / kFp8Block];
     }
-    blk[r * kBlkPitch + l] = v;
+    to_lds(blk, r, part, v);
   }
   __syncthreads();
-  write_block<FMT>(blk, true, d, c0, cols, r0);
+  write_columns<FMT>(blk, d, c0, cols, r0);
 }
 
 struct GateArgs {
@@ -138,43 +131,53 @@ struct GateArgs {
   Lines g_cols, u_cols;  // f lines each: one below the other
 };
 // dg and du of a 64 x 64 block of (row, column of f), laid out by rows and by columns
-template <int FMT, class T, bool FP8>
+template <int FMT, bool VEC, class T, bool FP8>
 __global__ void __launch_bounds__(256) glu_gate_kernel(GateArgs a) {
   __shared__ float dg[kBlk * kBlkPitch], du[kBlk * kBlkPitch];
+  using Held = std::conditional_t<FP8, uint8_t, T>;
   const int64_t r0 = (int64_t)blockIdx.x * kBlk, c0 = (int64_t)blockIdx.y * kBlk;
-  const int l = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int part = (threadIdx.x & 7) * 8;
   const int64_t blocks = (a.f + kFp8Block - 1) / kFp8Block;
-#pragma unroll 4
-  for (int i = 0; i < 16; ++i) {
-    const int r = w * 16 + i;
-    float vg = 0.f, vu = 0.f;
-    if (r0 + r < a.m && c0 + l < a.f) {
-      const int64_t at = (r0 + r) * a.f + c0 + l;
-      const float gh = (float)((const T*)a.gh)[at];
-      float g, u;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = (threadIdx.x >> 3) + 32 * i;
+    f32x8 vg = {}, vu = {};
+    if (r0 + r < a.m) {
+      const int64_t row = (r0 + r) * a.f;
+      const f32x8 gh = load8<VEC>((const T*)a.gh + row, c0 + part, a.f);
+      f32x8 g = load8<VEC>((const Held*)a.g + row, c0 + part, a.f);
+      f32x8 u = load8<VEC>((const Held*)a.u + row, c0 + part, a.f);
       if constexpr (FP8) {
         const int64_t b = (r0 + r) * blocks + c0 / kFp8Block;
-        g = fp8_value(((const uint8_t*)a.g)[at]) * a.gs[b];
-        u = fp8_value(((const uint8_t*)a.u)[at]) * a.us[b];
-      } else {
-        g = (float)((const T*)a.g)[at];
-        u = (float)((const T*)a.u)[at];
+        g *= a.gs[b];
+        u *= a.us[b];
       }
-      vg = gh * u * glu_act_grad(g, a.act);
-      vu = gh * glu_act(g, a.act);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const ActAndGrad ag = glu_act_grad(g[e], a.act);
+        vg[e] = gh[e] * u[e] * ag.grad;
+        vu[e] = gh[e] * ag.act;
+      }
+      if (!VEC) {  // past the row's end: zeros, whatever the block's scale
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (c0 + part + e >= a.f) vg[e] = vu[e] = 0.f;
+      }
+      if (VEC && c0 + part >= a.f) vg = vu = f32x8{};
+      if (a.by_rows) {
+        write8<FMT>(a.g_rows, r0 + r, c0 + part, vg);
+        write8<FMT>(a.u_rows, r0 + r, c0 + part, vu);
+      }
     }
-    dg[r * kBlkPitch + l] = vg;
-    du[r * kBlkPitch + l] = vu;
+    if (a.by_cols) {
+      to_lds(dg, r, part, vg);
+      to_lds(du, r, part, vu);
+    }
   }
+  if (!a.by_cols) return;
   __syncthreads();
-  if (a.by_rows) {
-    write_block<FMT>(dg, false, a.g_rows, r0, a.m, c0);
-    write_block<FMT>(du, false, a.u_rows, r0, a.m, c0);
-  }
-  if (a.by_cols) {
-    write_block<FMT>(dg, true, a.g_cols, c0, a.f, r0);
-    write_block<FMT>(du, true, a.u_cols, c0, a.f, r0);
-  }
+  write_columns<FMT>(dg, a.g_cols, c0, a.f, r0);
+  write_columns<FMT>(du, a.u_cols, c0, a.f, r0);
 }
 
 // ---- the sums of slices ---------------------------------------------------------------------------------------------------
@@ -240,11 +243,11 @@ __global__ void __launch_bounds__(256) glu_join_kernel(GemmArgs a) {
 // less than the operands' bytes at 5.5 TB/s; slices add the second launch and their sums' way to memory and back at
 // 4 TB/s. Measured steps (4096 x 4096 x 4096, all CUs busy), us; [mode][16, 64, 128, 256 rows]:
 constexpr float kStepUs[][4] = {
-    {1.3f, 4.0f, 3.83f, 7.46f},   // kF32
-    {0.45f, 1.12f, 0.96f, 1.75f}, // kBf16
-    {0.8f, 2.9f, 2.1f, 3.8f},     // kFp8x
-    {0.45f, 2.2f, 1.3f, 2.7f},    // kFp8
-    {0.8f, 2.3f, 1.52f, 2.86f},   // kSplit
+    {1.65f, 4.0f, 3.83f, 7.46f},  // kF32
+    {1.2f, 1.12f, 0.96f, 1.75f},  // kBf16
+    {2.1f, 2.9f, 2.1f, 3.8f},     // kFp8x
+    {1.6f, 2.2f, 1.3f, 2.7f},     // kFp8
+    {1.1f, 2.3f, 1.52f, 2.86f},   // kSplit
 };
 constexpr int kBm[4] = {16, 64, 128, 256}, kResident[4] = {2, 2, 1, 1};
 struct GemmPlan {
@@ -264,8 +267,9 @@ static GemmPlan plan_gemm(int mode, bool glu, int64_t m, int64_t n, int64_t row_
       const int64_t per = cdiv(steps, s), slices = cdiv(steps, per);
       if (slices != s) continue;
       const float rounds = (float)cdiv(gx * gy * s, 256 * kResident[v]);
-      // a CU's second workgroup slows the first: one alone takes about half the step that two take
-      const float step = kStepUs[mode][v] * (kResident[v] == 2 && gx * gy * s <= 256 ? 0.6f : 1.f);
+      // a workgroup alone on its CU takes about half the step that two take, but no less than a load's way, 0.9
+      const bool alone = kResident[v] == 2 && gx * gy * s <= 256;
+      const float step = alone ? std::max(0.9f, 0.6f * kStepUs[mode][v]) : kStepUs[mode][v];
       float us = std::max(rounds * (per * step + 1.5f), bytes_us);
       if (s > 1) us += 4.f + 2.f * s * sums * 4 / 4e6f;
       if (us < best.us) best = {kBm[v], (int)gx, (int)gy, (int)steps, (int)s, (int)per, us, 0};
@@ -278,9 +282,10 @@ static GemmPlan plan_gemm(int mode, bool glu, int64_t m, int64_t n, int64_t row_
 static int run_gemm(int mode, bool glu, const GemmPlan& p, GemmArgs a, void* parts, hipStream_t stream) {
   a.steps = p.steps, a.slices = p.slices, a.slice_steps = p.slice_steps, a.gx = p.gx, a.gy = p.gy;
   a.parts = (float*)parts;
-  int e = mode == kF32 ? ffn_gemm_f32(a, glu, p.bm, stream)
+  int e = mode == kF32 ? ffn_gemm_f32(a, p.bm, stream)
           : mode == kSplit ? ffn_gemm_split(a, glu, p.bm, stream)
-          : mode == kBf16 ? ffn_gemm_bf16(a, glu, p.bm, stream) : ffn_gemm_fp8(a, glu, p.bm, stream);
+          : mode == kBf16 ? ffn_gemm_bf16(a, glu, p.bm, stream)
+          : mode == kFp8 ? ffn_gemm_fp8(a, p.bm, stream) : ffn_gemm_fp8x(a, glu, p.bm, stream);
   if (e || p.slices == 1) return e;
   const bool vec = a.n % 8 == 0;
   if (glu) {
@@ -336,7 +341,7 @@ static Lines place_rows(Space& sp, int mode, int64_t rows, int64_t cols) {
 }
 static int lay_rows(const Lines& d, int mode, const void* src, int64_t rows, int64_t cols, hipStream_t stream) {
   if (mode == kSplit) {
-    const dim3 grid((unsigned)cdiv(rows, kBlk), (unsigned)cdiv(cols, kBlk));
+    const dim3 grid((unsigned)cdiv(rows, 32), (unsigned)cdiv(cols, kBlk));
     if (cols % 8 == 0) hipLaunchKernelGGL(split_rows_kernel<true>, grid, dim3(256), 0, stream, (const float*)src, rows, cols, d);
     else hipLaunchKernelGGL(split_rows_kernel<false>, grid, dim3(256), 0, stream, (const float*)src, rows, cols, d);
     return launch_check("split_rows_kernel");
@@ -388,12 +393,15 @@ static int need_space(const char* fn, size_t need, const void* ws, size_t bytes)
   return OMT_OK;
 }
 
+// The 8-bit matrix cores round inside the sum of a block (1.3e-5 of a block's sum over Gaussian values, where bfloat16's on
+// the same values are 1e-8 off): nothing beside a bfloat16 result's 2^-9, too much for a float32 one.
+static int fp8_mode(int out_dtype) { return out_dtype == OMT_DT_BF16 ? kFp8 : kFp8x; }
 struct MatmulFp8 {
   GemmPlan p;
   Lines a, b;
   void* parts;
-  MatmulFp8(Space& sp, int64_t m, int64_t n, int64_t k)
-      : p(plan_gemm(kFp8x, false, m, n, k)), a(place_rows(sp, kFp8x, m, k)), b(place_rows(sp, kFp8x, n, k)),
+  MatmulFp8(Space& sp, int mode, int64_t m, int64_t n, int64_t k)
+      : p(plan_gemm(mode, false, m, n, k)), a(place_rows(sp, kFp8x, m, k)), b(place_rows(sp, kFp8x, n, k)),
         parts(sp.take(p.parts_bytes)) {}
 };
 // float32: on fp32 MFMA as it is, or as halves on float16 MFMA, three products for one. Laying out the halves reads and
@@ -440,10 +448,10 @@ template <class S>
 static int run_transpose(int mode, const S* src, const float* scale, int64_t rows, int64_t cols, const Lines& d,
                          hipStream_t stream) {
   const dim3 grid((unsigned)cdiv(rows, kBlk), (unsigned)cdiv(cols, kBlk));
-  if (mode == kSplit)
-    hipLaunchKernelGGL((transpose_kernel<kSplit, S>), grid, dim3(256), 0, stream, src, scale, rows, cols, d);
-  else
-    hipLaunchKernelGGL((transpose_kernel<kBf16, S>), grid, dim3(256), 0, stream, src, scale, rows, cols, d);
+  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, src, scale, rows, cols, d); };
+  const bool vec = cols % 8 == 0 && on16({src});
+  if (mode == kSplit) vec ? go(transpose_kernel<kSplit, true, S>) : go(transpose_kernel<kSplit, false, S>);
+  else vec ? go(transpose_kernel<kBf16, true, S>) : go(transpose_kernel<kBf16, false, S>);
   return launch_check("transpose_kernel");
 }
 // the product of operands laid out as lines: x's lines by w's
@@ -460,10 +468,10 @@ static int run_lines(int mode, const GemmPlan& p, GemmArgs a, const Lines& x, co
 
 using namespace omt;
 
-OMT_EXPORT size_t omt_matmul_fp8_workspace(int64_t m, int64_t n, int64_t k) {
+OMT_EXPORT size_t omt_matmul_fp8_workspace(int64_t m, int64_t n, int64_t k, int out_dtype) {
   if (product_check("omt_matmul_fp8_workspace", m, n, k) || m == 0) return 0;
   Space sp{nullptr};
-  MatmulFp8(sp, m, n, k);
+  MatmulFp8(sp, fp8_mode(out_dtype), m, n, k);
   return sp.used;
 }
 
@@ -476,16 +484,17 @@ OMT_EXPORT int omt_matmul_fp8(int64_t m, int64_t n, int64_t k, const void* a, co
   if (m == 0) return OMT_OK;
   if (!a || !a_scale || !b || !b_scale || !c) return fail(OMT_INVALID, "%s: null pointer", fn);
   if (!on16({a, b, c})) return fail(OMT_INVALID, "%s: an operand is not on 16 bytes", fn);
-  if (int e = need_space(fn, omt_matmul_fp8_workspace(m, n, k), workspace, workspace_bytes)) return e;
+  if (int e = need_space(fn, omt_matmul_fp8_workspace(m, n, k, out_dtype), workspace, workspace_bytes)) return e;
   Space sp{(char*)workspace};
-  const MatmulFp8 l(sp, m, n, k);
+  const int mode = fp8_mode(out_dtype);
+  const MatmulFp8 l(sp, mode, m, n, k);
   hipStream_t st = stream_of(stream);
   GemmArgs g{};
-  if (int e = lay_operands(g, kFp8x, l.a, l.b, {}, a, b, nullptr, m, n, k, st)) return e;
+  if (int e = lay_operands(g, mode, l.a, l.b, {}, a, b, nullptr, m, n, k, st)) return e;
   g.sx = a_scale, g.sw = b_scale;
   g.sx_row = g.sw_row = (int)cdiv(k, kFp8Block), g.sx_step = g.sw_step = 1;
   g.out = c, g.out_kind = out_dtype == OMT_DT_BF16 ? kOutBf16 : kOutF32;
-  return run_gemm(kFp8x, false, l.p, g, l.parts, st);
+  return run_gemm(mode, false, l.p, g, l.parts, st);
 }
 
 OMT_EXPORT size_t omt_glu_fwd_workspace(int dtype, int64_t m, int64_t k, int64_t f) {
@@ -588,8 +597,12 @@ OMT_EXPORT int omt_glu_bwd(int dtype, int64_t m, int64_t k, int64_t f, int act, 
                     l.gate_rows, from(l.gate_rows, mode, 0, l.half), l.gate_cols, from(l.gate_cols, mode, f, 0)};
   const dim3 grid((unsigned)cdiv(m, kBlk), (unsigned)cdiv(f, kBlk));
   auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, st, ga); };
-  if (mode == kSplit) fp8 ? go(glu_gate_kernel<kSplit, float, true>) : go(glu_gate_kernel<kSplit, float, false>);
-  else fp8 ? go(glu_gate_kernel<kBf16, __bf16, true>) : go(glu_gate_kernel<kBf16, __bf16, false>);
+  auto pick = [&](auto vec) {
+    constexpr bool V = decltype(vec)::value;
+    if (mode == kSplit) fp8 ? go(glu_gate_kernel<kSplit, V, float, true>) : go(glu_gate_kernel<kSplit, V, float, false>);
+    else fp8 ? go(glu_gate_kernel<kBf16, V, __bf16, true>) : go(glu_gate_kernel<kBf16, V, __bf16, false>);
+  };
+  f % 8 == 0 && on16({gh, g, u}) ? pick(std::true_type{}) : pick(std::false_type{});
   if (int err = launch_check("glu_gate_kernel")) return err;
 
   auto transpose = [&](const void* src, int64_t rows, int64_t cols, const Lines& d) {

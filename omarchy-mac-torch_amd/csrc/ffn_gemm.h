@@ -51,19 +51,29 @@ struct GemmArgs {
   float *keep_gs, *keep_us;
 };
 
+// exp(-g) by the exponential instruction, a few ulp and |g| 2^-24 of it off, and reciprocals to 1 ulp: the sums that they
+// meet are no better in float32.
+__device__ __forceinline__ float sigmoid(float g) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.442695040888963f * g));
+}
 __device__ __forceinline__ float glu_act(float g, int act) {
-  if (act == OMT_GLU_SILU) return g / (1.f + expf(-g));
+  if (act == OMT_GLU_SILU) return g * sigmoid(g);
   if (act == OMT_GLU_GELU) return 0.5f * g * erfcf(-0.70710678118654752f * g);
   return g < 0.f ? 0.f : g;  // NaN stays
 }
-__device__ __forceinline__ float glu_act_grad(float g, int act) {
+struct ActAndGrad {
+  float act, grad;
+};
+__device__ __forceinline__ ActAndGrad glu_act_grad(float g, int act) {
   if (act == OMT_GLU_SILU) {
-    const float p = 1.f / (1.f + expf(-g));
-    return p * (1.f + g * (1.f - p));
+    const float p = sigmoid(g);
+    return {g * p, p * (1.f + g * (1.f - p))};
   }
-  if (act == OMT_GLU_GELU)
-    return 0.5f * erfcf(-0.70710678118654752f * g) + 0.3989422804014327f * g * expf(-0.5f * g * g);
-  return g > 0.f ? 1.f : 0.f;
+  if (act == OMT_GLU_GELU) {
+    const float phi = 0.5f * erfcf(-0.70710678118654752f * g);
+    return {g * phi, phi + 0.3989422804014327f * g * __builtin_amdgcn_exp2f(-0.7213475204444817f * g * g)};
+  }
+  return {g < 0.f ? 0.f : g, g > 0.f ? 1.f : 0.f};
 }
 
 // four consecutive columns c.. of a row of `cols`, at p (the row's start)
@@ -411,18 +421,20 @@ int launch_gemm(const GemmArgs& a, hipStream_t stream) {
 // bm rows of x to a tile: 16, 64, 128 or 256 (a.gx, a.gy in those units). Two stages: two workgroups of the small tiles
 // fit a CU's 160 KB together and hide each other's waits better than a third stage does (64 rows bf16, 4096 x 4096 x
 // 4096: 144 us with two, 226 with three and one workgroup); 128 rows gain 1-3% from a third where it fits.
-template <int MODE>
-int launch_gemm_of(const GemmArgs& a, bool glu, int bm, hipStream_t stream) {
+template <int MODE, bool GLU>
+int launch_gemm_of(const GemmArgs& a, int bm, hipStream_t stream) {
   switch (bm) {
-    case 16: return glu ? launch_gemm<MODE, true, 16, 2>(a, stream) : launch_gemm<MODE, false, 16, 2>(a, stream);
-    case 64: return glu ? launch_gemm<MODE, true, 64, 2>(a, stream) : launch_gemm<MODE, false, 64, 2>(a, stream);
-    case 128: return glu ? launch_gemm<MODE, true, 128, 3>(a, stream) : launch_gemm<MODE, false, 128, 3>(a, stream);
-    default: return glu ? launch_gemm<MODE, true, 256, 2>(a, stream) : launch_gemm<MODE, false, 256, 2>(a, stream);
+    case 16: return launch_gemm<MODE, GLU, 16, 2>(a, stream);
+    case 64: return launch_gemm<MODE, GLU, 64, 2>(a, stream);
+    case 128: return launch_gemm<MODE, GLU, 128, 3>(a, stream);
+    default: return launch_gemm<MODE, GLU, 256, 2>(a, stream);
   }
 }
-int ffn_gemm_f32(const GemmArgs& a, bool glu, int bm, hipStream_t stream);
+// kF32 in the gated form only, kFp8 in the plain one only
+int ffn_gemm_f32(const GemmArgs& a, int bm, hipStream_t stream);
 int ffn_gemm_bf16(const GemmArgs& a, bool glu, int bm, hipStream_t stream);
 int ffn_gemm_split(const GemmArgs& a, bool glu, int bm, hipStream_t stream);
-int ffn_gemm_fp8(const GemmArgs& a, bool glu, int bm, hipStream_t stream);
+int ffn_gemm_fp8x(const GemmArgs& a, bool glu, int bm, hipStream_t stream);
+int ffn_gemm_fp8(const GemmArgs& a, int bm, hipStream_t stream);
 
 }  // namespace omt

@@ -3,7 +3,7 @@
 namespace omt {
 
 int ffn_gemm_split(const GemmArgs& a, bool glu, int bm, hipStream_t stream) {
-  return launch_gemm_of<kSplit>(a, glu, bm, stream);
+  return glu ? launch_gemm_of<kSplit, true>(a, bm, stream) : launch_gemm_of<kSplit, false>(a, bm, stream);
 }
 
 }  // namespace omt

@@ -155,21 +155,28 @@ __global__ void __launch_bounds__(RT == 64 ? 256 : RT) rms_norm_bwd_kernel(NormB
     store8<false>(a.parts + (int64_t)blockIdx.x * a.dim, (int64_t)(i * RT + t) * 8, a.dim, gw[i]);
 }
 
-// gw[c] = sum over the workgroups' sums: 32 columns to a workgroup, 32 threads a column, each a strided share in order,
+// gw[c] = sum over the workgroups' sums: 16 columns to a workgroup, 64 threads a column, each a strided share in order,
 // then their sums in order
 template <class W>
 __global__ void __launch_bounds__(1024) rms_norm_weight_kernel(const float* __restrict__ parts, int count, int64_t dim,
                                                                W* __restrict__ gw) {
-  __shared__ float red[32][33];
-  const int l = threadIdx.x & 31, k = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + l;
+  __shared__ float red[64][17];
+  const int l = threadIdx.x & 15, k = threadIdx.x >> 4;
+  const int64_t c = (int64_t)blockIdx.x * 16 + l;
   float s = 0.f;
   if (c < dim)
-    for (int p = k; p < count; p += 32) s += parts[(int64_t)p * dim + c];
+    for (int p = k; p < count; p += 64) s += parts[(int64_t)p * dim + c];
   red[k][l] = s;
   __syncthreads();
+  if (k < 8) {
+    s = 0.f;
+    for (int i = 0; i < 8; ++i) s += red[k * 8 + i][l];
+  }
+  __syncthreads();
+  if (k < 8) red[k][l] = s;
+  __syncthreads();
   if (k == 0 && c < dim) {
-    for (int i = 1; i < 32; ++i) s += red[i][l];
+    for (int i = 1; i < 8; ++i) s += red[i][l];
     gw[c] = (W)s;
   }
 }
@@ -245,9 +252,11 @@ static void for_dim(int64_t dim, F f) {
   else if (dim <= 16384) f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
   else f(integral_constant<int, 1024>{}, integral_constant<int, 4>{});
 }
-static int64_t norm_groups(int64_t rows, int64_t dim) {  // workgroups of the backward
-  const int64_t at_once = dim <= 2048 ? 4 : 1;
-  return std::max<int64_t>(1, std::min<int64_t>(cdiv(rows, at_once), 1024));
+// Workgroups of the backward: four to a CU, each summing the weight gradient of at least four rounds of rows (where there
+// are as many as 256 workgroups), so that their sums stay a small part of the traffic.
+static int64_t norm_groups(int64_t rows, int64_t dim) {
+  const int64_t rounds = cdiv(rows, dim <= 2048 ? 4 : 1);
+  return std::max<int64_t>(1, std::min(rounds, std::max<int64_t>(256, std::min<int64_t>(cdiv(rounds, 4), 1024))));
 }
 
 }  // namespace omt
@@ -302,7 +311,7 @@ OMT_EXPORT int omt_rms_norm_bwd(int dtype, int weight_dtype, int64_t rows, int64
   });
   if (int e = launch_check("rms_norm_bwd_kernel")) return e;
   if (!gweight) return OMT_OK;
-  const dim3 grid((unsigned)cdiv(dim, 32));
+  const dim3 grid((unsigned)cdiv(dim, 16));
   if (weight_dtype == OMT_DT_F32)
     hipLaunchKernelGGL(rms_norm_weight_kernel<float>, grid, dim3(1024), 0, stream_of(stream), (const float*)workspace,
                        (int)groups, dim, (float*)gweight);

@@ -222,7 +222,7 @@ SIGNATURES = {
     "omt_rms_norm_bwd": (I32, [I32, I32, I64, I64] + [VP] * 8 + [SZ, VP]),
     "omt_quantize_fp8": (I32, [I32, I64, I64, VP, I32, VP, VP, VP]),
     "omt_quantize_fp8_weight": (I32, [I32, I64, I64, VP, VP, VP, VP]),
-    "omt_matmul_fp8_workspace": (SZ, [I64, I64, I64]),
+    "omt_matmul_fp8_workspace": (SZ, [I64, I64, I64, I32]),
     "omt_matmul_fp8": (I32, [I64, I64, I64, VP, VP, VP, VP, I32, VP, VP, SZ, VP]),
     "omt_glu_fwd_workspace": (SZ, [I32, I64, I64, I64]),
     "omt_glu_fwd": (I32, [I32, I64, I64, I64, I32, I32] + [VP] * 11 + [SZ, VP]),

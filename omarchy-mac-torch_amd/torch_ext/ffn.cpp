@@ -193,7 +193,7 @@ Tensor matmul_fp8(const Tensor& a_, const Tensor& a_scale, const Tensor& b_, con
   const int64_t n = b.q.size(0);
   Site at(a);
   Tensor c = make(a, with_last(a.sizes(), n), type);
-  const size_t need = omt_matmul_fp8_workspace(r.rows, n, r.cols);
+  const size_t need = omt_matmul_fp8_workspace(r.rows, n, r.cols, dtype_of(c));
   void* ws = at.scratch(a, need);
   ok(omt_matmul_fp8(r.rows, n, r.cols, raw(a), rawf(sa), raw(b.q), rawf(b.s), dtype_of(c), raw(c), ws, need, at.stream),
      "matmul_fp8");
