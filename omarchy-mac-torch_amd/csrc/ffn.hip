@@ -239,16 +239,18 @@ __global__ void __launch_bounds__(256) glu_join_kernel(GemmArgs a) {
 
 // The launch of a product of m rows by n (of each weight, if gated) with rows of row_bytes. Every choice of rows to a
 // tile and slices of the reduction is priced, in microseconds, and the cheapest taken: rounds of workgroups over the 256
-// CUs (two at a time of the tiles of 16 and 64 rows, whose stages leave room), each its steps and a fixed 1.5, but no
-// less than the operands' bytes at 5.5 TB/s; slices add the second launch and their sums' way to memory and back at
-// 4 TB/s. Measured steps (4096 x 4096 x 4096, all CUs busy), us; [mode][16, 64, 128, 256 rows]:
+// CUs (two at a time of the tiles of 16 and 64 rows, whose stages leave room), each its steps and what a tile costs before
+// its first and after its last, but no less than the operands' bytes at 5.5 TB/s; slices add the second launch and their
+// sums' way to memory and back at 4 TB/s. Measured steps (8192 x 4096 x 16384, and 64 x 4096 x 4096 for 16 rows, all CUs
+// busy), us, [mode][16, 64, 128, 256 rows], and the rest of a tile (from 4096 x 4096 x 4096):
 constexpr float kStepUs[][4] = {
-    {1.65f, 4.0f, 3.83f, 7.46f},  // kF32
-    {1.2f, 1.12f, 0.96f, 1.75f},  // kBf16
-    {2.1f, 2.9f, 2.1f, 3.8f},     // kFp8x
-    {1.6f, 2.2f, 1.3f, 2.7f},     // kFp8
-    {1.1f, 2.3f, 1.52f, 2.86f},   // kSplit
+    {1.65f, 3.9f, 3.75f, 7.3f},  // kF32
+    {1.2f, 1.1f, 0.85f, 1.56f},  // kBf16
+    {2.1f, 2.8f, 1.8f, 3.4f},    // kFp8x
+    {1.6f, 2.0f, 1.11f, 1.92f},  // kFp8
+    {1.1f, 2.2f, 1.55f, 2.8f},   // kSplit
 };
+constexpr float kTileUs[4] = {1.5f, 4.f, 7.f, 13.f};
 constexpr int kBm[4] = {16, 64, 128, 256}, kResident[4] = {2, 2, 1, 1};
 struct GemmPlan {
   int bm, gx, gy, steps, slices, slice_steps;
@@ -270,7 +272,7 @@ static GemmPlan plan_gemm(int mode, bool glu, int64_t m, int64_t n, int64_t row_
       // a workgroup alone on its CU takes about half the step that two take, but no less than a load's way, 0.9
       const bool alone = kResident[v] == 2 && gx * gy * s <= 256;
       const float step = alone ? std::max(0.9f, 0.6f * kStepUs[mode][v]) : kStepUs[mode][v];
-      float us = std::max(rounds * (per * step + 1.5f), bytes_us);
+      float us = std::max(rounds * (per * step + kTileUs[v]), bytes_us);
       if (s > 1) us += 4.f + 2.f * s * sums * 4 / 4e6f;
       if (us < best.us) best = {kBm[v], (int)gx, (int)gy, (int)steps, (int)s, (int)per, us, 0};
       if (gx * gy * s > 2048) break;
