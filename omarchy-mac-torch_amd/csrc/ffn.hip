@@ -17,14 +17,21 @@ namespace omt {
 
 // ---- operands laid out for the tiles ------------------------------------------------------------------------------------
 
-// Rows copied to a pitch that is a multiple of 16 bytes, zeros past their end.
+// Rows copied to a pitch that is a multiple of 16 bytes, zeros past their end; 16 bytes to a thread.
 template <class T>
 __global__ void __launch_bounds__(256) pad_rows_kernel(const T* __restrict__ src, int64_t rows, int64_t cols,
                                                        int64_t pitch, T* __restrict__ dst) {
-  const int64_t total = rows * pitch, step = (int64_t)gridDim.x * 256;
+  constexpr int N = 16 / sizeof(T);
+  const int64_t per = pitch / N, total = rows * per, step = (int64_t)gridDim.x * 256;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
-    const int64_t r = i / pitch, c = i - r * pitch;
-    dst[i] = c < cols ? src[r * cols + c] : T(0);
+    const int64_t r = i / per, c = (i - r * per) * N;
+    union {
+      T e[N];
+      uint4 all;
+    } v;
+#pragma unroll
+    for (int e = 0; e < N; ++e) v.e[e] = c + e < cols ? src[r * cols + c + e] : T(0);
+    *(uint4*)(dst + r * pitch + c) = v.all;
   }
 }
 
@@ -258,7 +265,7 @@ struct GemmPlan {
   size_t parts_bytes;
 };
 static GemmPlan plan_gemm(int mode, bool glu, int64_t m, int64_t n, int64_t row_bytes) {
-  const int64_t gx = cdiv(n, glu ? 128 : 256), steps = cdiv(row_bytes, 128), sums = m * n * (glu ? 2 : 1);
+  const int64_t gx = cdiv(n, glu ? 128 : 256), steps = std::max<int64_t>(cdiv(row_bytes & ~15, 128), 1), sums = m * n * (glu ? 2 : 1);
   const float bytes_us = (float)(m + n * (glu ? 2 : 1)) * (float)row_bytes / 5.5e6f;
   GemmPlan best{};
   best.us = 1e30f;
@@ -332,13 +339,16 @@ static Lines from(Lines d, int fmt, int64_t line, int64_t at) {
   return d;
 }
 
-// An operand's rows as the tiles read them: in place where every row starts on 16 bytes, else copied; kSplit always copied.
+// An operand's rows as the tiles read them: in place where every row starts on 4 bytes (any float32, an even number of
+// bfloat16, a multiple of four e4m3), else copied; kSplit always copied.
 static Lines place_rows(Space& sp, int mode, int64_t rows, int64_t cols) {
   if (mode == kSplit) return take_lines(sp, kSplit, rows, up(cols, kBlk));
   Lines d;
-  const int64_t bytes = cols * elem_bytes(mode);
-  d.pitch = up(bytes, 16);
-  if (d.pitch != bytes) d.p = (char*)sp.take((size_t)(rows * d.pitch));
+  d.pitch = cols * elem_bytes(mode);
+  if (d.pitch % 4) {
+    d.pitch = up(d.pitch, 16);
+    d.p = (char*)sp.take((size_t)(rows * d.pitch));
+  }
   return d;
 }
 static int lay_rows(const Lines& d, int mode, const void* src, int64_t rows, int64_t cols, hipStream_t stream) {
@@ -350,12 +360,12 @@ static int lay_rows(const Lines& d, int mode, const void* src, int64_t rows, int
   }
   if (!d.p) return OMT_OK;
   const int64_t pitch = d.pitch / elem_bytes(mode);
-  const dim3 grid(grid1d(rows * pitch, 256, 1 << 16));
+  const dim3 grid(grid1d(rows * d.pitch / 16, 256, 1 << 16));
   auto go = [&](auto zero) {
     using T = decltype(zero);
     hipLaunchKernelGGL(pad_rows_kernel<T>, grid, dim3(256), 0, stream, (const T*)src, rows, cols, pitch, (T*)d.p);
   };
-  mode == kF32 ? go(uint32_t(0)) : mode == kBf16 ? go(uint16_t(0)) : go(uint8_t(0));
+  mode == kBf16 ? go(uint16_t(0)) : go(uint8_t(0));
   return launch_check("pad_rows_kernel");
 }
 // Lays out x [m][k] and the weights [n][k] (w_up may be null) and points a at them.
@@ -399,11 +409,11 @@ static int need_space(const char* fn, size_t need, const void* ws, size_t bytes)
 // the same values are 1e-8 off): nothing beside a bfloat16 result's 2^-9, too much for a float32 one.
 static int fp8_mode(int out_dtype) { return out_dtype == OMT_DT_BF16 ? kFp8 : kFp8x; }
 struct MatmulFp8 {
-  GemmPlan p;
   Lines a, b;
+  GemmPlan p;
   void* parts;
   MatmulFp8(Space& sp, int mode, int64_t m, int64_t n, int64_t k)
-      : p(plan_gemm(mode, false, m, n, k)), a(place_rows(sp, kFp8x, m, k)), b(place_rows(sp, kFp8x, n, k)),
+      : a(place_rows(sp, mode, m, k)), b(place_rows(sp, mode, n, k)), p(plan_gemm(mode, false, m, n, a.pitch)),
         parts(sp.take(p.parts_bytes)) {}
 };
 // float32: on fp32 MFMA as it is, or as halves on float16 MFMA, three products for one. Laying out the halves reads and

@@ -34,7 +34,7 @@ __device__ __forceinline__ const T* uniform(const T* p) {
 }
 
 struct GemmArgs {
-  const void *x, *w, *w_up;           // rows of xpitch / wpitch bytes on 16-byte boundaries; w_up: the gated form's
+  const void *x, *w, *w_up;           // rows of xpitch / wpitch bytes, a multiple of 4; w_up: the gated form's
   const float *sx, *sw, *sw_up;       // 8 bits: x's scales [m][blocks], w's [ceil(n / 128)][blocks]
   int sx_row, sw_row, sx_step, sw_step;  // floats from a row's scale to the next row's, and to its next step's
   int64_t xpitch, wpitch;
@@ -94,9 +94,8 @@ __device__ __forceinline__ void store4_any(void* p, int64_t row, int c, int cols
   if (kind == kOutBf16) store4((__bf16*)p + row * cols, c, cols, vec, v);
   else store4((float*)p + row * cols, c, cols, vec, v);
 }
-__device__ __forceinline__ void store4_fp8(void* p, int64_t row, int c, int cols, bool vec, f32x4 v, float inv) {
+__device__ __forceinline__ void store4_fp8(uint8_t* q, int c, int cols, bool vec, f32x4 v, float inv) {
   const uint32_t w = pack_fp8(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv);
-  uint8_t* q = (uint8_t*)p + row * cols;
   if (vec) {
     if (c < cols) *(uint32_t*)(q + c) = w;
   } else {
@@ -140,7 +139,7 @@ __global__ void __launch_bounds__((GemmTile<MODE, BM, NS>::THREADS), (GemmTile<M
 ffn_gemm_kernel(GemmArgs a) {
   using Tl = GemmTile<MODE, BM, NS>;
   constexpr int TI = Tl::TI, TJ = Tl::TJ, NT = GLU ? 128 : 256;
-  static_assert(Tl::LDS >= 3 * 4 * BM * 4, "the epilogue's maxima lie where the stages were");
+  static_assert(Tl::LDS >= 2 * 4 * BM * 4, "the epilogue's maxima lie where the stages were");
   __shared__ __attribute__((aligned(128))) unsigned char lds[Tl::LDS];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -188,12 +187,13 @@ ffn_gemm_kernel(GemmArgs a) {
     }
   }
   auto slot_of_x = [&](int t) { return wave + Tl::NW * t < Tl::SROWS / 64; };
+  const int whole = a.row_bytes & ~15;  // what the 16-byte loads take of a row
   const uint32_t lds0 = lds_addr((const float*)lds);
   // Step s into stage `buf`. Past the slice's last step every lane's offset is out of range: the loads count, and read
   // nothing.
   auto issue = [&](int buf, int s) {
     const uint32_t at = lds0 + buf * Tl::STAGE;
-    const uint32_t left = s < s1 ? (uint32_t)(a.row_bytes - s * 128) : 0u;
+    const uint32_t left = s < s1 && s * 128 < whole ? (uint32_t)(whole - s * 128) : 0u;
     const bool in = chunk16 < left;
 #pragma unroll
     for (int t = 0; t < Tl::DW; ++t)
@@ -203,7 +203,7 @@ ffn_gemm_kernel(GemmArgs a) {
 #pragma unroll
       for (int t = 0; t < Tl::SW; ++t)
         lds_load_b32(rsrc_words(uniform(sbase[t] + (slot_of_x(t) ? s * (int64_t)a.sx_step : s * (int64_t)a.sw_step)), 0x7fffffffu),
-                     __builtin_amdgcn_readfirstlane(at + sdst[t]), left ? soff[t] : kOOB, 0);
+                     __builtin_amdgcn_readfirstlane(at + sdst[t]), s < s1 ? soff[t] : kOOB, 0);
     }
   };
 
@@ -219,6 +219,34 @@ ffn_gemm_kernel(GemmArgs a) {
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+  };
+
+  // The last one to three words of rows that are no multiple of 16 bytes, as a step of their own after the others, zeros
+  // beside them: laid into stage 0 by hand, with their block's scales. (In the loop they cost it 6%.)
+  const bool ragged = MODE != kSplit && whole != a.row_bytes && s1 == a.steps;
+  auto lay_rest = [&]() {
+    meet(std::integral_constant<int, 0>{});
+    for (int r = threadIdx.x; r < BM + 256; r += Tl::THREADS) {
+      const bool of_x = r < BM;
+      const int w = GLU ? (r - BM) & 127 : r - BM, part = GLU && r - BM >= 128;
+      const bool in = of_x ? m0 + r < a.m : n0 + w < a.n;
+      const unsigned char* src = of_x ? (const unsigned char*)a.x + (m0 + r) * a.xpitch
+                                      : (const unsigned char*)(part ? a.w_up : a.w) + (n0 + w) * a.wpitch;
+      omt_u32x4 rest = {};
+#pragma unroll
+      for (int e = 0; e < 3; ++e)
+        if (in && whole + 4 * e < a.row_bytes) rest[e] = *(const uint32_t*)(src + whole + 4 * e);
+      omt_u32x4* row = (omt_u32x4*)(lds + r * 128);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) row[c] = c == (r & 7) ? rest : omt_u32x4{};
+      if constexpr (Tl::SCALED) {
+        const int64_t block = (a.row_bytes - 1) >> 7;
+        float* scales = (float*)(lds + (BM + 256) * 128);
+        if (of_x) scales[r] = in ? a.sx[(m0 + r) * (int64_t)a.sx_row + block * a.sx_step] : 0.f;
+        else scales[Tl::SROWS + r - BM] = in ? (part ? a.sw_up : a.sw)[((n0 + w) >> 7) * (int64_t)a.sw_row + block * a.sw_step] : 0.f;
+      }
+    }
+    __syncthreads();
   };
 
   // kF32, kBf16: a step in two halves, each of them its products while the next half's chunks come from LDS
@@ -277,6 +305,11 @@ ffn_gemm_kernel(GemmArgs a) {
       multiply(1);
       blend();
       cur = nxt;
+    }
+    if (ragged) {
+      lay_rest();
+      read(0, 0);
+      multiply(0);
     }
   } else {
     auto compute = [&](int buf) {
@@ -367,6 +400,10 @@ ffn_gemm_kernel(GemmArgs a) {
       cur = cur + 1 == NS ? 0 : cur + 1;
       nxt = nxt + 1 == NS ? 0 : nxt + 1;
     }
+    if (ragged) {
+      lay_rest();
+      compute(0);
+    }
   }
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0) & ~0xF00);
   asm volatile("" ::: "memory");
@@ -401,34 +438,44 @@ ffn_gemm_kernel(GemmArgs a) {
                    a.out_kind, acc[i][j]);
     }
   } else {
-    uint32_t* top = (uint32_t*)lds;  // [g, u, h][wave][row]: each wave's largest magnitudes of 32 columns
-    const bool keep8 = a.keep == kKeepFp8, out8 = a.out_kind == kOutFp8;
+    uint32_t* top = (uint32_t*)lds;  // [g, u or h][wave][row]: each wave's largest magnitudes of 32 columns
+    constexpr bool out8 = MODE == kFp8x;  // 8-bit operands give an 8-bit result and keep nothing
+    const bool keep8 = !out8 && a.keep == kKeepFp8;
     auto h4 = [&](f32x4 gv, f32x4 uv) {
       f32x4 h;
 #pragma unroll
       for (int e = 0; e < 4; ++e) h[e] = glu_act(gv[e], a.act) * uv[e];
       return h;
     };
-    if (keep8 || out8) {
+    auto note = [&](int z, int i, uint32_t b) {
+      b = max_u32(b, (uint32_t)__shfl_xor((int)b, 16));
+      b = max_u32(b, (uint32_t)__shfl_xor((int)b, 32));
+      if (g == 0) top[(z * 4 + wn) * BM + xrow + i * 16 + r16] = b;
+    };
+    auto abs_bits4 = [](f32x4 v) {
+      return max_u32(max_u32(abs_bits(v[0]), abs_bits(v[1])), max_u32(abs_bits(v[2]), abs_bits(v[3])));
+    };
+    // the block's scale (by a product with 1 / 448 rounded) and its reciprocal to 1 ulp
+    auto scale_of = [&](int z, int lr, float* inv) {
+      const uint32_t* p = top + z * 4 * BM + lr;
+      const uint32_t b = max_u32(max_u32(p[0], p[BM]), max_u32(p[2 * BM], p[3 * BM]));
+      const float s = __builtin_bit_cast(float, max_u32(b, __builtin_bit_cast(uint32_t, kFp8Floor))) * (1.f / kFp8Max);
+      *inv = __builtin_amdgcn_rcpf(s);
+      return s;
+    };
+    if constexpr (out8) {  // h in the place of g
 #pragma unroll
       for (int i = 0; i < TI; ++i) {
-        uint32_t b[3] = {0, 0, 0};
+        acc[i][0] = h4(acc[i][0], acc[i][2]);
+        acc[i][1] = h4(acc[i][1], acc[i][3]);
+        note(0, i, max_u32(abs_bits4(acc[i][0]), abs_bits4(acc[i][1])));
+      }
+      __syncthreads();
+    } else if (keep8) {
 #pragma unroll
-        for (int jj = 0; jj < 2; ++jj) {
-          const f32x4 h = out8 ? h4(acc[i][jj], acc[i][jj + 2]) : f32x4{};
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            b[0] = max_u32(b[0], abs_bits(acc[i][jj][e]));
-            b[1] = max_u32(b[1], abs_bits(acc[i][jj + 2][e]));
-            b[2] = max_u32(b[2], abs_bits(h[e]));
-          }
-        }
-#pragma unroll
-        for (int z = 0; z < 3; ++z) {
-          b[z] = max_u32(b[z], (uint32_t)__shfl_xor((int)b[z], 16));
-          b[z] = max_u32(b[z], (uint32_t)__shfl_xor((int)b[z], 32));
-          if (g == 0) top[(z * 4 + wn) * BM + xrow + i * 16 + r16] = b[z];
-        }
+      for (int i = 0; i < TI; ++i) {
+        note(0, i, max_u32(abs_bits4(acc[i][0]), abs_bits4(acc[i][1])));
+        note(1, i, max_u32(abs_bits4(acc[i][2]), abs_bits4(acc[i][3])));
       }
       __syncthreads();
     }
@@ -436,34 +483,38 @@ ffn_gemm_kernel(GemmArgs a) {
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
       const int lr = xrow + i * 16 + r16, m = m0 + lr;
-      float s[3] = {1.f, 1.f, 1.f}, inv[3];
-      if (keep8 || out8) {
-#pragma unroll
-        for (int z = 0; z < 3; ++z) {
-          const uint32_t* p = top + z * 4 * BM + lr;
-          s[z] = block_scale(max_u32(max_u32(p[0], p[BM]), max_u32(p[2 * BM], p[3 * BM])));
-        }
-      }
-#pragma unroll
-      for (int z = 0; z < 3; ++z) inv[z] = 1.f / s[z];
       if (m >= a.m) continue;
-      if (wn == 0 && g == 0) {
-        const int64_t at = (int64_t)m * blocks + (n0 >> 7);
-        if (keep8) a.keep_gs[at] = s[0], a.keep_us[at] = s[1];
-        if (out8) a.out_scale[at] = s[2];
+      const int64_t row = (int64_t)m * a.n, at = (int64_t)m * blocks + (n0 >> 7);
+      const int c = n0 + wn * 32 + 4 * g;
+      const bool first = wn == 0 && g == 0;
+      float inv;
+      if constexpr (out8) {
+        const float s = scale_of(0, lr, &inv);
+        if (first) a.out_scale[at] = s;
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) store4_fp8((uint8_t*)a.out + row, c + 16 * jj, a.n, vec, acc[i][jj], inv);
+        continue;
       }
 #pragma unroll
       for (int jj = 0; jj < 2; ++jj) {
-        const int c = n0 + wrow(jj) + 4 * g;
-        const f32x4 gv = acc[i][jj], uv = acc[i][jj + 2], h = h4(gv, uv);
-        if (out8) store4_fp8(a.out, m, c, a.n, vec, h, inv[2]);
-        else store4_any(a.out, m, c, a.n, vec, a.out_kind, h);
-        if (keep8) {
-          store4_fp8(a.keep_g, m, c, a.n, vec, gv, inv[0]);
-          store4_fp8(a.keep_u, m, c, a.n, vec, uv, inv[1]);
-        } else if (a.keep == kKeepFull) {
-          store4_any(a.keep_g, m, c, a.n, vec, a.out_kind, gv);
-          store4_any(a.keep_u, m, c, a.n, vec, a.out_kind, uv);
+        const f32x4 h = h4(acc[i][jj], acc[i][jj + 2]);
+        if (a.out_kind == kOutBf16) store4((__bf16*)a.out + row, c + 16 * jj, a.n, vec, h);
+        else store4((float*)a.out + row, c + 16 * jj, a.n, vec, h);
+      }
+      if (keep8) {
+        float s = scale_of(0, lr, &inv);
+        if (first) a.keep_gs[at] = s;
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) store4_fp8((uint8_t*)a.keep_g + row, c + 16 * jj, a.n, vec, acc[i][jj], inv);
+        s = scale_of(1, lr, &inv);
+        if (first) a.keep_us[at] = s;
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) store4_fp8((uint8_t*)a.keep_u + row, c + 16 * jj, a.n, vec, acc[i][jj + 2], inv);
+      } else if (a.keep == kKeepFull) {
+#pragma unroll
+        for (int jj = 0; jj < 2; ++jj) {
+          store4_any(a.keep_g, m, c + 16 * jj, a.n, vec, a.out_kind, acc[i][jj]);
+          store4_any(a.keep_u, m, c + 16 * jj, a.n, vec, a.out_kind, acc[i][jj + 2]);
         }
       }
     }
