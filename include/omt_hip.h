@@ -665,6 +665,12 @@ int omt_glu_bwd(int dtype, int64_t m, int64_t k, int64_t f, int act, int keep, c
                 const float* x_scale, const void* g, const float* g_scale, const void* u, const float* u_scale,
                 const void* w_gate, const void* w_up, void* gx, void* gw_gate, void* gw_up, void* workspace,
                 size_t workspace_bytes, void* stream);
+/* How a product of these operators runs: m rows, a reduction of k (for the gradients: the block's k), n outputs (the
+ * block's f), dtype the result's (OMT_FFN_MATMUL_FP8) or the operands'. mode: 0 float32 matrix instructions, 1 bfloat16, 2
+ * e4m3 widened to bfloat16, 3 e4m3, 4 float32 as float16 halves; rows of x to a tile; slices of the reduction. */
+enum { OMT_FFN_MATMUL_FP8 = 0, OMT_FFN_GLU = 1, OMT_FFN_GLU_FP8 = 2, OMT_FFN_GLU_GX = 3, OMT_FFN_GLU_GW = 4 };
+int omt_ffn_plan(int op, int dtype, int64_t m, int64_t k, int64_t n, int* mode, int* rows, int* slices);
+
 /* omt_glu_fwd of operands in 8 bits (weights by 128 x 128), h in 8 bits. x, the weights and the workspace on 16 bytes. */
 size_t omt_glu_fp8_workspace(int64_t m, int64_t k, int64_t f);
 int omt_glu_fp8(int64_t m, int64_t k, int64_t f, int act, const void* x, const float* x_scale, const void* w_gate,

@@ -480,6 +480,25 @@ static int run_lines(int mode, const GemmPlan& p, GemmArgs a, const Lines& x, co
 
 using namespace omt;
 
+OMT_EXPORT int omt_ffn_plan(int op, int dtype, int64_t m, int64_t k, int64_t n, int* mode, int* rows, int* slices) {
+  const char* fn = "omt_ffn_plan";
+  if (!mode || !rows || !slices) return fail(OMT_INVALID, "%s: null pointer", fn);
+  if (int e = glu_check(fn, dtype, m, k, n, OMT_GLU_SILU)) return e;
+  if (m == 0) return fail(OMT_INVALID, "%s: no rows", fn);
+  Space sp{nullptr};
+  GemmPlan p;
+  switch (op) {
+    case OMT_FFN_MATMUL_FP8: *mode = fp8_mode(dtype), p = MatmulFp8(sp, *mode, m, n, k).p; break;
+    case OMT_FFN_GLU: *mode = glu_mode(dtype, m, k, n), p = GluFwd(sp, *mode, m, k, n).p; break;
+    case OMT_FFN_GLU_FP8: *mode = kFp8x, p = GluFwd(sp, kFp8x, m, k, n).p; break;
+    case OMT_FFN_GLU_GX: *mode = bwd_mode(dtype), p = GluBwd(sp, *mode, m, k, n).px; break;
+    case OMT_FFN_GLU_GW: *mode = bwd_mode(dtype), p = GluBwd(sp, *mode, m, k, n).pw; break;
+    default: return fail(OMT_INVALID, "%s: op %d", fn, op);
+  }
+  *rows = p.bm, *slices = p.slices;
+  return OMT_OK;
+}
+
 OMT_EXPORT size_t omt_matmul_fp8_workspace(int64_t m, int64_t n, int64_t k, int out_dtype) {
   if (product_check("omt_matmul_fp8_workspace", m, n, k) || m == 0) return 0;
   Space sp{nullptr};

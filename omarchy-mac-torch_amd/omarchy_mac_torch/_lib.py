@@ -22,6 +22,7 @@ NOALLOC_SCRATCH_BYTES = 64 << 20  # OMT_NOALLOC_SCRATCH_BYTES
  OMT_PW_HARDSIGMOID_BWD, OMT_PW_SCALE, OMT_PW_FILL, OMT_PW_ADD_SCALAR) = range(11)
 OMT_DT_F32, OMT_DT_I64, OMT_DT_BF16 = 0, 1, 2
 OMT_GLU_SILU, OMT_GLU_GELU, OMT_GLU_RELU = 0, 1, 2
+OMT_FFN_MATMUL_FP8, OMT_FFN_GLU, OMT_FFN_GLU_FP8, OMT_FFN_GLU_GX, OMT_FFN_GLU_GW = range(5)
 OMT_KEEP_NONE, OMT_KEEP_FP8, OMT_KEEP_FULL = 0, 1, 2
 OMT_ACT_NONE, OMT_ACT_RELU, OMT_ACT_HARDSWISH = 0, 1, 2
 FOREACH_MAX_NUMEL = 1 << 16  # OMT_FOREACH_MAX_NUMEL
@@ -222,6 +223,7 @@ SIGNATURES = {
     "omt_rms_norm_bwd": (I32, [I32, I32, I64, I64] + [VP] * 8 + [SZ, VP]),
     "omt_quantize_fp8": (I32, [I32, I64, I64, VP, I32, VP, VP, VP]),
     "omt_quantize_fp8_weight": (I32, [I32, I64, I64, VP, VP, VP, VP]),
+    "omt_ffn_plan": (I32, [I32, I32, I64, I64, I64] + [ctypes.POINTER(I32)] * 3),
     "omt_matmul_fp8_workspace": (SZ, [I64, I64, I64, I32]),
     "omt_matmul_fp8": (I32, [I64, I64, I64, VP, VP, VP, VP, I32, VP, VP, SZ, VP]),
     "omt_glu_fwd_workspace": (SZ, [I32, I64, I64, I64]),

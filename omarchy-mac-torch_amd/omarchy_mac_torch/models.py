@@ -1,4 +1,5 @@
-"""The convnets of the benchmark configurations, built from plain torch.nn modules.
+"""The convnets of the benchmark configurations, built from plain torch.nn modules, and a small language model of
+feed-forward sublayers.
 
     plain_cnn()              PlainCNN: four conv3x3 (32, 64, 128, 256) + BatchNorm + ReLU + maxpool2x2 blocks in one
                              nn.Sequential (a fused stack), global average pool, linear 256 -> classes
@@ -7,7 +8,11 @@
     mobilenet_v3_small()     MobileNetV3-Small-style: inverted residuals with stride-1 depthwise 3x3 / 5x5, 1x1 expand /
                              project, hardswish, BatchNorm, squeeze-excite (adaptive average pool + linear)
 
-Weights use Kaiming-normal initialization for convolutions (fan-in, ReLU gain), from torch's current RNG state.
+    mlp_lm()                 a next-token model without attention: embedding, feed-forward sublayers (ffn.FeedForward) on
+                             a residual stream, norm, linear to the vocabulary; serve() gives it with the sublayers'
+                             weights in 8 bits
+
+Convolution weights use Kaiming-normal initialization for convolutions (fan-in, ReLU gain), from torch's current RNG state.
 These are the model definitions the benchmark configurations name; the reference's own variants differ in input
 size, widths and classes (omarchy_mac_torch/models.py in the reference).
 """
@@ -130,3 +135,40 @@ class MobileNetV3Small(nn.Module):
 
 def mobilenet_v3_small(classes=1000):
     return MobileNetV3Small(classes)
+
+
+class MlpLM(nn.Module):
+    """Logits of the next token from the last `context` tokens' embeddings, side by side, through feed-forward sublayers."""
+
+    def __init__(self, vocab, dim, hidden, depth, context=4, act="silu", checkpoint="fp8"):
+        from omarchy_mac_torch import ffn  # the operators' library, which a user of the convnets' definitions need not have
+        super().__init__()
+        if dim % context:
+            raise ValueError(f"dim {dim} is not a multiple of the context, {context}")
+        self.context = context
+        self.embed = nn.Embedding(vocab, dim // context)
+        self.blocks = nn.ModuleList(ffn.FeedForward(dim, hidden, act, checkpoint) for _ in range(depth))
+        self.norm = ffn.RMSNorm(dim)
+        self.head = nn.Linear(dim, vocab, bias=False)
+        nn.init.normal_(self.head.weight, std=dim ** -0.5)
+
+    def forward(self, tokens):
+        """tokens [batch, length >= context] -> logits [batch, length - context + 1, vocab]"""
+        e = self.embed(tokens)
+        n = tokens.shape[1] - self.context + 1
+        x, stream = torch.cat([e[:, i:i + n] for i in range(self.context)], -1), None
+        for block in self.blocks:
+            x, stream = block(x, stream)
+        y = self.norm(x) if stream is None else self.norm(x, stream)[0]
+        return self.head(y)
+
+    def serve(self):
+        """The model for inference, its sublayers' weights in 8 bits (the rest is shared with this one)."""
+        import copy
+        served = copy.copy(self)
+        served._modules = dict(self._modules, blocks=nn.ModuleList(b.serve() for b in self.blocks))
+        return served.eval()
+
+
+def mlp_lm(vocab=256, dim=512, hidden=1408, depth=4, **options):
+    return MlpLM(vocab, dim, hidden, depth, **options)

@@ -419,3 +419,107 @@ def test_refusals(ops, cuda):
             (ValueError, lambda: ops.glu_backward(x, (x, None, x[:2], None, x, None), x[:, :8], x[:, :8]))]:
         with pytest.raises(error):
             call()
+
+
+# ---- every tile, in every mode, with the reduction whole and in slices ----------------------------------------------------------
+
+# (operator, type, m, k, n): (mode, rows of a tile, sliced)
+PLANS = {
+    (0, 0, 1, 8, 8): (2, 16, False), (0, 0, 1, 671, 8): (2, 16, True), (0, 0, 4103, 8, 307): (2, 64, False),
+    (0, 0, 758, 2738, 9): (2, 64, True), (0, 0, 4742, 394, 818): (2, 128, False), (0, 0, 3588, 3137, 8): (2, 128, True),
+    (0, 0, 3411, 258, 2353): (2, 256, False),
+    (0, 2, 1, 8, 8): (3, 16, False), (0, 2, 1, 921, 8): (3, 16, True), (0, 2, 4103, 8, 307): (3, 64, False),
+    (0, 2, 2243, 1177, 8): (3, 64, True), (0, 2, 4742, 394, 818): (3, 128, False), (0, 2, 3588, 3137, 8): (3, 128, True),
+    (0, 2, 3411, 258, 2353): (3, 256, False),
+    (1, 0, 1, 8, 8): (0, 16, False), (1, 0, 1, 277, 8): (0, 16, True), (1, 0, 3340, 8, 531): (0, 64, False),
+    (1, 0, 936, 1084, 8): (0, 64, True), (1, 0, 4713, 3959, 14): (0, 128, True),
+    (1, 2, 1, 8, 8): (1, 16, False), (1, 2, 1, 458, 8): (1, 16, True), (1, 2, 4112, 9, 140): (1, 64, False),
+    (1, 2, 703, 2126, 8): (1, 64, True), (1, 2, 3354, 931, 519): (1, 128, False), (1, 2, 3804, 3382, 130): (1, 128, True),
+    (1, 2, 1055, 476, 3985): (1, 256, False),
+    (1, 0, 1581, 749, 455): (4, 16, False), (1, 0, 2736, 383, 285): (4, 64, False), (1, 0, 1647, 871, 407): (4, 64, True),
+    (1, 0, 4182, 171, 429): (4, 128, False), (1, 0, 4136, 724, 150): (4, 128, True), (1, 0, 4999, 100, 787): (4, 256, False),
+    (1, 0, 3616, 2879, 287): (4, 256, True),
+    (2, 0, 1, 8, 8): (2, 16, False), (2, 0, 1, 671, 8): (2, 16, True), (2, 0, 4112, 9, 140): (2, 64, False),
+    (2, 0, 758, 2738, 9): (2, 64, True), (2, 0, 4253, 399, 412): (2, 128, False), (2, 0, 3588, 3137, 8): (2, 128, True),
+    (2, 0, 4189, 259, 956): (2, 256, False),
+    (3, 2, 1, 8, 8): (1, 16, False), (3, 2, 1, 8, 208): (1, 16, True), (3, 2, 4303, 297, 9): (1, 64, False),
+    (3, 2, 2317, 8, 262): (1, 64, True), (3, 2, 1264, 3108, 392): (1, 128, False), (3, 2, 4768, 8, 2625): (1, 128, True),
+    (3, 2, 2507, 3166, 194): (1, 256, False),
+    (3, 0, 1, 8, 69): (4, 16, True), (3, 0, 4303, 297, 9): (4, 64, False), (3, 0, 2732, 8, 130): (4, 64, True),
+    (3, 0, 3451, 1045, 71): (4, 128, False), (3, 0, 3599, 8, 537): (4, 128, True), (3, 0, 3754, 2109, 8): (4, 256, False),
+    (3, 0, 4768, 8, 2625): (4, 256, True),
+    (4, 2, 449, 8, 8): (1, 16, True), (4, 2, 1, 8, 4183): (1, 64, False), (4, 2, 1006, 8, 762): (1, 64, True),
+    (4, 2, 1063, 292, 4285): (1, 128, False), (4, 2, 2378, 9, 4361): (1, 128, True), (4, 2, 481, 1810, 2093): (1, 256, False),
+    (4, 0, 214, 8, 11): (4, 16, True), (4, 0, 1, 8, 4183): (4, 64, False), (4, 0, 573, 8, 830): (4, 64, True),
+    (4, 0, 138, 363, 4109): (4, 128, False), (4, 0, 393, 9, 4350): (4, 128, True), (4, 0, 70, 1094, 3315): (4, 256, False),
+    (4, 0, 2378, 9, 4361): (4, 256, True),
+}
+
+
+@pytest.mark.parametrize("op,dtype,m,k,n", list(PLANS))
+def test_every_tile(ops, cuda, op, dtype, m, k, n):
+    import ctypes
+    from omarchy_mac_torch import _lib
+    v = [ctypes.c_int() for _ in range(3)]
+    assert _lib.L.omt_ffn_plan(op, dtype, m, k, n, *v) == 0
+    print("plan", [x.value for x in v], flush=True)
+    t = F32 if dtype == 0 else BF16
+    g = torch.Generator(device=cuda).manual_seed(m + k + n)
+
+    def new(*shape):
+        return torch.randn(*shape, device=cuda, generator=g)
+
+    def near(got, want, bound):
+        assert float((got.double() - want).norm() / want.norm()) <= bound
+
+    def wide(q, s):
+        return q.double() * s.double().repeat_interleave(BLOCK, -1)[..., :q.shape[-1]]
+
+    def wide_weight(q, s):
+        return wide(q, s.repeat_interleave(BLOCK, 0)[:q.shape[0]])
+
+    if op == 0:
+        a, b = ops.quantize_fp8(new(m, k)), ops.quantize_fp8_weight(new(n, k))
+        near(ops.matmul_fp8(*a, *b, dtype=t), wide(*a) @ wide_weight(*b).T, tol(k, t))
+        return
+    x, wg, wu = new(m, k).to(t), (new(n, k) * k ** -0.5).to(t), (new(n, k) * k ** -0.5).to(t)
+    if op == 2:
+        a, b, c = ops.quantize_fp8(x), ops.quantize_fp8_weight(wg), ops.quantize_fp8_weight(wu)
+        p, q = wide(*a) @ wide_weight(*b).T, wide(*a) @ wide_weight(*c).T
+        check_fp8(*ops.glu_fp8(*a, *b, *c), (p * torch.sigmoid(p) * q).cpu())
+        return
+    if op == 1:
+        p, q = x.double() @ wg.double().T, x.double() @ wu.double().T
+        h, kept = ops.glu(x, wg, wu, checkpoint="fp8")
+        near(h, p * torch.sigmoid(p) * q, 2 * tol(k, t))
+        check_fp8(kept[2], kept[3], p.cpu())
+        check_fp8(kept[4], kept[5], q.cpu())
+        return
+    p, q, gh = new(m, n).to(t), new(m, n).to(t), new(m, n).to(t)
+    s = torch.sigmoid(p.double())
+    dg, du = gh.double() * q.double() * s * (1 + p.double() * (1 - s)), gh.double() * p.double() * s
+    got = ops.glu_backward(gh, (x, None, p, None, q, None), wg, wu, input_grad=op == 3, weight_grad=op == 4)
+    if op == 3:
+        near(got[0], dg @ wg.double() + du @ wu.double(), 2 * tol(2 * n, t, rounded=1))
+    else:
+        near(got[1], dg.T @ x.double(), 2 * tol(m, t, rounded=1))
+        near(got[2], du.T @ x.double(), 2 * tol(m, t, rounded=1))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_glu_infinities_and_nan_at_training_sizes(ops, cuda, dtype):
+    """An infinity or NaN of x, at sizes where float32 runs as halves: its own row of h, and no other, and infinities of
+    the sign that float32 gives where the activation passes them."""
+    m, k, f = 1647, 871, 407
+    x, wg, wu = (t.to(cuda) for t in glu_operands(m, k, f, dtype))
+    x[5, 3], x[600, 870], x[1646, 0] = float("inf"), float("nan"), -float("inf")
+    h, kept = ops.glu(x, wg, wu, act="relu", checkpoint="full")
+    bad = torch.zeros(m, dtype=torch.bool, device=cuda)
+    bad[[5, 600, 1646]] = True
+    assert bool(h[~bad].isfinite().all()) and bool(h[600].isnan().all())
+    for row, col in ((5, 3), (1646, 0)):
+        for got, w in ((kept[2], wg), (kept[4], wu)):
+            assert torch.equal(got[row].float(), (x[row, col].float() * w[:, col].float()).sign() * float("inf"))
+    gh = torch.ones_like(h)
+    gx, gwg, gwu = ops.glu_backward(gh, kept, wg, wu, act="relu")
+    assert bool(gx[~bad].isfinite().all()) and not bool(gx[600].isfinite().any())
