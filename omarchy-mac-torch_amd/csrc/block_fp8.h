@@ -17,7 +17,8 @@ constexpr float kFp8Max = 448.f;      // e4m3's largest value
 constexpr float kFp8Floor = 1e-30f;   // a block of smaller values is scaled as if this were its largest
 
 // ---- eight consecutive elements of a row, as floats; those from `cols` on read as 0 and are not written -------------
-// VEC: every row starts on 16 bytes and holds a multiple of eight elements, so the eight are in range together.
+// VEC: every row starts on 16 bytes and holds a multiple of eight elements, so the eight are in range together. Without it
+// they are read and written together where all are in range, at their type's alignment, and one by one at a row's end.
 
 template <bool VEC>
 __device__ __forceinline__ f32x8 load8(const float* p, int64_t c, int64_t cols) {
@@ -27,6 +28,8 @@ __device__ __forceinline__ f32x8 load8(const float* p, int64_t c, int64_t cols) 
       const f32x4 a = *(const f32x4*)(p + c), b = *(const f32x4*)(p + c + 4);
       v = f32x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     }
+  } else if (c + 8 <= cols) {
+    __builtin_memcpy(&v, p + c, sizeof(v));
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -39,6 +42,10 @@ __device__ __forceinline__ f32x8 load8(const __bf16* p, int64_t c, int64_t cols)
   f32x8 v = {};
   if constexpr (VEC) {
     if (c < cols) v = __builtin_convertvector(*(const bf16x8*)(p + c), f32x8);
+  } else if (c + 8 <= cols) {
+    bf16x8 b;
+    __builtin_memcpy(&b, p + c, sizeof(b));
+    v = __builtin_convertvector(b, f32x8);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -60,6 +67,8 @@ __device__ __forceinline__ f32x8 load8(const uint8_t* p, int64_t c, int64_t cols
   uint2 w = make_uint2(0, 0);
   if constexpr (VEC) {
     if (c < cols) w = *(const uint2*)(p + c);
+  } else if (c + 8 <= cols) {
+    __builtin_memcpy(&w, p + c, sizeof(w));
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -74,6 +83,8 @@ __device__ __forceinline__ void store8(float* p, int64_t c, int64_t cols, f32x8 
       *(f32x4*)(p + c) = f32x4{v[0], v[1], v[2], v[3]};
       *(f32x4*)(p + c + 4) = f32x4{v[4], v[5], v[6], v[7]};
     }
+  } else if (c + 8 <= cols) {
+    __builtin_memcpy(p + c, &v, sizeof(v));
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -84,6 +95,9 @@ template <bool VEC>
 __device__ __forceinline__ void store8(__bf16* p, int64_t c, int64_t cols, f32x8 v) {
   if constexpr (VEC) {
     if (c < cols) *(bf16x8*)(p + c) = __builtin_convertvector(v, bf16x8);
+  } else if (c + 8 <= cols) {
+    const bf16x8 b = __builtin_convertvector(v, bf16x8);
+    __builtin_memcpy(p + c, &b, sizeof(b));
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -142,6 +156,8 @@ template <bool VEC>
 __device__ __forceinline__ void store_fp8x8(uint8_t* p, int64_t c, int64_t cols, uint2 w) {
   if constexpr (VEC) {
     if (c < cols) *(uint2*)(p + c) = w;
+  } else if (c + 8 <= cols) {
+    __builtin_memcpy(p + c, &w, sizeof(w));
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)

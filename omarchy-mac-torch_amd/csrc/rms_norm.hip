@@ -112,13 +112,14 @@ __global__ void __launch_bounds__(RT == 64 ? 256 : RT) rms_norm_bwd_kernel(NormB
   for (int64_t row = (int64_t)blockIdx.x * ROWS + sub; row < a.rows; row += (int64_t)gridDim.x * ROWS) {
     const int64_t base = row * a.dim;
     const float r = a.rstd[row];
-    f32x8 g[NV], n[NV];
+    f32x8 g[NV], n[NV], gh[NV];
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int64_t c = (int64_t)(i * RT + t) * 8;
       const f32x8 gy = load8<VEC>((const T*)a.gy + base, c, a.dim);
       n[i] = load8<VEC>((const T*)a.h + base, c, a.dim) * r;
+      gh[i] = a.gh ? load8<VEC>((const T*)a.gh + base, c, a.dim) : f32x8{};  // on its way during the sum
       gw[i] += gy * n[i];
       g[i] = gy * w[i];
 #pragma unroll
@@ -128,9 +129,7 @@ __global__ void __launch_bounds__(RT == 64 ? 256 : RT) rms_norm_bwd_kernel(NormB
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int64_t c = (int64_t)(i * RT + t) * 8;
-      f32x8 gx = (g[i] - n[i] * mean) * r;
-      if (a.gh) gx += load8<VEC>((const T*)a.gh + base, c, a.dim);
-      store8<VEC>((T*)a.gx + base, c, a.dim, gx);
+      store8<VEC>((T*)a.gx + base, c, a.dim, (g[i] - n[i] * mean) * r + gh[i]);
     }
   }
   if (!a.parts) return;

@@ -801,15 +801,23 @@ def fused_sgd(params, grads, momentum_buffers=None, lr=1e-3, momentum=0.0, dampe
 # omarchy_mac_torch device (differentiable forms for the latter: omarchy_mac_torch.ffn). Held in 8 bits: a
 # torch.float8_e4m3fn tensor with float32 scales, one for each block of 128 along the last dimension (the last block may
 # be shorter), or of 128 x 128 for weights; scale = max(largest magnitude, 1e-30) / 448. A block that holds an infinity or
-# NaN stands for NaN throughout. The checks, and the launches, are torch.ops.omt's (torch_ext/ffn.cpp).
+# NaN stands for NaN throughout. The checks and the launches are in torch_ext/ffn.cpp, whose functions torch.ops.omt
+# registers too.
 
 _GLU_ACTS = {"silu": _lib.OMT_GLU_SILU, "gelu": _lib.OMT_GLU_GELU, "relu": _lib.OMT_GLU_RELU}
 _KEEPS = {None: _lib.OMT_KEEP_NONE, "fp8": _lib.OMT_KEEP_FP8, "full": _lib.OMT_KEEP_FULL}
 
 
+_native_ffn = None
+
+
 def _ffn(name, *args):
+    global _native_ffn
+    if _native_ffn is None:  # the extension loads after this module
+        from omarchy_mac_torch.native import core
+        _native_ffn = core.ffn
     try:
-        return getattr(torch.ops.omt, name).default(*args)
+        return getattr(_native_ffn, name)(*args)
     except NotImplementedError as e:
         raise _lib.Unsupported(_lib.OMT_UNSUPPORTED, str(e)) from None
 

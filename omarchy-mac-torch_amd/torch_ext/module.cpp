@@ -9,6 +9,7 @@ namespace omt {
 void bind_plans(pybind11::module_& m);
 void bind_tuning(pybind11::module_& m);
 void bind_replay(pybind11::module_& m);
+void bind_ffn(pybind11::module_& m);
 }
 
 PYBIND11_MODULE(_native, m) {
@@ -88,4 +89,5 @@ PYBIND11_MODULE(_native, m) {
   bind_plans(m);
   bind_tuning(m);
   bind_replay(m);
+  bind_ffn(m);
 }
