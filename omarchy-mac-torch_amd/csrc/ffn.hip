@@ -187,69 +187,86 @@ __global__ void __launch_bounds__(256) glu_gate_kernel(GateArgs a) {
   write_columns<FMT>(du, a.u_cols, c0, a.f, r0);
 }
 
-// ---- the sums of slices ---------------------------------------------------------------------------------------------------
+// ---- tiles whose steps are shared ---------------------------------------------------------------------------------------
 
-// out = the slices' sums, in slice order, in the output's type; rows from `split` on go to out2
-template <bool VEC>
-__global__ void __launch_bounds__(256) ffn_join_kernel(GemmArgs a) {
-  const int64_t vecs = (a.n + 7) / 8, total = a.m * vecs, step = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
-    const int64_t m = i / vecs, c = (i - m * vecs) * 8;
-    f32x8 v = {};
-    for (int s = 0; s < a.slices; ++s) v += load8<VEC>(a.parts + ((int64_t)s * a.m + m) * a.n, c, a.n);
-    void* out = m < a.split ? a.out : a.out2;
-    const int64_t row = m < a.split ? m : m - a.split;
-    if (a.out_kind == kOutBf16) store8<VEC>((__bf16*)out + row * a.n, c, a.n, v);
-    else store8<VEC>((float*)out + row * a.n, c, a.n, v);
+// The sum of the shares of eight columns of a row of shared tile j, in the shares' order; four loads in flight.
+__device__ __forceinline__ f32x8 join8(const GemmArgs& a, int bm, int j, int row, int col) {
+  const int64_t from = (int64_t)j * a.steps;
+  const int w0 = (int)(from / a.share), w1 = (int)((from + a.steps - 1) / a.share);
+  f32x8 sum = {};
+  // the first share that begins in an earlier tile holds this one's sum second
+  auto at = [&](int w) {
+    const int second = (int64_t)w * a.share < from;
+    return load8<true>(a.parts + (((int64_t)w * 2 + second) * bm + row) * 256, col, 256);
+  };
+  int w = w0;
+  for (; w + 3 <= w1; w += 4) {
+    const f32x8 v0 = at(w), v1 = at(w + 1), v2 = at(w + 2), v3 = at(w + 3);
+    sum += v0;
+    sum += v1;
+    sum += v2;
+    sum += v3;
   }
+  for (; w <= w1; ++w) sum += at(w);
+  return sum;
 }
 
-// The gated form's epilogue over the slices' sums: 16 lanes to a block of 128 outputs of a row.
+// Shared tiles' results: eight rows of a tile to a workgroup, eight columns to a thread. Rows from `split` on go to out2.
 template <bool VEC>
-__global__ void __launch_bounds__(256) glu_join_kernel(GemmArgs a) {
-  const int64_t blocks = (a.n + kFp8Block - 1) / kFp8Block, vecs = blocks * 16;
-  const int64_t total = a.m * vecs, step = (int64_t)gridDim.x * 256;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
-    const int64_t m = i / vecs, c = (i - m * vecs) * 8;
-    f32x8 g = {}, u = {}, h;
-    for (int s = 0; s < a.slices; ++s) {
-      const float* row = a.parts + ((int64_t)s * a.m + m) * 2 * a.n;
-      g += load8<VEC>(row, c, a.n);
-      u += load8<VEC>(row + a.n, c, a.n);
-    }
+__global__ void __launch_bounds__(256) ffn_join_kernel(GemmArgs a, int bm) {
+  const int per = bm / 8, j = blockIdx.x / per, row = blockIdx.x % per * 8 + (threadIdx.x >> 5);
+  const TileId id = tile_at(a.whole + j, a.gx, a.gy);
+  const int64_t m = (int64_t)id.y * bm + row, c = id.x * 256 + (threadIdx.x & 31) * 8;
+  if (m >= a.m || c >= a.n) return;
+  const f32x8 v = join8(a, bm, j, row, (threadIdx.x & 31) * 8);
+  void* out = m < a.split ? a.out : a.out2;
+  const int64_t at = (m < a.split ? m : m - a.split) * a.n;
+  if (a.out_kind == kOutBf16) store8<VEC>((__bf16*)out + at, c, a.n, v);
+  else store8<VEC>((float*)out + at, c, a.n, v);
+}
+
+// The gated form's epilogue over them: sixteen rows to a workgroup, 16 lanes to a row's block of 128.
+template <bool VEC>
+__global__ void __launch_bounds__(256) glu_join_kernel(GemmArgs a, int bm) {
+  const int per = bm / 16, j = blockIdx.x / per, row = blockIdx.x % per * 16 + (threadIdx.x >> 4);
+  const TileId id = tile_at(a.whole + j, a.gx, a.gy);
+  const int64_t m = (int64_t)id.y * bm + row, c = id.x * 128 + (threadIdx.x & 15) * 8;
+  if (m >= a.m) return;  // all sixteen lanes of a row
+  const f32x8 g = join8(a, bm, j, row, (threadIdx.x & 15) * 8), u = join8(a, bm, j, row, 128 + (threadIdx.x & 15) * 8);
+  f32x8 h;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) h[e] = glu_act(g[e], a.act) * u[e];
-    const int64_t row = m * a.n;
-    const bool first = (threadIdx.x & 15) == 0;
-    auto in_8 = [&](f32x8 v, void* q, float* scale) {
-      const float s = block_scale(row16_max(abs_bits8(v)));
-      store_fp8x8<VEC>((uint8_t*)q + row, c, a.n, pack_fp8x8(v, 1.f / s));
-      if (first) scale[i / 16] = s;
-    };
-    auto in_type = [&](f32x8 v, void* p) {
-      if (a.out_kind == kOutBf16) store8<VEC>((__bf16*)p + row, c, a.n, v);
-      else store8<VEC>((float*)p + row, c, a.n, v);
-    };
-    if (a.out_kind == kOutFp8) in_8(h, a.out, a.out_scale);
-    else in_type(h, a.out);
-    if (a.keep == kKeepFp8) {
-      in_8(g, a.keep_g, a.keep_gs);
-      in_8(u, a.keep_u, a.keep_us);
-    } else if (a.keep == kKeepFull) {
-      in_type(g, a.keep_g);
-      in_type(u, a.keep_u);
-    }
+  for (int e = 0; e < 8; ++e) h[e] = glu_act(g[e], a.act) * u[e];
+  const int64_t at = m * a.n, block = m * ((a.n + kFp8Block - 1) / kFp8Block) + id.x;
+  auto in_8 = [&](f32x8 v, void* q, float* scale) {
+    const float s = block_scale(row16_max(abs_bits8(v)));
+    store_fp8x8<VEC>((uint8_t*)q + at, c, a.n, pack_fp8x8(v, 1.f / s));
+    if ((threadIdx.x & 15) == 0) scale[block] = s;
+  };
+  auto in_type = [&](f32x8 v, void* p) {
+    if (a.out_kind == kOutBf16) store8<VEC>((__bf16*)p + at, c, a.n, v);
+    else store8<VEC>((float*)p + at, c, a.n, v);
+  };
+  if (a.out_kind == kOutFp8) in_8(h, a.out, a.out_scale);
+  else in_type(h, a.out);
+  if (a.keep == kKeepFp8) {
+    in_8(g, a.keep_g, a.keep_gs);
+    in_8(u, a.keep_u, a.keep_us);
+  } else if (a.keep == kKeepFull) {
+    in_type(g, a.keep_g);
+    in_type(u, a.keep_u);
   }
 }
 
 // ---- host -------------------------------------------------------------------------------------------------------------------
 
-// The launch of a product of m rows by n (of each weight, if gated) with rows of row_bytes. Every choice of rows to a
-// tile and slices of the reduction is priced, in microseconds, and the cheapest taken: rounds of workgroups over the 256
-// CUs (two at a time of the tiles of 16 and 64 rows, whose stages leave room), each its steps and what a tile costs before
-// its first and after its last, but no less than the operands' bytes at 5.5 TB/s; slices add the second launch and their
-// sums' way to memory and back at 4 TB/s. Measured steps (8192 x 4096 x 16384, and 64 x 4096 x 4096 for 16 rows, all CUs
-// busy), us, [mode][16, 64, 128, 256 rows], and the rest of a tile (from 4096 x 4096 x 4096):
+// The launch of a product of m rows by n (of each weight, if gated) with rows of row_bytes. As many tiles as fill all CUs
+// evenly are a workgroup's each; those left over, too few for a round of their own, can be shared, every workgroup taking
+// the same number of their steps, and joined by a second launch. Every choice of rows to a tile and of a share is priced, in
+// microseconds, and the cheapest taken: rounds of workgroups over the 256 CUs (two at a time of the tiles of 16 and 64
+// rows, whose stages leave room), each its steps and what a tile costs before its first and after its last, but no less
+// than the operands' bytes at 5.5 TB/s; sharing adds the second launch and the shares' sums to memory and back at 4 TB/s.
+// Measured steps (8192 x 4096 x 16384, and 64 x 4096 x 4096 for 16 rows, all CUs busy), us, [mode][16, 64, 128, 256 rows],
+// and the rest of a tile (from 4096 x 4096 x 4096):
 constexpr float kStepUs[][4] = {
     {1.65f, 3.9f, 3.75f, 7.3f},  // kF32
     {1.2f, 1.1f, 0.85f, 1.56f},  // kBf16
@@ -257,55 +274,66 @@ constexpr float kStepUs[][4] = {
     {1.6f, 2.0f, 1.11f, 1.92f},  // kFp8
     {1.1f, 2.2f, 1.55f, 2.8f},   // kSplit
 };
-constexpr float kTileUs[4] = {1.5f, 4.f, 7.f, 13.f};
-constexpr int kBm[4] = {16, 64, 128, 256}, kResident[4] = {2, 2, 1, 1};
+constexpr float kTileUs[4] = {1.5f, 4.f, 7.f, 13.f}, kJoinUs = 4.f;
+constexpr int kCus = 256, kBm[4] = {16, 64, 128, 256}, kResident[4] = {2, 2, 1, 1};
 struct GemmPlan {
-  int bm, gx, gy, steps, slices, slice_steps;
+  int bm, gx, gy, steps, whole, sharers, share;
   float us;
   size_t parts_bytes;
 };
 static GemmPlan plan_gemm(int mode, bool glu, int64_t m, int64_t n, int64_t row_bytes) {
-  const int64_t gx = cdiv(n, glu ? 128 : 256), steps = std::max<int64_t>(cdiv(row_bytes & ~15, 128), 1), sums = m * n * (glu ? 2 : 1);
+  const int64_t gx = cdiv(n, glu ? 128 : 256), steps = std::max<int64_t>(cdiv(row_bytes & ~15, 128), 1);
   const float bytes_us = (float)(m + n * (glu ? 2 : 1)) * (float)row_bytes / 5.5e6f;
   GemmPlan best{};
   best.us = 1e30f;
   for (int v = 0; v < 4; ++v) {
-    const int64_t gy = cdiv(m, kBm[v]);
     if (v > 0 && m <= kBm[v - 1]) break;
-    for (int64_t s = 1; s <= 32 && s * 2 <= std::max<int64_t>(steps, 2); ++s) {
-      const int64_t per = cdiv(steps, s), slices = cdiv(steps, per);
-      if (slices != s) continue;
-      const float rounds = (float)cdiv(gx * gy * s, 256 * kResident[v]);
-      // a workgroup alone on its CU takes about half the step that two take, but no less than a load's way, 0.9
-      const bool alone = kResident[v] == 2 && gx * gy * s <= 256;
-      const float step = alone ? std::max(0.9f, 0.6f * kStepUs[mode][v]) : kStepUs[mode][v];
-      float us = std::max(rounds * (per * step + kTileUs[v]), bytes_us);
-      if (s > 1) us += 4.f + 2.f * s * sums * 4 / 4e6f;
-      if (us < best.us) best = {kBm[v], (int)gx, (int)gy, (int)steps, (int)s, (int)per, us, 0};
-      if (gx * gy * s > 2048) break;
+    const int64_t gy = cdiv(m, kBm[v]), tiles = gx * gy, at_once = kCus * kResident[v], left = tiles % at_once;
+    // a workgroup alone on its CU takes about half the step that two take, but no less than a load's way, 0.9
+    auto step = [&](int64_t groups) {
+      return kResident[v] == 2 && groups <= kCus ? std::max(0.9f, 0.6f * kStepUs[mode][v]) : kStepUs[mode][v];
+    };
+    const float rounds_us = (float)(tiles / at_once) * (steps * kStepUs[mode][v] + kTileUs[v]);
+    auto consider = [&](float us, int64_t whole, int64_t sharers, int64_t share) {
+      us = std::max(us, bytes_us);
+      if (sharers) {  // a share begins a tile, and each tile's first and last shares may belong to two
+        const float sums = (float)(sharers + tiles - whole) * (float)std::min<int64_t>(m, kBm[v]) * 256 * 4;
+        us += kJoinUs + 2 * sums / 4e6f;
+      }
+      if (us < best.us)
+        best = {kBm[v], (int)gx, (int)gy, (int)steps, (int)whole, (int)sharers, (int)share, us,
+                (size_t)sharers * 2 * kBm[v] * 256 * sizeof(float)};
+    };
+    consider(rounds_us + (left ? steps * step(left) + kTileUs[v] : 0.f), tiles, 0, 0);
+    if (!left || steps < 4) continue;
+    for (int64_t k = 1; k <= 32; ++k) {  // a k-th of a tile's steps each, or all CUs' even share
+      const int64_t share = k == 1 ? std::max<int64_t>(cdiv(left * steps, at_once), 2) : cdiv(steps, k);
+      const int64_t sharers = cdiv(left * steps, share);
+      if (share < 2 || share >= steps || sharers > at_once) continue;
+      const float begins = steps % share ? 1.5f : 1.f;  // some shares cover the end of one tile and the start of the next
+      consider(rounds_us + share * step(sharers) + begins * kTileUs[v], tiles - left, sharers, share);
     }
   }
-  if (best.slices > 1) best.parts_bytes = (size_t)best.slices * sums * sizeof(float);
   return best;
 }
 static int run_gemm(int mode, bool glu, const GemmPlan& p, GemmArgs a, void* parts, hipStream_t stream) {
-  a.steps = p.steps, a.slices = p.slices, a.slice_steps = p.slice_steps, a.gx = p.gx, a.gy = p.gy;
+  a.steps = p.steps, a.gx = p.gx, a.gy = p.gy, a.whole = p.whole, a.sharers = p.sharers, a.share = p.share;
   a.parts = (float*)parts;
   int e = mode == kF32 ? ffn_gemm_f32(a, p.bm, stream)
           : mode == kSplit ? ffn_gemm_split(a, glu, p.bm, stream)
           : mode == kBf16 ? ffn_gemm_bf16(a, glu, p.bm, stream)
           : mode == kFp8 ? ffn_gemm_fp8(a, p.bm, stream) : ffn_gemm_fp8x(a, glu, p.bm, stream);
-  if (e || p.slices == 1) return e;
+  if (e || !p.sharers) return e;
   const bool vec = a.n % 8 == 0;
+  const int shared = p.gx * p.gy - p.whole;
+  auto go = [&](auto kernel, int rows) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(shared * (p.bm / rows))), dim3(256), 0, stream, a, p.bm);
+  };
   if (glu) {
-    const dim3 grid(grid1d(a.m * cdiv(a.n, kFp8Block) * 16, 256, 1 << 16));
-    if (vec) hipLaunchKernelGGL(glu_join_kernel<true>, grid, dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL(glu_join_kernel<false>, grid, dim3(256), 0, stream, a);
+    vec ? go(glu_join_kernel<true>, 16) : go(glu_join_kernel<false>, 16);
     return launch_check("glu_join_kernel");
   }
-  const dim3 grid(grid1d(a.m * cdiv(a.n, 8), 256, 1 << 16));
-  if (vec) hipLaunchKernelGGL(ffn_join_kernel<true>, grid, dim3(256), 0, stream, a);
-  else hipLaunchKernelGGL(ffn_join_kernel<false>, grid, dim3(256), 0, stream, a);
+  vec ? go(ffn_join_kernel<true>, 8) : go(ffn_join_kernel<false>, 8);
   return launch_check("ffn_join_kernel");
 }
 
@@ -480,9 +508,10 @@ static int run_lines(int mode, const GemmPlan& p, GemmArgs a, const Lines& x, co
 
 using namespace omt;
 
-OMT_EXPORT int omt_ffn_plan(int op, int dtype, int64_t m, int64_t k, int64_t n, int* mode, int* rows, int* slices) {
+OMT_EXPORT int omt_ffn_plan(int op, int dtype, int64_t m, int64_t k, int64_t n, int* mode, int* rows,
+                            int* sharers) {
   const char* fn = "omt_ffn_plan";
-  if (!mode || !rows || !slices) return fail(OMT_INVALID, "%s: null pointer", fn);
+  if (!mode || !rows || !sharers) return fail(OMT_INVALID, "%s: null pointer", fn);
   if (int e = glu_check(fn, dtype, m, k, n, OMT_GLU_SILU)) return e;
   if (m == 0) return fail(OMT_INVALID, "%s: no rows", fn);
   Space sp{nullptr};
@@ -495,7 +524,7 @@ OMT_EXPORT int omt_ffn_plan(int op, int dtype, int64_t m, int64_t k, int64_t n, 
     case OMT_FFN_GLU_GW: *mode = bwd_mode(dtype), p = GluBwd(sp, *mode, m, k, n).pw; break;
     default: return fail(OMT_INVALID, "%s: op %d", fn, op);
   }
-  *rows = p.bm, *slices = p.slices;
+  *rows = p.bm, *sharers = p.sharers;
   return OMT_OK;
 }
 

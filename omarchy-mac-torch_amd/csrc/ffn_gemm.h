@@ -33,15 +33,28 @@ __device__ __forceinline__ const T* uniform(const T* p) {
   return (const T*)((uint64_t)hi << 32 | lo);
 }
 
+// Tiles in groups of eight rows, the rows fastest within a group.
+__host__ __device__ __forceinline__ TileId tile_at(int t, int gx, int gy) {
+  const int group = t / (8 * gx), y0 = group * 8, rows = gy - y0 < 8 ? gy - y0 : 8, r = t - group * 8 * gx;
+  return {r / rows, y0 + r % rows, 0};
+}
+// The p-th of n workgroups' place among them, so that each XCD (p mod 8) has a run of places.
+__device__ __forceinline__ int xcd_place(int p, int n) {
+  const int per = n / kXCDs;
+  return p < per * kXCDs ? (p % kXCDs) * per + p / kXCDs : p;
+}
+
 struct GemmArgs {
   const void *x, *w, *w_up;           // rows of xpitch / wpitch bytes, a multiple of 4; w_up: the gated form's
   const float *sx, *sw, *sw_up;       // 8 bits: x's scales [m][blocks], w's [ceil(n / 128)][blocks]
   int sx_row, sw_row, sx_step, sw_step;  // floats from a row's scale to the next row's, and to its next step's
   int64_t xpitch, wpitch;
   int m, n, row_bytes, steps;         // n: rows of w (and of w_up); row_bytes: the reduction's length
-  int slices, slice_steps;            // steps of each slice of the reduction; more than one slice: sums go to parts
-  int gx, gy;                         // tiles
-  float* parts;                       // [slices][m][n], gated: [slices][m][2][n]
+  int gx, gy;                         // tiles, in the order of tile_at
+  // The first `whole` of them are a workgroup's each. The others' steps, one tile's after the other's, are cut into shares
+  // of `share` steps for `sharers` workgroups, at most two tiles' to a share, whose sums go to parts and are joined after.
+  int whole, sharers, share;
+  float* parts;                       // [sharers][2][rows of a tile][256]
   void *out, *out2;                   // rows of n; rows of x from split on go to out2
   int split, out_kind;
   // the gated form: out gets act(g) * u, in 8 bits with scales out_scale; keep: what the backward pass needs
@@ -142,11 +155,30 @@ ffn_gemm_kernel(GemmArgs a) {
   static_assert(Tl::LDS >= 2 * 4 * BM * 4, "the epilogue's maxima lie where the stages were");
   __shared__ __attribute__((aligned(128))) unsigned char lds[Tl::LDS];
 
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave >> 2, wn = wave & 3, r16 = lane & 15, g = lane >> 4;
-  const TileId id = xcd_tile(blockIdx.x, a.gx, a.gy, a.slices, 8);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wm = wave >> 2, wn = wave & 3;
+
+  // this workgroup's tile, or its share of the steps of one or two
+  int tile, s0 = 0, todo = a.steps;
+  float* part = nullptr;
+  if ((int)blockIdx.x < a.whole) {
+    tile = xcd_place(blockIdx.x, a.whole);
+  } else {
+    const int w = xcd_place(blockIdx.x - a.whole, a.sharers);
+    const int64_t begin = (int64_t)w * a.share, all = (int64_t)(a.gx * a.gy - a.whole) * a.steps;
+    tile = a.whole + (int)(begin / a.steps);
+    s0 = (int)(begin % a.steps);
+    todo = (int)(all - begin < a.share ? all - begin : a.share);
+    part = a.parts + (int64_t)w * 2 * BM * 256;
+  }
+  while (todo > 0) {
+  // Opaque, so that what follows from it is computed where it is used: taken out of this loop, which mostly runs once, the
+  // addresses of the epilogue would sit in 50 registers through the products.
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  const int r16 = lane & 15, g = lane >> 4;
+  const TileId id = tile_at(tile, a.gx, a.gy);
   const int m0 = id.y * BM, n0 = id.x * NT;
-  const int s0 = id.z * a.slice_steps, s1 = min(a.steps, s0 + a.slice_steps);
+  const int s1 = min(a.steps, s0 + todo);
 
   // where each of this wave's loads reads: a base that advances 128 bytes a step, and the lane's offset from it. Rows
   // past the operand's last read as 0 (an offset out of the range that the load checks).
@@ -226,7 +258,7 @@ ffn_gemm_kernel(GemmArgs a) {
   const bool ragged = MODE != kSplit && whole != a.row_bytes && s1 == a.steps;
   auto lay_rest = [&]() {
     meet(std::integral_constant<int, 0>{});
-    for (int r = threadIdx.x; r < BM + 256; r += Tl::THREADS) {
+    for (int r = wave * 64 + lane; r < BM + 256; r += Tl::THREADS) {
       const bool of_x = r < BM;
       const int w = GLU ? (r - BM) & 127 : r - BM, part = GLU && r - BM >= 128;
       const bool in = of_x ? m0 + r < a.m : n0 + w < a.n;
@@ -411,22 +443,21 @@ ffn_gemm_kernel(GemmArgs a) {
 
   // a lane holds four consecutive columns (4 g ..) of one row (r16) of each 16 x 16 tile
   const bool vec = (a.n & 3) == 0;
-  if (a.slices > 1) {
-    const int64_t width = GLU ? 2 * (int64_t)a.n : a.n;
+  if (part) {
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
-      const int m = m0 + xrow + i * 16 + r16;
-      if (m >= a.m) continue;
-      float* row = a.parts + ((int64_t)id.z * a.m + m) * width;
+      const int row = xrow + i * 16 + r16;
+      if (m0 + row >= a.m) continue;
 #pragma unroll
-      for (int j = 0; j < TJ; ++j) {
-        const int r = wrow(j) + 4 * g;
-        if constexpr (GLU) store4(row + (r >= 128 ? a.n : 0), n0 + (r & 127), a.n, vec, acc[i][j]);
-        else store4(row, n0 + r, a.n, vec, acc[i][j]);
-      }
+      for (int j = 0; j < TJ; ++j) *(f32x4*)(part + row * 256 + wrow(j) + 4 * g) = acc[i][j];
     }
-    return;
+    todo -= s1 - s0;
+    s0 = 0;
+    ++tile;
+    part += BM * 256;
+    continue;
   }
+  todo = 0;
   if constexpr (!GLU) {
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
@@ -519,11 +550,12 @@ ffn_gemm_kernel(GemmArgs a) {
       }
     }
   }
+  }
 }
 
 template <int MODE, bool GLU, int BM, int NS>
 int launch_gemm(const GemmArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL((ffn_gemm_kernel<MODE, GLU, BM, NS>), dim3((unsigned)(a.gx * a.gy * a.slices)),
+  hipLaunchKernelGGL((ffn_gemm_kernel<MODE, GLU, BM, NS>), dim3((unsigned)(a.whole + a.sharers)),
                      dim3(GemmTile<MODE, BM, NS>::THREADS), 0, stream, a);
   return launch_check("ffn_gemm_kernel");
 }

@@ -82,9 +82,9 @@ def test_workspaces_cover_what_they_say(lib):
     assert L.omt_glu_fp8_workspace(4096, 4096, 4096) == 0 and L.omt_matmul_fp8_workspace(4096, 4096, 4096, BF16) == 0
     # rows of an odd number of bytes are copied
     assert L.omt_matmul_fp8_workspace(4096, 4096, 4097, BF16) >= 2 * 4096 * 4112
-    # slices of the reduction: a sum of each
-    _, _, slices = plan(lib, lib.OMT_FFN_MATMUL_FP8, BF16, 1, 8192, 4096)
-    assert slices > 1 and L.omt_matmul_fp8_workspace(1, 4096, 8192, BF16) >= slices * 4096 * 4
+    # shared tiles: each workgroup's sums of two
+    _, rows, sharers = plan(lib, lib.OMT_FFN_MATMUL_FP8, BF16, 1, 8192, 4096)
+    assert sharers > 16 and L.omt_matmul_fp8_workspace(1, 4096, 8192, BF16) >= sharers * 2 * rows * 256 * 4
     # the backward: dg and du twice, the weights and x transposed
     m, k, f = 300, 200, 500
     for dtype, e in ((F32, 4), (BF16, 2)):
@@ -98,8 +98,8 @@ def test_plans_are_within_the_kernels_limits(lib):
         m, k, n = (int(2 ** (float(torch.rand((), generator=g)) * 13)) for _ in range(3))
         for op in range(5):
             for dtype in (F32, BF16):
-                mode, rows, slices = plan(lib, op, dtype, m, k, n)
-                assert rows in (16, 64, 128, 256) and 1 <= slices <= 32 and mode in range(5)
+                mode, rows, sharers = plan(lib, op, dtype, m, k, n)
+                assert rows in (16, 64, 128, 256) and 0 <= sharers <= (256 if rows >= 128 else 512) and mode in range(5)
                 assert rows <= 16 or rows // 4 < max(m, 2 * n if op == lib.OMT_FFN_GLU_GW else m)
 
 
