@@ -265,17 +265,19 @@ __global__ void __launch_bounds__(256) glu_join_kernel(GemmArgs a, int bm) {
 // microseconds, and the cheapest taken: rounds of workgroups over the 256 CUs (two at a time of the tiles of 16 and 64
 // rows, whose stages leave room), each its steps and what a tile costs before its first and after its last, but no less
 // than the operands' bytes at 5.5 TB/s; sharing adds the second launch and the shares' sums to memory and back at 4 TB/s.
-// Measured steps (8192 x 4096 x 16384, and 64 x 4096 x 4096 for 16 rows, all CUs busy), us, [mode][16, 64, 128, 256 rows],
-// and the rest of a tile (from 4096 x 4096 x 4096):
-constexpr float kStepUs[][4] = {
-    {1.65f, 3.9f, 3.75f, 7.3f},  // kF32
-    {1.2f, 1.1f, 0.85f, 1.56f},  // kBf16
-    {2.1f, 2.8f, 1.8f, 3.4f},    // kFp8x
-    {1.6f, 2.0f, 1.11f, 1.92f},  // kFp8
-    {1.1f, 2.2f, 1.55f, 2.8f},   // kSplit
+// Steps, and the rest of a tile, in us, measured with all CUs busy (16384 x 4096 x 4096 and x 8192, the gated form of kF32 at
+// 5120 x 4096 x 1024 and x 2048; 16 rows at 64 x 4096 x 4096), [mode][rows of a tile]:
+constexpr float kStepUs[][kHeights] = {
+    // 16    64    96    128    160    192    224   256
+    {1.65f, 3.55f, 2.8f, 3.72f, 4.55f, 5.45f, 6.35f, 7.15f},   // kF32
+    {1.2f, 1.0f, 0.62f, 0.76f, 0.88f, 1.1f, 1.25f, 1.4f},      // kBf16
+    {2.1f, 2.7f, 1.62f, 1.91f, 2.18f, 2.59f, 2.98f, 3.34f},    // kFp8x
+    {1.6f, 1.71f, 0.92f, 1.05f, 1.26f, 1.42f, 1.67f, 1.92f},   // kFp8
+    {1.1f, 2.35f, 1.25f, 1.5f, 1.82f, 2.1f, 2.48f, 2.8f},      // kSplit
 };
-constexpr float kTileUs[4] = {1.5f, 4.f, 7.f, 13.f}, kJoinUs = 4.f;
-constexpr int kCus = 256, kBm[4] = {16, 64, 128, 256}, kResident[4] = {2, 2, 1, 1};
+constexpr float kTileUs[kHeights] = {1.5f, 8.f, 5.f, 6.5f, 8.f, 8.5f, 10.f, 11.f}, kJoinUs = 4.f;
+constexpr int kCus = 256;
+constexpr int resident(int v) { return kBm[v] <= 64 ? 2 : 1; }
 struct GemmPlan {
   int bm, gx, gy, steps, whole, sharers, share;
   float us;
@@ -286,12 +288,12 @@ static GemmPlan plan_gemm(int mode, bool glu, int64_t m, int64_t n, int64_t row_
   const float bytes_us = (float)(m + n * (glu ? 2 : 1)) * (float)row_bytes / 5.5e6f;
   GemmPlan best{};
   best.us = 1e30f;
-  for (int v = 0; v < 4; ++v) {
+  for (int v = 0; v < kHeights; ++v) {
     if (v > 0 && m <= kBm[v - 1]) break;
-    const int64_t gy = cdiv(m, kBm[v]), tiles = gx * gy, at_once = kCus * kResident[v], left = tiles % at_once;
+    const int64_t gy = cdiv(m, kBm[v]), tiles = gx * gy, at_once = kCus * resident(v), left = tiles % at_once;
     // a workgroup alone on its CU takes about half the step that two take, but no less than a load's way, 0.9
     auto step = [&](int64_t groups) {
-      return kResident[v] == 2 && groups <= kCus ? std::max(0.9f, 0.6f * kStepUs[mode][v]) : kStepUs[mode][v];
+      return resident(v) == 2 && groups <= kCus ? std::max(0.9f, 0.6f * kStepUs[mode][v]) : kStepUs[mode][v];
     };
     const float rounds_us = (float)(tiles / at_once) * (steps * kStepUs[mode][v] + kTileUs[v]);
     auto consider = [&](float us, int64_t whole, int64_t sharers, int64_t share) {

@@ -133,13 +133,13 @@ __device__ __forceinline__ i32x8 join8(omt_u32x4 a, omt_u32x4 b) {
 
 template <int MODE, int BM, int NS>
 struct GemmTile {
-  static constexpr int WM = BM >= 128 ? 2 : 1;        // waves along the rows of x; 4 along the rows of w
+  static constexpr int WM = BM >= 96 ? 2 : 1;        // waves along the rows of x; 4 along the rows of w
   static constexpr int NW = WM * 4, THREADS = NW * 64;
   static constexpr int TI = BM / WM / 16, TJ = 4;      // a wave's 16 x 16 tiles
   static constexpr int XI = BM / 8, DI = XI + 32;      // loads of 8 rows a step
   static constexpr int DW = (DI + NW - 1) / NW;        // ... by each wave (some repeated, so that all waves' counts are one)
   static constexpr bool SCALED = MODE != kF32 && MODE != kBf16;
-  static constexpr int SROWS = BM < 64 ? 64 : BM;
+  static constexpr int SROWS = (BM + 63) / 64 * 64;
   static constexpr int SI = SROWS / 64 + 4;            // loads of 64 scales a step
   static constexpr int SW = SCALED ? (SI + NW - 1) / NW : 0;
   static constexpr int LOADS = DW + SW;
@@ -274,6 +274,7 @@ ffn_gemm_kernel(GemmArgs a) {
       if constexpr (Tl::SCALED) {
         const int64_t block = (a.row_bytes - 1) >> 7;
         float* scales = (float*)(lds + (BM + 256) * 128);
+        // (rows between BM and SROWS are no tile's)
         if (of_x) scales[r] = in ? a.sx[(m0 + r) * (int64_t)a.sx_row + block * a.sx_step] : 0.f;
         else scales[Tl::SROWS + r - BM] = in ? (part ? a.sw_up : a.sw)[((n0 + w) >> 7) * (int64_t)a.sw_row + block * a.sw_step] : 0.f;
       }
@@ -560,17 +561,21 @@ int launch_gemm(const GemmArgs& a, hipStream_t stream) {
   return launch_check("ffn_gemm_kernel");
 }
 
-// bm rows of x to a tile: 16, 64, 128 or 256 (a.gx, a.gy in those units). Two stages: two workgroups of the small tiles
-// fit a CU's 160 KB together and hide each other's waits better than a third stage does (64 rows bf16, 4096 x 4096 x
-// 4096: 144 us with two, 226 with three and one workgroup); 128 rows gain 1-3% from a third where it fits.
-template <int MODE, bool GLU>
+// Two stages, or three where they fit the CU's 160 KB: two workgroups of the small tiles fit it together and hide each
+// other's waits better than a third stage does (64 rows bf16, 4096 x 4096 x 4096: 144 us with two, 226 with three and one
+// workgroup); 128 rows gain 1-3% from a third.
+template <int MODE, int BM>
+constexpr int gemm_stages() {
+  return BM > 64 && 3 * GemmTile<MODE, BM, 1>::STAGE <= 160 * 1024 ? 3 : 2;
+}
+// bm rows of x to a tile (a.gx, a.gy in those units). The heights between 64 and 256 are there for the rows that a whole
+// number of tiles leaves over, and the CUs: 777 rows by 20 columns of tiles are 140 workgroups of 128 rows, 180 of 96.
+constexpr int kHeights = 8, kBm[kHeights] = {16, 64, 96, 128, 160, 192, 224, 256};
+template <int MODE, bool GLU, int V = 0>
 int launch_gemm_of(const GemmArgs& a, int bm, hipStream_t stream) {
-  switch (bm) {
-    case 16: return launch_gemm<MODE, GLU, 16, 2>(a, stream);
-    case 64: return launch_gemm<MODE, GLU, 64, 2>(a, stream);
-    case 128: return launch_gemm<MODE, GLU, 128, 3>(a, stream);
-    default: return launch_gemm<MODE, GLU, 256, 2>(a, stream);
-  }
+  if constexpr (V + 1 < kHeights)
+    if (bm != kBm[V]) return launch_gemm_of<MODE, GLU, V + 1>(a, bm, stream);
+  return launch_gemm<MODE, GLU, kBm[V], gemm_stages<MODE, kBm[V]>()>(a, stream);
 }
 // kF32 in the gated form only, kFp8 in the plain one only
 int ffn_gemm_f32(const GemmArgs& a, int bm, hipStream_t stream);

@@ -99,8 +99,23 @@ def test_plans_are_within_the_kernels_limits(lib):
         for op in range(5):
             for dtype in (F32, BF16):
                 mode, rows, sharers = plan(lib, op, dtype, m, k, n)
-                assert rows in (16, 64, 128, 256) and 0 <= sharers <= (256 if rows >= 128 else 512) and mode in range(5)
-                assert rows <= 16 or rows // 4 < max(m, 2 * n if op == lib.OMT_FFN_GLU_GW else m)
+                assert rows in (16, 64, 96, 128, 160, 192, 224, 256) and mode in range(5)
+                assert 0 <= sharers <= (256 if rows > 64 else 512)
+                assert rows <= 16 or rows // 4 < (2 * n if op == lib.OMT_FFN_GLU_GW else m)
+
+
+def test_the_tested_sizes_reach_the_tiles(lib):
+    """Three quarters at least of the combinations (operator, mode, rows of a tile, shared or not) that random sizes lead to
+    are among those of the sizes that the GPU tests run."""
+    import test_gpu_ffn
+    def kind(op, *size):
+        mode, rows, sharers = plan(lib, op, *size)
+        return op, mode, rows, sharers > 0
+    tested = {kind(*p) for p in test_gpu_ffn.PLANS}
+    g = torch.Generator().manual_seed(1)
+    met = {kind(op, dtype, *(int(8 * 2 ** (float(torch.rand((), generator=g)) * 9)) for _ in range(3)))
+           for _ in range(1000) for op in range(5) for dtype in (F32, BF16)}
+    assert len(met & tested) >= 0.75 * len(met), sorted(met - tested)
 
 
 def test_operators_refuse_cpu_tensors():
