@@ -272,8 +272,8 @@ constexpr float kStepUs[][kHeights] = {
     {1.65f, 3.55f, 2.8f, 3.72f, 4.55f, 5.45f, 6.35f, 7.15f},   // kF32
     {1.2f, 1.0f, 0.62f, 0.76f, 0.88f, 1.1f, 1.25f, 1.4f},      // kBf16
     {2.1f, 2.7f, 1.62f, 1.91f, 2.18f, 2.59f, 2.98f, 3.34f},    // kFp8x
-    {1.6f, 1.71f, 0.92f, 1.05f, 1.26f, 1.42f, 1.67f, 1.92f},   // kFp8
-    {1.1f, 2.35f, 1.25f, 1.5f, 1.82f, 2.1f, 2.48f, 2.8f},      // kSplit
+    {1.6f, 1.6f, 0.86f, 1.02f, 1.2f, 1.32f, 1.55f, 1.85f},     // kFp8
+    {1.1f, 2.3f, 1.16f, 1.4f, 1.68f, 1.95f, 2.3f, 2.7f},       // kSplit
 };
 constexpr float kTileUs[kHeights] = {1.5f, 8.f, 5.f, 6.5f, 8.f, 8.5f, 10.f, 11.f}, kJoinUs = 4.f;
 constexpr int kCus = 256;

@@ -345,97 +345,142 @@ ffn_gemm_kernel(GemmArgs a) {
       multiply(0);
     }
   } else {
-    auto compute = [&](int buf) {
-      const unsigned char* xs = lds + buf * Tl::STAGE + xrow * 128;
-      const unsigned char* ws = lds + buf * Tl::STAGE + BM * 128;
-      // a block's sum, then times both scales, onto the sum of the blocks
-      const float* sx = (const float*)(lds + buf * Tl::STAGE + (BM + 256) * 128) + xrow + r16;
-      const float* sw = (const float*)(lds + buf * Tl::STAGE + (BM + 256) * 128) + Tl::SROWS;
-      constexpr int KQ = MODE == kFp8x ? 4 : 2;
-      auto fragments = [&](omt_u32x4* f, const unsigned char* row) {
-        const omt_u32x4 lo = chunk(row + frag), hi = chunk(row + (frag ^ 64));
-        if constexpr (MODE == kFp8x) {
-          f[0] = widen_fp8(lo[0], lo[1]), f[1] = widen_fp8(lo[2], lo[3]);
-          f[2] = widen_fp8(hi[0], hi[1]), f[3] = widen_fp8(hi[2], hi[3]);
-        } else {
-          f[0] = lo, f[1] = hi;
-        }
-      };
-      omt_u32x4 wv[TJ][KQ];
-      using Scale = std::conditional_t<MODE == kSplit, f32x4, float>;
-      Scale ws4[TJ];
-#pragma unroll
-      for (int j = 0; j < TJ; ++j) {
-        fragments(wv[j], ws + wrow(j) * 128);
-        if constexpr (MODE == kSplit) ws4[j] = *(const f32x4*)(sw + wrow(j) + 4 * g);
-        else ws4[j] = sw[wrow(j)];  // one block of 128 rows
-      }
-      auto products = [&](f32x4* part, const omt_u32x4* xv) {
-#pragma unroll
-        for (int j = 0; j < TJ; ++j) part[j] = f32x4{};
-        if constexpr (MODE == kFp8x) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q)
-#pragma unroll
-            for (int j = 0; j < TJ; ++j)
-              part[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[j][q]),
-                                                                __builtin_bit_cast(bf16x8, xv[q]), part[j], 0, 0, 0);
-        } else if constexpr (MODE == kFp8) {
-#pragma unroll
-          for (int j = 0; j < TJ; ++j)
-            part[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join8(wv[j][0], wv[j][1]), join8(xv[0], xv[1]),
-                                                                       part[j], 0, 0, 0, 0, 0, 0);
-        } else {  // high by low, low by high, high by high
-#pragma unroll
-          for (int q = 0; q < 3; ++q)
-#pragma unroll
-            for (int j = 0; j < TJ; ++j)
-              part[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, wv[j][q == 1]),
-                                                               __builtin_bit_cast(f16x8, xv[q == 0]), part[j], 0, 0, 0);
-        }
-      };
-      auto scaled = [&](f32x4* a4, const f32x4* part, float xscale) {
-#pragma unroll
-        for (int j = 0; j < TJ; ++j) a4[j] += part[j] * (ws4[j] * xscale);
-      };
-      if constexpr (MODE == kFp8x) {  // its fragments take four times the registers: one row of tiles at a time
-#pragma unroll
-        for (int i = 0; i < TI; ++i) {
-          omt_u32x4 xv[KQ];
-          f32x4 part[TJ];
-          fragments(xv, xs + i * 2048);
-          products(part, xv);
-          scaled(acc[i], part, sx[i * 16]);
-        }
+    // a block's sum, then times both scales, onto the sum of the blocks
+    constexpr int KQ = MODE == kFp8x ? 4 : 2;
+    using Scale = std::conditional_t<MODE == kSplit, f32x4, float>;
+    omt_u32x4 wv[TJ][KQ];
+    Scale wscale[TJ];
+    float xscale[TI];
+    auto fragments = [&](omt_u32x4* f, const unsigned char* row) {
+      const omt_u32x4 lo = chunk(row + frag), hi = chunk(row + (frag ^ 64));
+      if constexpr (MODE == kFp8x) {
+        f[0] = widen_fp8(lo[0], lo[1]), f[1] = widen_fp8(lo[2], lo[3]);
+        f[2] = widen_fp8(hi[0], hi[1]), f[3] = widen_fp8(hi[2], hi[3]);
       } else {
-        // one row of tiles ahead: its products run while the sums of the last are scaled (8192 x 4096 x 16384: e4m3 550 ->
-        // 492 us, halves 2955 -> 2850)
-        omt_u32x4 xv[2][KQ];
-        f32x4 part[2][TJ];
-        fragments(xv[0], xs);
-        if (TI > 1) fragments(xv[1], xs + 2048);
-        products(part[0], xv[0]);
-#pragma unroll
-        for (int i = 0; i < TI; ++i) {
-          if (i + 2 < TI) fragments(xv[i & 1], xs + (i + 2) * 2048);
-          if (i + 1 < TI) products(part[(i + 1) & 1], xv[(i + 1) & 1]);
-          scaled(acc[i], part[i & 1], sx[i * 16]);
-        }
+        f[0] = lo, f[1] = hi;
       }
     };
+    auto read_x = [&](omt_u32x4* f, int buf, int i) { fragments(f, lds + buf * Tl::STAGE + (xrow + i * 16) * 128); };
+    auto read_w = [&](int buf) {
 #pragma unroll
-    for (int p = 0; p < NS - 1; ++p) issue(p, s0 + p);
-    int cur = 0, nxt = NS - 1;
-    for (int s = s0; s < s1; ++s) {
-      meet(std::integral_constant<int, NS - 2>{});
-      issue(nxt, s + NS - 1);
-      compute(cur);
-      cur = cur + 1 == NS ? 0 : cur + 1;
-      nxt = nxt + 1 == NS ? 0 : nxt + 1;
+      for (int j = 0; j < TJ; ++j) fragments(wv[j], lds + buf * Tl::STAGE + (BM + wrow(j)) * 128);
+    };
+    auto read_xscale = [&](int buf, int i) {
+      xscale[i] = ((const float*)(lds + buf * Tl::STAGE + (BM + 256) * 128))[xrow + i * 16 + r16];
+    };
+    auto read_wscales = [&](int buf) {
+      const float* sw = (const float*)(lds + buf * Tl::STAGE + (BM + 256) * 128) + Tl::SROWS;
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) {
+        if constexpr (MODE == kSplit) wscale[j] = *(const f32x4*)(sw + wrow(j) + 4 * g);
+        else wscale[j] = sw[wrow(j)];  // one block of 128 rows
+      }
+    };
+    auto products = [&](f32x4* part, const omt_u32x4* xv) {
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) part[j] = f32x4{};
+      if constexpr (MODE == kFp8x) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+          for (int j = 0; j < TJ; ++j)
+            part[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[j][q]),
+                                                              __builtin_bit_cast(bf16x8, xv[q]), part[j], 0, 0, 0);
+      } else if constexpr (MODE == kFp8) {
+#pragma unroll
+        for (int j = 0; j < TJ; ++j)
+          part[j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(join8(wv[j][0], wv[j][1]), join8(xv[0], xv[1]),
+                                                                     part[j], 0, 0, 0, 0, 0, 0);
+      } else {  // high by low, low by high, high by high
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+#pragma unroll
+          for (int j = 0; j < TJ; ++j)
+            part[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, wv[j][q == 1]),
+                                                             __builtin_bit_cast(f16x8, xv[q == 0]), part[j], 0, 0, 0);
+      }
+    };
+    auto scaled = [&](int i, const f32x4* part) {
+#pragma unroll
+      for (int j = 0; j < TJ; ++j) acc[i][j] += part[j] * (wscale[j] * xscale[i]);
+    };
+    auto row_by_row = [&](int buf) {
+      read_w(buf);
+      read_wscales(buf);
+#pragma unroll
+      for (int i = 0; i < TI; ++i) {
+        omt_u32x4 xv[KQ];
+        f32x4 part[TJ];
+        read_x(xv, buf, i);
+        read_xscale(buf, i);
+        products(part, xv);
+        scaled(i, part);
+      }
+    };
+    // A row of tiles ahead: its products run while the sums of the last are scaled (8192 x 4096 x 16384 at 256 rows: e4m3 550
+    // -> 492 us, halves 2955 -> 2850). xv and wv hold the step's first fragments; `meet_here` is called before the last
+    // row's products, when all of the step is in registers, `then` after them.
+    omt_u32x4 xv[2][KQ];
+    auto read_first = [&](int buf) {
+      read_w(buf);
+      read_x(xv[0], buf, 0);
+      if (TI > 1) read_x(xv[1], buf, 1);
+    };
+    auto rows_ahead = [&](int buf, auto meet_here, auto then) {
+      f32x4 part[2][TJ];
+      read_wscales(buf);
+#pragma unroll
+      for (int i = 0; i < TI; ++i) read_xscale(buf, i);
+      products(part[0], xv[0]);
+#pragma unroll
+      for (int i = 0; i < TI; ++i) {
+        constexpr int kLast = TI > 1 ? TI - 2 : 0;
+        if (i + 2 < TI) read_x(xv[i & 1], buf, i + 2);
+        if (i == kLast) meet_here();
+        if (i + 1 < TI) products(part[(i + 1) & 1], xv[(i + 1) & 1]);
+        if (i == kLast) then();
+        scaled(i, part[i & 1]);
+      }
+    };
+    if constexpr (MODE == kFp8x || BM == 256) {
+      // the widened fragments take four times the registers, and 256 rows leave none: a step's first reads wait for the waves
+      // to meet
+#pragma unroll
+      for (int p = 0; p < NS - 1; ++p) issue(p, s0 + p);
+      int cur = 0, nxt = NS - 1;
+      for (int s = s0; s < s1; ++s) {
+        meet(std::integral_constant<int, NS - 2>{});
+        issue(nxt, s + NS - 1);
+        if constexpr (MODE == kFp8x) {
+          row_by_row(cur);
+        } else {
+          read_first(cur);
+          rows_ahead(cur, [] {}, [] {});
+        }
+        cur = cur + 1 == NS ? 0 : cur + 1;
+        nxt = nxt + 1 == NS ? 0 : nxt + 1;
+      }
+    } else {
+      // the next step's first reads in the shadow of the last row's products (8192 x 4096 x 8192 at 128 rows: e4m3 312 -> 298
+      // us, halves 1675 -> 1567)
+#pragma unroll
+      for (int p = 0; p < NS; ++p) issue(p, s0 + p);
+      meet(std::integral_constant<int, NS - 1>{});
+      read_first(0);
+      int cur = 0;
+      for (int s = s0; s < s1; ++s) {
+        const int nxt = cur + 1 == NS ? 0 : cur + 1;
+        rows_ahead(cur, [&] { meet(std::integral_constant<int, NS - 2>{}); },
+                   [&] {
+                     read_first(nxt);
+                     issue(cur, s + NS);
+                   });
+        cur = nxt;
+      }
     }
     if (ragged) {
       lay_rest();
-      compute(0);
+      row_by_row(0);
     }
   }
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0) & ~0xF00);
