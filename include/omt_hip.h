@@ -659,7 +659,8 @@ int omt_glu_fwd(int dtype, int64_t m, int64_t k, int64_t f, int act, int keep, c
                 const void* w_up, void* h, void* x_q, float* x_scale, void* g, float* g_scale, void* u, float* u_scale,
                 void* workspace, size_t workspace_bytes, void* stream);
 /* The gradients of x (gx), w_gate and w_up (each may be null) from gh, the gradient of h, and what the forward pass
- * kept: OMT_KEEP_FP8 or, with x in x and no scales, OMT_KEEP_FULL. The workspace on 16 bytes. */
+ * kept: OMT_KEEP_FP8 or, with x in x and no scales, OMT_KEEP_FULL. x, the weights, the gradients and the workspace on 16
+ * bytes. */
 size_t omt_glu_bwd_workspace(int dtype, int64_t m, int64_t k, int64_t f);
 int omt_glu_bwd(int dtype, int64_t m, int64_t k, int64_t f, int act, int keep, const void* gh, const void* x,
                 const float* x_scale, const void* g, const float* g_scale, const void* u, const float* u_scale,

@@ -56,7 +56,8 @@ struct GemmArgs {
   int whole, sharers, share;
   float* parts;                       // [sharers][2][rows of a tile][256]
   void *out, *out2;                   // rows of n; rows of x from split on go to out2
-  int split, out_kind;
+  int split, limit, out_kind;         // rows of out, and of out2, from limit on are no one's
+  int t_rows, up_step;                // operands with the reduction along their columns: rows of each, see below
   // the gated form: out gets act(g) * u, in 8 bits with scales out_scale; keep: what the backward pass needs
   int act, keep;
   float* out_scale;
@@ -147,10 +148,16 @@ struct GemmTile {
   static constexpr int LDS = NS * STAGE;
 };
 
-template <int MODE, bool GLU, int BM, int NS>
+// XT, WT (kBf16): x, or w, lies with the reduction along its columns, [reduction][m] or [reduction][n], a multiple of 8
+// columns and rows on 16 bytes. Its stages are 64 rows of the reduction; the LDS reads that transpose 4 x 16 elements give
+// the matrix instructions what they take. A row's 16-byte chunk c lies at c ^ 2 (row & 3): the four rows of such a read
+// would share their banks. w may be two matrices one after the other along the reduction, w and from step up_step w_up.
+template <int MODE, bool GLU, int BM, int NS, bool XT, bool WT>
 __global__ void __launch_bounds__((GemmTile<MODE, BM, NS>::THREADS), (GemmTile<MODE, BM, NS>::NW / 4))
 ffn_gemm_kernel(GemmArgs a) {
   using Tl = GemmTile<MODE, BM, NS>;
+  static_assert(!(XT || WT) || (MODE == kBf16 && !GLU), "transposed operands: bfloat16, plain");
+  static_assert(!XT || BM == 128 || BM == 256, "a row of x's stage: 16 or 32 chunks");
   constexpr int TI = Tl::TI, TJ = Tl::TJ, NT = GLU ? 128 : 256;
   static_assert(Tl::LDS >= 2 * 4 * BM * 4, "the epilogue's maxima lie where the stages were");
   __shared__ __attribute__((aligned(128))) unsigned char lds[Tl::LDS];
@@ -189,7 +196,13 @@ ffn_gemm_kernel(GemmArgs a) {
   for (int t = 0; t < Tl::DW; ++t) {
     const int slot = min(wave + Tl::NW * t, Tl::DI - 1);
     ddst[t] = slot * 1024;
-    if (slot < Tl::XI) {
+    if ((XT && slot < Tl::XI) || (WT && slot >= Tl::XI)) {
+      const bool of_x = slot < Tl::XI;
+      const int row_size = of_x ? BM * 2 : 512, at = (of_x ? slot : slot - Tl::XI) * 1024 + lane * 16;
+      const int k = at / row_size, c = (at % row_size / 16) ^ ((k & 3) * 2);
+      dbase[t] = of_x ? (const unsigned char*)a.x + m0 * 2 : (const unsigned char*)a.w + n0 * 2;
+      doff[t] = c * 8 < (of_x ? a.m - m0 : a.n - n0) ? (uint32_t)k * (uint32_t)(of_x ? a.xpitch : a.wpitch) + c * 16 : kOOB;
+    } else if (slot < Tl::XI) {
       const int r = slot * 8 + (lane >> 3);
       dbase[t] = (const unsigned char*)a.x + m0 * a.xpitch;
       doff[t] = m0 + r < a.m ? (uint32_t)r * (uint32_t)a.xpitch + chunk16 : kOOB;
@@ -228,9 +241,24 @@ ffn_gemm_kernel(GemmArgs a) {
     const uint32_t left = s < s1 && s * 128 < whole ? (uint32_t)(whole - s * 128) : 0u;
     const bool in = chunk16 < left;
 #pragma unroll
-    for (int t = 0; t < Tl::DW; ++t)
+    for (int t = 0; t < Tl::DW; ++t) {
+      if constexpr (XT || WT) {
+        const int slot = min(wave + Tl::NW * t, Tl::DI - 1);
+        const bool of_x = slot < Tl::XI;
+        if (of_x ? XT : WT) {
+          const int row_size = of_x ? BM * 2 : 512, k = ((of_x ? slot : slot - Tl::XI) * 1024 + lane * 16) / row_size;
+          const bool second = !of_x && s >= a.up_step;
+          const int row = (second ? s - a.up_step : s) * 64;
+          const unsigned char* p = second ? (const unsigned char*)a.w_up + n0 * 2 : dbase[t];
+          const bool there = s < s1 && row + k < a.t_rows;
+          lds_load_b128(rsrc_words(uniform(p + row * (of_x ? a.xpitch : a.wpitch)), 0x7fffffffu),
+                        __builtin_amdgcn_readfirstlane(at + ddst[t]), there ? doff[t] : kOOB);
+          continue;
+        }
+      }
       lds_load_b128(rsrc_words(uniform(dbase[t] + (int64_t)s * 128), 0x7fffffffu),
                     __builtin_amdgcn_readfirstlane(at + ddst[t]), in ? doff[t] : kOOB);
+    }
     if constexpr (Tl::SCALED) {
 #pragma unroll
       for (int t = 0; t < Tl::SW; ++t)
@@ -255,7 +283,7 @@ ffn_gemm_kernel(GemmArgs a) {
 
   // The last one to three words of rows that are no multiple of 16 bytes, as a step of their own after the others, zeros
   // beside them: laid into stage 0 by hand, with their block's scales. (In the loop they cost it 6%.)
-  const bool ragged = MODE != kSplit && whole != a.row_bytes && s1 == a.steps;
+  const bool ragged = MODE != kSplit && !XT && whole != a.row_bytes && s1 == a.steps;
   auto lay_rest = [&]() {
     meet(std::integral_constant<int, 0>{});
     for (int r = wave * 64 + lane; r < BM + 256; r += Tl::THREADS) {
@@ -285,13 +313,33 @@ ffn_gemm_kernel(GemmArgs a) {
   // kF32, kBf16: a step in two halves, each of them its products while the next half's chunks come from LDS
   if constexpr (!Tl::SCALED) {
     omt_u32x4 wv[2][TJ], xv[2][TI];
+    // Columns from + 16 i.. of a stage with the reduction along its columns: a lane's eight of the reduction (32 kk + 8 g ..)
+    // for column r16. In a transposing read of a group of 16 lanes, lane p gives four columns (4 (p & 3) ..) of row p / 4 and
+    // gets four rows of column p.
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4* LdsQuad;
+    const int turn = (r16 >> 2) * 2, quad = ((r16 >> 1) & 1) * 16 + (r16 & 1) * 8;
+    auto across = [&](unsigned char* stage, int row_size, int from, int i, int kk) {
+      unsigned char* p = stage + (kk * 32 + g * 8 + (r16 >> 2)) * row_size + (from + i / 4 * 64) * 2 +
+                         (((i % 4) * 2) ^ turn) * 16 + quad;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad)p);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsQuad)(p + 4 * row_size));
+      const uint2 l = __builtin_bit_cast(uint2, lo), h = __builtin_bit_cast(uint2, hi);
+      return omt_u32x4{l.x, l.y, h.x, h.y};
+    };
     auto read = [&](int buf, int kk) {
       const unsigned char* xs = lds + buf * Tl::STAGE + xrow * 128 + (frag ^ (kk * 64));
       const unsigned char* ws = lds + buf * Tl::STAGE + BM * 128 + (frag ^ (kk * 64));
 #pragma unroll
-      for (int j = 0; j < TJ; ++j) wv[kk][j] = chunk(ws + wrow(j) * 128);
+      for (int j = 0; j < TJ; ++j) {
+        if constexpr (WT) wv[kk][j] = across(lds + buf * Tl::STAGE + BM * 128, 512, wn * 64, j, kk);
+        else wv[kk][j] = chunk(ws + wrow(j) * 128);
+      }
 #pragma unroll
-      for (int i = 0; i < TI; ++i) xv[kk][i] = chunk(xs + i * 2048);
+      for (int i = 0; i < TI; ++i) {
+        if constexpr (XT) xv[kk][i] = across(lds + buf * Tl::STAGE, BM * 2, xrow, i, kk);
+        else xv[kk][i] = chunk(xs + i * 2048);
+      }
     };
     auto multiply = [&](int kk) {
 #pragma unroll
@@ -311,7 +359,7 @@ ffn_gemm_kernel(GemmArgs a) {
     };
     // a read, then the products that hide it
     auto blend = [&]() {
-      constexpr int kReads = TI + TJ, kMfma = TI * TJ * (MODE == kF32 ? 4 : 1), kEach = kMfma / kReads;
+      constexpr int kReads = TI * (XT ? 2 : 1) + TJ * (WT ? 2 : 1), kMfma = TI * TJ * (MODE == kF32 ? 4 : 1), kEach = kMfma / kReads;
 #pragma unroll
       for (int r = 0; r < kReads; ++r) {
         __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
@@ -508,10 +556,11 @@ ffn_gemm_kernel(GemmArgs a) {
 #pragma unroll
     for (int i = 0; i < TI; ++i) {
       const int m = m0 + xrow + i * 16 + r16;
-      if (m >= a.m) continue;
+      const int row = m < a.split ? m : m - a.split;
+      if (m >= a.m || row >= a.limit) continue;
 #pragma unroll
       for (int j = 0; j < TJ; ++j)
-        store4_any(m < a.split ? a.out : a.out2, m < a.split ? m : m - a.split, n0 + wrow(j) + 4 * g, a.n, vec,
+        store4_any(m < a.split ? a.out : a.out2, row, n0 + wrow(j) + 4 * g, a.n, vec,
                    a.out_kind, acc[i][j]);
     }
   } else {
@@ -599,9 +648,9 @@ ffn_gemm_kernel(GemmArgs a) {
   }
 }
 
-template <int MODE, bool GLU, int BM, int NS>
+template <int MODE, bool GLU, int BM, int NS, bool XT = false, bool WT = false>
 int launch_gemm(const GemmArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL((ffn_gemm_kernel<MODE, GLU, BM, NS>), dim3((unsigned)(a.whole + a.sharers)),
+  hipLaunchKernelGGL((ffn_gemm_kernel<MODE, GLU, BM, NS, XT, WT>), dim3((unsigned)(a.whole + a.sharers)),
                      dim3(GemmTile<MODE, BM, NS>::THREADS), 0, stream, a);
   return launch_check("ffn_gemm_kernel");
 }
@@ -616,12 +665,15 @@ constexpr int gemm_stages() {
 // bm rows of x to a tile (a.gx, a.gy in those units). The heights between 64 and 256 are there for the rows that a whole
 // number of tiles leaves over, and the CUs: 777 rows by 20 columns of tiles are 140 workgroups of 128 rows, 180 of 96.
 constexpr int kHeights = 8, kBm[kHeights] = {16, 64, 96, 128, 160, 192, 224, 256};
-template <int MODE, bool GLU, int V = 0>
+template <int MODE, bool GLU, bool WT = false, int V = 0>
 int launch_gemm_of(const GemmArgs& a, int bm, hipStream_t stream) {
   if constexpr (V + 1 < kHeights)
-    if (bm != kBm[V]) return launch_gemm_of<MODE, GLU, V + 1>(a, bm, stream);
-  return launch_gemm<MODE, GLU, kBm[V], gemm_stages<MODE, kBm[V]>()>(a, stream);
+    if (bm != kBm[V]) return launch_gemm_of<MODE, GLU, WT, V + 1>(a, bm, stream);
+  return launch_gemm<MODE, GLU, kBm[V], gemm_stages<MODE, kBm[V]>(), false, WT>(a, stream);
 }
+// kBf16, plain, with w, or both operands, along their columns (the latter: 128 or 256 rows)
+int ffn_gemm_bf16_w(const GemmArgs& a, int bm, hipStream_t stream);
+int ffn_gemm_bf16_xw(const GemmArgs& a, int bm, hipStream_t stream);
 // kF32 in the gated form only, kFp8 in the plain one only
 int ffn_gemm_f32(const GemmArgs& a, int bm, hipStream_t stream);
 int ffn_gemm_bf16(const GemmArgs& a, bool glu, int bm, hipStream_t stream);
