@@ -455,9 +455,16 @@ PLANS = [
     (4, 0, 1, 1373, 3436), (4, 0, 4869, 2892, 644), (4, 0, 1, 1422, 4103), (4, 0, 3449, 1613, 4089),
     (4, 0, 1, 1648, 4162), (4, 0, 3920, 4310, 2409),
 ]
+# the same for the bfloat16 gradients whose products run across the reduction (k and n multiples of 8)
+ACROSS = [
+    (3, 2, 1, 8, 8), (3, 2, 1, 8, 200), (3, 2, 17, 4296, 4184), (3, 2, 4230, 8, 144), (3, 2, 1034, 8, 1008),
+    (3, 2, 3096, 1800, 8), (3, 2, 113, 1112, 2920), (3, 2, 4974, 1592, 8), (3, 2, 3136, 3120, 8), (3, 2, 4500, 2696, 8),
+    (3, 2, 4292, 3192, 8), (3, 2, 4783, 3504, 3008), (4, 2, 449, 8, 8), (4, 2, 1, 864, 4176), (4, 2, 1739, 2496, 3296),
+    (4, 2, 65, 264, 72), (3, 2, 200, 264, 72), (4, 2, 4096, 128, 512),
+]
 
 
-@pytest.mark.parametrize("op,dtype,m,k,n", PLANS)
+@pytest.mark.parametrize("op,dtype,m,k,n", PLANS + ACROSS)
 def test_every_tile(ops, cuda, op, dtype, m, k, n):
     import ctypes
     from omarchy_mac_torch import _lib
