@@ -668,8 +668,9 @@ int omt_glu_bwd(int dtype, int64_t m, int64_t k, int64_t f, int act, int keep, c
                 size_t workspace_bytes, void* stream);
 /* How a product of these operators runs: m rows, a reduction of k (for the gradients: the block's k), n outputs (the
  * block's f), dtype the result's (OMT_FFN_MATMUL_FP8) or the operands'. mode: 0 float32 matrix instructions, 1 bfloat16, 2
- * e4m3 widened to bfloat16, 3 e4m3, 4 float32 as float16 halves; rows of x to a tile; workgroups that share the steps of
- * tiles (0: a workgroup to each tile). */
+ * e4m3 widened to bfloat16, 3 e4m3, 4 float32 as float16 halves, 5 e4m3 widened to bfloat16 and a workgroup to a few rows
+ * of the weight over the whole reduction; rows of x to a tile; workgroups that share the steps of tiles (0: a workgroup to
+ * each tile). */
 enum { OMT_FFN_MATMUL_FP8 = 0, OMT_FFN_GLU = 1, OMT_FFN_GLU_FP8 = 2, OMT_FFN_GLU_GX = 3, OMT_FFN_GLU_GW = 4 };
 int omt_ffn_plan(int op, int dtype, int64_t m, int64_t k, int64_t n, int* mode, int* rows, int* sharers);
 

@@ -13,7 +13,7 @@
 // take 57 us for dg and du, 72 for the weights and 25 for x; a product across costs 0 to 3% more than one along.
 #include <algorithm>
 
-#include "ffn_gemm.h"
+#include "ffn_few.h"
 
 namespace omt {
 
@@ -459,12 +459,16 @@ static int need_space(const char* fn, size_t need, const void* ws, size_t bytes)
 // the same values are 1e-8 off): nothing beside a bfloat16 result's 2^-9, too much for a float32 one.
 static int fp8_mode(int out_dtype) { return out_dtype == OMT_DT_BF16 ? kFp8 : kFp8x; }
 struct MatmulFp8 {
+  int few, mode;
   Lines a, b;
-  GemmPlan p;
-  void* parts;
-  MatmulFp8(Space& sp, int mode, int64_t m, int64_t n, int64_t k)
-      : a(place_rows(sp, mode, m, k)), b(place_rows(sp, mode, n, k)), p(plan_gemm(mode, false, m, n, a.pitch)),
-        parts(sp.take(p.parts_bytes)) {}
+  GemmPlan p{};
+  void* parts = nullptr;
+  MatmulFp8(Space& sp, int out_dtype, int64_t m, int64_t n, int64_t k)
+      : few(few_rows(m, n, k)), mode(fp8_mode(out_dtype)), a(place_rows(sp, mode, m, k)), b(place_rows(sp, mode, n, k)) {
+    if (few) return;
+    p = plan_gemm(mode, false, m, n, a.pitch);
+    parts = sp.take(p.parts_bytes);
+  }
 };
 // float32: on fp32 MFMA as it is, or as halves on float16 MFMA, three products for one. Laying out the halves reads and
 // writes the operands once (4 TB/s, three launches); it is taken where the products win that back.
@@ -549,7 +553,12 @@ OMT_EXPORT int omt_ffn_plan(int op, int dtype, int64_t m, int64_t k, int64_t n, 
   Space sp{nullptr};
   GemmPlan p;
   switch (op) {
-    case OMT_FFN_MATMUL_FP8: *mode = fp8_mode(dtype), p = MatmulFp8(sp, *mode, m, n, k).p; break;
+    case OMT_FFN_MATMUL_FP8: {
+      const MatmulFp8 l(sp, dtype, m, n, k);
+      *mode = l.few ? 5 : l.mode, p = l.p;
+      if (l.few) p.bm = l.few;
+      break;
+    }
     case OMT_FFN_GLU: *mode = glu_mode(dtype, m, k, n), p = GluFwd(sp, *mode, m, k, n).p; break;
     case OMT_FFN_GLU_FP8: *mode = kFp8x, p = GluFwd(sp, kFp8x, m, k, n).p; break;
     case OMT_FFN_GLU_GX: *mode = bwd_mode(dtype), p = GluBwd(sp, *mode, m, k, n).px; break;
@@ -563,7 +572,7 @@ OMT_EXPORT int omt_ffn_plan(int op, int dtype, int64_t m, int64_t k, int64_t n, 
 OMT_EXPORT size_t omt_matmul_fp8_workspace(int64_t m, int64_t n, int64_t k, int out_dtype) {
   if (product_check("omt_matmul_fp8_workspace", m, n, k) || m == 0) return 0;
   Space sp{nullptr};
-  MatmulFp8(sp, fp8_mode(out_dtype), m, n, k);
+  MatmulFp8(sp, out_dtype, m, n, k);
   return sp.used;
 }
 
@@ -578,15 +587,15 @@ OMT_EXPORT int omt_matmul_fp8(int64_t m, int64_t n, int64_t k, const void* a, co
   if (!on16({a, b, c})) return fail(OMT_INVALID, "%s: an operand is not on 16 bytes", fn);
   if (int e = need_space(fn, omt_matmul_fp8_workspace(m, n, k, out_dtype), workspace, workspace_bytes)) return e;
   Space sp{(char*)workspace};
-  const int mode = fp8_mode(out_dtype);
-  const MatmulFp8 l(sp, mode, m, n, k);
+  const MatmulFp8 l(sp, out_dtype, m, n, k);
   hipStream_t st = stream_of(stream);
   GemmArgs g{};
-  if (int e = lay_operands(g, mode, l.a, l.b, {}, a, b, nullptr, m, n, k, st)) return e;
+  if (int e = lay_operands(g, l.mode, l.a, l.b, {}, a, b, nullptr, m, n, k, st)) return e;
   g.sx = a_scale, g.sw = b_scale;
   g.sx_row = g.sw_row = (int)cdiv(k, kFp8Block), g.sx_step = g.sw_step = 1;
   g.out = c, g.out_kind = out_dtype == OMT_DT_BF16 ? kOutBf16 : kOutF32;
-  return run_gemm(mode, false, l.p, g, l.parts, st);
+  if (l.few) return matmul_fp8_few({g.x, g.w, g.sx, g.sw, c, g.m, g.n, g.row_bytes, g.out_kind}, st);
+  return run_gemm(l.mode, false, l.p, g, l.parts, st);
 }
 
 OMT_EXPORT size_t omt_glu_fwd_workspace(int dtype, int64_t m, int64_t k, int64_t f) {

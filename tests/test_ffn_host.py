@@ -83,8 +83,8 @@ def test_workspaces_cover_what_they_say(lib):
     # rows of an odd number of bytes are copied
     assert L.omt_matmul_fp8_workspace(4096, 4096, 4097, BF16) >= 2 * 4096 * 4112
     # shared tiles: each workgroup's sums of two
-    _, rows, sharers = plan(lib, lib.OMT_FFN_MATMUL_FP8, BF16, 1, 8192, 4096)
-    assert sharers > 16 and L.omt_matmul_fp8_workspace(1, 4096, 8192, BF16) >= sharers * 2 * rows * 256 * 4
+    _, rows, sharers = plan(lib, lib.OMT_FFN_MATMUL_FP8, BF16, 17, 8192, 4096)
+    assert sharers > 16 and L.omt_matmul_fp8_workspace(17, 4096, 8192, BF16) >= sharers * 2 * rows * 256 * 4
     # the backward: dg and du twice, the weights and x transposed
     m, k, f = 300, 200, 500
     for dtype, e in ((F32, 4), (BF16, 2)):
@@ -102,6 +102,10 @@ def test_plans_are_within_the_kernels_limits(lib):
         for op in range(5):
             for dtype in (F32, BF16):
                 mode, rows, sharers = plan(lib, op, dtype, m, k, n)
+                if mode == 5:  # few rows: all of them at once, nothing shared
+                    assert op == lib.OMT_FFN_MATMUL_FP8 and m <= rows <= 64 and sharers == 0 and rows * k <= 16 * 8192
+                    assert k % 4 or lib.L.omt_matmul_fp8_workspace(m, n, k, dtype) == 0
+                    continue
                 assert rows in (16, 64, 96, 128, 160, 192, 224, 256) and mode in range(5)
                 assert 0 <= sharers <= (256 if rows > 64 else 512)
                 if op != lib.OMT_FFN_GLU_GW:  # (of the weights' gradients in bfloat16 the tiles have 128 rows or 256)
@@ -115,7 +119,7 @@ def test_the_tested_sizes_reach_the_tiles(lib):
     def kind(op, *size):
         mode, rows, sharers = plan(lib, op, *size)
         return op, mode, rows, sharers > 0
-    tested = {kind(*p) for p in test_gpu_ffn.PLANS}
+    tested = {kind(*p) for p in test_gpu_ffn.PLANS + test_gpu_ffn.FEW}
     g = torch.Generator().manual_seed(1)
     met = {kind(op, dtype, *(int(8 * 2 ** (float(torch.rand((), generator=g)) * 9)) for _ in range(3)))
            for _ in range(1000) for op in range(5) for dtype in (F32, BF16)}

@@ -462,9 +462,15 @@ ACROSS = [
     (3, 2, 4292, 3192, 8), (3, 2, 4783, 3504, 3008), (4, 2, 449, 8, 8), (4, 2, 1, 864, 4176), (4, 2, 1739, 2496, 3296),
     (4, 2, 65, 264, 72), (3, 2, 200, 264, 72), (4, 2, 4096, 128, 512),
 ]
+# 8-bit products of few rows: rows and weights that fill a workgroup or not, the reduction in whole blocks, ending inside one,
+# on no word, shorter than the waves; and their neighbours that go to the tiles
+FEW = [(0, d, *s) for d in (0, 2) for s in (
+    (1, 4, 1), (1, 128, 16), (3, 132, 17), (16, 8192, 15), (15, 2052, 4097), (5, 130, 300), (16, 257, 128), (1, 8192, 8192),
+    (16, 1000, 8209), (7, 129, 8200), (17, 64, 31), (32, 4096, 100), (30, 515, 4096), (33, 2048, 129), (64, 1924, 33),
+    (50, 1023, 257), (16, 8196, 64), (32, 4100, 64), (64, 2052, 64), (17, 128, 4100))]
 
 
-@pytest.mark.parametrize("op,dtype,m,k,n", PLANS + ACROSS)
+@pytest.mark.parametrize("op,dtype,m,k,n", PLANS + ACROSS + FEW)
 def test_every_tile(ops, cuda, op, dtype, m, k, n):
     import ctypes
     from omarchy_mac_torch import _lib
