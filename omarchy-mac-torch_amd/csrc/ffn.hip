@@ -99,20 +99,29 @@ __device__ __forceinline__ void write_columns(const float* blk, const Lines& d, 
   }
 }
 
-// rows of floats as kSplit lines, zeros past their end up to a multiple of 64
+// Up to three matrices of floats with rows of one length as kSplit lines, zeros past their end up to a multiple of 64: one
+// launch for all (4096 x 1024 x 4096: 20.0 us, 5 TB/s; three launches took 23.7).
+struct SplitArgs {
+  const float* src[3];
+  int64_t rows[3];
+  Lines d[3];
+};
 template <bool VEC>
-__global__ void __launch_bounds__(256) split_rows_kernel(const float* __restrict__ src, int64_t rows, int64_t cols,
-                                                         Lines d) {
+__global__ void __launch_bounds__(256) split_rows_kernel(SplitArgs a, int64_t cols) {
+  const int z = blockIdx.z;
   const int64_t line = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
   const int64_t at = (int64_t)blockIdx.y * kBlk + (threadIdx.x & 7) * 8;
-  if (line < rows) write8<kSplit>(d, line, at, load8<VEC>(src + line * cols, at, cols));
+  if (line < a.rows[z]) write8<kSplit>(a.d[z], line, at, load8<VEC>(a.src[z] + line * cols, at, cols));
 }
 
-// The columns of src [rows][cols] as lines of d, zeros from `rows` on up to a multiple of 64; S float, __bf16, or e4m3 with
-// its scales.
+// The columns of src [rows][cols] as lines of d, zeros from `rows` on up to a multiple of 64, and a second matrix's, where there
+// is one, as lines of d2; S float, __bf16, or e4m3 with its scales (one matrix).
 template <int FMT, bool VEC, class S>
-__global__ void __launch_bounds__(256) transpose_kernel(const S* __restrict__ src, const float* __restrict__ scale,
-                                                        int64_t rows, int64_t cols, Lines d) {
+__global__ void __launch_bounds__(256) transpose_kernel(const S* __restrict__ src1, const S* __restrict__ src2,
+                                                        const float* __restrict__ scale, int64_t rows, int64_t cols,
+                                                        Lines d1, Lines d2) {
+  const S* src = blockIdx.z ? src2 : src1;
+  const Lines& d = blockIdx.z ? d2 : d1;
   __shared__ float blk[kBlk * kBlkPitch];
   const int64_t r0 = (int64_t)blockIdx.x * kBlk, c0 = (int64_t)blockIdx.y * kBlk;
   const int part = (threadIdx.x & 7) * 8;
@@ -402,12 +411,6 @@ static Lines place_rows(Space& sp, int mode, int64_t rows, int64_t cols) {
   return d;
 }
 static int lay_rows(const Lines& d, int mode, const void* src, int64_t rows, int64_t cols, hipStream_t stream) {
-  if (mode == kSplit) {
-    const dim3 grid((unsigned)cdiv(rows, 32), (unsigned)cdiv(cols, kBlk));
-    if (cols % 8 == 0) hipLaunchKernelGGL(split_rows_kernel<true>, grid, dim3(256), 0, stream, (const float*)src, rows, cols, d);
-    else hipLaunchKernelGGL(split_rows_kernel<false>, grid, dim3(256), 0, stream, (const float*)src, rows, cols, d);
-    return launch_check("split_rows_kernel");
-  }
   if (!d.p) return OMT_OK;
   const int64_t pitch = d.pitch / elem_bytes(mode);
   const dim3 grid(grid1d(rows * d.pitch / 16, 256, 1 << 16));
@@ -421,10 +424,18 @@ static int lay_rows(const Lines& d, int mode, const void* src, int64_t rows, int
 // Lays out x [m][k] and the weights [n][k] (w_up may be null) and points a at them.
 static int lay_operands(GemmArgs& a, int mode, const Lines& x, const Lines& w, const Lines& w_up, const void* px,
                         const void* pw, const void* pw_up, int64_t m, int64_t n, int64_t k, hipStream_t stream) {
-  if (int e = lay_rows(x, mode, px, m, k, stream)) return e;
-  if (int e = lay_rows(w, mode, pw, n, k, stream)) return e;
-  if (pw_up)
-    if (int e = lay_rows(w_up, mode, pw_up, n, k, stream)) return e;
+  if (mode == kSplit) {
+    const SplitArgs s{{(const float*)px, (const float*)pw, (const float*)pw_up}, {m, n, n}, {x, w, w_up}};
+    const dim3 grid((unsigned)cdiv(std::max(m, n), 32), (unsigned)cdiv(k, kBlk), pw_up ? 3 : 2);
+    if (k % 8 == 0) hipLaunchKernelGGL(split_rows_kernel<true>, grid, dim3(256), 0, stream, s, k);
+    else hipLaunchKernelGGL(split_rows_kernel<false>, grid, dim3(256), 0, stream, s, k);
+    if (int e = launch_check("split_rows_kernel")) return e;
+  } else {
+    if (int e = lay_rows(x, mode, px, m, k, stream)) return e;
+    if (int e = lay_rows(w, mode, pw, n, k, stream)) return e;
+    if (pw_up)
+      if (int e = lay_rows(w_up, mode, pw_up, n, k, stream)) return e;
+  }
   a.x = x.p ? x.p : px, a.w = w.p ? w.p : pw, a.w_up = w_up.p ? w_up.p : pw_up;
   a.xpitch = x.pitch, a.wpitch = w.pitch, a.row_bytes = (int)x.pitch;
   a.m = (int)m, a.n = (int)n, a.split = a.limit = (int)m;
@@ -471,10 +482,10 @@ struct MatmulFp8 {
   }
 };
 // float32: on fp32 MFMA as it is, or as halves on float16 MFMA, three products for one. Laying out the halves reads and
-// writes the operands once (4 TB/s, three launches); it is taken where the products win that back.
+// writes the operands once, at 4 TB/s; it is taken where the products win that back.
 static int glu_mode(int dtype, int64_t m, int64_t k, int64_t f) {
   if (dtype == OMT_DT_BF16) return kBf16;
-  const float lay_us = 8.f * (float)(m + 2 * f) * (float)k / 4e6f + 9.f;
+  const float lay_us = 8.f * (float)(m + 2 * f) * (float)k / 4e6f + 3.f;
   return plan_gemm(kSplit, true, m, f, up(k, kBlk) * 4).us + lay_us < plan_gemm(kF32, true, m, f, k * 4).us ? kSplit : kF32;
 }
 struct GluFwd {
@@ -520,12 +531,15 @@ static int glu_check(const char* fn, int dtype, int64_t m, int64_t k, int64_t f,
 
 static int bwd_mode(int dtype) { return dtype == OMT_DT_F32 ? kSplit : kBf16; }
 
+// src2: null, or a second matrix, its lines d2
 template <class S>
-static int run_transpose(int mode, const S* src, const float* scale, int64_t rows, int64_t cols, const Lines& d,
-                         hipStream_t stream) {
-  const dim3 grid((unsigned)cdiv(rows, kBlk), (unsigned)cdiv(cols, kBlk));
-  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, src, scale, rows, cols, d); };
-  const bool vec = cols % 8 == 0 && on16({src});
+static int run_transpose(int mode, const S* src, const S* src2, const float* scale, int64_t rows, int64_t cols,
+                         const Lines& d, const Lines& d2, hipStream_t stream) {
+  const dim3 grid((unsigned)cdiv(rows, kBlk), (unsigned)cdiv(cols, kBlk), src2 ? 2 : 1);
+  auto go = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, stream, src, src2, scale, rows, cols, d, d2);
+  };
+  const bool vec = cols % 8 == 0 && on16({src, src2});
   if (mode == kSplit) vec ? go(transpose_kernel<kSplit, true, S>) : go(transpose_kernel<kSplit, false, S>);
   else vec ? go(transpose_kernel<kBf16, true, S>) : go(transpose_kernel<kBf16, false, S>);
   return launch_check("transpose_kernel");
@@ -707,9 +721,10 @@ OMT_EXPORT int omt_glu_bwd(int dtype, int64_t m, int64_t k, int64_t f, int act, 
   f % 8 == 0 && on16({gh, g, u}) ? pick(std::true_type{}) : pick(std::false_type{});
   if (int err = launch_check("glu_gate_kernel")) return err;
 
-  auto transpose = [&](const void* src, int64_t rows, int64_t cols, const Lines& d) {
-    return dtype == OMT_DT_F32 ? run_transpose(mode, (const float*)src, nullptr, rows, cols, d, st)
-                               : run_transpose(mode, (const __bf16*)src, nullptr, rows, cols, d, st);
+  auto transpose = [&](const void* src, const void* src2, int64_t rows, int64_t cols, const Lines& d, const Lines& d2) {
+    return dtype == OMT_DT_F32
+               ? run_transpose(mode, (const float*)src, (const float*)src2, nullptr, rows, cols, d, d2, st)
+               : run_transpose(mode, (const __bf16*)src, (const __bf16*)src2, nullptr, rows, cols, d, d2, st);
   };
   if (l.across) {
     GemmArgs a{};
@@ -735,15 +750,14 @@ OMT_EXPORT int omt_glu_bwd(int dtype, int64_t m, int64_t k, int64_t f, int act, 
     return OMT_OK;
   }
   if (gx) {  // [m][dg | du] by [k][Wg^T | Wu^T]
-    if (int err = transpose(w_gate, f, k, l.w_cols)) return err;
-    if (int err = transpose(w_up, f, k, from(l.w_cols, mode, 0, l.half))) return err;
+    if (int err = transpose(w_gate, w_up, f, k, l.w_cols, from(l.w_cols, mode, 0, l.half))) return err;
     GemmArgs a{};
     a.out = gx, a.split = a.limit = (int)m, a.out_kind = out_kind;
     if (int err = run_lines(mode, l.px, a, l.gate_rows, l.w_cols, m, k, l.parts, st)) return err;
   }
   if (gw_gate) {  // [dg^T over du^T] by [k][x^T]
-    if (int err = fp8 ? run_transpose(mode, (const uint8_t*)x, x_scale, m, k, l.x_cols, st)
-                      : transpose(x, m, k, l.x_cols))
+    if (int err = fp8 ? run_transpose(mode, (const uint8_t*)x, (const uint8_t*)nullptr, x_scale, m, k, l.x_cols, {}, st)
+                      : transpose(x, nullptr, m, k, l.x_cols, {}))
       return err;
     GemmArgs a{};
     a.out = gw_gate, a.out2 = gw_up, a.split = a.limit = (int)f, a.out_kind = out_kind;
