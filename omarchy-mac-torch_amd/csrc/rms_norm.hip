@@ -13,6 +13,10 @@
 // of 128 and find its largest magnitude without leaving the row of lanes. The weight gradient sums rows in registers
 // over a workgroup's rows, then the workgroups' sums in a fixed order in a second launch: no atomics, the same bits
 // each time.
+//
+// 8192 x 4096 bfloat16 with a residual: forward 47 us (5.7 TB/s), backward 51 and its weights' sums 7; 3001 x 1000 float32: 10.6,
+// 10.2 and 2.7; one row: 3.3, a launch. A copy of large tensors reaches 4.7 TB/s on this card: part of these is still in the
+// caches.
 #include <algorithm>
 
 #include "block_fp8.h"
@@ -180,6 +184,7 @@ __global__ void __launch_bounds__(1024) rms_norm_weight_kernel(const float* __re
   }
 }
 
+// Bound by memory: 8192 x 4096 bfloat16 20 us, 5 TB/s
 template <bool VEC, class T>
 __global__ void __launch_bounds__(256) quantize_fp8_kernel(const T* __restrict__ x, int64_t rows, int64_t cols,
                                                            int64_t vecs, int pow2, uint8_t* __restrict__ q,
@@ -196,7 +201,7 @@ __global__ void __launch_bounds__(256) quantize_fp8_kernel(const T* __restrict__
   }
 }
 
-// a block of 128 x 128 to a workgroup
+// a block of 128 x 128 to a workgroup, in registers (8192 x 4096 bfloat16: 18 us, 5.6 TB/s)
 template <bool VEC, class T>
 __global__ void __launch_bounds__(256) quantize_fp8_weight_kernel(const T* __restrict__ w, int64_t rows, int64_t cols,
                                                                   uint8_t* __restrict__ q, float* __restrict__ scale) {
