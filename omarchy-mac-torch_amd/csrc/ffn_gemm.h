@@ -79,9 +79,29 @@ struct GemmArgs {
 __device__ __forceinline__ float sigmoid(float g) {
   return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.442695040888963f * g));
 }
+// The normal distribution's Phi(g) and, where asked for, its density. The tail Phi(-|g|) is exp(-z^2) times half of
+// erfcx(z), z = |g| / sqrt 2, which over t = 1 / (1 + z / 2) is t times a polynomial in t: of degree 8, fitted for the smallest
+// relative error (4.4e-8; in float32 with the exponential instruction 4e-7 of g Phi(g) over -1, 3e-6 at -8). The gated form by
+// 777 x 1928 x 2504 in 8 bits takes 37.7 us with it, 39.9 with erfcf.
+__device__ __forceinline__ float normal_cdf(float g, float* density) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.35355339059327373f, fabsf(g), 1.f));
+  const float e = __builtin_amdgcn_exp2f(-0.7213475204444817f * g * g);
+  float q = -0.0296387915f;
+  q = fmaf(q, t, 0.142796934f);
+  q = fmaf(q, t, -0.244655848f);
+  q = fmaf(q, t, 0.140242666f);
+  q = fmaf(q, t, -0.014146396f);
+  q = fmaf(q, t, 0.10169632f);
+  q = fmaf(q, t, 0.121462673f);
+  q = fmaf(q, t, 0.141199917f);
+  q = fmaf(q, t, 0.141042516f);
+  const float tail = t * q * e;
+  if (density) *density = 0.3989422804014327f * e;
+  return g < 0.f ? tail : 1.f - tail;
+}
 __device__ __forceinline__ float glu_act(float g, int act) {
   if (act == OMT_GLU_SILU) return g * sigmoid(g);
-  if (act == OMT_GLU_GELU) return 0.5f * g * erfcf(-0.70710678118654752f * g);
+  if (act == OMT_GLU_GELU) return g * normal_cdf(g, nullptr);
   return g < 0.f ? 0.f : g;  // NaN stays
 }
 struct ActAndGrad {
@@ -93,8 +113,9 @@ __device__ __forceinline__ ActAndGrad glu_act_grad(float g, int act) {
     return {g * p, p * (1.f + g * (1.f - p))};
   }
   if (act == OMT_GLU_GELU) {
-    const float phi = 0.5f * erfcf(-0.70710678118654752f * g);
-    return {g * phi, phi + 0.3989422804014327f * g * __builtin_amdgcn_exp2f(-0.7213475204444817f * g * g)};
+    float density;
+    const float phi = normal_cdf(g, &density);
+    return {g * phi, phi + g * density};
   }
   return {g < 0.f ? 0.f : g, g > 0.f ? 1.f : 0.f};
 }
