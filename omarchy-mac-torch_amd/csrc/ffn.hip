@@ -303,7 +303,7 @@ constexpr float kStepUs[][kHeights] = {
     // 16    64    96    128    160    192    224   256
     {1.65f, 3.55f, 2.8f, 3.72f, 4.55f, 5.45f, 6.35f, 7.15f},   // kF32
     {1.2f, 1.0f, 0.62f, 0.76f, 0.88f, 1.1f, 1.25f, 1.4f},      // kBf16
-    {2.1f, 2.7f, 1.62f, 1.91f, 2.18f, 2.59f, 2.98f, 3.34f},    // kFp8x
+    {1.95f, 2.7f, 1.42f, 1.68f, 2.02f, 2.46f, 2.98f, 3.34f},   // kFp8x
     {1.6f, 1.6f, 0.86f, 1.02f, 1.2f, 1.32f, 1.55f, 1.85f},     // kFp8
     {1.1f, 2.3f, 1.16f, 1.4f, 1.68f, 1.95f, 2.3f, 2.7f},       // kSplit
 };

@@ -533,9 +533,10 @@ ffn_gemm_kernel(GemmArgs a) {
         scaled(i, part[i & 1]);
       }
     };
-    if constexpr (MODE == kFp8x || BM == 256) {
-      // the widened fragments take four times the registers, and 256 rows leave none: a step's first reads wait for the waves
-      // to meet
+    if constexpr (BM == 256 || (MODE == kFp8x && (BM == 224 || BM == 64))) {
+      // 256 rows leave no registers, nor do 224 beside widened fragments, of four times the size: a step's first reads wait for
+      // the waves to meet (and of 64 rows widened two workgroups to a CU hide each other's waits: 175 us for 187, 4096 x 4096
+      // x 4096)
 #pragma unroll
       for (int p = 0; p < NS - 1; ++p) issue(p, s0 + p);
       int cur = 0, nxt = NS - 1;
@@ -553,7 +554,7 @@ ffn_gemm_kernel(GemmArgs a) {
       }
     } else {
       // the next step's first reads in the shadow of the last row's products (8192 x 4096 x 8192 at 128 rows: e4m3 312 -> 298
-      // us, halves 1675 -> 1567)
+      // us, halves 1675 -> 1567; 4096 x 4096 x 4096 widened 132 -> 117)
 #pragma unroll
       for (int p = 0; p < NS; ++p) issue(p, s0 + p);
       meet(std::integral_constant<int, NS - 1>{});
