@@ -304,7 +304,7 @@ constexpr float kStepUs[][kHeights] = {
     {1.65f, 3.55f, 2.8f, 3.72f, 4.55f, 5.45f, 6.35f, 7.15f},   // kF32
     {1.2f, 1.0f, 0.62f, 0.76f, 0.88f, 1.1f, 1.25f, 1.4f},      // kBf16
     {1.95f, 2.7f, 1.42f, 1.68f, 2.02f, 2.46f, 2.98f, 3.34f},   // kFp8x
-    {1.6f, 1.6f, 0.86f, 1.02f, 1.2f, 1.32f, 1.55f, 1.85f},     // kFp8
+    {1.6f, 1.6f, 0.86f, 1.02f, 1.2f, 1.32f, 1.55f, 1.78f},     // kFp8
     {1.1f, 2.3f, 1.16f, 1.4f, 1.68f, 1.95f, 2.3f, 2.7f},       // kSplit
 };
 constexpr float kTileUs[kHeights] = {1.5f, 8.f, 5.f, 6.5f, 8.f, 8.5f, 10.f, 11.f}, kJoinUs = 4.f;

@@ -9,13 +9,14 @@
 // the same for both operands, and a sum does not mind.
 //
 // Tiles of 256 rows with all CUs busy, m x n x k (Gaussian values, short runs; long ones are up to a tenth slower, the clock
-// giving way to power): bfloat16 8192 x 4096 x 8192 370 us, 1480 TFLOP/s; e4m3 236 us, 2330; halves 1470 us, 375 (1120 of
-// the float16 products); e4m3 widened 1290 TFLOP/s, float32 150. A step of 256 rows takes the LDS as long as the matrix cores
-// (192 KB of reads and 64 KB of loads at 128 bytes a clock, 64 products of 16 clocks to each of a SIMD's two waves), so
-// the wave's tile is as large as its registers hold, 128 x 64, and the matrix cores are busy for 61% of the clocks (gated, bfloat16,
-// 8192 x 4096 x 8192). The scaled modes add vector instructions, which the matrix cores' work hides in part: 42% in e4m3 (4096 x
-// 8192 x 4096), 44% in halves (gated, 4096 x 1024 x 4096). A wave tile of 128 x 128 (four waves, accumulators in the second half of the register file)
-// reads a third less and took as long (355 to 370 us): then a lone wave's other instructions are in the products' way.
+// giving way to power): bfloat16 8192 x 4096 x 8192 370 us, 1480 TFLOP/s; e4m3 227 us, 2420; halves 1470 us, 375 (1120 of
+// the float16 products); e4m3 widened 1210 TFLOP/s (4096 x 4096 x 4096), float32 150. A step of 256 rows takes the LDS as
+// long as the matrix cores (192 KB of reads and 64 KB of loads at 128 bytes a clock; 64 products of 16 clocks to each of a
+// SIMD's two waves), so the wave's tile is as large as its registers hold, 128 x 64, and the matrix cores are busy for 61% of
+// the clocks (gated, bfloat16, 8192 x 4096 x 8192). The scaled modes add vector instructions, which the matrix cores' work
+// hides in part: 42% in e4m3 (4096 x 8192 x 4096), 44% in halves (gated, 4096 x 1024 x 4096). A wave tile of 128 x 128 (four
+// waves, accumulators in the second half of the register file) reads a third less and took as long (355 to 370 us for 361 to
+// 373): a lone wave's other instructions are in its products' way.
 #pragma once
 
 #include "block_fp8.h"
@@ -533,10 +534,10 @@ ffn_gemm_kernel(GemmArgs a) {
         scaled(i, part[i & 1]);
       }
     };
-    if constexpr (BM == 256 || (MODE == kFp8x && (BM == 224 || BM == 64))) {
-      // 256 rows leave no registers, nor do 224 beside widened fragments, of four times the size: a step's first reads wait for
-      // the waves to meet (and of 64 rows widened two workgroups to a CU hide each other's waits: 175 us for 187, 4096 x 4096
-      // x 4096)
+    if constexpr (BM == 256 ? MODE != kFp8 : MODE == kFp8x && (BM == 224 || BM == 64)) {
+      // 256 rows of halves leave no registers, nor do 224 beside widened fragments, of four times the size: a step's first reads
+      // wait for the waves to meet (and of 64 rows widened two workgroups to a CU hide each other's waits: 175 us for 187,
+      // 4096 x 4096 x 4096)
 #pragma unroll
       for (int p = 0; p < NS - 1; ++p) issue(p, s0 + p);
       int cur = 0, nxt = NS - 1;
