@@ -14,7 +14,7 @@
 // long as the matrix cores (192 KB of reads and 64 KB of loads at 128 bytes a clock; 64 products of 16 clocks to each of a
 // SIMD's two waves), so the wave's tile is as large as its registers hold, 128 x 64, and the matrix cores are busy for 61% of
 // the clocks (gated, bfloat16, 8192 x 4096 x 8192). The scaled modes add vector instructions, which the matrix cores' work
-// hides in part: 42% in e4m3 (4096 x 8192 x 4096), 44% in halves (gated, 4096 x 1024 x 4096). A wave tile of 128 x 128 (four
+// hides in part: 46% in e4m3 (4096 x 4096 x 8192), 44% in halves (gated, 4096 x 1024 x 4096). A wave tile of 128 x 128 (four
 // waves, accumulators in the second half of the register file) reads a third less and took as long (355 to 370 us for 361 to
 // 373): a lone wave's other instructions are in its products' way.
 #pragma once
