@@ -104,7 +104,8 @@ __global__ void __launch_bounds__(WAVES * 64) matmul_fp8_few_kernel(FewArgs a) {
 
 template <int WAVES, int MT, int NT>
 static int launch_few(const FewArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL((matmul_fp8_few_kernel<WAVES, MT, NT>), dim3((unsigned)cdiv(a.n, 16 * NT)), dim3(WAVES * 64), 0, stream, a);
+  const dim3 grid((unsigned)cdiv(a.n, 16 * NT));
+  hipLaunchKernelGGL((matmul_fp8_few_kernel<WAVES, MT, NT>), grid, dim3(WAVES * 64), 0, stream, a);
   return launch_check("matmul_fp8_few_kernel");
 }
 

@@ -278,7 +278,7 @@ ffn_gemm_kernel(GemmArgs a) {
   auto slot_of_x = [&](int t) { return wave + Tl::NW * t < Tl::SROWS / 64; };
   const int whole = a.row_bytes & ~15;  // what the 16-byte loads take of a row
   const uint32_t lds0 = lds_addr((const float*)lds);
-  // Step s into stage `buf`. Past the slice's last step every lane's offset is out of range: the loads count, and read
+  // Step s into stage `buf`. Past the share's last step every lane's offset is out of range: the loads count, and read
   // nothing.
   auto issue = [&](int buf, int s) {
     const uint32_t at = lds0 + buf * Tl::STAGE;
