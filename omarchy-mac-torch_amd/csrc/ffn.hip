@@ -46,8 +46,12 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const T* __restrict__ src
 // Where lines of an operand go: bfloat16 (kBf16), or float32 as two halves (kSplit). There the 32 elements that a step of
 // the tiles reads of a line are scaled by one power of two, so that the largest lies in [2^14, 2^15), and each is held as
 // the nearest float16 and the float16 nearest to what is left: 22 bits, or 2^-40 of the largest where that is more. 32
-// high halves, then the 32 low ones; the scales lie by step, then line. Where a group holds an infinity its scale is
-// infinite, with +-1 for the infinities and 0 for the rest; where it holds NaN, NaN.
+// high halves, then the 32 low ones; the scales lie by step, then line.
+// A group that holds an infinity or NaN gives nothing finite, whatever it meets; what counts is where each product is
+// infinite, of which sign, and where it is NaN. Its high halves are the signs (0 for zeros, NaN for NaN), its low ones 0 but for the
+// infinities, which lie there, and its scale is 1. An infinity then meets the other line's high half once, and not its low one,
+// whose sign is its own: inf times v is inf by v's sign, and NaN for 0; two infinities meet each other's sign. So that a high
+// half is 0 for zeros alone, smaller values have float16's smallest there, and the low half takes it back.
 struct Lines {
   char* p = nullptr;
   int64_t pitch = 0;       // bytes
@@ -65,20 +69,27 @@ __device__ __forceinline__ void write8(const Lines& d, int64_t line, int64_t at,
     uint32_t b = abs_bits8(v);
     b = max_u32(b, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)b, 0xB1, 0xF, 0xF, false));  // quad_perm [1,0,3,2]
     b = max_u32(b, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)b, 0x4E, 0xF, 0xF, false));  // quad_perm [2,3,0,1]
-    float scale;
+    float scale = 1.f;
+    half8 hi, lo = {};
     if (b < 0x7f800000u) {
       const uint32_t e = max_u32(b >> 23, 15u);
-      v *= __builtin_bit_cast(float, (268u - e) << 23);
+      const f32x8 w = v * __builtin_bit_cast(float, (268u - e) << 23);
       scale = __builtin_bit_cast(float, (e - 14u) << 23);
-    } else {
-      scale = __builtin_bit_cast(float, b);
+      hi = __builtin_convertvector(w, half8);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = abs_bits(v[e]) == 0x7f800000u ? copysignf(1.f, v[e]) : 0.f;
+      for (int e = 0; e < 8; ++e)
+        if (hi[e] == 0 && v[e] != 0.f) hi[e] = (_Float16)copysignf(0x1p-24f, v[e]);
+      lo = __builtin_convertvector(w - __builtin_convertvector(hi, f32x8), half8);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        hi[e] = (_Float16)(v[e] == 0.f || v[e] != v[e] ? v[e] : copysignf(1.f, v[e]));
+        if (abs_bits(v[e]) == 0x7f800000u) lo[e] = (_Float16)v[e];
+      }
     }
     char* p = d.p + line * d.pitch + (at >> 5) * 128 + (at & 31) * 2;
-    const half8 h = __builtin_convertvector(v, half8);
-    *(half8*)p = h;
-    *(half8*)(p + 64) = __builtin_convertvector(v - __builtin_convertvector(h, f32x8), half8);
+    *(half8*)p = hi;
+    *(half8*)(p + 64) = lo;
     if ((at & 31) == 0) d.scale[(at >> 5) * d.scale_lines + line] = scale;
   }
 }

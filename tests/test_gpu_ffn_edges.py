@@ -1,0 +1,86 @@
+"""The feed-forward operators where they can go wrong: infinities and NaN in each form of the products, sums whose terms
+cancel, every row and column of a gradient by itself, scales to the bit, long and wide norms. Oracles in float64, on the CPU
+or the GPU; tolerances are derived beside each test."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BLOCK = 128
+F32, BF16, FP8 = torch.float32, torch.bfloat16, torch.float8_e4m3fn
+INF, NAN = float("inf"), float("nan")
+
+
+@pytest.fixture(scope="module")
+def ops(cuda):
+    from omarchy_mac_torch import hip_ops
+    return hip_ops
+
+
+def rnd(shape, seed, scale=1.0):
+    return torch.randn(shape, generator=torch.Generator().manual_seed(seed), dtype=torch.float64) * scale
+
+
+def mode_of(op, dtype, m, k, n):
+    import ctypes
+    from omarchy_mac_torch import _lib
+    v = [ctypes.c_int() for _ in range(3)]
+    assert _lib.L.omt_ffn_plan(op, dtype, m, k, n, *v) == 0
+    return v[0].value
+
+
+def same_kind(got, want):
+    """Both +inf, both -inf, both NaN, or both finite, element by element."""
+    got, want = got.double().cpu(), want.double().cpu()
+    return (torch.equal(got.isnan(), want.isnan()) and torch.equal(got.isposinf(), want.isposinf())
+            and torch.equal(got.isneginf(), want.isneginf()))
+
+
+def products(x, w):
+    """x w^T, one rounding to each product, as IEEE has infinities and NaN."""
+    return torch.stack([(x.double()[:, None, :] * r.double()).sum(-1) for r in w.split(1)], 1)[..., 0]
+
+
+# ---- what is not finite ------------------------------------------------------------------------------------------------
+
+def test_glu_infinities_of_both_operands(ops, cuda):
+    """float32 as float16 halves: infinities of x and of the weights in one group of 32 (at one place, at two), of both
+    signs, beside zeros and beside values far below their group's largest: as float32 has them, one by one."""
+    m, k, f = 1647, 871, 407
+    assert mode_of(1, 0, m, k, f) == 4
+    x, wg, wu = rnd((m, k), 1).float(), rnd((f, k), 2, k ** -0.5).float(), rnd((f, k), 3, k ** -0.5).float()
+    x[5, 3], x[6, 3], x[6, 9] = INF, INF, INF       # one; two, whose signs the weight decides
+    x[7, 3], x[7, 9] = INF, -INF
+    x[8, 40], x[9, 870] = -INF, INF                 # another group; the last element
+    x[10, 3], x[10, 5] = INF, NAN
+    x[11, 7] = 0
+    wg[2, 7], wg[3, 3], wg[4, 3] = -INF, INF, -INF  # elsewhere in x's group; at its own place
+    wg[5, 3], wg[5, 40] = 0, 1e-30
+    wg[6, 3], wg[6, 9], wg[7, 870] = -0.0, 1e-38, NAN
+    wu[2, 3], wu[2, 7], wu[3] = INF, -INF, 0
+    rows, cols = torch.tensor([4, 5, 6, 7, 8, 9, 10, 11, 12, 1646]), torch.arange(12)
+    h, kept = ops.glu(x.to(cuda), wg.to(cuda), wu.to(cuda), act="relu", checkpoint="full")
+    for got, w in ((kept[2], wg), (kept[4], wu)):
+        got = got.cpu()
+        assert same_kind(got[rows][:, cols], products(x[rows], w[cols]))
+        plain = torch.ones(m, dtype=torch.bool)
+        plain[5:11] = False
+        finite = w.isfinite().all(1)
+        assert bool(got[plain][:, finite].isfinite().all()) and not bool(got[5:11].isfinite().any())
+
+
+def test_glu_backward_infinities_of_the_weights(ops, cuda):
+    """gx = dg Wg + du Wu with an infinity in a weight: by the sign of dg, NaN where dg is 0."""
+    m, k, f = 1647, 871, 407
+    assert mode_of(3, 0, m, k, f) == 4 and mode_of(4, 0, m, k, f) == 4
+    x, g, u, gh = (rnd(s, i).float() for i, s in enumerate(((m, k), (m, f), (m, f), (m, f))))
+    wg, wu = rnd((f, k), 7, k ** -0.5).float(), rnd((f, k), 8, k ** -0.5).float()
+    wg[9, 7], wu[40, 8] = INF, -INF
+    gh[3] = 0
+    gx, gwg, gwu = ops.glu_backward(gh.to(cuda), (x.to(cuda), None, g.to(cuda), None, u.to(cuda), None), wg.to(cuda),
+                                    wu.to(cuda), act="relu")
+    dg, du = gh.double() * u.double() * (g > 0), gh.double() * g.double().clamp(min=0)
+    assert same_kind(gx[:, 7], dg[:, 9] * INF) and same_kind(gx[:, 8], du[:, 40] * -INF)
+    gx[:, 7:9] = 0
+    assert bool(gx.isfinite().all()) and bool(gwg.isfinite().all()) and bool(gwu.isfinite().all())
