@@ -626,12 +626,11 @@ ffn_gemm_kernel(GemmArgs a) {
       b = max_u32(b, (uint32_t)__shfl_xor((int)b, 32));
       if (g == 0) top[(z * 4 + wn) * BM + xrow + i * 16 + r16] = b;
     };
-    // the block's scale (by a product with 1 / 448 rounded) and its reciprocal to 1 ulp
+    // the block's scale and its reciprocal, as the other kernels have them
     auto scale_of = [&](int z, int lr, float* inv) {
       const uint32_t* p = top + z * 4 * BM + lr;
-      const uint32_t b = max_u32(max_u32(p[0], p[BM]), max_u32(p[2 * BM], p[3 * BM]));
-      const float s = __builtin_bit_cast(float, max_u32(b, __builtin_bit_cast(uint32_t, kFp8Floor))) * (1.f / kFp8Max);
-      *inv = __builtin_amdgcn_rcpf(s);
+      const float s = block_scale(max_u32(max_u32(p[0], p[BM]), max_u32(p[2 * BM], p[3 * BM])));
+      *inv = 1.f / s;
       return s;
     };
     const int blocks = (a.n + kFp8Block - 1) / kFp8Block, c = n0 + wcol(0);

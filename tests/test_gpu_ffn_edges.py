@@ -84,3 +84,23 @@ def test_glu_backward_infinities_of_the_weights(ops, cuda):
     assert same_kind(gx[:, 7], dg[:, 9] * INF) and same_kind(gx[:, 8], du[:, 40] * -INF)
     gx[:, 7:9] = 0
     assert bool(gx.isfinite().all()) and bool(gwg.isfinite().all()) and bool(gwu.isfinite().all())
+
+
+# ---- scales ------------------------------------------------------------------------------------------------------------
+
+# float32 instructions and halves, tiles a workgroup's own and shared (the second, fourth and sixth)
+@pytest.mark.parametrize("m,k,f", [(16, 64, 128), (1, 512, 700), (4868, 397, 157), (1951, 1569, 134), (4096, 256, 1024),
+                                   (889, 1380, 1058)])
+def test_glu_checkpoints_to_the_bit(ops, cuda, m, k, f):
+    """A block's scale is float32's max(largest magnitude, 1e-30) / 448, and its values float32's product with 1 / scale rounded
+    to e4m3, of the same projections that the whole checkpoints give."""
+    x, wg, wu = (t.float().to(cuda) for t in (rnd((m, k), 1), rnd((f, k), 2, k ** -0.5), rnd((f, k), 3, k ** -0.5)))
+    _, full = ops.glu(x, wg, wu, checkpoint="full")
+    _, kept = ops.glu(x, wg, wu, checkpoint="fp8")
+    for i in (2, 4):
+        t = full[i].cpu()
+        blocks = torch.nn.functional.pad(t, (0, -f % BLOCK)).unflatten(-1, (-1, BLOCK))
+        scale = blocks.abs().amax(-1).clamp(min=1e-30) / 448
+        assert torch.equal(kept[i + 1].cpu(), scale)
+        q = (blocks * (1 / scale)[..., None]).flatten(-2)[:, :f].to(FP8)
+        assert torch.equal(kept[i].cpu().view(torch.uint8), q.contiguous().view(torch.uint8))
