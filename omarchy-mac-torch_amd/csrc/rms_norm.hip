@@ -59,9 +59,10 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 template <class T, bool VEC, int RT, int NV>
 __global__ void __launch_bounds__(RT == 64 ? 256 : RT) rms_norm_fwd_kernel(NormArgs a) {
   __shared__ float red[16];
-  const int64_t row = RT == 64 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : (int64_t)blockIdx.x;
+  const int64_t group = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+  const int64_t row = RT == 64 ? group * 4 + (threadIdx.x >> 6) : group;
   const int t = RT == 64 ? threadIdx.x & 63 : threadIdx.x;
-  if (row >= a.rows) return;  // a whole wave, and only where no barrier follows
+  if (row >= a.rows) return;  // a whole wave where no barrier follows, or the workgroup
   const int64_t base = row * a.dim;
   f32x8 v[NV];
   float ss = 0.f;
@@ -278,8 +279,10 @@ OMT_EXPORT int omt_rms_norm_fwd(int dtype, int weight_dtype, int64_t rows, int64
   const NormArgs a{x, residual, weight, y, h, rstd, (uint8_t*)q, scale, rows, dim, eps, weight_dtype == OMT_DT_F32};
   for_dim(dim, [&](auto rt, auto nv) {
     constexpr int RT = decltype(rt)::value, NV = decltype(nv)::value;
+    // a dimension of the grid holds fewer than 2^32 threads: 2^21 workgroups along it, the rest along the other
+    const int64_t groups = RT == 64 ? cdiv(rows, 4) : rows, along = std::min<int64_t>(groups, 1 << 21);
     auto go = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3((unsigned)(RT == 64 ? cdiv(rows, 4) : rows)), dim3(RT == 64 ? 256 : RT), 0,
+      hipLaunchKernelGGL(kernel, dim3((unsigned)along, (unsigned)cdiv(groups, along)), dim3(RT == 64 ? 256 : RT), 0,
                          stream_of(stream), a);
     };
     if (dtype == OMT_DT_F32) vec ? go(rms_norm_fwd_kernel<float, true, RT, NV>) : go(rms_norm_fwd_kernel<float, false, RT, NV>);

@@ -104,3 +104,22 @@ def test_glu_checkpoints_to_the_bit(ops, cuda, m, k, f):
         assert torch.equal(kept[i + 1].cpu(), scale)
         q = (blocks * (1 / scale)[..., None]).flatten(-2)[:, :f].to(FP8)
         assert torch.equal(kept[i].cpu().view(torch.uint8), q.contiguous().view(torch.uint8))
+
+
+# ---- norms ---------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("rows,dim", [(2 ** 26 + 5, 8), (2 ** 23 + 3, 8), (2 ** 21 + 2, 2056)])
+def test_rms_norm_of_more_rows_than_a_grid_dimension_holds(ops, cuda, rows, dim):
+    """A workgroup to four short rows or to one long one: 2^24 of them of 256 threads pass a dimension's 2^32 threads. Rows
+    differ in size, so that each shows whose statistics it has. bfloat16: 2^-8 for the result's rounding, and as much again
+    for float32's sums, far below it."""
+    x = torch.ones(rows, dim, device=cuda, dtype=BF16)
+    x[:, 0] = (torch.arange(rows, device=cuda) % 97).to(BF16)
+    w = torch.ones(dim, device=cuda, dtype=BF16)
+    y, _, rstd = ops.rms_norm(x, w)
+    want = torch.rsqrt(((torch.arange(rows, device=cuda) % 97).double().square() + dim - 1) / dim + 1e-6)
+    assert float((rstd.double() / want - 1).abs().max()) <= (8 + dim) * 2 ** -24
+    assert float((y[:, 1].double() / want - 1).abs().max()) <= 2 ** -7
+    q, scale, _ = ops.rms_norm_fp8(x, w)
+    top = torch.maximum(torch.arange(rows, device=cuda) % 97, torch.ones((), device=cuda)).double() * want
+    assert float((scale[:, 0].double() * 448 / top - 1).abs().max()) <= (16 + dim) * 2 ** -24
