@@ -126,9 +126,10 @@ struct SplitArgs {
 template <bool VEC>
 __global__ void __launch_bounds__(256) split_rows_kernel(SplitArgs a, int64_t cols) {
   const int z = blockIdx.z;
-  const int64_t line = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
   const int64_t at = (int64_t)blockIdx.y * kBlk + (threadIdx.x & 7) * 8;
-  if (line < a.rows[z]) write8<kSplit>(a.d[z], line, at, load8<VEC>(a.src[z] + line * cols, at, cols));
+  // one line to a thread, but for those past the 2^32 threads that a dimension of the grid cannot hold
+  for (int64_t line = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3); line < a.rows[z]; line += (int64_t)gridDim.x * 32)
+    write8<kSplit>(a.d[z], line, at, load8<VEC>(a.src[z] + line * cols, at, cols));
 }
 
 // The columns of src [rows][cols] as lines of d, zeros from `rows` on up to a multiple of 64, and a second matrix's, where there
@@ -449,7 +450,7 @@ static int lay_operands(GemmArgs& a, int mode, const Lines& x, const Lines& w, c
                         const void* pw, const void* pw_up, int64_t m, int64_t n, int64_t k, hipStream_t stream) {
   if (mode == kSplit) {
     const SplitArgs s{{(const float*)px, (const float*)pw, (const float*)pw_up}, {m, n, n}, {x, w, w_up}};
-    const dim3 grid((unsigned)cdiv(std::max(m, n), 32), (unsigned)cdiv(k, kBlk), pw_up ? 3 : 2);
+    const dim3 grid(grid1d(std::max(m, n), 32), (unsigned)cdiv(k, kBlk), pw_up ? 3 : 2);
     if (k % 8 == 0) hipLaunchKernelGGL(split_rows_kernel<true>, grid, dim3(256), 0, stream, s, k);
     else hipLaunchKernelGGL(split_rows_kernel<false>, grid, dim3(256), 0, stream, s, k);
     if (int e = launch_check("split_rows_kernel")) return e;

@@ -86,6 +86,21 @@ def test_glu_backward_infinities_of_the_weights(ops, cuda):
     assert bool(gx.isfinite().all()) and bool(gwg.isfinite().all()) and bool(gwu.isfinite().all())
 
 
+# ---- very many rows ------------------------------------------------------------------------------------------------------
+
+def test_glu_of_more_rows_than_a_grid_dimension_holds(ops, cuda):
+    """2^29 rows, as halves: laid out 32 to a workgroup of 256 they are 2^32 threads. Products of small whole numbers, exact."""
+    m = 2 ** 29 + 40
+    if torch.cuda.mem_get_info()[0] < 200 << 30:
+        pytest.skip("needs 160 GB of GPU memory")
+    assert mode_of(1, 0, m, 1, 1) == 4
+    x = (torch.arange(m, device=cuda, dtype=torch.int32) % 61).to(F32).view(m, 1)
+    h, _ = ops.glu(x, torch.full((1, 1), 2.0, device=cuda), torch.full((1, 1), 3.0, device=cuda), act="relu")
+    assert torch.equal(h, x.square_().mul_(6))
+    del h, x
+    torch.cuda.empty_cache()
+
+
 # ---- scales ------------------------------------------------------------------------------------------------------------
 
 # float32 instructions and halves, tiles a workgroup's own and shared (the second, fourth and sixth)
