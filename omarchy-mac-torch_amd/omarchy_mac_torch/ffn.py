@@ -40,10 +40,9 @@ class _RmsNorm(torch.autograd.Function):
 class _Glu(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, act, checkpoint):
-        h, kept = hip_ops.glu(x, w_gate, w_up, act, checkpoint if any(ctx.needs_input_grad[:3]) else None)
-        if kept is not None:
-            ctx.save_for_backward(w_gate, w_up, *kept)
-            ctx.act = act
+        h, kept = hip_ops.glu(x, w_gate, w_up, act, checkpoint)
+        ctx.save_for_backward(w_gate, w_up, *kept)
+        ctx.act = act
         return h
 
     @staticmethod
@@ -65,9 +64,12 @@ def rms_norm(x, weight, residual=None, eps=1e-6):
 @torch.compiler.disable
 def glu(x, w_gate, w_up, act="silu", checkpoint="fp8"):
     """hip_ops.glu's h, differentiable; `checkpoint` says how x and both projections are kept for the backward: "fp8" or
-    "full"."""
+    "full". Nothing is kept where no gradient can be asked for."""
     if checkpoint not in ("fp8", "full"):
         raise ValueError(f"checkpoint: expected 'fp8' or 'full', got {checkpoint!r}")
+    # (inside the function grad mode is always off, and ctx.needs_input_grad says what the inputs require whatever the mode)
+    if not torch.is_grad_enabled() or not any(t.requires_grad for t in (x, w_gate, w_up)):
+        return hip_ops.glu(x, w_gate, w_up, act)[0]
     return _Glu.apply(x, w_gate, w_up, act, checkpoint)
 
 
