@@ -163,11 +163,13 @@ class MlpLM(nn.Module):
         return self.head(y)
 
     def serve(self):
-        """The model for inference, its sublayers' weights in 8 bits (the rest is shared with this one)."""
+        """A model for inference with the weights of now, its sublayers' in 8 bits: nothing of it is this one's, which stays
+        as it is and may train on."""
         import copy
         served = copy.copy(self)
-        served._modules = dict(self._modules, blocks=nn.ModuleList(b.serve() for b in self.blocks))
-        return served.eval()
+        served._modules = {name: nn.ModuleList(b.serve() for b in m) if name == "blocks" else copy.deepcopy(m)
+                           for name, m in self._modules.items()}
+        return served.eval().requires_grad_(False)
 
 
 def mlp_lm(vocab=256, dim=512, hidden=1408, depth=4, **options):

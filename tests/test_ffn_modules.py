@@ -40,3 +40,34 @@ def test_nothing_is_kept_where_no_gradient_can_be_asked_for(glu_calls, checkpoin
     m.down.weight.requires_grad_(True)
     m(x.detach())
     assert glu_calls[5:] == [None, None]
+
+
+@pytest.fixture
+def quantized(monkeypatch):
+    """hip_ops.quantize_fp8_weight by plain torch."""
+    from omarchy_mac_torch import hip_ops
+
+    def quantize(w):
+        n, k = w.shape
+        b = torch.nn.functional.pad(w.float(), (0, -k % 128, 0, -n % 128)).unflatten(1, (-1, 128)).unflatten(0, (-1, 128))
+        s = b.abs().amax((1, 3)).clamp(min=1e-30) / 448
+        return (b / s[:, None, :, None]).flatten(2).flatten(0, 1)[:n, :k].contiguous().to(torch.float8_e4m3fn), s
+
+    monkeypatch.setattr(hip_ops, "quantize_fp8_weight", quantize)
+
+
+def test_serving_leaves_the_model_as_it_is(quantized):
+    from omarchy_mac_torch import models
+    lm = models.mlp_lm(32, 64, 96, 2).train()
+    served = lm.serve()
+    assert not any(m.training for m in served.modules())
+    assert all(m.training for m in lm.modules()) and all(p.requires_grad for p in lm.parameters())
+    assert isinstance(served, models.MlpLM) and served.context == lm.context
+    before = [v.clone() for v in served.state_dict().values()]
+    own = {v.data_ptr() for v in lm.state_dict().values()}
+    assert not any(v.data_ptr() in own for v in served.state_dict().values())
+    with torch.no_grad():
+        for p in lm.parameters():
+            p.add_(1)
+    after = served.state_dict().values()
+    assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(before, after))
