@@ -138,6 +138,16 @@ class ServedFeedForward(nn.Module):
             self.register_buffer(name, q)
             self.register_buffer(name + "_scale", scale)
 
+    def _apply(self, fn, recurse=True):
+        # a change of type (to(dtype), float(), bfloat16()) is for the norm's weight: values in 8 bits and their scales move only
+        def apply(t):
+            if t is not self.weight:
+                like = fn(t.new_empty(0))
+                if like.dtype != t.dtype:
+                    return t.to(like.device)
+            return fn(t)
+        return super()._apply(apply, recurse)
+
     @torch.no_grad()
     def forward(self, x, residual=None):
         q, scale, h = hip_ops.rms_norm_fp8(x, self.weight, residual, self.eps)

@@ -71,3 +71,17 @@ def test_serving_leaves_the_model_as_it_is(quantized):
             p.add_(1)
     after = served.state_dict().values()
     assert all(torch.equal(a.view(torch.uint8), b.view(torch.uint8)) for a, b in zip(before, after))
+
+
+def test_a_served_sublayer_keeps_its_8_bit_types(quantized):
+    from omarchy_mac_torch import ffn
+    served = ffn.FeedForward(64, 96).serve()
+    kept = {k: v.clone() for k, v in served.state_dict().items() if k != "weight"}
+    for change in (lambda: served.to(torch.bfloat16), served.float, served.half, lambda: served.to("cpu", torch.float64)):
+        change()
+        for name, v in kept.items():
+            now = getattr(served, name)
+            assert now.dtype == v.dtype and torch.equal(now.view(torch.uint8), v.view(torch.uint8))
+    assert served.weight.dtype == torch.float64
+    assert all(b.device.type == "meta" for b in served.to("meta", torch.bfloat16).buffers())
+    assert all(getattr(served, name).dtype == v.dtype for name, v in kept.items())
