@@ -148,6 +148,7 @@ class ServedFeedForward(nn.Module):
             return fn(t)
         return super()._apply(apply, recurse)
 
+    @torch.compiler.disable
     @torch.no_grad()
     def forward(self, x, residual=None):
         q, scale, h = hip_ops.rms_norm_fp8(x, self.weight, residual, self.eps)
