@@ -6,7 +6,8 @@
 //
 // with gh the gradient that reaches h past the norm; gx is the gradient of x and of the residual. Statistics and sums
 // are float32. Bound by memory: a forward reads x and residual and writes h and y (or 1 byte per value and 4 per block
-// of 128), the backward reads gy, h and gh and writes gx; each exactly once, a row in registers between the passes.
+// of 128), the backward reads gy, h and gh and writes gx; each exactly once, a row in registers between the passes (gh of over
+// 16384 columns is read after the sum).
 //
 // A row takes a wave (up to 2048 columns; four rows to a workgroup, no barrier), a workgroup of 256 (up to 8192) or
 // one of 1024 threads (up to 32768), eight consecutive columns to a thread and vector, so that 16 lanes hold a block
@@ -107,26 +108,40 @@ __global__ void __launch_bounds__(RT == 64 ? 256 : RT) rms_norm_bwd_kernel(NormB
   constexpr int ROWS = RT == 64 ? 4 : 1;  // rows of a workgroup at a time
   __shared__ float red[16];
   __shared__ f32x4 sums[ROWS == 4 ? 3 * 64 * NV * 2 : 1];
-  const int t = RT == 64 ? threadIdx.x & 63 : threadIdx.x, sub = RT == 64 ? threadIdx.x >> 6 : 0;
-  f32x8 w[NV], gw[NV];
+  int t = RT == 64 ? threadIdx.x & 63 : threadIdx.x;
+  const int sub = RT == 64 ? threadIdx.x >> 6 : 0;
+  // Whether a thread's registers hold the weight and its gradient through all rows, and gh through a row's sum. At 32768
+  // columns they do not: the gradient is held in LDS, each thread's sums in its own place, and the others are loaded where
+  // they are used (2048 x 32768 float32 253 us for 440 with registers spilled to memory, bfloat16 144 for 438).
+  constexpr bool kHold = RT * NV <= 2048;
+  __shared__ f32x4 held[kHold ? 1 : NV * 2 * RT];
+  f32x8 w[kHold ? NV : 1], gw[kHold ? NV : 1];
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
-    w[i] = load_weight<VEC>(a.weight, a.weight_f32, (int64_t)(i * RT + t) * 8, a.dim);
-    gw[i] = f32x8{};
+    if constexpr (kHold) w[i] = load_weight<VEC>(a.weight, a.weight_f32, (int64_t)(i * RT + t) * 8, a.dim), gw[i] = f32x8{};
+    else held[i * 2 * RT + t] = held[(i * 2 + 1) * RT + t] = f32x4{};
   }
   for (int64_t row = (int64_t)blockIdx.x * ROWS + sub; row < a.rows; row += (int64_t)gridDim.x * ROWS) {
     const int64_t base = row * a.dim;
     const float r = a.rstd[row];
-    f32x8 g[NV], n[NV], gh[NV];
+    // (opaque: what follows from it, as whether a column is there, would sit in registers through all rows)
+    if constexpr (!kHold) asm volatile("" : "+v"(t));
+    f32x8 g[NV], n[NV], gh[kHold ? NV : 1];
     float dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int64_t c = (int64_t)(i * RT + t) * 8;
       const f32x8 gy = load8<VEC>((const T*)a.gy + base, c, a.dim);
       n[i] = load8<VEC>((const T*)a.h + base, c, a.dim) * r;
-      gh[i] = a.gh ? load8<VEC>((const T*)a.gh + base, c, a.dim) : f32x8{};  // on its way during the sum
-      gw[i] += gy * n[i];
-      g[i] = gy * w[i];
+      if constexpr (kHold) gh[i] = a.gh ? load8<VEC>((const T*)a.gh + base, c, a.dim) : f32x8{};  // on its way during the sum
+      if constexpr (kHold) {
+        gw[i] += gy * n[i];
+      } else if (a.parts) {
+        const f32x8 p = gy * n[i];
+        held[i * 2 * RT + t] += f32x4{p[0], p[1], p[2], p[3]};
+        held[(i * 2 + 1) * RT + t] += f32x4{p[4], p[5], p[6], p[7]};
+      }
+      g[i] = gy * (kHold ? w[kHold ? i : 0] : load_weight<VEC>(a.weight, a.weight_f32, c, a.dim));
 #pragma unroll
       for (int e = 0; e < 8; ++e) dot = fmaf(g[i][e], n[i][e], dot);
     }
@@ -134,7 +149,8 @@ __global__ void __launch_bounds__(RT == 64 ? 256 : RT) rms_norm_bwd_kernel(NormB
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int64_t c = (int64_t)(i * RT + t) * 8;
-      store8<VEC>((T*)a.gx + base, c, a.dim, (g[i] - n[i] * mean) * r + gh[i]);
+      if constexpr (!kHold) gh[0] = a.gh ? load8<VEC>((const T*)a.gh + base, c, a.dim) : f32x8{};
+      store8<VEC>((T*)a.gx + base, c, a.dim, (g[i] - n[i] * mean) * r + gh[kHold ? i : 0]);
     }
   }
   if (!a.parts) return;
@@ -155,8 +171,13 @@ __global__ void __launch_bounds__(RT == 64 ? 256 : RT) rms_norm_bwd_kernel(NormB
       }
   }
 #pragma unroll
-  for (int i = 0; i < NV; ++i)
-    store8<false>(a.parts + (int64_t)blockIdx.x * a.dim, (int64_t)(i * RT + t) * 8, a.dim, gw[i]);
+  for (int i = 0; i < NV; ++i) {
+    if constexpr (!kHold) {
+      const f32x4 lo = held[i * 2 * RT + t], hi = held[(i * 2 + 1) * RT + t];
+      gw[0] = f32x8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+    }
+    store8<false>(a.parts + (int64_t)blockIdx.x * a.dim, (int64_t)(i * RT + t) * 8, a.dim, gw[kHold ? i : 0]);
+  }
 }
 
 // gw[c] = sum over the workgroups' sums: 16 columns to a workgroup, 64 threads a column, each a strided share in order,

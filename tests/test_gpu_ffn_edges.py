@@ -138,3 +138,28 @@ def test_rms_norm_of_more_rows_than_a_grid_dimension_holds(ops, cuda, rows, dim)
     q, scale, _ = ops.rms_norm_fp8(x, w)
     top = torch.maximum(torch.arange(rows, device=cuda) % 97, torch.ones((), device=cuda)).double() * want
     assert float((scale[:, 0].double() * 448 / top - 1).abs().max()) <= (16 + dim) * 2 ** -24
+
+
+@pytest.mark.parametrize("dim", [16400, 24577, 32766, 32768])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_rms_norm_backward_of_wide_rows(ops, cuda, dim, dtype):
+    """More rows than workgroups, so that each sums the weight's gradient over some. Per row and per column: float32's sums of
+    `dim` or `rows` terms, (8 + 2 sqrt(n)) 2^-24 of the terms' norm for random signs, twice for the two terms of gx, and for
+    bfloat16 results 2^-8."""
+    rows = 700
+    g = torch.Generator(device=cuda).manual_seed(dim)
+    h, gy, gh = (torch.randn(rows, dim, device=cuda, generator=g).to(dtype) for _ in range(3))
+    w = (1 + 0.2 * torch.randn(dim, device=cuda, generator=g)).to(dtype)
+    _, _, rstd = ops.rms_norm(h, w)
+    hd, gyd, r = h.double(), gy.double(), torch.rsqrt(h.double().square().mean(-1, keepdim=True) + 1e-6)
+    n, t = hd * r, gyd * w.double()
+    want = r * (t - n * (t * n).mean(-1, keepdim=True))
+    rounded = 2 ** -8 if dtype == BF16 else 0
+    for use_gh in (True, False):
+        gx, gw = ops.rms_norm_backward(gy, h, w, rstd, gh=gh if use_gh else None)
+        v = want + gh.double() if use_gh else want
+        assert bool(((gx.double() - v).norm(dim=1) <= (2 * (8 + 2 * dim ** 0.5) * 2 ** -24 + rounded) * v.norm(dim=1)).all())
+        off = (gw.double() - (gyd * n).sum(0)).abs()
+        assert bool((off <= 4 * (8 + 2 * rows ** 0.5) * 2 ** -24 * (gyd * n).norm(dim=0) + rounded * gw.double().abs()).all())
+        alone, none = ops.rms_norm_backward(gy, h, w, rstd, gh=gh if use_gh else None, weight_grad=False)
+        assert none is None and torch.equal(alone, gx)
