@@ -308,22 +308,38 @@ __global__ void __launch_bounds__(256) glu_join_kernel(GemmArgs a, int bm) {
 // The launch of a product of m rows by n (of each weight, if gated) with rows of row_bytes. As many tiles as fill all CUs
 // evenly are a workgroup's each; those left over, too few for a round of their own, can be shared, every workgroup taking
 // the same number of their steps, and joined by a second launch. Every choice of rows to a tile and of a share is priced, in
-// microseconds, and the cheapest taken: rounds of workgroups over the 256 CUs (two at a time of the tiles of 16 and 64
-// rows, whose stages leave room), each its steps and what a tile costs before its first and after its last, but no less
-// than the operands' bytes at 5.5 TB/s; sharing adds the second launch and the shares' sums to memory and back at 4 TB/s.
-// Steps, and the rest of a tile, in us, measured with all CUs busy (16384 x 4096 x 4096 and x 8192, the gated form of kF32 at
-// 5120 x 4096 x 1024 and x 2048; 16 rows at 64 x 4096 x 4096), [mode][rows of a tile]:
+// microseconds, and the cheapest taken: rounds of workgroups over the 256 CUs (two at a time to a CU whose LDS holds the
+// stages of two: tiles of 16 rows, and of 64 without scales), each its steps and what a tile costs before its first and after
+// its last, but no less than the operands' bytes at 5.5 TB/s; sharing adds the second launch and the shares' sums to memory
+// and back at 4 TB/s. Steps, and the rest of a tile, in us, measured with all CUs busy (16384 x 4096 x 4096 and x 8192, the
+// gated form of kF32 at 5120 x 4096 x 1024 and x 2048; 16 rows at 64 x 4096 x 4096; 64 rows with scales beside 96 in one round of
+// 256 workgroups, where both take as long), [mode][rows of a tile]:
 constexpr float kStepUs[][kHeights] = {
     // 16    64    96    128    160    192    224   256
     {1.65f, 3.55f, 2.8f, 3.72f, 4.55f, 5.45f, 6.35f, 7.15f},   // kF32
     {1.2f, 1.0f, 0.62f, 0.76f, 0.88f, 1.1f, 1.25f, 1.4f},      // kBf16
-    {1.95f, 2.7f, 1.42f, 1.68f, 2.02f, 2.46f, 2.98f, 3.34f},   // kFp8x
-    {1.6f, 1.6f, 0.86f, 1.02f, 1.2f, 1.32f, 1.55f, 1.78f},     // kFp8
-    {1.1f, 2.3f, 1.16f, 1.4f, 1.68f, 1.95f, 2.3f, 2.7f},       // kSplit
+    {1.95f, 1.35f, 1.42f, 1.68f, 2.02f, 2.46f, 2.98f, 3.34f},   // kFp8x
+    {1.6f, 0.9f, 0.86f, 1.02f, 1.2f, 1.32f, 1.55f, 1.78f},     // kFp8
+    {1.1f, 1.25f, 1.16f, 1.4f, 1.68f, 1.95f, 2.3f, 2.7f},      // kSplit
 };
-constexpr float kTileUs[kHeights] = {1.5f, 8.f, 5.f, 6.5f, 8.f, 8.5f, 10.f, 11.f}, kJoinUs = 4.f;
-constexpr int kCus = 256;
-constexpr int resident(int v) { return kBm[v] <= 64 ? 2 : 1; }
+constexpr float kJoinUs = 4.f;
+constexpr int kCus = 256, kCuLds = 160 * 1024;
+template <int MODE, int V>
+constexpr int resident_of() {
+  return 2 * GemmTile<MODE, kBm[V], gemm_stages<MODE, kBm[V]>()>::LDS <= kCuLds ? 2 : 1;
+}
+template <int V = 0>
+static int resident(int mode, int v) {
+  if constexpr (V + 1 < kHeights)
+    if (v != V) return resident<V + 1>(mode, v);
+  constexpr int of[] = {resident_of<kF32, V>(), resident_of<kBf16, V>(), resident_of<kFp8x, V>(), resident_of<kFp8, V>(),
+                        resident_of<kSplit, V>()};
+  return of[mode];
+}
+static float tile_us(int mode, int v) {  // 64 rows: of two workgroups, or of one
+  constexpr float us[kHeights] = {1.5f, 8.f, 5.f, 6.5f, 8.f, 8.5f, 10.f, 11.f};
+  return kBm[v] == 64 && resident(mode, v) == 1 ? 5.f : us[v];
+}
 struct GemmPlan {
   int bm, gx, gy, steps, whole, sharers, share;
   float us;
@@ -340,12 +356,14 @@ static GemmPlan plan_gemm(int mode, bool glu, int64_t m, int64_t n, int64_t row_
     if (v > 0 && m <= kBm[v - 1] && best.bm) break;
     if (across == kAcrossBoth && kBm[v] != 128 && kBm[v] != 256) continue;
     const float full = kStepUs[mode][v] * (across != kAlong && kBm[v] < 256 ? 1.1f : 1.f);
-    const int64_t gy = cdiv(m, kBm[v]), tiles = gx * gy, at_once = kCus * resident(v), left = tiles % at_once;
+    const bool two = resident(mode, v) == 2;
+    const float tile = tile_us(mode, v);
+    const int64_t gy = cdiv(m, kBm[v]), tiles = gx * gy, at_once = two ? 2 * kCus : kCus, left = tiles % at_once;
     // a workgroup alone on its CU takes about half the step that two take, but no less than a load's way, 0.9
     auto step = [&](int64_t groups) {
-      return resident(v) == 2 && groups <= kCus ? std::max(0.9f, 0.6f * full) : full;
+      return two && groups <= kCus ? std::max(0.9f, 0.6f * full) : full;
     };
-    const float rounds_us = (float)(tiles / at_once) * (steps * full + kTileUs[v]);
+    const float rounds_us = (float)(tiles / at_once) * (steps * full + tile);
     auto consider = [&](float us, int64_t whole, int64_t sharers, int64_t share) {
       us = std::max(us, bytes_us);
       if (sharers) {  // a share begins a tile, and each tile's first and last shares may belong to two
@@ -356,14 +374,14 @@ static GemmPlan plan_gemm(int mode, bool glu, int64_t m, int64_t n, int64_t row_
         best = {kBm[v], (int)gx, (int)gy, (int)steps, (int)whole, (int)sharers, (int)share, us,
                 (size_t)sharers * 2 * kBm[v] * 256 * sizeof(float)};
     };
-    consider(rounds_us + (left ? steps * step(left) + kTileUs[v] : 0.f), tiles, 0, 0);
+    consider(rounds_us + (left ? steps * step(left) + tile : 0.f), tiles, 0, 0);
     if (!left || steps < 4) continue;
     for (int64_t k = 1; k <= 32; ++k) {  // a k-th of a tile's steps each, or all CUs' even share
       const int64_t share = k == 1 ? std::max<int64_t>(cdiv(left * steps, at_once), 2) : cdiv(steps, k);
       const int64_t sharers = cdiv(left * steps, share);
       if (share < 2 || share >= steps || sharers > at_once) continue;
       const float begins = steps % share ? 1.5f : 1.f;  // some shares cover the end of one tile and the start of the next
-      consider(rounds_us + share * step(sharers) + begins * kTileUs[v], tiles - left, sharers, share);
+      consider(rounds_us + share * step(sharers) + begins * tile, tiles - left, sharers, share);
     }
   }
   return best;

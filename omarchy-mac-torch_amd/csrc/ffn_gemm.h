@@ -536,8 +536,7 @@ ffn_gemm_kernel(GemmArgs a) {
     };
     if constexpr (BM == 256 ? MODE != kFp8 : MODE == kFp8x && (BM == 224 || BM == 64)) {
       // 256 rows of halves leave no registers, nor do 224 beside widened fragments, of four times the size: a step's first reads
-      // wait for the waves to meet (and of 64 rows widened two workgroups to a CU hide each other's waits: 175 us for 187,
-      // 4096 x 4096 x 4096)
+      // wait for the waves to meet. (64 rows widened are faster so too: 175 us for 187, 4096 x 4096 x 4096.)
 #pragma unroll
       for (int p = 0; p < NS - 1; ++p) issue(p, s0 + p);
       int cur = 0, nxt = NS - 1;
@@ -702,9 +701,10 @@ int launch_gemm(const GemmArgs& a, hipStream_t stream) {
   return launch_check("ffn_gemm_kernel");
 }
 
-// Two stages, or three where they fit the CU's 160 KB: two workgroups of the small tiles fit it together and hide each
-// other's waits better than a third stage does (64 rows bf16, 4096 x 4096 x 4096: 144 us with two, 226 with three and one
-// workgroup); 128 rows gain 1-3% from a third.
+// Two stages, or three where they fit the CU's 160 KB. Two workgroups of 16 rows fit it together, and two of 64 without
+// scales, and hide each other's waits better than a third stage does (64 rows bf16, 4096 x 4096 x 4096: 144 us with two, 226
+// with three and one workgroup). Of 64 rows with scales one fits, and gains nothing from a third (16384 x 4096 x 8192 e4m3 964 us
+// with two, 960 with three; widened 1388 and 1539; halves, x 2048, 1159 and 1161); 128 rows gain 1-3%.
 template <int MODE, int BM>
 constexpr int gemm_stages() {
   return BM > 64 && 3 * GemmTile<MODE, BM, 1>::STAGE <= 160 * 1024 ? 3 : 2;
