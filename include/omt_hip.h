@@ -640,6 +640,8 @@ int omt_quantize_fp8(int dtype, int64_t rows, int64_t cols, const void* x, int p
 int omt_quantize_fp8_weight(int dtype, int64_t rows, int64_t cols, const void* w, void* q, float* scale, void* stream);
 
 /* c[m][n] = sum over k of a[m][k] b[n][k], both in 8 bits with scales (a by 1 x 128, b by 128 x 128); c in out_dtype.
+ * OMT_DT_F32: float32 sums of exact products. OMT_DT_BF16: of eight consecutive products, what is under 2^-13 of the largest may
+ * be lost, by the 8-bit matrix instructions.
  * a, b and the workspace on 16 bytes. */
 size_t omt_matmul_fp8_workspace(int64_t m, int64_t n, int64_t k, int out_dtype);
 int omt_matmul_fp8(int64_t m, int64_t n, int64_t k, const void* a, const float* a_scale, const void* b,

@@ -861,7 +861,9 @@ def quantize_fp8_weight(w):
 
 def matmul_fp8(a, a_scale, b, b_scale, dtype=torch.bfloat16):
     """a b^T of operands held in 8 bits: a [..., k] with scales by blocks of 128 along k, b [n, k] with scales by
-    128 x 128. Returns [..., n] of dtype (bfloat16 or float32)."""
+    128 x 128. Returns [..., n] of dtype (bfloat16 or float32). float32: float32 sums of exact products. bfloat16: of eight
+    consecutive products, what is under 2^-13 of the largest may be lost (the 8-bit matrix instructions' sums), which shows
+    where large products cancel."""
     return _ffn("matmul_fp8", a, a_scale, b, b_scale, dtype)
 
 

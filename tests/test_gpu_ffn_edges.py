@@ -86,6 +86,52 @@ def test_glu_backward_infinities_of_the_weights(ops, cuda):
     assert bool(gx.isfinite().all()) and bool(gwg.isfinite().all()) and bool(gwu.isfinite().all())
 
 
+# few rows (16, 32 and 64 of them), tiles, a reduction that ends inside a block
+@pytest.mark.parametrize("m,n,k", [(2, 140, 300), (16, 200, 512), (30, 140, 384), (64, 257, 300), (70, 140, 300), (300, 260, 640)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_matmul_fp8_blocks_that_stand_for_nan(ops, cuda, m, n, k, dtype):
+    """An infinity or NaN before quantization makes its block NaN throughout: of x its row of the result, of the weight the
+    columns of its 128 rows. Every form, both result types."""
+    x, w = rnd((m, k), 1).float(), rnd((n, k), 2).float()
+    x[1, 5], x[m - 1, k - 1] = INF, NAN
+    a, b = ops.quantize_fp8(x.to(cuda)), ops.quantize_fp8_weight(w.to(cuda))
+    got = ops.matmul_fp8(*a, *b, dtype=dtype).cpu()
+    rows = torch.zeros(m, dtype=torch.bool)
+    rows[[1, m - 1]] = True
+    assert bool(got[rows].isnan().all()) and bool(got[~rows].isfinite().all())
+    for bad in (-INF, NAN):
+        w[n - 1, k - 1] = bad
+        c = ops.quantize_fp8_weight(w.to(cuda))
+        got = ops.matmul_fp8(*a, *c, dtype=dtype).cpu()
+        cols = torch.arange(n) // BLOCK == (n - 1) // BLOCK
+        assert bool(got[:, cols].isnan().all()) and bool(got[~rows][:, ~cols].isfinite().all())
+
+
+# ---- sums that cancel ----------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("m", [1, 16, 40, 80, 300])
+def test_matmul_fp8_terms_that_cancel(ops, cuda, m):
+    """Large products that cancel beside small ones, in every block. A float32 result has float32's sums. A bfloat16 one may lose
+    what is under 2^-13 of the largest of eight consecutive products: at most 7 such parts to eight products, each 2^-13 of the
+    largest, and 2^-8 of the result."""
+    n, k = 256, 512
+    a, b = rnd((m, k), 1, 2.0), rnd((n, k), 2, 2.0)
+    for block in range(0, k, 128):
+        a[:, block + 3], a[:, block + 5], a[:, block + 9] = 448, -448, 384  # within eight, and over two eights
+        a[:, block + 90] = -384
+        b[:, [block + 3, block + 5]] = 256
+        b[:, [block + 9, block + 90]] = 448
+    a, b = a.to(FP8).to(cuda), b.to(FP8).to(cuda)
+    sa, sb = torch.ones(m, k // BLOCK, device=cuda), torch.ones(n // BLOCK, k // BLOCK, device=cuda)
+    terms = a.double()[:, None] * b.double()
+    want = terms.sum(-1)
+    exact = ops.matmul_fp8(a, sa, b, sb, dtype=F32).double()
+    assert bool(((exact - want).abs() <= (16 + 4 * k ** 0.5) * 2 ** -24 * terms.norm(dim=-1)).all())
+    got = ops.matmul_fp8(a, sa, b, sb, dtype=BF16).double()
+    lost = 7 * 2 ** -13 * terms.abs().unflatten(-1, (-1, 8)).amax(-1).sum(-1)
+    assert bool(((got - want).abs() <= 2 ** -8 * want.abs() + lost + (16 + 4 * k ** 0.5) * 2 ** -24 * terms.norm(dim=-1)).all())
+
+
 # ---- very many rows ------------------------------------------------------------------------------------------------------
 
 def test_glu_of_more_rows_than_a_grid_dimension_holds(ops, cuda):
