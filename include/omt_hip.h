@@ -620,7 +620,8 @@ int omt_fused_sgd(const omt_sgd_params* params, const omt_sgd_tensor* tensors, i
  * 8 bits: e4m3 values with a float32 scale for each block of 128 consecutive ones of a row ([rows][ceil(cols / 128)];
  * the last block of a row may be shorter), scale = max(largest magnitude, 1e-30) / 448; for weights of 128 x 128
  * ([ceil(rows / 128)][ceil(cols / 128)]). A block that holds an infinity or NaN stands for NaN throughout.
- * Arrays need the alignment of their type only, except where a line below says 16 bytes. */
+ * Arrays need the alignment of their type only, except where a line below says 16 bytes (OMT_INVALID for others). Products take
+ * up to 2^30 rows, and weights of up to 2^20 rows and columns; else OMT_UNSUPPORTED. */
 
 /* h = x + residual (residual may be null: h = x, not written); y = h / sqrt(mean(h^2) + eps) * weight, written to y in
  * x's type and / or to q and scale in 8 bits; rstd (may be null) gets 1 / sqrt(mean(h^2) + eps) of each row. The weight
@@ -642,7 +643,7 @@ int omt_quantize_fp8_weight(int dtype, int64_t rows, int64_t cols, const void* w
 /* c[m][n] = sum over k of a[m][k] b[n][k], both in 8 bits with scales (a by 1 x 128, b by 128 x 128); c in out_dtype.
  * OMT_DT_F32: float32 sums of exact products. OMT_DT_BF16: of eight consecutive products, what is under 2^-13 of the largest may
  * be lost, by the 8-bit matrix instructions.
- * a, b and the workspace on 16 bytes. */
+ * a, b, c and the workspace on 16 bytes. */
 size_t omt_matmul_fp8_workspace(int64_t m, int64_t n, int64_t k, int out_dtype);
 int omt_matmul_fp8(int64_t m, int64_t n, int64_t k, const void* a, const float* a_scale, const void* b,
                    const float* b_scale, int out_dtype, void* c, void* workspace, size_t workspace_bytes, void* stream);
@@ -654,15 +655,15 @@ enum { OMT_GLU_SILU = 0, OMT_GLU_GELU = 1, OMT_GLU_RELU = 2 };
  * omt_quantize_fp8); or g and u in x's type, and x itself. */
 enum { OMT_KEEP_NONE = 0, OMT_KEEP_FP8 = 1, OMT_KEEP_FULL = 2 };
 
-/* keep OMT_KEEP_FP8: x_q and x_scale, g and g_scale, u and u_scale are written; OMT_KEEP_FULL: g and u. x, the weights
- * and the workspace on 16 bytes. */
+/* keep OMT_KEEP_FP8: x_q and x_scale, g and g_scale, u and u_scale are written; OMT_KEEP_FULL: g and u. x, the weights,
+ * h, g, u and the workspace on 16 bytes. */
 size_t omt_glu_fwd_workspace(int dtype, int64_t m, int64_t k, int64_t f);
 int omt_glu_fwd(int dtype, int64_t m, int64_t k, int64_t f, int act, int keep, const void* x, const void* w_gate,
                 const void* w_up, void* h, void* x_q, float* x_scale, void* g, float* g_scale, void* u, float* u_scale,
                 void* workspace, size_t workspace_bytes, void* stream);
-/* The gradients of x (gx), w_gate and w_up (each may be null) from gh, the gradient of h, and what the forward pass
+/* The gradients of x (gx, may be null), w_gate and w_up (both or neither) from gh, the gradient of h, and what the forward pass
  * kept: OMT_KEEP_FP8 or, with x in x and no scales, OMT_KEEP_FULL. x, the weights, the gradients and the workspace on 16
- * bytes. */
+ * bytes. Up to 2^20 rows, f up to 2^18. */
 size_t omt_glu_bwd_workspace(int dtype, int64_t m, int64_t k, int64_t f);
 int omt_glu_bwd(int dtype, int64_t m, int64_t k, int64_t f, int act, int keep, const void* gh, const void* x,
                 const float* x_scale, const void* g, const float* g_scale, const void* u, const float* u_scale,
@@ -676,7 +677,8 @@ int omt_glu_bwd(int dtype, int64_t m, int64_t k, int64_t f, int act, int keep, c
 enum { OMT_FFN_MATMUL_FP8 = 0, OMT_FFN_GLU = 1, OMT_FFN_GLU_FP8 = 2, OMT_FFN_GLU_GX = 3, OMT_FFN_GLU_GW = 4 };
 int omt_ffn_plan(int op, int dtype, int64_t m, int64_t k, int64_t n, int* mode, int* rows, int* sharers);
 
-/* omt_glu_fwd of operands in 8 bits (weights by 128 x 128), h in 8 bits. x, the weights and the workspace on 16 bytes. */
+/* omt_glu_fwd of operands in 8 bits (weights by 128 x 128), h in 8 bits. x, the weights, h_q and the workspace on 16
+ * bytes. */
 size_t omt_glu_fp8_workspace(int64_t m, int64_t k, int64_t f);
 int omt_glu_fp8(int64_t m, int64_t k, int64_t f, int act, const void* x, const float* x_scale, const void* w_gate,
                 const float* gate_scale, const void* w_up, const float* up_scale, void* h_q, float* h_scale,

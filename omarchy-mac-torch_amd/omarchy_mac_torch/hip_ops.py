@@ -871,7 +871,7 @@ def glu(x, w_gate, w_up, act="silu", checkpoint=None):
     """The gated feed-forward block's first half: h = act(x w_gate^T) * (x w_up^T), x [..., k], weights [f, k], act
     "silu", "gelu" (by erf) or "relu". Returns (h, kept): kept is what glu_backward needs, as `checkpoint` says: None;
     "fp8": (x, x's scales, g, g's, u, u's), x and both projections in 8 bits (x's scales are powers of two); or "full":
-    (x, None, g, None, u, None) in x's type."""
+    (x, None, g, None, u, None) in x's type. Up to 2^30 rows of x, and weights of up to 2^20 rows and columns."""
     if checkpoint not in _KEEPS:
         raise ValueError(f"checkpoint: expected None, 'fp8' or 'full', got {checkpoint!r}")
     h, *kept = _ffn("glu", x, w_gate, w_up, _glu_act(act), _KEEPS[checkpoint])
@@ -882,7 +882,7 @@ def glu(x, w_gate, w_up, act="silu", checkpoint=None):
 
 def glu_backward(gh, kept, w_gate, w_up, act="silu", input_grad=True, weight_grad=True):
     """The gradients of glu's x, w_gate and w_up from gh, the gradient of h, and what glu kept. A gradient that is not
-    asked for is None."""
+    asked for is None. Up to 2^20 rows of x, and weights of up to 2^18 rows."""
     if len(kept) != 6:
         raise ValueError(f"kept: expected glu's six values, got {len(kept)}")
     return _ffn("glu_backward", gh, *kept, w_gate, w_up, _glu_act(act), input_grad, weight_grad)

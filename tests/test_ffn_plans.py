@@ -1,4 +1,4 @@
-"""Which tiles and shares the feed-forward products take, without a GPU."""
+"""Which tiles and shares the feed-forward products take, and which addresses and sizes, without a GPU."""
 
 import ctypes
 
@@ -60,3 +60,36 @@ def test_every_combination_that_random_sizes_lead_to_is_run(plan):
     tested = {kind(*p) for p in test_gpu_ffn.PLANS + test_gpu_ffn.ACROSS + test_gpu_ffn.FEW + test_gpu_ffn_plans.MORE}
     met = {kind(op, dtype, *size) for size in random_sizes(1, 4000, 1, 13) for op in OPS for dtype in (F32, BF16)}
     assert len(met) > 100 and met <= tested, sorted(met - tested)
+
+
+def test_alignment_and_sizes_as_the_header_has_them():
+    """Every address that the header wants on 16 bytes is refused off them before anything runs, and every size past its limits."""
+    from omarchy_mac_torch import _lib
+    L, on, off = _lib.L, 4096, 4100
+    big = 1 << 40  # of workspace
+
+    def refused(entry, sizes, pointers, tail, aligned):
+        for i in aligned:
+            args = [ctypes.c_void_p(off if j == i else on) for j in range(len(pointers))]
+            assert entry(*sizes, *args, *tail) == _lib.OMT_INVALID, (entry.__name__, pointers[i])
+
+    def product(a, a_scale, b, b_scale, c, ws):
+        return L.omt_matmul_fp8(8, 16, 33, a, a_scale, b, b_scale, F32, c, ws, big, None)
+
+    product.__name__ = "omt_matmul_fp8"
+    refused(product, (), ["a", "a_scale", "b", "b_scale", "c", "workspace"], (), [0, 2, 4, 5])
+    names = ["x", "w_gate", "w_up", "h", "x_q", "x_scale", "g", "g_scale", "u", "u_scale", "workspace"]
+    refused(L.omt_glu_fwd, (BF16, 8, 33, 16, 0, 1), names, (big, None), [0, 1, 2, 3, 6, 8, 10])
+    names = ["gh", "x", "x_scale", "g", "g_scale", "u", "u_scale", "w_gate", "w_up", "gx", "gw_gate", "gw_up", "workspace"]
+    refused(L.omt_glu_bwd, (BF16, 8, 32, 16, 0, 1), names, (big, None), [1, 7, 8, 9, 10, 11, 12])
+    names = ["x", "x_scale", "w_gate", "gate_scale", "w_up", "up_scale", "h_q", "h_scale", "workspace"]
+    refused(L.omt_glu_fp8, (8, 33, 16, 0), names, (big, None), [0, 2, 4, 6, 8])
+
+    p = ctypes.c_void_p(on)
+    over = (1 << 30) + 1, (1 << 20) + 1
+    for m, n, k in ((over[0], 8, 8), (8, over[1], 8), (8, 8, over[1])):
+        assert L.omt_matmul_fp8(m, n, k, p, p, p, p, F32, p, p, big, None) == _lib.OMT_UNSUPPORTED
+        assert L.omt_glu_fwd(F32, m, k, n, 0, 0, *[p] * 11, big, None) == _lib.OMT_UNSUPPORTED
+        assert L.omt_glu_fp8(m, k, n, 0, *[p] * 9, big, None) == _lib.OMT_UNSUPPORTED
+    for m, n in (((1 << 20) + 1, 8), (8, (1 << 18) + 1)):
+        assert L.omt_glu_bwd(F32, m, 8, n, 0, 1, *[p] * 13, big, None) == _lib.OMT_UNSUPPORTED
