@@ -621,7 +621,8 @@ int omt_fused_sgd(const omt_sgd_params* params, const omt_sgd_tensor* tensors, i
  * the last block of a row may be shorter), scale = max(largest magnitude, 1e-30) / 448; for weights of 128 x 128
  * ([ceil(rows / 128)][ceil(cols / 128)]). A block that holds an infinity or NaN stands for NaN throughout.
  * Arrays need the alignment of their type only, except where a line below says 16 bytes (OMT_INVALID for others). Products take
- * up to 2^30 rows, and weights of up to 2^20 rows and columns; else OMT_UNSUPPORTED. */
+ * up to 2^30 rows, weights of up to 2^20 rows and columns, and fewer than 2^23 tiles (of up to 256 x 256 results, 256 x 128 of the
+ * gated block); else OMT_UNSUPPORTED. */
 
 /* h = x + residual (residual may be null: h = x, not written); y = h / sqrt(mean(h^2) + eps) * weight, written to y in
  * x's type and / or to q and scale in 8 bits; rstd (may be null) gets 1 / sqrt(mean(h^2) + eps) of each row. The weight

@@ -696,8 +696,11 @@ ffn_gemm_kernel(GemmArgs a) {
 
 template <int MODE, bool GLU, int BM, int NS, bool XT = false, bool WT = false>
 int launch_gemm(const GemmArgs& a, hipStream_t stream) {
-  hipLaunchKernelGGL((ffn_gemm_kernel<MODE, GLU, BM, NS, XT, WT>), dim3((unsigned)(a.whole + a.sharers)),
-                     dim3(GemmTile<MODE, BM, NS>::THREADS), 0, stream, a);
+  constexpr int kThreads = GemmTile<MODE, BM, NS>::THREADS;
+  const int64_t tiles = (int64_t)a.gx * a.gy, groups = (int64_t)a.whole + a.sharers;
+  if ((tiles > groups ? tiles : groups) * kThreads > UINT32_MAX)  // what a launch holds; one of more runs a part of it and says nothing
+    return fail(OMT_UNSUPPORTED, "ffn_gemm_kernel: %lld tiles", (long long)tiles);
+  hipLaunchKernelGGL((ffn_gemm_kernel<MODE, GLU, BM, NS, XT, WT>), dim3((unsigned)groups), dim3(kThreads), 0, stream, a);
   return launch_check("ffn_gemm_kernel");
 }
 

@@ -93,3 +93,11 @@ def test_alignment_and_sizes_as_the_header_has_them():
         assert L.omt_glu_fp8(m, k, n, 0, *[p] * 9, big, None) == _lib.OMT_UNSUPPORTED
     for m, n in (((1 << 20) + 1, 8), (8, (1 << 18) + 1)):
         assert L.omt_glu_bwd(F32, m, 8, n, 0, 1, *[p] * 13, big, None) == _lib.OMT_UNSUPPORTED
+
+
+def test_products_of_more_tiles_than_a_launch_holds():
+    """2^23 tiles of 512 threads are 2^32: refused, where a launch would run a part of them with no error."""
+    from omarchy_mac_torch import _lib
+    p = ctypes.c_void_p(4096)
+    for f in (256, 1 << 20):  # the latter are 2^35
+        assert _lib.L.omt_glu_fp8(1 << 30, 64, f, 0, *[p] * 9, 1 << 40, None) == _lib.OMT_UNSUPPORTED
