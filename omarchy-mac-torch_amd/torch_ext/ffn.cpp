@@ -5,61 +5,21 @@
 //
 // Arguments are checked here: a wrong type or device raises TypeError, a wrong shape or value ValueError, sizes that no
 // kernel covers NotImplementedError. Operands that are not contiguous, or not on 16 bytes, are copied first.
-#include <ATen/hip/EmptyTensor.h>
-#include <c10/core/DeviceGuard.h>
-#include <c10/hip/HIPFunctions.h>
-#include <c10/hip/HIPStream.h>
-
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 #include <torch/extension.h>
 
-#include "omt_torch.h"
+#include "operands.h"
 
 namespace omt {
 
 namespace {
 
-using OptTensor = std::optional<Tensor>;
 constexpr int64_t kBlock = 128;
 constexpr at::ScalarType kFp8 = at::kFloat8_e4m3fn;
 
 int64_t blocks(int64_t n) { return (n + kBlock - 1) / kBlock; }
-bool on_gpu(const Tensor& t) { return t.device().type() == kDev || t.device().is_cuda(); }
-int dtype_of(const Tensor& t) { return t.scalar_type() == at::kFloat ? OMT_DT_F32 : OMT_DT_BF16; }
 
-// t, contiguous and on 16 bytes, after checking it against a type, and the device and shape of the other operands
-Tensor take(const Tensor& t, const char* name, at::ScalarType type, const Tensor* beside = nullptr,
-            at::OptionalIntArrayRef shape = std::nullopt) {
-  TORCH_CHECK_TYPE(t.defined() && on_gpu(t) && t.scalar_type() == type, name, ": expected ", type,
-                   " on the HIP device, got ", t.defined() ? t.scalar_type() : at::ScalarType::Undefined, " on ",
-                   t.defined() ? t.device() : c10::Device(c10::kCPU));
-  if (beside)
-    TORCH_CHECK_VALUE(t.device() == beside->device(), name, ": on ", t.device(), ", the other operands on ",
-                      beside->device());
-  if (shape) TORCH_CHECK_VALUE(t.sizes().equals(*shape), name, ": expected ", *shape, ", got ", t.sizes());
-  Tensor c = t.contiguous();
-  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
-}
-at::ScalarType real_type(const Tensor& t, const char* name) {
-  TORCH_CHECK_TYPE(t.defined() && (t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16), name,
-                   ": expected float32 or bfloat16 on the HIP device, got ",
-                   t.defined() ? t.scalar_type() : at::ScalarType::Undefined);
-  return t.scalar_type();
-}
-struct Rows {
-  int64_t rows, cols;
-};
-Rows rows_of(const Tensor& t, const char* name) {
-  TORCH_CHECK_VALUE(t.dim() >= 1 && t.size(-1) >= 1, name, ": expected rows of at least one value, got ", t.sizes());
-  return {t.numel() / t.size(-1), t.size(-1)};
-}
-// `shape` with its last dimension replaced
-std::vector<int64_t> with_last(IntArrayRef shape, int64_t last) {
-  auto v = shape.vec();
-  v.back() = last;
-  return v;
-}
 Tensor take_scale(const Tensor& s, const char* name, const Tensor& q) {
   return take(s, name, at::kFloat, &q, with_last(q.sizes(), blocks(q.size(-1))));
 }
@@ -74,41 +34,9 @@ Weight8 take_weight8(const Tensor& q, const Tensor& s, const char* name, const c
   return {c, take(s, scale_name, at::kFloat, &beside, IntArrayRef{blocks(c.size(0)), blocks(cols)})};
 }
 
-// (straight from the allocator: an at::empty through the dispatcher takes twice as long, and a small call makes three)
-Tensor make(const Tensor& like, IntArrayRef shape, at::ScalarType type) {
-  if (is_dev(like)) return empty_dev(shape, type);
-  return Tensor(at::detail::empty_cuda(shape, type, like.device(), std::nullopt));
-}
 Tensor make_scale(const Tensor& like, IntArrayRef shape) {
   return make(like, with_last(shape, blocks(shape.back())), at::kFloat);
 }
-void* raw(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
-float* rawf(const Tensor& t) { return (float*)raw(t); }
-
-// Where a call runs: t's device, its current stream, and scratch memory of that stream.
-struct Site {
-  c10::OptionalDeviceGuard guard;
-  void* stream;
-  Tensor ws;
-  explicit Site(const Tensor& t) {
-    if (!is_dev(t) && t.device().index() != c10::hip::current_device()) guard.reset_device(t.device());
-    stream = cur_stream();
-  }
-  void* scratch(const Tensor& like, size_t bytes) {
-    if (bytes) ws = make(like, {(int64_t)bytes}, at::kByte);
-    return raw(ws);
-  }
-};
-void ok(int status, const char* what) {
-  if (status == OMT_UNSUPPORTED) TORCH_CHECK_NOT_IMPLEMENTED(false, what, ": ", omt_last_error());
-  check(status, what);
-}
-// A call under the device's lock (library calls on one stream are serialized), with its debug check.
-#define FFN_OP(name) \
-  OMT_LOCK;          \
-  struct AtEnd {     \
-    ~AtEnd() noexcept(false) { if (debug_mode() && !std::uncaught_exceptions()) debug_point("omt::" name); } \
-  } at_end_
 
 struct NormOperands {
   Tensor x, weight, other;
@@ -127,7 +55,7 @@ NormOperands norm_operands(const Tensor& x_, const Tensor& weight_, const OptTen
 
 std::tuple<Tensor, Tensor, Tensor> rms_norm(const Tensor& x_, const Tensor& weight_, const OptTensor& residual,
                                             double eps) {
-  FFN_OP("rms_norm");
+  OMT_OP("rms_norm");
   const auto o = norm_operands(x_, weight_, residual, "x", "residual");
   Site at(o.x);
   Tensor y = make(o.x, o.x.sizes(), o.x.scalar_type());
@@ -141,7 +69,7 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm(const Tensor& x_, const Tensor& weig
 
 std::tuple<Tensor, Tensor, Tensor> rms_norm_fp8(const Tensor& x_, const Tensor& weight_, const OptTensor& residual,
                                                 double eps) {
-  FFN_OP("rms_norm_fp8");
+  OMT_OP("rms_norm_fp8");
   const auto o = norm_operands(x_, weight_, residual, "x", "residual");
   Site at(o.x);
   Tensor q = make(o.x, o.x.sizes(), kFp8), scale = make_scale(o.x, o.x.sizes());
@@ -154,7 +82,7 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_fp8(const Tensor& x_, const Tensor& 
 
 std::tuple<Tensor, Tensor> rms_norm_backward(const Tensor& gy_, const Tensor& h_, const Tensor& weight_,
                                              const Tensor& rstd_, const OptTensor& gh, bool weight_grad) {
-  FFN_OP("rms_norm_backward");
+  OMT_OP("rms_norm_backward");
   const auto o = norm_operands(h_, weight_, gh, "h", "gh");
   Tensor gy = take(gy_, "gy", o.x.scalar_type(), &o.x, o.x.sizes());
   Tensor rstd = take(rstd_, "rstd", at::kFloat, &o.x, o.x.sizes().slice(0, o.x.dim() - 1));
@@ -170,7 +98,7 @@ std::tuple<Tensor, Tensor> rms_norm_backward(const Tensor& gy_, const Tensor& h_
 }
 
 std::tuple<Tensor, Tensor> quantize_fp8(const Tensor& x_, bool pow2) {
-  FFN_OP("quantize_fp8");
+  OMT_OP("quantize_fp8");
   Tensor x = take(x_, "x", real_type(x_, "x"));
   const Rows r = rows_of(x, "x");
   Site at(x);
@@ -180,7 +108,7 @@ std::tuple<Tensor, Tensor> quantize_fp8(const Tensor& x_, bool pow2) {
 }
 
 std::tuple<Tensor, Tensor> quantize_fp8_weight(const Tensor& w_) {
-  FFN_OP("quantize_fp8_weight");
+  OMT_OP("quantize_fp8_weight");
   Tensor w = take(w_, "w", real_type(w_, "w"));
   TORCH_CHECK_VALUE(w.dim() == 2 && w.numel() > 0, "w: expected a matrix, got ", w.sizes());
   Site at(w);
@@ -192,7 +120,7 @@ std::tuple<Tensor, Tensor> quantize_fp8_weight(const Tensor& w_) {
 
 Tensor matmul_fp8(const Tensor& a_, const Tensor& a_scale, const Tensor& b_, const Tensor& b_scale,
                   at::ScalarType type) {
-  FFN_OP("matmul_fp8");
+  OMT_OP("matmul_fp8");
   TORCH_CHECK_TYPE(type == at::kFloat || type == at::kBFloat16, "dtype: expected bfloat16 or float32, got ", type);
   Tensor a = take(a_, "a", kFp8);
   const Rows r = rows_of(a, "a");
@@ -220,7 +148,7 @@ GluWeights glu_weights(const Tensor& gate, const Tensor& up, at::ScalarType type
 // (h, x_q, x_scale, g, g_scale, u, u_scale); what `keep` (OMT_KEEP_*) does not ask for is undefined
 std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> glu(const Tensor& x_, const Tensor& w_gate,
                                                                        const Tensor& w_up, int64_t act, int64_t keep) {
-  FFN_OP("glu");
+  OMT_OP("glu");
   Tensor x = take(x_, "x", real_type(x_, "x"));
   const Rows r = rows_of(x, "x");
   const GluWeights w = glu_weights(w_gate, w_up, x.scalar_type(), r.cols, x);
@@ -247,7 +175,7 @@ std::tuple<Tensor, Tensor, Tensor> glu_backward(const Tensor& gh_, const Tensor&
                                                 const Tensor& g_, const OptTensor& g_scale, const Tensor& u_,
                                                 const OptTensor& u_scale, const Tensor& w_gate, const Tensor& w_up,
                                                 int64_t act, bool input_grad, bool weight_grad) {
-  FFN_OP("glu_backward");
+  OMT_OP("glu_backward");
   const at::ScalarType type = real_type(gh_, "gh");
   Tensor gh = take(gh_, "gh", type);
   const Rows r = rows_of(gh, "gh");
@@ -282,7 +210,7 @@ std::tuple<Tensor, Tensor, Tensor> glu_backward(const Tensor& gh_, const Tensor&
 
 std::tuple<Tensor, Tensor> glu_fp8(const Tensor& x_, const Tensor& x_scale, const Tensor& w_gate,
                                    const Tensor& gate_scale, const Tensor& w_up, const Tensor& up_scale, int64_t act) {
-  FFN_OP("glu_fp8");
+  OMT_OP("glu_fp8");
   Tensor x = take(x_, "x", kFp8);
   const Rows r = rows_of(x, "x");
   Tensor xs = take_scale(x_scale, "x's scales", x);
