@@ -506,7 +506,7 @@ int omt_pointwise(int op, int64_t n, const float* a, const float* b, float alpha
  * OMT_FOREACH_MAX_NUMEL each; host arrays) in one launch per 64 tensors: dtype OMT_DT_F32 adds fvalue, OMT_DT_I64 adds
  * ivalue. The optimizers' step counts and BatchNorm's batch counters. Replaces the reference's _foreach_* handling,
  * which loops the per-tensor add on the device (csrc/device.cpp:220-225). */
-enum { OMT_DT_F32 = 0, OMT_DT_I64 = 1, OMT_DT_BF16 = 2 };
+enum { OMT_DT_F32 = 0, OMT_DT_I64 = 1, OMT_DT_BF16 = 2, OMT_DT_I32 = 3 };
 #define OMT_FOREACH_MAX_NUMEL (1 << 16)
 int omt_foreach_add_scalar(int count, void* const* ptrs, const int64_t* numels, int dtype, int64_t ivalue,
                            float fvalue, void* stream);
@@ -684,6 +684,90 @@ size_t omt_glu_fp8_workspace(int64_t m, int64_t k, int64_t f);
 int omt_glu_fp8(int64_t m, int64_t k, int64_t f, int act, const void* x, const float* x_scale, const void* w_gate,
                 const float* gate_scale, const void* w_up, const float* up_scale, void* h_q, float* h_scale,
                 void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- both ends of a language model's training step: embedding, losses on logits, AdamW ------------------------------
+ *
+ * No counterpart in the reference. Types are OMT_DT_F32 or OMT_DT_BF16; arrays need the alignment of their type only (those on 16
+ * bytes, with rows of a multiple of eight elements, take the vector paths), workspaces 16 bytes. Every sum runs in a fixed order. */
+
+/* y[i] = scale * weight[tokens[i]], weight [vocab][dim], tokens of OMT_DT_I64 or OMT_DT_I32. A token outside the vocabulary gives
+ * a row of NaN and touches no memory. */
+int omt_embedding_fwd(int dtype, int token_dtype, int64_t n, int64_t vocab, int64_t dim, const void* tokens, const void* weight,
+                      float scale, void* y, void* stream);
+/* gweight[v] = scale * sum of gy[i] over the i with tokens[i] = v, in their order, float32 sums rounded once; zeros for v =
+ * padding_idx (negative: none) and for rows without positions. Tokens outside the vocabulary take no part. Up to 2^28 tokens and
+ * rows and 2^16 columns, and fewer than 2^24 workgroups (OMT_UNSUPPORTED otherwise). */
+size_t omt_embedding_bwd_workspace(int64_t n, int64_t vocab, int64_t dim);
+int omt_embedding_bwd(int dtype, int token_dtype, int64_t n, int64_t vocab, int64_t dim, const void* gy, const void* tokens,
+                      int64_t padding_idx, float scale, void* gweight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Logits x [sequences][length][vocab], each row dense, strides in elements, with labels [sequences][length] (dense). A row whose
+ * label is ignore_index does not count and is not read; another label outside the vocabulary makes the loss and the row's gradient
+ * NaN. Up to 2^28 rows and columns (OMT_UNSUPPORTED otherwise). Gradients gx are dense, in x's type. */
+typedef struct omt_logits {
+  const void* x;
+  const int64_t* labels;
+  int64_t ignore_index;
+  int64_t sequences, length, vocab;
+  int64_t sequence_stride, row_stride;
+  int dtype;
+} omt_logits;
+
+/* logps = x[label] - lse, lse = log(sum exp x), each [sequences][length]; 0 in both where a row does not count. The backward:
+ * gx = g (onehot(label) - exp(x - lse)), g the gradient of logps. */
+int omt_token_logps_fwd(const omt_logits* logits, float* logps, float* lse, void* stream);
+int omt_token_logps_bwd(const omt_logits* logits, const float* lse, const float* g, void* gx, void* stream);
+
+/* Pairs of sequences, the chosen ones in the first half and the rejected ones, in the same order, in the second. L: the sum of a
+ * sequence's logps, or with `average` their mean (0 where none counts); R: reference[sequences]; d = (L - R of the chosen) - (L - R
+ * of the rejected). Loss, the mean over pairs of
+ *   OMT_PREFERENCE_SIGMOID  -(1 - smoothing) log sigmoid(beta d) - smoothing log sigmoid(-beta d)
+ *   OMT_PREFERENCE_HINGE    max(0, 1 - beta d)
+ *   OMT_PREFERENCE_IPO      (d - 1 / (2 beta))^2
+ * rewards[sequences] = beta (L - R). gx: the loss's gradient (null: not asked for). beta > 0, smoothing in [0, 1]. */
+enum { OMT_PREFERENCE_SIGMOID = 0, OMT_PREFERENCE_HINGE = 1, OMT_PREFERENCE_IPO = 2 };
+size_t omt_preference_workspace(int64_t sequences, int64_t length);
+int omt_preference_loss(const omt_logits* logits, const float* reference, int kind, double beta, double smoothing, int average,
+                        float* loss, float* rewards, void* gx, void* workspace, size_t workspace_bytes, void* stream);
+
+/* r = exp(logps - old_logps); a token's loss is -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_weight k with k =
+ * exp(reference - logps) - (reference - logps) - 1 (0 where reference is null); old_logps and reference [sequences][length], A =
+ * advantages[sequence * advantage_sequence_stride + row * advantage_row_stride]. loss, and kl of k: the mean over all tokens
+ * that count or, by_sequence, over sequences of each one's mean (0 of one where none counts). logps as omt_token_logps_fwd's. gx:
+ * the loss's gradient (null: not asked for). */
+size_t omt_policy_workspace(int64_t sequences, int64_t length, int by_sequence);
+int omt_policy_loss(const omt_logits* logits, const float* old_logps, const float* reference, const float* advantages,
+                    int64_t advantage_sequence_stride, int64_t advantage_row_stride, double clip_low, double clip_high,
+                    double kl_weight, int by_sequence, float* loss, float* kl, float* logps, void* gx, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/* x *= *factor (a float on the device), in place; nothing is read or written where it is 1. */
+int omt_scale_by(int dtype, int64_t n, void* x, const float* factor, void* stream);
+
+/* One parameter of an AdamW step: param and grad of the call's type, its step count (a float on the device, already incremented).
+ * master (bfloat16 parameters; of all tensors of a call, or null in all): the float32 copy that is updated, param its rounding.
+ * States of 32 bits: float32, no scales. Of 8 bits: e4m3 with a scale for each block of 128 consecutive elements
+ * ([ceil(numel / 128)]), max(largest magnitude, 1e-30) / 448; exp_avg_sq then holds the second moment's square root, and what is
+ * over 0 as e4m3's smallest value at least. */
+typedef struct omt_adamw_tensor {
+  void* param;
+  const void* grad;
+  float* master;
+  void* exp_avg;
+  float* exp_avg_scale;
+  void* exp_avg_sq;
+  float* exp_avg_sq_scale;
+  const float* step;
+  int64_t numel;
+} omt_adamw_tensor;
+/* lr_dev (a float on the device) overrides lr; grad_scale divides the gradients (which stay as they are), found_inf == 1 on the
+ * device skips the step; all optional. */
+typedef struct omt_adamw_params {
+  double lr, beta1, beta2, weight_decay, eps;
+  const float *lr_dev, *grad_scale, *found_inf;
+  int maximize;
+} omt_adamw_params;
+int omt_adamw(int dtype, int state_bits, const omt_adamw_params* params, const omt_adamw_tensor* tensors, int count, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,477 @@
+// Embedding: y[i] = scale * weight[token_i], and its gradient gw[v] = scale * (sum over i with token_i = v of gy[i]), the
+// positions of a token in their order, so that the same inputs give the same bits: no atomics on values.
+//
+// The gradient sorts the positions by token (a stable sort by digits of up to 9 bits: a workgroup in LDS up to 8192
+// positions; above, at most 64 workgroups, which count and then scatter each digit), cuts the sorted positions into runs of
+// equal length, whatever the tokens' frequencies, and sums each run's rows of gy in float32: what begins and ends within a run
+// is rounded and written at once, the sums of a token that reaches over runs are joined by a second launch. Rows that no
+// position holds are written as zeros by the workgroups behind the runs'. Bound by memory: gy is read once, gw written once.
+//
+// Tokens outside the vocabulary: a row of NaN, and no part in the gradient; no memory is touched for them.
+#include <algorithm>
+
+#include "block_fp8.h"
+
+namespace omt {
+
+struct TokenArray {
+  const void* p;
+  int wide;  // int64, else int32
+  __device__ __forceinline__ int64_t operator[](int64_t i) const {
+    return wide ? ((const int64_t*)p)[i] : (int64_t)((const int32_t*)p)[i];
+  }
+};
+
+// ---- forward --------------------------------------------------------------------------------------------------------
+
+struct EmbedArgs {
+  TokenArray tokens;
+  const void* weight;
+  void* y;
+  int64_t n, vocab, dim;
+  float scale;
+};
+
+// LANES threads to a row, eight consecutive columns to a thread at a time
+template <class T, bool VEC, int LANES>
+__global__ void __launch_bounds__(256) embedding_kernel(EmbedArgs a) {
+  const int64_t row = ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * (256 / LANES) + threadIdx.x / LANES;
+  if (row >= a.n) return;
+  const int64_t token = a.tokens[row];
+  const bool known = (uint64_t)token < (uint64_t)a.vocab;
+  const T* w = (const T*)a.weight + (known ? token : 0) * a.dim;
+  T* y = (T*)a.y + row * a.dim;
+  const float scale = known ? a.scale : __builtin_nanf("");
+  constexpr int U = 4;
+  for (int64_t c = (int64_t)(threadIdx.x % LANES) * 8; c < a.dim; c += LANES * 8 * U) {
+    f32x8 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = load8<VEC>(w, c + u * LANES * 8, a.dim);
+#pragma unroll
+    for (int u = 0; u < U; ++u) store8<VEC>(y, c + u * LANES * 8, a.dim, v[u] * scale);
+  }
+}
+
+// ---- sorting positions by token -------------------------------------------------------------------------------------
+
+constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
+constexpr int kDigitBits = 9, kBins = 1 << kDigitBits;
+constexpr int kSmallSort = 8192;  // positions that one workgroup sorts in LDS
+constexpr int kSortTiles = 64;    // workgroups of a larger sort at most: each adds up the counts of all
+
+// Tokens as keys: those that take part in the gradient, `vocab` for the others, which so come last.
+struct KeyOf {
+  TokenArray tokens;
+  int64_t vocab, padding;
+  __device__ __forceinline__ uint32_t operator()(int64_t i) const {
+    const int64_t t = tokens[i];
+    return (uint64_t)t < (uint64_t)vocab && t != padding ? (uint32_t)t : (uint32_t)vocab;
+  }
+};
+
+// the wave's lanes, among those that are `on`, with this lane's digit
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, bool on, int bits) {
+  uint64_t m = __ballot(on);
+  for (int b = 0; b < bits; ++b) {
+    const bool one = digit >> b & 1;
+    const uint64_t with = __ballot(on && one);
+    m &= one ? with : ~with;
+  }
+  return m;
+}
+__device__ __forceinline__ uint64_t lanes_below() { return (1ull << (threadIdx.x & 63)) - 1; }
+
+// counts[digit] += the keys of [beg, end) with it, by one wave
+template <class Key>
+__device__ __forceinline__ void count_digits(uint32_t* counts, int64_t beg, int64_t end, Key key, int shift, int bits) {
+  for (int64_t i = beg; i < end; i += 64) {
+    const int64_t j = i + (threadIdx.x & 63);
+    const bool on = j < end;
+    const uint32_t digit = on ? key(j) >> shift & ((1u << bits) - 1) : 0;
+    const uint64_t same = same_digit(digit, on, bits);
+    if (on && !(same & lanes_below())) atomicAdd(&counts[digit], (uint32_t)__popcll(same));
+  }
+}
+// put(j, place) for the keys of [beg, end) in order, by one wave; at[digit] is the digit's next place
+template <class Key, class Put>
+__device__ __forceinline__ void place_digits(uint32_t* at, int64_t beg, int64_t end, Key key, int shift, int bits, Put put) {
+  for (int64_t i = beg; i < end; i += 64) {
+    const int64_t j = i + (threadIdx.x & 63);
+    const bool on = j < end;
+    const uint32_t digit = on ? key(j) >> shift & ((1u << bits) - 1) : 0;
+    const uint64_t same = same_digit(digit, on, bits), below = same & lanes_below();
+    uint32_t first = 0;
+    if (on && !below) first = atomicAdd(&at[digit], (uint32_t)__popcll(same));
+    first = __shfl(first, on ? __ffsll((unsigned long long)same) - 1 : 0);
+    if (on) put(j, first + (uint32_t)__popcll(below));
+  }
+}
+// Of kBins values, one to each of the first kBins threads, the sum of those before it; all threads call it.
+__device__ __forceinline__ uint32_t exclusive_scan(uint32_t v, uint32_t* sums) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t run = v;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    const uint32_t up = __shfl_up(run, d);
+    if (lane >= d) run += up;
+  }
+  __syncthreads();
+  if (lane == 63) sums[wave] = run;
+  __syncthreads();
+  for (int i = 0; i < wave; ++i) run += sums[i];
+  return run - v;
+}
+
+// Up to kSmallSort positions, all digits, in one workgroup.
+__global__ void __launch_bounds__(kSortThreads) sort_small_kernel(KeyOf key, int n, int bits, int passes, uint32_t* keys_out,
+                                                                  uint32_t* pos_out) {
+  __shared__ uint32_t keys[2][kSmallSort];
+  __shared__ uint16_t pos[2][kSmallSort];
+  __shared__ uint32_t counts[kSortWaves][kBins];
+  __shared__ uint32_t sums[kSortWaves];
+  const int wave = threadIdx.x >> 6;
+  for (int i = threadIdx.x; i < n; i += kSortThreads) keys[0][i] = key(i), pos[0][i] = (uint16_t)i;
+  const int share = (n + kSortThreads - 1) / kSortThreads * 64;  // consecutive positions of a wave
+  const int beg = min(wave * share, n), end = min(beg + share, n);
+  for (int p = 0; p < passes; ++p) {
+    const uint32_t* from = keys[p & 1];
+    const uint16_t* from_pos = pos[p & 1];
+    uint32_t* to = keys[~p & 1];
+    uint16_t* to_pos = pos[~p & 1];
+    for (int i = threadIdx.x; i < kSortWaves * kBins; i += kSortThreads) counts[0][i] = 0;
+    __syncthreads();
+    auto at = [&](int64_t j) { return from[j]; };
+    count_digits(counts[wave], beg, end, at, p * bits, bits);
+    __syncthreads();
+    uint32_t total = 0;
+    if (threadIdx.x < kBins)
+      for (int w = 0; w < kSortWaves; ++w) total += counts[w][threadIdx.x];
+    uint32_t first = exclusive_scan(total, sums);
+    if (threadIdx.x < kBins)
+      for (int w = 0; w < kSortWaves; ++w) {
+        const uint32_t c = counts[w][threadIdx.x];
+        counts[w][threadIdx.x] = first;
+        first += c;
+      }
+    __syncthreads();
+    place_digits(counts[wave], beg, end, at, p * bits, bits, [&](int64_t j, uint32_t place) {
+      to[place] = from[j];
+      to_pos[place] = from_pos[j];
+    });
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < n; i += kSortThreads) keys_out[i] = keys[passes & 1][i], pos_out[i] = pos[passes & 1][i];
+}
+
+// The keys and positions that a pass of a larger sort reads: the tokens themselves (keys null), or the pass before.
+struct SortFrom {
+  KeyOf key;
+  const uint32_t *keys, *pos;
+};
+struct SortArgs {
+  SortFrom from;
+  uint32_t *keys, *pos;  // what it writes
+  uint32_t* counts;      // [workgroups][kBins]
+  int64_t n, tile;       // positions, and how many to a workgroup
+  int shift, bits;
+};
+
+template <bool FIRST>
+__device__ __forceinline__ uint32_t key_at(const SortFrom& f, int64_t j) {
+  return FIRST ? f.key(j) : f.keys[j];
+}
+
+template <bool FIRST>
+__global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortArgs a) {
+  __shared__ uint32_t counts[kBins];
+  if (threadIdx.x < kBins) counts[threadIdx.x] = 0;
+  __syncthreads();
+  const int64_t share = a.tile / kSortWaves;
+  const int64_t beg = min(blockIdx.x * a.tile + (threadIdx.x >> 6) * share, a.n), end = min(beg + share, a.n);
+  count_digits(counts, beg, end, [&](int64_t j) { return key_at<FIRST>(a.from, j); }, a.shift, a.bits);
+  __syncthreads();
+  if (threadIdx.x < kBins) a.counts[blockIdx.x * kBins + threadIdx.x] = counts[threadIdx.x];
+}
+
+template <bool FIRST>
+__global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortArgs a) {
+  __shared__ uint32_t counts[kSortWaves][kBins];
+  __shared__ uint32_t sums[kSortWaves];
+  const int wave = threadIdx.x >> 6;
+  for (int i = threadIdx.x; i < kSortWaves * kBins; i += kSortThreads) counts[0][i] = 0;
+  __syncthreads();
+  const int64_t share = a.tile / kSortWaves;
+  const int64_t beg = min(blockIdx.x * a.tile + wave * share, a.n), end = min(beg + share, a.n);
+  auto key = [&](int64_t j) { return key_at<FIRST>(a.from, j); };
+  count_digits(counts[wave], beg, end, key, a.shift, a.bits);
+  uint32_t total = 0, before = 0;  // of this thread's digit, over all workgroups and over those before this one
+  if (threadIdx.x < kBins)
+    for (unsigned t = 0; t < gridDim.x; ++t) {
+      const uint32_t c = a.counts[t * kBins + threadIdx.x];
+      total += c;
+      before += t < blockIdx.x ? c : 0;
+    }
+  uint32_t first = exclusive_scan(total, sums) + before;  // (its barriers stand between the counts above and their use below)
+  if (threadIdx.x < kBins)
+    for (int w = 0; w < kSortWaves; ++w) {
+      const uint32_t c = counts[w][threadIdx.x];
+      counts[w][threadIdx.x] = first;
+      first += c;
+    }
+  __syncthreads();
+  place_digits(counts[wave], beg, end, key, a.shift, a.bits, [&](int64_t j, uint32_t place) {
+    a.keys[place] = key(j);
+    a.pos[place] = FIRST ? (uint32_t)j : a.from.pos[j];
+  });
+}
+
+// ---- sums of the sorted rows ----------------------------------------------------------------------------------------
+
+struct SumArgs {
+  const void* gy;
+  const uint32_t *keys, *pos;  // sorted
+  float* parts;                // [runs][2][dim]: what a run holds of a token that began before it, and of one that goes on after
+  void* gw;
+  int64_t n, vocab, dim;
+  int64_t run, runs;   // positions to a run, and how many
+  int64_t sum_groups;  // workgroups that sum; those behind them write zeros
+  float scale;
+};
+
+constexpr int kZeroRows = 64;  // rows of the weight to a workgroup that writes zeros
+
+// the first place in the sorted keys from which on they are `key` or more
+__device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t n, uint32_t key) {
+  int64_t lo = 0, hi = n;
+  while (lo < hi) {
+    const int64_t mid = (lo + hi) / 2;
+    if (keys[mid] < key) lo = mid + 1; else hi = mid;
+  }
+  return lo;
+}
+
+template <class T, bool VEC>
+__device__ __forceinline__ void write_zero_rows(const SumArgs& a, int64_t first) {
+  __shared__ uint8_t empty[kZeroRows];
+  const int rows = (int)min((int64_t)kZeroRows, a.vocab - first);
+  if ((int)threadIdx.x < rows) {
+    const uint32_t v = (uint32_t)(first + threadIdx.x);
+    const int64_t at = lower_bound(a.keys, a.n, v);
+    empty[threadIdx.x] = !(at < a.n && a.keys[at] == v);
+  }
+  __syncthreads();
+  const int lane = threadIdx.x & 63;
+  for (int r = threadIdx.x >> 6; r < rows; r += 4)
+    if (empty[r])
+      for (int64_t c = lane * 8; c < a.dim; c += 512) store8<VEC>((T*)a.gw + (first + r) * a.dim, c, a.dim, f32x8{});
+}
+
+// LANES threads to a run and 8 LANES columns
+template <class T, bool VEC, int LANES>
+__global__ void __launch_bounds__(256) embedding_sum_kernel(SumArgs a) {
+  if ((int64_t)blockIdx.x >= a.sum_groups) return write_zero_rows<T, VEC>(a, (blockIdx.x - a.sum_groups) * (int64_t)kZeroRows);
+  const int64_t chunks = (a.dim + LANES * 8 - 1) / (LANES * 8);
+  const int64_t unit = blockIdx.x * (int64_t)(256 / LANES) + threadIdx.x / LANES;
+  const int64_t run = unit / chunks, c = (unit % chunks * LANES + threadIdx.x % LANES) * 8;
+  if (run >= a.runs || c >= a.dim) return;
+  const int64_t beg = run * a.run, end = min(beg + a.run, a.n);
+  const uint32_t none = (uint32_t)a.vocab;
+  uint32_t key = a.keys[beg];
+  bool began = beg > 0 && a.keys[beg - 1] == key;  // before this run
+  f32x8 sum = {};
+  auto put = [&](bool goes_on) {
+    if (key == none) return;
+    if (began || goes_on) store8<false>(a.parts + (run * 2 + (began ? 0 : 1)) * a.dim, c, a.dim, sum);
+    else store8<VEC>((T*)a.gw + key * a.dim, c, a.dim, sum * a.scale);
+  };
+  constexpr int U = 4;
+  for (int64_t i = beg; i < end; i += U) {
+    f32x8 v[U];
+    uint32_t k[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      k[u] = i + u < end ? a.keys[i + u] : none;
+      v[u] = k[u] != none ? load8<VEC>((const T*)a.gy + (int64_t)a.pos[i + u] * a.dim, c, a.dim) : f32x8{};
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (i + u >= end) break;
+      if (k[u] != key) {
+        put(false);
+        key = k[u], began = false, sum = f32x8{};
+      }
+      sum += v[u];
+    }
+  }
+  put(end < a.n && a.keys[end] == key);
+}
+
+// gw of the tokens that began in run blockIdx.x and go on after it: the runs' sums, in order
+template <class T, bool VEC, int LANES>
+__global__ void __launch_bounds__(256) embedding_join_kernel(SumArgs a) {
+  __shared__ f32x8 sums[256];
+  const int64_t run = blockIdx.x, beg = run * a.run, end = min(beg + a.run, a.n);
+  const uint32_t key = a.keys[end - 1];
+  if (key == (uint32_t)a.vocab || end == a.n || a.keys[end] != key) return;  // (the same for the whole workgroup)
+  if (beg > 0 && a.keys[beg - 1] == key) return;                            // began before
+  const int64_t last = (lower_bound(a.keys, a.n, key + 1) - 1) / a.run;      // the run where it ends
+  constexpr int GROUPS = 256 / LANES;
+  const int g = threadIdx.x / LANES;
+  const int64_t count = last - run, share = (count + GROUPS - 1) / GROUPS;  // runs after this one, and to a group of threads
+  const int64_t from = run + 1 + min(g * share, count), to = min(from + share, last + 1);
+  for (int64_t c0 = 0; c0 < a.dim; c0 += LANES * 8) {
+    const int64_t c = c0 + threadIdx.x % LANES * 8;
+    f32x8 sum = {};
+    if (g == 0) sum = load8<false>(a.parts + (run * 2 + 1) * a.dim, c, a.dim);
+#pragma unroll 4
+    for (int64_t r = from; r < to; ++r) sum += load8<false>(a.parts + r * 2 * a.dim, c, a.dim);
+    sums[threadIdx.x] = sum;
+    __syncthreads();
+    if (g == 0) {
+      for (int i = 1; i < GROUPS; ++i) sum += sums[i * LANES + threadIdx.x];
+      store8<VEC>((T*)a.gw + key * a.dim, c, a.dim, sum * a.scale);
+    }
+    __syncthreads();
+  }
+}
+
+// Limits: positions are 32-bit, and a launch holds fewer than 2^24 workgroups of 256 threads along one dimension.
+constexpr int64_t kEmbedMaxTokens = 1 << 28, kEmbedMaxVocab = 1 << 28, kEmbedMaxDim = 1 << 16;
+
+// ---- plans ----------------------------------------------------------------------------------------------------------
+
+// Positions to a run: enough runs for the card's threads, no fewer positions than keep the joined sums few.
+static int64_t run_length(int64_t n, int64_t dim) {
+  const int64_t units = cdiv(dim, 512);
+  return std::min<int64_t>(256, std::max<int64_t>(16, cdiv(n * units, 4096)));
+}
+static int digits_of(int64_t vocab) {
+  int bits = 1;
+  while ((int64_t)1 << bits <= vocab) ++bits;  // the key `vocab` among them
+  return bits;
+}
+struct EmbedPlan {
+  int64_t run, runs;
+  size_t counts, sorted, parts;  // bytes: of one array each
+  size_t total() const { return counts + 4 * sorted + parts; }
+};
+static EmbedPlan embed_plan(int64_t n, int64_t dim) {
+  EmbedPlan p;
+  p.run = run_length(n, dim);
+  p.runs = cdiv(n, p.run);
+  p.counts = (size_t)kSortTiles * kBins * 4;
+  p.sorted = (size_t)cdiv(n, 64) * 256;
+  p.parts = (size_t)p.runs * 2 * dim * 4;
+  return p;
+}
+
+static bool on16(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if ((uintptr_t)p & 15) return false;
+  return true;
+}
+static int embed_check(const char* fn, int dtype, int token_dtype, int64_t n, int64_t vocab, int64_t dim) {
+  if (dtype != OMT_DT_F32 && dtype != OMT_DT_BF16) return fail(OMT_INVALID, "%s: dtype %d", fn, dtype);
+  if (token_dtype != OMT_DT_I64 && token_dtype != OMT_DT_I32) return fail(OMT_INVALID, "%s: tokens of dtype %d", fn, token_dtype);
+  if (n < 0 || vocab < 1 || dim < 1)
+    return fail(OMT_INVALID, "%s: %lld tokens, weight %lld x %lld", fn, (long long)n, (long long)vocab, (long long)dim);
+  return OMT_OK;
+}
+// go(LANES): threads to a row of `dim`
+template <class Go>
+static void for_lanes(int64_t dim, Go go) {
+  if (dim <= 64) go(std::integral_constant<int, 8>());
+  else if (dim <= 128) go(std::integral_constant<int, 16>());
+  else if (dim <= 256) go(std::integral_constant<int, 32>());
+  else go(std::integral_constant<int, 64>());
+}
+
+}  // namespace omt
+
+using namespace omt;
+
+OMT_EXPORT int omt_embedding_fwd(int dtype, int token_dtype, int64_t n, int64_t vocab, int64_t dim, const void* tokens,
+                                 const void* weight, float scale, void* y, void* stream) {
+  if (int e = embed_check("omt_embedding_fwd", dtype, token_dtype, n, vocab, dim)) return e;
+  if (n == 0) return OMT_OK;
+  if (!tokens || !weight || !y) return fail(OMT_INVALID, "omt_embedding_fwd: null pointer");
+  const bool vec = dim % 8 == 0 && on16({weight, y});
+  const EmbedArgs a{{tokens, token_dtype == OMT_DT_I64}, weight, y, n, vocab, dim, scale};
+  for_lanes(dim, [&](auto lanes) {
+    constexpr int LANES = decltype(lanes)::value;
+    // a dimension of the grid holds fewer than 2^32 threads: 2^21 workgroups along it, the rest along the other
+    const int64_t groups = cdiv(n, 256 / LANES), along = std::min<int64_t>(groups, 1 << 21);
+    auto go = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, dim3((unsigned)along, (unsigned)cdiv(groups, along)), dim3(256), 0, stream_of(stream), a);
+    };
+    if (dtype == OMT_DT_F32) vec ? go(embedding_kernel<float, true, LANES>) : go(embedding_kernel<float, false, LANES>);
+    else vec ? go(embedding_kernel<__bf16, true, LANES>) : go(embedding_kernel<__bf16, false, LANES>);
+  });
+  return launch_check("embedding_kernel");
+}
+
+OMT_EXPORT size_t omt_embedding_bwd_workspace(int64_t n, int64_t vocab, int64_t dim) {
+  if (n < 0 || n > kEmbedMaxTokens || vocab < 1 || dim < 1) return 0;
+  return embed_plan(n, dim).total();
+}
+
+OMT_EXPORT int omt_embedding_bwd(int dtype, int token_dtype, int64_t n, int64_t vocab, int64_t dim, const void* gy,
+                                 const void* tokens, int64_t padding_idx, float scale, void* gweight, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  const char* fn = "omt_embedding_bwd";
+  if (int e = embed_check(fn, dtype, token_dtype, n, vocab, dim)) return e;
+  if (n > kEmbedMaxTokens || vocab > kEmbedMaxVocab || dim > kEmbedMaxDim)
+    return fail(OMT_UNSUPPORTED, "%s: %lld tokens, weight %lld x %lld", fn, (long long)n, (long long)vocab, (long long)dim);
+  if (!gweight || (n > 0 && (!gy || !tokens))) return fail(OMT_INVALID, "%s: null pointer", fn);
+  const EmbedPlan p = embed_plan(n, dim);
+  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.total())
+    return fail(OMT_INVALID, "%s: workspace of %zu bytes at %p", fn, workspace_bytes, workspace);
+  hipStream_t s = stream_of(stream);
+  char* at = (char*)workspace;
+  uint32_t* counts = (uint32_t*)at;
+  uint32_t *keys[2], *pos[2];
+  at += p.counts;
+  for (int i = 0; i < 2; ++i) {
+    keys[i] = (uint32_t*)at, at += p.sorted;
+    pos[i] = (uint32_t*)at, at += p.sorted;
+  }
+  const KeyOf key{{tokens, token_dtype == OMT_DT_I64}, vocab, padding_idx};
+  const int all = digits_of(vocab), passes = (all + kDigitBits - 1) / kDigitBits, bits = (all + passes - 1) / passes;
+  int last = 0;
+  if (n > 0 && n <= kSmallSort) {
+    hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(kSortThreads), 0, s, key, (int)n, bits, passes, keys[0], pos[0]);
+    if (int e = launch_check("sort_small_kernel")) return e;
+  } else if (n > 0) {
+    const int64_t tile = cdiv(std::max<int64_t>(4096, cdiv(n, kSortTiles)), kSortThreads) * kSortThreads;
+    const unsigned tiles = (unsigned)cdiv(n, tile);
+    for (int q = 0; q < passes; ++q) {
+      const SortArgs a{{key, keys[~q & 1], pos[~q & 1]}, keys[q & 1], pos[q & 1], counts, n, tile, q * bits, bits};
+      hipLaunchKernelGGL(q ? sort_count_kernel<false> : sort_count_kernel<true>, dim3(tiles), dim3(kSortThreads), 0, s, a);
+      if (int e = launch_check("sort_count_kernel")) return e;
+      hipLaunchKernelGGL(q ? sort_place_kernel<false> : sort_place_kernel<true>, dim3(tiles), dim3(kSortThreads), 0, s, a);
+      if (int e = launch_check("sort_place_kernel")) return e;
+      last = q & 1;
+    }
+  }
+  const bool vec = dim % 8 == 0 && on16({gy, gweight});
+  int status = OMT_OK;
+  for_lanes(dim, [&](auto lanes) {
+    constexpr int LANES = decltype(lanes)::value;
+    const int64_t units = p.runs * cdiv(dim, LANES * 8), groups = cdiv(units, 256 / LANES);
+    const SumArgs a{gy, keys[last], pos[last], (float*)at, gweight, n, vocab, dim, p.run, p.runs, groups, scale};
+    auto go = [&](auto kernel, int64_t grid) { hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, s, a); };
+    const int64_t grid = groups + cdiv(vocab, kZeroRows);
+    if (grid >= 1 << 24) {
+      status = fail(OMT_UNSUPPORTED, "%s: %lld tokens, weight %lld x %lld", fn, (long long)n, (long long)vocab, (long long)dim);
+      return;
+    }
+    if (dtype == OMT_DT_F32) vec ? go(embedding_sum_kernel<float, true, LANES>, grid) : go(embedding_sum_kernel<float, false, LANES>, grid);
+    else vec ? go(embedding_sum_kernel<__bf16, true, LANES>, grid) : go(embedding_sum_kernel<__bf16, false, LANES>, grid);
+    status = launch_check("embedding_sum_kernel");
+    if (status || p.runs < 2) return;
+    if (dtype == OMT_DT_F32) vec ? go(embedding_join_kernel<float, true, LANES>, p.runs) : go(embedding_join_kernel<float, false, LANES>, p.runs);
+    else vec ? go(embedding_join_kernel<__bf16, true, LANES>, p.runs) : go(embedding_join_kernel<__bf16, false, LANES>, p.runs);
+    status = launch_check("embedding_join_kernel");
+  });
+  return status;
+}

@@ -20,8 +20,9 @@ TILE_SPLIT = 256  # OMT_TILE_SPLIT
 NOALLOC_SCRATCH_BYTES = 64 << 20  # OMT_NOALLOC_SCRATCH_BYTES
 (OMT_PW_ADD, OMT_PW_MUL, OMT_PW_RELU, OMT_PW_THRESHOLD_BWD, OMT_PW_HARDSWISH, OMT_PW_HARDSWISH_BWD, OMT_PW_HARDSIGMOID,
  OMT_PW_HARDSIGMOID_BWD, OMT_PW_SCALE, OMT_PW_FILL, OMT_PW_ADD_SCALAR) = range(11)
-OMT_DT_F32, OMT_DT_I64, OMT_DT_BF16 = 0, 1, 2
+OMT_DT_F32, OMT_DT_I64, OMT_DT_BF16, OMT_DT_I32 = 0, 1, 2, 3
 OMT_GLU_SILU, OMT_GLU_GELU, OMT_GLU_RELU = 0, 1, 2
+OMT_PREFERENCE_SIGMOID, OMT_PREFERENCE_HINGE, OMT_PREFERENCE_IPO = 0, 1, 2
 OMT_FFN_MATMUL_FP8, OMT_FFN_GLU, OMT_FFN_GLU_FP8, OMT_FFN_GLU_GX, OMT_FFN_GLU_GW = range(5)
 OMT_KEEP_NONE, OMT_KEEP_FP8, OMT_KEEP_FULL = 0, 1, 2
 OMT_ACT_NONE, OMT_ACT_RELU, OMT_ACT_HARDSWISH = 0, 1, 2
@@ -85,10 +86,32 @@ class SgdParams(ctypes.Structure):
                 ("found_inf", ctypes.c_void_p)]
 
 
+class Logits(ctypes.Structure):
+    """omt_logits: logits [sequences][length][vocab] and their labels."""
+    _fields_ = [("x", ctypes.c_void_p), ("labels", ctypes.c_void_p), ("ignore_index", ctypes.c_int64),
+                ("sequences", ctypes.c_int64), ("length", ctypes.c_int64), ("vocab", ctypes.c_int64),
+                ("sequence_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64), ("dtype", ctypes.c_int)]
+
+
+class AdamwTensor(ctypes.Structure):
+    """omt_adamw_tensor: one parameter of an AdamW step with states in 32 bits or in 8."""
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("master", ctypes.c_void_p),
+                ("exp_avg", ctypes.c_void_p), ("exp_avg_scale", ctypes.c_void_p), ("exp_avg_sq", ctypes.c_void_p),
+                ("exp_avg_sq_scale", ctypes.c_void_p), ("step", ctypes.c_void_p), ("numel", ctypes.c_int64)]
+
+
+class AdamwParams(ctypes.Structure):
+    """omt_adamw_params: hyper-parameters of that step."""
+    _fields_ = [("lr", ctypes.c_double), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double),
+                ("weight_decay", ctypes.c_double), ("eps", ctypes.c_double), ("lr_dev", ctypes.c_void_p),
+                ("grad_scale", ctypes.c_void_p), ("found_inf", ctypes.c_void_p), ("maximize", ctypes.c_int)]
+
+
 I64, U32, I32, F32, F64, SZ, VP = (ctypes.c_int64, ctypes.c_uint, ctypes.c_int, ctypes.c_float, ctypes.c_double,
                                    ctypes.c_size_t, ctypes.c_void_p)
 G = ctypes.POINTER(ConvGeo)
 PL = ctypes.POINTER(ConvPlan)
+LG = ctypes.POINTER(Logits)
 
 # name -> (restype, argtypes); the full exported surface of include/omt_hip.h
 SIGNATURES = {
@@ -232,6 +255,17 @@ SIGNATURES = {
     "omt_glu_bwd": (I32, [I32, I64, I64, I64, I32, I32] + [VP] * 13 + [SZ, VP]),
     "omt_glu_fp8_workspace": (SZ, [I64, I64, I64]),
     "omt_glu_fp8": (I32, [I64, I64, I64, I32] + [VP] * 9 + [SZ, VP]),
+    "omt_embedding_fwd": (I32, [I32, I32, I64, I64, I64, VP, VP, F32, VP, VP]),
+    "omt_embedding_bwd_workspace": (SZ, [I64, I64, I64]),
+    "omt_embedding_bwd": (I32, [I32, I32, I64, I64, I64, VP, VP, I64, F32, VP, VP, SZ, VP]),
+    "omt_token_logps_fwd": (I32, [LG, VP, VP, VP]),
+    "omt_token_logps_bwd": (I32, [LG, VP, VP, VP, VP]),
+    "omt_preference_workspace": (SZ, [I64, I64]),
+    "omt_preference_loss": (I32, [LG, VP, I32, F64, F64, I32, VP, VP, VP, VP, SZ, VP]),
+    "omt_policy_workspace": (SZ, [I64, I64, I32]),
+    "omt_policy_loss": (I32, [LG, VP, VP, VP, I64, I64, F64, F64, F64, I32] + [VP] * 5 + [SZ, VP]),
+    "omt_scale_by": (I32, [I32, I64, VP, VP, VP]),
+    "omt_adamw": (I32, [I32, I32, ctypes.POINTER(AdamwParams), ctypes.POINTER(AdamwTensor), I32, VP]),
 }
 
 ABI_VERSION = 5

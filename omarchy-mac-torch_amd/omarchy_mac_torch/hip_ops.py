@@ -808,18 +808,21 @@ _GLU_ACTS = {"silu": _lib.OMT_GLU_SILU, "gelu": _lib.OMT_GLU_GELU, "relu": _lib.
 _KEEPS = {None: _lib.OMT_KEEP_NONE, "fp8": _lib.OMT_KEEP_FP8, "full": _lib.OMT_KEEP_FULL}
 
 
-_native_ffn = None
+_native = {}
+
+
+def _call(module, name, args):
+    if module not in _native:  # the extension loads after this module
+        from omarchy_mac_torch.native import core
+        _native[module] = getattr(core, module)
+    try:
+        return getattr(_native[module], name)(*args)
+    except NotImplementedError as e:
+        raise _lib.Unsupported(_lib.OMT_UNSUPPORTED, str(e)) from None
 
 
 def _ffn(name, *args):
-    global _native_ffn
-    if _native_ffn is None:  # the extension loads after this module
-        from omarchy_mac_torch.native import core
-        _native_ffn = core.ffn
-    try:
-        return getattr(_native_ffn, name)(*args)
-    except NotImplementedError as e:
-        raise _lib.Unsupported(_lib.OMT_UNSUPPORTED, str(e)) from None
+    return _call("ffn", name, args)
 
 
 def _glu_act(act):
@@ -891,3 +894,98 @@ def glu_backward(gh, kept, w_gate, w_up, act="silu", input_grad=True, weight_gra
 def glu_fp8(x, x_scale, w_gate, gate_scale, w_up, up_scale, act="silu"):
     """glu of operands held in 8 bits, for serving: returns h in 8 bits, (q, scale)."""
     return _ffn("glu_fp8", x, x_scale, w_gate, gate_scale, w_up, up_scale, _glu_act(act))
+
+
+# ---- both ends of a language model's training step: embedding, losses on logits, AdamW -------------------------------
+#
+# No counterpart in the reference. Tensors of float32 or bfloat16, on torch.cuda or on the omarchy_mac_torch device
+# (differentiable forms for the latter: omarchy_mac_torch.lm; the optimizer: omarchy_mac_torch.optim.AdamW). Every sum runs in
+# a fixed order: the same inputs give the same bits. The checks and the launches are in torch_ext/lm.cpp, whose functions
+# torch.ops.omt registers too.
+
+_PREFERENCES = {"sigmoid": _lib.OMT_PREFERENCE_SIGMOID, "hinge": _lib.OMT_PREFERENCE_HINGE, "ipo": _lib.OMT_PREFERENCE_IPO}
+
+
+def _lm(name, *args):
+    return _call("lm", name, args)
+
+
+def _choice(name, value, choices):
+    if value not in choices:
+        raise ValueError(f"{name}: expected one of {sorted(choices)}, got {value!r}")
+    return choices[value]
+
+
+def embedding(tokens, weight, scale=1.0):
+    """scale * weight[tokens]: weight [vocab, dim], tokens int64 or int32 of any shape. A token outside the vocabulary gives a
+    row of NaN (the device cannot raise)."""
+    return _lm("embedding", tokens, weight, float(scale))
+
+
+def embedding_backward(gy, tokens, vocab, scale=1.0, padding_idx=None):
+    """The gradient [vocab, dim] of embedding's weight from gy, the gradient of its result: each row's positions in their
+    order, summed in float32. The row padding_idx gets zeros; tokens outside the vocabulary take no part."""
+    if padding_idx is not None and not -vocab <= padding_idx < vocab:
+        raise ValueError(f"padding_idx: expected a row of {vocab}, got {padding_idx}")
+    padding_idx = -1 if padding_idx is None else padding_idx % vocab
+    return _lm("embedding_backward", gy, tokens, int(vocab), float(scale), padding_idx)
+
+
+def token_logps(logits, labels, ignore_index=-100):
+    """log softmax(logits)[label] of each label: logits [sequences, length, vocab] (rows dense, any other strides), labels int64
+    [sequences, length]. Returns (logps, lse) in float32, lse each row's log sum exp; both 0 where the label is ignore_index, whose
+    rows are not read. A label outside the vocabulary gives NaN."""
+    return _lm("token_logps", logits, labels, int(ignore_index))
+
+
+def token_logps_backward(g, logits, labels, lse, ignore_index=-100):
+    """The gradient of token_logps' logits from g, the gradient of its logps, and its lse."""
+    return _lm("token_logps_backward", g, logits, labels, lse, int(ignore_index))
+
+
+def preference_loss(logits, labels, reference, beta=0.1, kind="sigmoid", smoothing=0.0, average=False, ignore_index=-100,
+                    grad=True):
+    """A loss on pairs of sequences: logits and labels as token_logps', the chosen sequences in the first half and the rejected
+    ones, in the same order, in the second. With L the sum of a sequence's logps (average: their mean), R = reference
+    [sequences] the same of a reference model, d = (L - R of the chosen) - (L - R of the rejected), the mean over pairs of
+
+        "sigmoid"  -(1 - smoothing) log sigmoid(beta d) - smoothing log sigmoid(-beta d)
+        "hinge"    max(0, 1 - beta d)
+        "ipo"      (d - 1 / (2 beta))^2
+
+    Returns (loss, rewards [sequences] = beta (L - R), the logits' gradient or, without grad, None)."""
+    return _lm("preference_loss", logits, labels, reference, float(beta), _choice("kind", kind, _PREFERENCES), float(smoothing),
+               bool(average), int(ignore_index), bool(grad))
+
+
+def policy_loss(logits, labels, old_logps, advantages, reference=None, clip=(0.2, 0.2), kl=0.0, reduction="token",
+                ignore_index=-100, grad=True):
+    """The clipped policy loss: logits and labels as token_logps', r = exp(logps - old_logps) against the probabilities that
+    the tokens were sampled with, A = advantages ([sequences] or [sequences, length]); of each token
+    -min(r A, clamp(r, 1 - clip[0], 1 + clip[1]) A) + kl k, k = exp(reference - logps) - (reference - logps) - 1 (0 without a
+    reference); old_logps and reference are float32 [sequences, length]. reduction: the mean over all "token"s that count, or over
+    "sequence"s of each one's mean. Returns (loss, k's mean, logps, the logits' gradient or, without grad, None)."""
+    by_sequence = _choice("reduction", reduction, {"token": False, "sequence": True})
+    return _lm("policy_loss", logits, labels, old_logps, advantages, reference, float(clip[0]), float(clip[1]), float(kl),
+               by_sequence, int(ignore_index), bool(grad))
+
+
+def adamw(params, grads, exp_avgs, exp_avg_sqs, step, exp_avg_scales=None, exp_avg_sq_scales=None, masters=None, lr=1e-3,
+          betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, maximize=False, grad_scale=None, found_inf=None):
+    """One AdamW step over lists of tensors, in place: parameters and gradients all of float32, or all of bfloat16, which may
+    have `masters`, float32 copies that are updated in their place. States of float32; or, with lists of scales (float32, one for
+    each block of 128 elements of a tensor in memory), of torch.float8_e4m3fn, exp_avg_sqs then holding the second moments' square
+    roots. step: a one-element float32 tensor already incremented for this step, or a list of them; lr may be one too.
+    grad_scale divides the gradients (which stay as they are); found_inf == 1 skips the step."""
+    n = len(params)
+    steps = [step] * n if isinstance(step, torch.Tensor) else step
+    lr_dev = lr if isinstance(lr, torch.Tensor) else None
+    _lm("adamw_", params, grads, exp_avgs, exp_avg_sqs, steps, exp_avg_scales or [], exp_avg_sq_scales or [], masters or [],
+        0.0 if lr_dev is not None else float(lr), lr_dev, float(betas[0]), float(betas[1]), float(eps), float(weight_decay),
+        grad_scale, found_inf, bool(maximize))
+
+
+def scale_by_(x, factor):
+    """x *= factor, a one-element float32 tensor on the device; x is left untouched where it is 1."""
+    _lm("scale_by_", x, factor)
+    return x

@@ -1,0 +1,106 @@
+"""Both ends of a language model's training step on the omarchy_mac_torch device, beside its feed-forward sublayers (ffn):
+
+    embedding        scale * weight[tokens], its gradient summed in the order of positions
+    token_logps      log softmax(logits)[label]: a reference's log-probabilities, or those that tokens were sampled with
+    preference_loss  training on pairs of sequences: one chosen, one rejected
+    policy_loss      training on rewards: clipped probability ratios times advantages, with a KL term to a reference
+
+Differentiable functions over torch.ops.omt's operators. The two losses compute the logits' gradient with the loss, where
+one can be asked for, and hand it on in the backward pass, which therefore runs once. optim.AdamW is the step at the end.
+
+No counterpart in the reference. hip_ops has the same operators as plain functions, for torch.cuda tensors too.
+"""
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from omarchy_mac_torch import hip_ops
+
+__all__ = ["embedding", "policy_loss", "preference_loss", "token_logps"]
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, weight, scale, padding_idx):
+        ctx.save_for_backward(tokens)
+        ctx.vocab, ctx.scale, ctx.padding_idx = weight.shape[0], scale, padding_idx
+        return hip_ops.embedding(tokens, weight, scale)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        tokens, = ctx.saved_tensors
+        return None, hip_ops.embedding_backward(gy, tokens, ctx.vocab, ctx.scale, ctx.padding_idx), None, None
+
+
+class _TokenLogps(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, labels, ignore_index):
+        logps, lse = hip_ops.token_logps(logits, labels, ignore_index)
+        ctx.save_for_backward(logits, labels, lse)
+        ctx.ignore_index = ignore_index
+        return logps
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g):
+        return hip_ops.token_logps_backward(g, *ctx.saved_tensors, ctx.ignore_index), None, None
+
+
+class _Loss(torch.autograd.Function):
+    """A loss whose operator, op(logits, **arguments), gives (loss, others..., the logits' gradient)."""
+
+    @staticmethod
+    def forward(ctx, logits, op, arguments):
+        loss, *others, ctx.gradient = op(logits, **arguments)
+        ctx.mark_non_differentiable(*others)
+        ctx.set_materialize_grads(False)
+        return loss, *others
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gloss, *_):
+        if gloss is None:
+            return None, None, None
+        if ctx.gradient is None:
+            raise RuntimeError("the loss's gradient has been handed on already: its backward pass runs once")
+        gradient, ctx.gradient = ctx.gradient, None
+        return hip_ops.scale_by_(gradient, gloss), None, None
+
+
+def _loss(op, logits, arguments):
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _Loss.apply(logits, op, arguments)
+    return op(logits, **arguments, grad=False)[:-1]
+
+
+@torch.compiler.disable  # one operator each way: nothing for a compiler to fuse
+def embedding(tokens, weight, scale=1.0, padding_idx=None):
+    """hip_ops.embedding, differentiable in the weight; the row padding_idx gets no gradient."""
+    if padding_idx is not None and not -weight.shape[0] <= padding_idx < weight.shape[0]:
+        raise ValueError(f"padding_idx: expected a row of {weight.shape[0]}, got {padding_idx}")
+    return _Embedding.apply(tokens, weight, scale, padding_idx)
+
+
+@torch.compiler.disable
+def token_logps(logits, labels, ignore_index=-100):
+    """hip_ops.token_logps' logps, differentiable in the logits."""
+    return _TokenLogps.apply(logits, labels, ignore_index)
+
+
+@torch.compiler.disable
+def preference_loss(logits, labels, reference, beta=0.1, kind="sigmoid", smoothing=0.0, average=False, ignore_index=-100):
+    """hip_ops.preference_loss, differentiable in the logits: (loss, rewards), the rewards without a gradient."""
+    return _loss(hip_ops.preference_loss, logits,
+                 dict(labels=labels, reference=reference, beta=beta, kind=kind, smoothing=smoothing, average=average,
+                      ignore_index=ignore_index))
+
+
+@torch.compiler.disable
+def policy_loss(logits, labels, old_logps, advantages, reference=None, clip=(0.2, 0.2), kl=0.0, reduction="token",
+                ignore_index=-100):
+    """hip_ops.policy_loss, differentiable in the logits: (loss, the KL term's mean, logps), the latter two without a
+    gradient (the loss holds the KL term's)."""
+    return _loss(hip_ops.policy_loss, logits,
+                 dict(labels=labels, old_logps=old_logps, advantages=advantages, reference=reference, clip=clip, kl=kl,
+                      reduction=reduction, ignore_index=ignore_index))

@@ -138,14 +138,15 @@ def mobilenet_v3_small(classes=1000):
 
 
 class MlpLM(nn.Module):
-    """Logits of the next token from the last `context` tokens' embeddings, side by side, through feed-forward sublayers."""
+    """Logits of the next token from the last `context` tokens' embeddings (times embed_scale), side by side, through
+    feed-forward sublayers."""
 
-    def __init__(self, vocab, dim, hidden, depth, context=4, act="silu", checkpoint="fp8"):
+    def __init__(self, vocab, dim, hidden, depth, context=4, act="silu", checkpoint="fp8", embed_scale=1.0):
         from omarchy_mac_torch import ffn  # the operators' library, which a user of the convnets' definitions need not have
         super().__init__()
         if dim % context:
             raise ValueError(f"dim {dim} is not a multiple of the context, {context}")
-        self.context = context
+        self.context, self.embed_scale = context, embed_scale
         self.embed = nn.Embedding(vocab, dim // context)
         self.blocks = nn.ModuleList(ffn.FeedForward(dim, hidden, act, checkpoint) for _ in range(depth))
         self.norm = ffn.RMSNorm(dim)
@@ -154,7 +155,8 @@ class MlpLM(nn.Module):
 
     def forward(self, tokens):
         """tokens [batch, length >= context] -> logits [batch, length - context + 1, vocab]"""
-        e = self.embed(tokens)
+        from omarchy_mac_torch import lm
+        e = lm.embedding(tokens, self.embed.weight, self.embed_scale)
         n = tokens.shape[1] - self.context + 1
         x, stream = torch.cat([e[:, i:i + n] for i in range(self.context)], -1), None
         for block in self.blocks:

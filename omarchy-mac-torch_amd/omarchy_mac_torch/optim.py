@@ -6,13 +6,18 @@ has no hook for a device's preferred implementation, so `enable_fused_defaults` 
 parameters are all on the device, and that chose neither fused= nor foreach= (nor differentiable=, nor a tensor lr),
 gets fused=True. `keeps_torch_default` says why a call is left alone. OMARCHY_MAC_TORCH_FUSED_OPTIM=0 leaves
 torch.optim untouched.
+
+AdamW is this package's own, for language models: parameters in float32 or bfloat16, these with float32 master copies, and
+states in 8 bits or in 32 (no counterpart in the reference).
 """
 
 import functools
+import itertools
 import os
 
 import torch
 
+from omarchy_mac_torch import hip_ops
 from omarchy_mac_torch.native import DEVICE
 
 _MARK = "_omarchy_mac_torch_fused_default"
@@ -69,6 +74,77 @@ def enable_fused_defaults(classes=DEFAULT_CLASSES):
     """Applies fused_default to each class (the package does this on import unless OMARCHY_MAC_TORCH_FUSED_OPTIM=0);
     returns the classes."""
     return [fused_default(cls) for cls in classes]
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW over hip_ops.adamw: one launch for each 32 parameters of a group and type. Parameters in float32 or bfloat16, on the
+    device (or on torch.cuda); gradients of their type.
+
+    state_bits: 8 (e4m3 with a scale for each block of 128, two bytes and 1/16 a parameter; the second moment as its root) or 32
+    (eight bytes). masters: bfloat16 parameters keep a float32 copy, which is what is updated; without one, an update below half a
+    parameter's last place is lost. lr may be a one-element float32 tensor on the device. The step's counters are on the device,
+    so a step may be captured into a graph once it has run eagerly (which makes the states)."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, *, state_bits=8, masters=True,
+                 maximize=False):
+        if state_bits not in (8, 32):
+            raise ValueError(f"state_bits: expected 8 or 32, got {state_bits!r}")
+        if not isinstance(lr, torch.Tensor) and not lr >= 0:
+            raise ValueError(f"lr: expected at least 0, got {lr!r}")
+        if not all(0 <= b < 1 for b in betas):
+            raise ValueError(f"betas: expected from 0 to below 1, got {betas!r}")
+        if not eps >= 0 or not weight_decay >= 0:
+            raise ValueError(f"eps, weight_decay: expected at least 0, got {eps!r}, {weight_decay!r}")
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      masters=masters, maximize=maximize))
+
+    @staticmethod
+    def _new_state(p, group):
+        state = {"step": torch.zeros((), device=p.device)}
+        held = torch.float8_e4m3fn if group["state_bits"] == 8 else torch.float32
+        for name in ("exp_avg", "exp_avg_sq"):
+            state[name] = torch.zeros_like(p, dtype=torch.float32).to(held)
+            if group["state_bits"] == 8:
+                state[name + "_scale"] = torch.zeros(-(-p.numel() // 128), device=p.device)
+        if group["masters"] and p.dtype == torch.bfloat16:
+            state["master"] = p.detach().float()
+        return state
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        for group in self.param_groups:
+            by_type = {}
+            for p in group["params"]:
+                if p.grad is None:
+                    continue
+                if p.grad.is_sparse:
+                    raise TypeError("AdamW: sparse gradients are not covered")
+                if not self.state[p]:
+                    self.state[p] = self._new_state(p, group)
+                by_type.setdefault((p.dtype, p.device), []).append(p)
+            for ps in by_type.values():
+                def of(name):
+                    return [self.state[p][name] for p in ps] if name in self.state[ps[0]] else None
+
+                steps = of("step")
+                torch._foreach_add_(steps, 1)
+                hip_ops.adamw(ps, [p.grad for p in ps], of("exp_avg"), of("exp_avg_sq"), steps, of("exp_avg_scale"),
+                              of("exp_avg_sq_scale"), of("master"), lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                              weight_decay=group["weight_decay"], maximize=group["maximize"])
+        return loss
+
+    def load_state_dict(self, state_dict):
+        super().load_state_dict(state_dict)
+        # (torch casts states to their parameter's type; these keep their own)
+        ids = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
+        params = itertools.chain.from_iterable(g["params"] for g in self.param_groups)
+        for i, p in zip(ids, params):
+            for name, t in state_dict["state"].get(i, {}).items():
+                self.state[p][name] = t.detach().to(p.device, copy=True)
 
 
 if os.environ.get("OMARCHY_MAC_TORCH_FUSED_OPTIM", "1") != "0":

@@ -10,6 +10,7 @@ void bind_plans(pybind11::module_& m);
 void bind_tuning(pybind11::module_& m);
 void bind_replay(pybind11::module_& m);
 void bind_ffn(pybind11::module_& m);
+void bind_lm(pybind11::module_& m);
 }
 
 PYBIND11_MODULE(_native, m) {
@@ -90,4 +91,5 @@ PYBIND11_MODULE(_native, m) {
   bind_tuning(m);
   bind_replay(m);
   bind_ffn(m);
+  bind_lm(m);
 }

@@ -1,0 +1,286 @@
+"""Both ends of a language model's training step on the omarchy_mac_torch device: autograd, the small language model trained on pairs
+and on rewards with AdamW in 8 bits, against the same mathematics in plain torch on the CPU in float64."""
+
+import math
+
+import pytest
+import torch
+import torch.nn.functional as F
+
+from test_gpu_ffn_device import plain_lm, rel
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def omt(cuda):
+    import omarchy_mac_torch
+    return omarchy_mac_torch
+
+
+def test_embedding_gradient(omt):
+    from omarchy_mac_torch import lm
+    g = torch.Generator().manual_seed(0)
+    w, t = torch.randn(50, 24, generator=g), torch.randint(50, (3, 70), generator=g)
+    gy = torch.randn(3, 70, 24, generator=g)
+    dev = w.to(omt.DEVICE).requires_grad_(True)
+    y = lm.embedding(t.to(omt.DEVICE), dev, scale=0.5, padding_idx=-50)
+    assert torch.equal(y.detach().cpu(), 0.5 * w[t])
+    y.backward(gy.to(omt.DEVICE))
+    ref = w.double().requires_grad_(True)
+    (0.5 * F.embedding(t, ref, padding_idx=0)).backward(gy.double())
+    assert rel(dev.grad, ref.grad) <= 2e-6 and not bool(dev.grad.cpu()[0].any())  # float32 sums of a few terms
+    with torch.no_grad():
+        assert lm.embedding(t.to(omt.DEVICE), dev).grad_fn is None
+
+
+@pytest.mark.parametrize("scale", [1.0, 3.0])
+def test_losses_hand_their_gradient_on(omt, scale):
+    """Through what comes before them and with what comes after; against differences too."""
+    from omarchy_mac_torch import lm
+    g = torch.Generator().manual_seed(1)
+    h, w = torch.randn(4, 6, 16, generator=g), torch.randn(40, 16, generator=g)
+    labels = torch.randint(40, (4, 7), generator=g)
+    labels[:, :2] = -100
+    labels[3, 5:] = -100
+    target = labels[:, 1:]
+    ref, old, adv = -30 + torch.randn(4, generator=g), -5 + 0.1 * torch.randn(4, 6, generator=g), torch.randn(4, generator=g)
+
+    def plain(logits):
+        lp = torch.log_softmax(logits, -1).gather(2, target.clamp(min=0)[..., None])[..., 0] * (target != -100)
+        gain = lp.sum(1) - ref.double()
+        pref = -F.logsigmoid(0.1 * (gain[:2] - gain[2:])).mean()
+        on = (target != -100).double()
+        r, a = (lp - old.double()).exp(), adv.double()[:, None]
+        pol = (-torch.minimum(r * a, r.clamp(0.8, 1.2) * a) * on).sum() / on.sum()
+        return pref, pol, (lp * torch.arange(6)).sum()
+
+    def ours(logits):
+        t = target.to(omt.DEVICE)
+        return (lm.preference_loss(logits, t, ref.to(omt.DEVICE))[0],
+                lm.policy_loss(logits, t, old.to(omt.DEVICE), adv.to(omt.DEVICE))[0],
+                (lm.token_logps(logits, t) * torch.arange(6, device=omt.DEVICE)).sum())
+
+    for k in range(3):
+        leaves = [[t.double().requires_grad_(True) for t in (h, w)], [t.to(omt.DEVICE).requires_grad_(True) for t in (h, w)]]
+        a, b = plain(leaves[0][0] @ leaves[0][1].T)[k], ours(leaves[1][0] @ leaves[1][1].T)[k]
+        assert abs(float(b) - float(a)) <= 2e-5 * max(1, abs(float(a)))
+        (scale * a).backward()
+        (scale * b).backward()
+        for p, q in zip(leaves[1], leaves[0]):
+            assert rel(p.grad, q.grad) <= 2e-5
+        with torch.no_grad():  # along a direction, by differences of the device's losses: their float32 limits the step
+            d = torch.randn(4, 6, 16, generator=g)
+            step = 1e-2
+            up, down = (ours((h + s * step * d).to(omt.DEVICE) @ w.to(omt.DEVICE).T)[k] for s in (1, -1))
+            slope = float((leaves[0][0].grad * d.double()).sum()) / scale
+            exact = [plain((h + s * step * d).double() @ w.double().T)[k] for s in (1, -1)]
+            difference = float(exact[0] - exact[1]) / (2 * step)
+            assert abs((float(up) - float(down)) / (2 * step) - difference) <= 2e-5 * max(1, abs(float(a))) / step
+            assert abs(difference - slope) <= 0.05 * float(leaves[0][0].grad.norm()) / scale * float(d.norm())
+
+
+def test_a_loss_of_a_view_keeps_the_rest_at_zero(omt):
+    from omarchy_mac_torch import lm
+    x = torch.randn(2, 5, 12).to(omt.DEVICE).requires_grad_(True)
+    labels = torch.randint(12, (2, 4)).to(omt.DEVICE)
+    loss, rewards = lm.preference_loss(x[:, :-1], labels, torch.zeros(2).to(omt.DEVICE))
+    loss.backward()
+    assert not rewards.requires_grad and not bool(x.grad[:, -1].cpu().any()) and bool(x.grad[:, :-1].cpu().any())
+
+
+def reference_adamw(p, g, state, lr, betas, eps, decay):
+    state["t"] = state.get("t", 0) + 1
+    state["m"] = betas[0] * state.get("m", 0) + (1 - betas[0]) * g
+    state["v"] = betas[1] * state.get("v", 0) + (1 - betas[1]) * g * g
+    m, v = state["m"] / (1 - betas[0] ** state["t"]), state["v"] / (1 - betas[1] ** state["t"])
+    return p - lr * decay * p - lr * m / (v.sqrt() + eps)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_optimizer(omt, bits):
+    """Float32 parameters over several steps: states in 32 bits follow float64 to its rounding; in 8 bits, the first step too, and
+    later ones to the states' rounding: m within 2^-4 and sqrt(v) within 2^-4 of the exact, each step's from what was held."""
+    from omarchy_mac_torch import optim
+    g = torch.Generator().manual_seed(2)
+    shapes = [(33, 40), (7,), (256,)]
+    start = [torch.randn(s, generator=g) for s in shapes]
+    params = [torch.nn.Parameter(p.to(omt.DEVICE)) for p in start]
+    opt = optim.AdamW(params, lr=1e-2, betas=(0.9, 0.99), weight_decay=0.05, state_bits=bits)
+    exact, states = [p.double() for p in start], [{} for _ in start]
+    for k in range(4):
+        grads = [torch.randn(s, generator=g) for s in shapes]
+        for p, d in zip(params, grads):
+            p.grad = d.to(omt.DEVICE)
+        opt.step()
+        before = exact
+        exact = [reference_adamw(p, d.double(), s, 1e-2, (0.9, 0.99), 1e-8, 0.05) for p, d, s in zip(exact, grads, states)]
+        for p, e, b in zip(params, exact, before):
+            off = (p.detach().cpu().double() - e).abs()
+            if bits == 32 or k == 0:
+                # float32: of the parameter 3 roundings a step, of the update 16
+                assert bool((off <= (k + 1) * 2.0 ** -24 * (4 * e.abs() + 4 * b.abs() + 16 * 1e-2 * 10)).all())
+            else:  # a step's update is at most lr (1 - b1) / sqrt(1 - b2) over the corrections, here 2.8 lr
+                assert bool((off <= k * 2.8e-2 * 3 * 2.0 ** -4 * 2).all())
+    assert float(opt.state[params[0]]["step"]) == 4
+
+
+def test_optimizer_resumes_from_its_state(omt):
+    from omarchy_mac_torch import optim
+    g = torch.Generator().manual_seed(3)
+    start, grads = torch.randn(300, generator=g), [torch.randn(300, generator=g) for _ in range(4)]
+
+    def made(p):
+        p = torch.nn.Parameter(p.to(omt.DEVICE, torch.bfloat16))
+        return p, optim.AdamW([p], lr=1e-2)
+
+    def run(p, opt, ds):
+        for d in ds:
+            p.grad = d.to(omt.DEVICE, torch.bfloat16)
+            opt.step()
+
+    p, opt = made(start)
+    run(p, opt, grads[:2])
+    q, other = made(p.detach().cpu())
+    other.load_state_dict(opt.state_dict())
+    run(p, opt, grads[2:])
+    run(q, other, grads[2:])
+    assert torch.equal(p.detach().cpu(), q.detach().cpu())
+    for name, t in opt.state[p].items():
+        assert torch.equal(t.float().cpu(), other.state[q][name].float().cpu()), name
+
+
+def sequences(g, n, length, vocab):
+    t = torch.randint(vocab, (n, length), generator=g)
+    for i in range(4, length):
+        t[:, i] = (t[:, i - 1] + t[:, i - 4]) % vocab
+    return t
+
+
+@pytest.mark.parametrize("loss", ["preference", "policy"])
+def test_language_model_is_tuned(omt, loss):
+    """The operators together: embedding with a scale, the sublayers, the head, a loss on the logits, AdamW in 8 bits. The first
+    step's loss and gradients against float64, and that the steps after it run."""
+    from omarchy_mac_torch import lm, models, optim
+    torch.manual_seed(0)
+    ref = models.mlp_lm(64, 128, 320, 2, checkpoint="full", embed_scale=128 ** 0.5)
+    dev = models.mlp_lm(64, 128, 320, 2, checkpoint="full", embed_scale=128 ** 0.5)
+    dev.load_state_dict(ref.state_dict())
+    ref, dev = ref.double(), dev.to(omt.DEVICE)
+    g = torch.Generator().manual_seed(1)
+    tokens = torch.cat([sequences(g, 4, 24, 64), torch.randint(64, (4, 24), generator=g)])
+    labels = tokens[:, 4:].clone()
+    labels[:, :5] = -100
+    labels[2, 15:] = labels[6, 9:] = -100
+    t, y = tokens.to(omt.DEVICE), labels.to(omt.DEVICE)
+    with torch.no_grad():
+        held = lm.token_logps(dev(t[:, :-1]), y)
+    opt = optim.AdamW(dev.parameters(), lr=1e-3)
+    adv = torch.tensor([1.0] * 4 + [-1.0] * 4)
+    names = dict(ref.named_parameters())
+    for k in range(4):
+        logits = dev(t[:, :-1])
+        if loss == "preference":
+            out, rewards = lm.preference_loss(logits, y, held.sum(1), beta=0.5)
+        else:
+            out, kl, _ = lm.policy_loss(logits, y, held, adv.to(omt.DEVICE), reference=held, kl=0.1, reduction="sequence")
+        opt.zero_grad()
+        out.backward()
+        if k == 0:
+            plain = plain_lm_scaled(ref, tokens[:, :-1])
+            lp = torch.log_softmax(plain, -1).gather(2, labels.clamp(min=0)[..., None])[..., 0] * (labels != -100)
+            was = held.cpu().double()
+            if loss == "preference":
+                gain = lp.sum(1) - was.sum(1)
+                want = -F.logsigmoid(0.5 * (gain[:4] - gain[4:])).mean()
+            else:
+                on = (labels != -100).double()
+                r, more = (lp - was).exp(), was - lp
+                each = -torch.minimum(r * adv.double()[:, None], r.clamp(0.8, 1.2) * adv.double()[:, None])
+                want = (((each + 0.1 * (more.exp() - more - 1)) * on).sum(1) / on.sum(1)).mean()
+            want.backward()
+            assert abs(float(out) - float(want)) <= 1e-4
+            for name, p in dev.named_parameters():
+                # float32 matrix products of up to 320 terms, four sublayers deep: 2e-5 each, as the sublayers' own tests have
+                assert rel(p.grad, names[name].grad) <= 1e-4, name
+        opt.step()
+        assert math.isfinite(float(out))
+    assert all(bool(torch.isfinite(p.detach().cpu()).all()) for p in dev.parameters())
+    assert not any(k.startswith("omt::") for k in omt.FALLBACKS)
+
+
+def plain_lm_scaled(m, tokens):
+    embed = m.embed
+
+    class Scaled(torch.nn.Module):
+        def forward(self, t):
+            return embed(t) * m.embed_scale
+
+    m.embed = Scaled()
+    try:
+        return plain_lm(m, tokens)
+    finally:
+        m.embed = embed
+
+
+def test_a_captured_training_step(omt):
+    """Embedding, loss and optimizer of a step in one graph, replayed on new tokens with eager work between."""
+    from omarchy_mac_torch import graphs, lm, optim
+    torch.manual_seed(4)
+    start = [torch.randn(50, 32), torch.randn(50, 32)]
+    tokens = [torch.randint(50, (4, 9)) for _ in range(8)]
+
+    def made():
+        ps = [torch.nn.Parameter(p.to(omt.DEVICE)) for p in start]
+        return ps, optim.AdamW(ps, lr=1e-2), torch.zeros(4, 9, dtype=torch.int64).to(omt.DEVICE)
+
+    def step(ps, opt, t):
+        logits = lm.embedding(t[:, :-1], ps[0], scale=2.0) @ ps[1].T
+        loss, _ = lm.preference_loss(logits, t[:, 1:], torch.zeros(4, device=omt.DEVICE))
+        for p in ps:
+            p.grad = None
+        loss.backward()
+        opt.step()
+        return loss.detach()
+
+    ps, opt, t = made()
+    t.copy_(tokens[0])
+    replay, _ = graphs.graphed(lambda: step(ps, opt, t), warmup=2)
+    qs, other, u = made()
+    u.copy_(tokens[0])
+    for _ in range(2):
+        step(qs, other, u)
+    for k in range(1, 8):
+        t.copy_(tokens[k])
+        got = replay()
+        u.copy_(tokens[k])
+        want = step(qs, other, u)
+        torch.cuda.synchronize()
+        assert torch.equal(got.cpu(), want.cpu()), k
+        for p, q in zip(ps, qs):
+            assert torch.equal(p.detach().cpu(), q.detach().cpu()), k
+    replay.graph.release()
+
+
+def test_operators_of_the_dispatcher(omt):
+    """torch.ops.omt on device tensors gives what hip_ops gives on torch.cuda tensors."""
+    ops = omt.hip_ops
+    w, t, x, y = torch.randn(20, 16), torch.randint(20, (30,)), torch.randn(2, 5, 20), torch.randint(20, (2, 5))
+    d = omt.DEVICE
+    got = torch.ops.omt.embedding(t.to(d), w.to(d), 2.0)
+    assert got.device.type == d and torch.equal(got.cpu(), ops.embedding(t.cuda(), w.cuda(), 2.0).cpu())
+    got = torch.ops.omt.embedding_backward(w[t].to(d), t.to(d), 20, 1.0, -1)
+    assert torch.equal(got.cpu(), ops.embedding_backward(w[t].cuda(), t.cuda(), 20).cpu())
+    for a, b in zip(torch.ops.omt.preference_loss(x.to(d), y.to(d), w[:2, 0].to(d), 0.1, 0, 0.0, False, -100, True),
+                    ops.preference_loss(x.cuda(), y.cuda(), w[:2, 0].cuda())):
+        assert torch.equal(a.cpu(), b.cpu())
+    for a, b in zip(torch.ops.omt.policy_loss(x.to(d), y.to(d), x[..., 0].to(d), w[:2, 0].to(d), None, 0.2, 0.2, 0.0, False, -100, True),
+                    ops.policy_loss(x.cuda(), y.cuda(), x[..., 0].cuda(), w[:2, 0].cuda())):
+        assert torch.equal(a.cpu(), b.cpu())
+    p, q = w.to(d), w.cuda()
+    torch.ops.omt.adamw_([p], [p * 1], [p * 0], [p * 0], [torch.ones((), device=d)], [], [], [], 0.1, None, 0.9, 0.99, 1e-8, 0.0, None,
+                         None, False)
+    ops.adamw([q], [q * 1], [q * 0], [q * 0], torch.ones((), device="cuda"), lr=0.1, betas=(0.9, 0.99), weight_decay=0.0)
+    assert torch.equal(p.cpu(), q.cpu())
+    with pytest.raises(ValueError):
+        ops.embedding(t.to(d), w.cuda())

@@ -1,0 +1,217 @@
+"""The embedding's, the losses' and AdamW's host side, without a GPU: argument statuses of every entry point, workspaces, the
+differentiable functions' dealings with autograd (their operators replaced by plain torch), the optimizer's arguments."""
+
+import ctypes
+
+import pytest
+import torch
+
+F32, I64, BF16, I32 = 0, 1, 2, 3
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from omarchy_mac_torch import _lib
+    return _lib
+
+
+def test_embedding_statuses(lib):
+    L, p, bad, no, ok = lib.L, ctypes.c_void_p(4096), lib.OMT_INVALID, lib.OMT_UNSUPPORTED, lib.OMT_OK
+    f = L.omt_embedding_fwd
+    assert f(I64, I64, 4, 8, 16, p, p, 1.0, p, None) == bad
+    assert f(F32, F32, 4, 8, 16, p, p, 1.0, p, None) == bad  # tokens that are no integers
+    assert f(F32, I64, -1, 8, 16, p, p, 1.0, p, None) == bad
+    assert f(F32, I64, 4, 0, 16, p, p, 1.0, p, None) == bad
+    assert f(F32, I64, 4, 8, 0, p, p, 1.0, p, None) == bad
+    assert f(F32, I32, 4, 8, 16, None, p, 1.0, p, None) == bad
+    assert f(F32, I32, 0, 8, 16, None, None, 1.0, None, None) == ok
+    b, ws = L.omt_embedding_bwd, L.omt_embedding_bwd_workspace
+    assert b(F32, I64, 4, 8, 16, p, p, -1, 1.0, p, None, 0, None) == bad  # no workspace
+    assert b(F32, I64, 4, 8, 16, p, p, -1, 1.0, p, p, ws(4, 8, 16) - 1, None) == bad
+    assert b(F32, I64, 4, 8, 16, p, p, -1, 1.0, p, ctypes.c_void_p(4100), 1 << 30, None) == bad
+    assert b(F32, I64, 4, 8, 16, p, p, -1, 1.0, None, p, 1 << 30, None) == bad
+    assert b(F32, I64, 4, 8, 16, None, p, -1, 1.0, p, p, 1 << 30, None) == bad
+    assert b(F32, I64, (1 << 28) + 1, 8, 16, p, p, -1, 1.0, p, p, 1 << 40, None) == no
+    assert b(F32, I64, 4, 8, (1 << 16) + 1, p, p, -1, 1.0, p, p, 1 << 40, None) == no
+    assert b(F32, I64, 4, (1 << 28) + 1, 16, p, p, -1, 1.0, p, p, 1 << 40, None) == no
+    # sorted tokens and positions twice, each run's two sums
+    assert ws(100000, 50000, 1024) >= 4 * 4 * 100000 and ws(-1, 8, 16) == 0 and ws(4, 8, 1 << 17) >= 0
+
+
+def logits(lib, sequences=2, length=3, vocab=10, dtype=F32, x=4096, labels=4096):
+    return ctypes.byref(lib.Logits(x, labels, -100, sequences, length, vocab, length * vocab, vocab, dtype))
+
+
+def test_loss_statuses(lib):
+    L, p, bad, no, ok = lib.L, ctypes.c_void_p(4096), lib.OMT_INVALID, lib.OMT_UNSUPPORTED, lib.OMT_OK
+    f, b = L.omt_token_logps_fwd, L.omt_token_logps_bwd
+    assert f(None, p, p, None) == bad
+    for wrong in (dict(dtype=I64), dict(sequences=-1), dict(vocab=0), dict(x=None), dict(labels=None)):
+        assert f(logits(lib, **wrong), p, p, None) == bad and b(logits(lib, **wrong), p, p, p, None) == bad
+    assert f(logits(lib, length=1 << 28), p, p, None) == no
+    assert f(logits(lib, vocab=(1 << 28) + 1), p, p, None) == no
+    assert f(logits(lib), None, p, None) == bad and f(logits(lib), p, None, None) == bad
+    assert b(logits(lib), p, None, p, None) == bad and b(logits(lib), p, p, None, None) == bad
+    for empty in (dict(sequences=0, x=None, labels=None), dict(length=0, x=None, labels=None)):
+        assert f(logits(lib, **empty), None, None, None) == ok and b(logits(lib, **empty), None, None, None, None) == ok
+
+    need = L.omt_preference_workspace(2, 3)
+    g = lambda q, ref=p, kind=0, beta=0.1, smooth=0.0, loss=p, rewards=p, ws=p, size=need: \
+        L.omt_preference_loss(q, ref, kind, beta, smooth, 0, loss, rewards, p, ws, size, None)  # noqa: E731
+    assert g(logits(lib, sequences=3)) == bad and g(logits(lib, sequences=0)) == bad
+    assert g(logits(lib), kind=3) == bad and g(logits(lib), kind=-1) == bad
+    assert g(logits(lib), beta=0.0) == bad and g(logits(lib), beta=float("nan")) == bad
+    assert g(logits(lib), smooth=-0.1) == bad and g(logits(lib), smooth=1.1) == bad
+    assert g(logits(lib), ref=None) == bad and g(logits(lib), loss=None) == bad and g(logits(lib), rewards=None) == bad
+    assert g(logits(lib), ws=None) == bad and g(logits(lib), size=need - 1) == bad
+    assert g(logits(lib), ws=ctypes.c_void_p(4104)) == bad
+    assert L.omt_preference_workspace(1 << 20, 1 << 20) == 0
+
+    need = L.omt_policy_workspace(2, 3, 1)
+    h = lambda q, old=p, adv=p, lo=0.2, hi=0.2, loss=p, kl=p, logps=p, ws=p, size=need: \
+        L.omt_policy_loss(q, old, None, adv, 1, 0, lo, hi, 0.0, 1, loss, kl, logps, p, ws, size, None)  # noqa: E731
+    assert h(logits(lib), old=None) == bad and h(logits(lib), adv=None) == bad and h(logits(lib), logps=None) == bad
+    assert h(logits(lib), loss=None) == bad and h(logits(lib), kl=None) == bad
+    assert h(logits(lib), lo=-0.1) == bad and h(logits(lib), hi=float("nan")) == bad
+    assert h(logits(lib), ws=None) == bad and h(logits(lib), size=need - 1) == bad
+    assert h(logits(lib, length=1 << 28)) == no
+    assert L.omt_policy_workspace(-1, 3, 0) == 0
+
+    s = L.omt_scale_by
+    assert s(I64, 4, p, p, None) == bad and s(F32, -1, p, p, None) == bad and s(F32, 4, None, p, None) == bad
+    assert s(BF16, 0, None, None, None) == ok
+
+
+def test_adamw_statuses(lib):
+    L, bad, no, ok = lib.L, lib.OMT_INVALID, lib.OMT_UNSUPPORTED, lib.OMT_OK
+    hp = lib.AdamwParams(1e-3, 0.9, 0.999, 0.01, 1e-8, None, None, None, 0)
+
+    def f(tensors, dtype=F32, bits=32, params=hp, count=None):
+        arr = (lib.AdamwTensor * max(1, len(tensors)))(*tensors)
+        return L.omt_adamw(dtype, bits, ctypes.byref(params) if params else None, arr, len(tensors) if count is None else count, None)
+
+    def t(param=4096, grad=4096, master=None, m=4096, ms=4096, v=4096, vs=4096, step=4096, n=0):
+        return lib.AdamwTensor(param, grad, master, m, ms, v, vs, step, n)
+
+    assert f([]) == ok and f([t()]) == ok
+    assert f([t()], dtype=I64) == bad and f([t()], bits=16) == bad and f([t()], params=None) == bad and f([], count=-1) == bad
+    for missing in (dict(param=None), dict(grad=None), dict(m=None), dict(v=None), dict(step=None)):
+        assert f([t(n=5, **missing)]) == bad
+    for missing in (dict(ms=None), dict(vs=None)):
+        assert f([t(n=5, **missing)], bits=8) == bad
+    assert f([t(n=-1)]) == bad and f([t(n=1 << 40)]) == no
+    assert f([t(master=4096, n=5)]) == bad                               # a master copy of float32
+    assert f([t(master=4096, n=5), t(n=5)], dtype=BF16) == bad           # of some alone
+
+
+def test_operators_refuse_cpu_tensors_and_wrong_choices():
+    from omarchy_mac_torch import hip_ops as ops
+    x, labels = torch.ones(2, 3, 5), torch.zeros(2, 3, dtype=torch.int64)
+    for call in (lambda: ops.embedding(labels, x[0]), lambda: ops.embedding_backward(x, labels, 4),
+                 lambda: ops.token_logps(x, labels), lambda: ops.token_logps_backward(x[..., 0], x, labels, x[..., 0]),
+                 lambda: ops.preference_loss(x, labels, x[:, 0, 0]), lambda: ops.policy_loss(x, labels, x[..., 0], x[:, 0, 0]),
+                 lambda: ops.adamw([x], [x], [x], [x], x[0, 0, 0])):
+        with pytest.raises(TypeError, match="HIP device"):
+            call()
+    with pytest.raises(ValueError, match="kind"):
+        ops.preference_loss(x, labels, x[:, 0, 0], kind="other")
+    with pytest.raises(ValueError, match="reduction"):
+        ops.policy_loss(x, labels, x[..., 0], x[:, 0, 0], reduction="batch")
+    for row in (4, -5):
+        with pytest.raises(ValueError, match="padding_idx"):
+            ops.embedding_backward(x, labels, 4, padding_idx=row)
+    ops.adamw([], [], [], [], x[0, 0, 0])
+
+
+@pytest.fixture
+def plain_losses(monkeypatch):
+    """hip_ops' losses in plain torch, with a record of whether a gradient was asked for."""
+    from omarchy_mac_torch import hip_ops
+    asked = []
+
+    def preference(logits, labels, reference, grad=True, **_):
+        asked.append(grad)
+        return logits.sum(), reference * 2, torch.ones_like(logits) if grad else None
+
+    def policy(logits, labels, old_logps, advantages, grad=True, **_):
+        asked.append(grad)
+        return logits.sum(), old_logps.sum(), old_logps * 1, torch.ones_like(logits) if grad else None
+
+    monkeypatch.setattr(hip_ops, "preference_loss", preference)
+    monkeypatch.setattr(hip_ops, "policy_loss", policy)
+    monkeypatch.setattr(hip_ops, "scale_by_", lambda x, f: x.mul_(f))
+    return asked
+
+
+def test_losses_compute_a_gradient_only_where_one_can_be_asked_for(plain_losses):
+    from omarchy_mac_torch import lm
+    x, labels, ref = torch.ones(2, 3, 5, requires_grad=True), torch.zeros(2, 3, dtype=torch.int64), torch.ones(2)
+    for call, others in ((lambda t: lm.preference_loss(t, labels, ref), 1),
+                         (lambda t: lm.policy_loss(t, labels, torch.ones(2, 3), ref), 2)):
+        plain_losses.clear()
+        out = call(x)
+        assert len(out) == 1 + others and out[0].requires_grad and not any(t.requires_grad for t in out[1:])
+        with torch.no_grad():
+            assert len(call(x)) == 1 + others
+        call(x.detach())
+        assert plain_losses == [True, False, False]
+        (3 * out[0]).backward()
+        assert torch.equal(x.grad, torch.full_like(x, 3.0))
+        x.grad = None
+
+
+def test_a_losss_gradient_is_handed_on_once(plain_losses):
+    from omarchy_mac_torch import lm
+    x, labels, ref = torch.ones(2, 3, 5, requires_grad=True), torch.zeros(2, 3, dtype=torch.int64), torch.ones(2)
+    loss, _ = lm.preference_loss(x, labels, ref)
+    loss.backward(retain_graph=True)
+    with pytest.raises(RuntimeError, match="runs once"):
+        loss.backward()
+
+
+def test_padding_rows_are_checked():
+    from omarchy_mac_torch import lm
+    with pytest.raises(ValueError, match="padding_idx"):
+        lm.embedding(torch.zeros(2, dtype=torch.int64), torch.ones(4, 8), padding_idx=4)
+
+
+def test_optimizer_arguments():
+    from omarchy_mac_torch import optim
+    p = [torch.nn.Parameter(torch.ones(3))]
+    for wrong in (dict(state_bits=16), dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1.0), dict(weight_decay=-1.0)):
+        with pytest.raises(ValueError):
+            optim.AdamW(p, **wrong)
+    opt = optim.AdamW(p)
+    opt.step()  # no gradients: nothing to do
+    assert not opt.state
+    p[0].grad = torch.ones(3)
+    with pytest.raises(TypeError, match="HIP device"):
+        opt.step()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_optimizer_states_keep_their_types_through_a_state_dict(monkeypatch, dtype, bits):
+    from omarchy_mac_torch import hip_ops, optim
+    monkeypatch.setattr(hip_ops, "adamw", lambda *args, **options: None)
+    def made():
+        p = torch.nn.Parameter(torch.linspace(-1, 1, 130).to(dtype))
+        p.grad = torch.ones_like(p)
+        return p, optim.AdamW([p], state_bits=bits)
+
+    p, opt = made()
+    opt.step()
+    state = opt.state[p]
+    held = torch.float8_e4m3fn if bits == 8 else torch.float32
+    assert state["exp_avg"].dtype == state["exp_avg_sq"].dtype == held and state["exp_avg"].shape == p.shape
+    assert ("exp_avg_scale" in state) == (bits == 8) and ("master" in state) == (dtype == torch.bfloat16)
+    if bits == 8:
+        assert state["exp_avg_scale"].shape == state["exp_avg_sq_scale"].shape == (2,)
+    if "master" in state:
+        state["master"] += 1e-5  # what the parameter's type cannot hold
+    q, other = made()
+    other.load_state_dict(opt.state_dict())
+    assert other.state[q].keys() == state.keys() and float(other.state[q]["step"]) == 1
+    for name, t in state.items():
+        mine = other.state[q][name]
+        assert mine.dtype == t.dtype and torch.equal(mine.float(), t.float()) and mine.data_ptr() != t.data_ptr()
