@@ -346,6 +346,7 @@ _PLAIN = {"embed": _plain_embed, "embed_grad": _plain_embed, "preference": _plai
 
 # ---- the framework's operators --------------------------------------------------------------------------------------
 
+@functools.lru_cache(maxsize=None)  # as a program imports it: once
 def _hip_ops():
     package = str(pathlib.Path(__file__).resolve().parent.parent / "omarchy-mac-torch_amd")
     if package not in sys.path:
