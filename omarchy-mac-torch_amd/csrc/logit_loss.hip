@@ -72,46 +72,103 @@ __device__ __forceinline__ float row_total(float v, float* red) {
   return v;
 }
 
-// eight logits from column c on, minus infinity behind the row
-template <bool VEC, class T>
-__device__ __forceinline__ f32x8 load_logits(const T* p, int64_t c, int64_t cols) {
-  f32x8 v = load8<VEC>(p, c, cols);
-  if (c + 8 > cols)
+// A row is a body of vectors of 16 bytes, on 16 bytes, and up to 14 single columns before and behind it, of which a thread has
+// one at most: rows of any size, at any alignment, are read by whole vectors.
+template <class T> struct Lanes;
+template <> struct Lanes<float> {
+  typedef f32x4 raw, wide;
+  static constexpr int W = 4;
+};
+template <> struct Lanes<__bf16> {
+  typedef bf16x8 raw;
+  typedef f32x8 wide;
+  static constexpr int W = 8;
+};
+template <class T>
+struct Row {
+  typedef typename Lanes<T>::raw Raw;
+  typedef typename Lanes<T>::wide Wide;
+  static constexpr int W = Lanes<T>::W;
+  const T* p;
+  int cols, head, body;  // columns, those before the body, and its vectors
+  __device__ __forceinline__ Row(const T* at, int64_t n) : p(at), cols((int)n) {
+    head = min((int)((0 - (uintptr_t)at) & 15) / (int)sizeof(T), cols);
+    body = (cols - head) / W;
+  }
+  __device__ __forceinline__ Raw load(int j) const {
+    Raw v;
+    if (j < body) {
+      v = *(const Raw*)(p + head + j * W);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (c + e >= cols) v[e] = -kInf;
-  return v;
-}
-__device__ __forceinline__ float max8(f32x8 v) {
+      for (int e = 0; e < W; ++e) v[e] = (T)-kInf;
+    }
+    return v;
+  }
+  // the single column of thread t; -1 where it has none
+  __device__ __forceinline__ int single(int t) const {
+    const int c = t < head ? t : body * W + t;
+    return c < cols && t < 2 * W ? c : -1;
+  }
+  __device__ __forceinline__ int column(int j) const { return head + j * W; }
+};
+__device__ __forceinline__ f32x4 widen(f32x4 v) { return v; }
+__device__ __forceinline__ f32x8 widen(bf16x8 v) { return __builtin_convertvector(v, f32x8); }
+__device__ __forceinline__ float largest(f32x4 v) { return fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])); }
+__device__ __forceinline__ float largest(f32x8 v) {
   return fmaxf(fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])), fmaxf(fmaxf(v[4], v[5]), fmaxf(v[6], v[7])));
 }
 // exp(v - m): the difference first, which is exact or nearly so for what counts
 __device__ __forceinline__ float exp_from(float v, float m) { return __builtin_amdgcn_exp2f((v - m) * kLog2e); }
 
+// The gradient's row: written past the caches, which so keep what is read again, where it lies as the logits' row does.
+template <class T>
+struct GradRow {
+  T* g;
+  bool aligned;
+  __device__ __forceinline__ GradRow(T* at, const Row<T>& r) : g(at), aligned(!((uintptr_t)(at + r.head) & 15)) {}
+  __device__ __forceinline__ void store(int c, typename Lanes<T>::wide v) const {
+    typename Lanes<T>::raw r = __builtin_convertvector(v, typename Lanes<T>::raw);
+    if (aligned) __builtin_nontemporal_store(r, (typename Lanes<T>::raw*)(g + c));
+    else __builtin_memcpy(g + c, &r, sizeof(r));
+  }
+};
+
 // The largest and the sum of exp(x - largest) of a row of memory, in every one of its RT threads.
 struct RowStats {
   float top, sum;
 };
-template <class T, bool VEC, int RT>
-__device__ __forceinline__ RowStats row_stats(const T* x, int64_t vocab, float* red) {
+template <class T, int RT>
+__device__ __forceinline__ RowStats row_stats(const Row<T>& x, float* red) {
+  constexpr int U = 4, W = Row<T>::W;
   const int t = RT == 64 ? threadIdx.x & 63 : threadIdx.x;
-  float m = -kInf, s = 0.f;
-  constexpr int U = 4;
-  for (int64_t c0 = (int64_t)t * 8; c0 < vocab; c0 += RT * 8 * U) {
-    f32x8 v[U];
+  const int single = x.single(t);
+  float m = single >= 0 ? (float)x.p[single] : -kInf, s = single >= 0 && m != -kInf ? 1.f : 0.f;
+  if (m != m) s = m;
+  typename Row<T>::Raw now[U], next[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = load_logits<VEC>(x, c0 + u * RT * 8, vocab);
+  for (int u = 0; u < U; ++u) now[u] = x.load(t + u * RT);
+  for (int j = t;; j += RT * U) {
+    const bool more = j - t + RT * U < x.body;  // (the same for the row's threads)
+    if (more)
+#pragma unroll
+      for (int u = 0; u < U; ++u) next[u] = x.load(j + (U + u) * RT);
     float top = m;
 #pragma unroll
-    for (int u = 0; u < U; ++u) top = fmaxf(top, max8(v[u]));
+    for (int u = 0; u < U; ++u) top = fmaxf(top, largest(widen(now[u])));
     // (a thread that has met nothing over minus infinity: differences to 0 instead, so that none is NaN)
     const float from = top == -kInf ? 0.f : top;
     s *= exp_from(m, from);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u) {
+      const auto v = widen(now[u]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s += exp_from(v[u][e], from);
+      for (int e = 0; e < W; ++e) s += exp_from(v[e], from);
+    }
     m = top;
+    if (!more) break;
+#pragma unroll
+    for (int u = 0; u < U; ++u) now[u] = next[u];
   }
   const float top = row_max<RT>(m, red), from = top == -kInf ? 0.f : top;
   return {top, row_total<RT>(s * exp_from(m, from), red)};
@@ -135,7 +192,7 @@ __device__ __forceinline__ int64_t this_row(int64_t rows) {
   return row < rows ? row : -1;
 }
 
-template <class T, bool VEC, int RT>
+template <class T, int RT>
 __global__ void __launch_bounds__(RT == 64 ? 256 : RT) token_logps_kernel(LogitRows a, float* logps, float* lse) {
   __shared__ float red[16];
   const int64_t row = this_row<RT>(a.rows);
@@ -146,69 +203,103 @@ __global__ void __launch_bounds__(RT == 64 ? 256 : RT) token_logps_kernel(LogitR
     if (first) logps[row] = 0.f, lse[row] = 0.f;
     return;
   }
-  const T* x = (const T*)a.x + a.offset(row);
-  const RowStats st = row_stats<T, VEC, RT>(x, a.vocab, red);
+  const Row<T> x((const T*)a.x + a.offset(row), a.vocab);
+  const RowStats st = row_stats<T, RT>(x, red);
   if (first) {
-    logps[row] = (float)label_logp(x, label, a.vocab, st);
+    logps[row] = (float)label_logp(x.p, label, a.vocab, st);
     lse[row] = (float)((double)st.top + log((double)st.sum));
   }
 }
 
 // ---- the gradient of rows -------------------------------------------------------------------------------------------
 
-// c (onehot(label) - p) of the eight columns from c0 on, p = exp(x - lse)
-__device__ __forceinline__ f32x8 row_gradient(f32x8 p, float c, int64_t c0, int64_t label) {
-  f32x8 g = p * -c;
-  if ((uint64_t)(label - c0) < 8)
+template <class T, int RT>
+__device__ __forceinline__ void write_zeros(const GradRow<T>& g, const Row<T>& x) {
+  const int t = RT == 64 ? threadIdx.x & 63 : threadIdx.x;
+  const int single = x.single(t);
+  if (single >= 0) g.g[single] = (T)0.f;
+  for (int j = t; j < x.body; j += RT) g.store(x.column(j), typename Row<T>::Wide{});
+}
+
+// c (onehot(label) - exp(x - lse)) of the columns from c0 on
+template <class Wide>
+__device__ __forceinline__ Wide row_gradient(Wide v, float lse, float c, int c0, int64_t label) {
+  constexpr int W = sizeof(Wide) / 4;
+  Wide g;
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+  for (int e = 0; e < W; ++e) g[e] = exp_from(v[e], lse) * -c;
+  if ((uint64_t)(label - c0) < W)
+#pragma unroll
+    for (int e = 0; e < W; ++e)
       if (c0 + e == label) g[e] += c;
   return g;
 }
-
-template <class T, bool VEC, int RT>
-__device__ __forceinline__ void write_zeros(T* g, int64_t vocab) {
+// of the thread's single column
+template <class T>
+__device__ __forceinline__ void single_gradient(const Row<T>& x, T* g, int t, float lse, float c, int64_t label) {
+  const int single = x.single(t);
+  if (single >= 0) g[single] = (T)(exp_from((float)x.p[single], lse) * -c + (single == label ? c : 0.f));
+}
+// of a row of memory
+template <class T, int RT>
+__device__ __forceinline__ void write_gradient(const Row<T>& x, const GradRow<T>& g, float lse, float c, int64_t label) {
+  constexpr int U = 4;
   const int t = RT == 64 ? threadIdx.x & 63 : threadIdx.x;
-  for (int64_t c = (int64_t)t * 8; c < vocab; c += RT * 8) store8<VEC>(g, c, vocab, f32x8{});
+  single_gradient(x, g.g, t, lse, c, label);
+  for (int j = t; j < x.body; j += RT * U) {
+    typename Row<T>::Raw v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = x.load(j + u * RT);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (j + u * RT < x.body) g.store(x.column(j + u * RT), row_gradient(widen(v[u]), lse, c, x.column(j + u * RT), label));
+  }
 }
 
-// per_row: coefs holds one for each row, else one for each sequence
-template <class T, bool VEC, int RT>
-__global__ void __launch_bounds__(RT == 64 ? 256 : RT) logit_grad_kernel(LogitRows a, const float* lse, const float* coefs,
-                                                                         int per_row, T* gx) {
-  const int64_t row = this_row<RT>(a.rows);
+// per_row: coefs holds one for each row, else one for each sequence. backwards: the last rows first, which a pass over all rows
+// has left in the last cache. losses (or null): the mean of so many goes to loss, by the first workgroup.
+struct GradArgs {
+  const float *lse, *coefs;
+  int per_row, backwards;
+  const double* losses;
+  int64_t count;
+  float* loss;
+};
+__device__ __forceinline__ void mean_loss(const double* losses, int64_t count, float* loss) {  // by one wave
+  double s = 0.0;
+  for (int64_t i = threadIdx.x; i < count; i += 64) s += losses[i];
+  s = wave_sum(s);
+  if (threadIdx.x == 0) *loss = (float)(s / (double)count);
+}
+template <class T, int RT>
+__global__ void __launch_bounds__(RT == 64 ? 256 : RT) logit_grad_kernel(LogitRows a, GradArgs q, T* gx) {
+  if (q.losses && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 64) mean_loss(q.losses, q.count, q.loss);
+  int64_t row = this_row<RT>(a.rows);
   if (row < 0) return;
-  const int t = RT == 64 ? threadIdx.x & 63 : threadIdx.x;
+  if (q.backwards) row = a.rows - 1 - row;
   const int64_t label = a.labels[row];
-  const float coef = coefs[per_row ? row : row / a.length];
-  T* g = gx + row * a.vocab;
-  if (label == a.ignore || coef == 0.f) return write_zeros<T, VEC, RT>(g, a.vocab);
-  const float c = in_vocab(label, a.vocab) ? coef : __builtin_nanf(""), l = lse[row];
-  const T* x = (const T*)a.x + a.offset(row);
-  constexpr int U = 4;
-  for (int64_t c0 = (int64_t)t * 8; c0 < a.vocab; c0 += RT * 8 * U) {
-    f32x8 v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) v[u] = load8<VEC>(x, c0 + u * RT * 8, a.vocab);
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t cu = c0 + u * RT * 8;
-      f32x8 p;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) p[e] = exp_from(v[u][e], l);
-      store8<VEC>(g, cu, a.vocab, row_gradient(p, c, cu, label));
-    }
-  }
+  const float coef = q.coefs[q.per_row ? row : row / a.length];
+  const Row<T> x((const T*)a.x + a.offset(row), a.vocab);
+  const GradRow<T> g(gx + row * a.vocab, x);
+  if (label == a.ignore || coef == 0.f) return write_zeros<T, RT>(g, x);
+  write_gradient<T, RT>(x, g, q.lse[row], in_vocab(label, a.vocab) ? coef : __builtin_nanf(""), label);
+}
+__global__ void __launch_bounds__(64) mean_loss_kernel(const double* losses, int64_t count, float* loss) {
+  mean_loss(losses, count, loss);
 }
 
 // ---- pairs ----------------------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ double block_sum(double v, double* red) {  // 256 threads, in every one of them
-  v = wave_sum(v);
+// two sums over the workgroup's THREADS, in every one of them
+template <int THREADS>
+__device__ __forceinline__ void block_sums(double& u, double& v, double* red) {
+  u = wave_sum(u), v = wave_sum(v);
   __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  if ((threadIdx.x & 63) == 0) red[(threadIdx.x >> 6) * 2] = u, red[(threadIdx.x >> 6) * 2 + 1] = v;
   __syncthreads();
-  return (red[0] + red[1]) + (red[2] + red[3]);
+  u = v = 0.0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) u += red[w * 2], v += red[w * 2 + 1];
 }
 
 struct PairArgs {
@@ -226,17 +317,19 @@ __device__ __forceinline__ double softplus_neg(double z) { return (z < 0 ? -z : 
 __device__ __forceinline__ double sigmoid(double z) { return 1.0 / (1.0 + exp(-z)); }
 
 __global__ void __launch_bounds__(256) preference_pair_kernel(PairArgs a) {
-  __shared__ double red[4];
+  __shared__ double red[8];
   const int64_t pair = blockIdx.x;
   double ratio[2], share[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
     const int64_t seq = pair + k * a.pairs, base = seq * a.length;
     double sum = 0.0, count = 0.0;
-    for (int64_t i = threadIdx.x; i < a.length; i += 256)
-      if (a.labels[base + i] != a.ignore) sum += (double)a.logps[base + i], count += 1.0;
-    sum = block_sum(sum, red);
-    count = block_sum(count, red);
+#pragma unroll 4
+    for (int64_t i = threadIdx.x; i < a.length; i += 256) {  // (logps of labels that do not count are 0)
+      sum += (double)a.logps[base + i];
+      count += a.labels[base + i] != a.ignore ? 1.0 : 0.0;
+    }
+    block_sums<256>(sum, count, red);
     share[k] = a.average ? 1.0 / fmax(count, 1.0) : 1.0;
     ratio[k] = sum * share[k] - (double)a.reference[seq];
   }
@@ -261,33 +354,26 @@ __global__ void __launch_bounds__(256) preference_pair_kernel(PairArgs a) {
   }
 }
 
-// out = scale * (sum of v), in a fixed order
-__global__ void __launch_bounds__(256) mean_kernel(const double* v, int64_t n, double scale, float* out) {
-  __shared__ double red[4];
-  double s = 0.0;
-  for (int64_t i = threadIdx.x; i < n; i += 256) s += v[i];
-  s = block_sum(s, red);
-  if (threadIdx.x == 0) *out = (float)(s * scale);
-}
-
 // ---- policy ---------------------------------------------------------------------------------------------------------
 
 // counts[segment] = the labels of it that count: segments of `span` labels
 __global__ void __launch_bounds__(256) count_labels_kernel(const int64_t* labels, int64_t n, int64_t span, int64_t ignore,
                                                            double* counts) {
-  __shared__ double red[4];
+  __shared__ double red[8];
   const int64_t beg = blockIdx.x * span, end = min(beg + span, n);
   int64_t c = 0;
+#pragma unroll 4
   for (int64_t i = beg + threadIdx.x; i < end; i += 256) c += labels[i] != ignore;
-  const double all = block_sum((double)c, red);
+  double all = (double)c, none = 0.0;
+  block_sums<256>(all, none, red);
   if (threadIdx.x == 0) counts[blockIdx.x] = all;
 }
 
 struct PolicyArgs {
   const float *old, *reference, *advantages;
   int64_t advantage_sequence, advantage_row;  // strides
-  const double* counts;
-  int64_t segments;  // counts of the whole batch's parts, or (by_sequence) of each sequence
+  const double* counts;  // null: each row's threads count for themselves
+  int64_t segments;      // counts of the whole batch's parts, 64 at most, or (by_sequence) of each sequence
   int by_sequence;
   double lo, hi, kl;
   float* logps;
@@ -300,10 +386,15 @@ struct TokenLoss {
   double loss, kl, slope;
 };
 __device__ __forceinline__ double token_share(const PolicyArgs& p, const LogitRows& a, int64_t row) {
-  if (p.by_sequence) return 1.0 / (p.counts[row / a.length] * (double)(a.rows / a.length));
-  double n = 0.0;
-  for (int64_t i = 0; i < p.segments; ++i) n += p.counts[i];
-  return 1.0 / n;
+  const double sequences = p.by_sequence ? (double)(a.rows / a.length) : 1.0;
+  if (!p.counts) {
+    const int64_t beg = p.by_sequence ? row / a.length * a.length : 0, n = p.by_sequence ? a.length : a.rows;
+    int c = 0;
+    for (int64_t i = threadIdx.x & 63; i < n; i += 64) c += a.labels[beg + i] != a.ignore;
+    return 1.0 / (wave_sum((double)c) * sequences);
+  }
+  if (p.by_sequence) return 1.0 / (p.counts[row / a.length] * sequences);
+  return 1.0 / wave_sum((threadIdx.x & 63) < p.segments ? p.counts[threadIdx.x & 63] : 0.0);
 }
 __device__ __forceinline__ TokenLoss token_loss(const PolicyArgs& p, const LogitRows& a, int64_t row, double lp) {
   const double share = token_share(p, a, row);
@@ -320,100 +411,73 @@ __device__ __forceinline__ TokenLoss token_loss(const PolicyArgs& p, const Logit
   return {t.loss * share, t.kl * share, t.slope * share};
 }
 
-// eight logits of a row as they are in memory, minus infinity behind it
-template <bool VEC>
-__device__ __forceinline__ f32x8 load_raw(const float* p, int64_t c, int64_t cols) { return load_logits<VEC>(p, c, cols); }
-template <bool VEC>
-__device__ __forceinline__ bf16x8 load_raw(const __bf16* p, int64_t c, int64_t cols) {
-  bf16x8 v;
-  if (c + 8 <= cols) {
-    if constexpr (VEC) v = *(const bf16x8*)(p + c);
-    else __builtin_memcpy(&v, p + c, sizeof(v));
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = !VEC && c + e < cols ? p[c + e] : (__bf16)-kInf;
-  }
-  return v;
-}
-__device__ __forceinline__ f32x8 widen(f32x8 v) { return v; }
-__device__ __forceinline__ f32x8 widen(bf16x8 v) { return __builtin_convertvector(v, f32x8); }
-
-// NV vectors of eight logits to a thread hold the row; NV = 0: the row is read again for the gradient
-template <class T, bool VEC, int RT, int NV>
+// NV vectors to a thread hold the row's body; NV = 0: the row is read again for the gradient
+template <class T, int RT, int NV>
 __global__ void __launch_bounds__(RT == 64 ? 256 : RT) policy_kernel(LogitRows a, PolicyArgs p) {
   __shared__ float red[16];
   const int64_t row = this_row<RT>(a.rows);
   if (row < 0) return;
   const int t = RT == 64 ? threadIdx.x & 63 : threadIdx.x;
   const int64_t label = a.labels[row];
-  T* g = p.gx ? (T*)p.gx + row * a.vocab : nullptr;
+  const Row<T> x((const T*)a.x + a.offset(row), a.vocab);
+  const GradRow<T> g((T*)p.gx + row * a.vocab, x);
   if (label == a.ignore) {
     if (t == 0) p.logps[row] = 0.f, p.terms[row * 2] = p.terms[row * 2 + 1] = 0.0;
-    if (g) write_zeros<T, VEC, RT>(g, a.vocab);
+    if (p.gx) write_zeros<T, RT>(g, x);
     return;
   }
-  const T* x = (const T*)a.x + a.offset(row);
-  decltype(load_raw<VEC>(x, 0, 0)) held[NV ? NV : 1];
+  typename Row<T>::Raw held[NV ? NV : 1];
   RowStats st;
   if constexpr (NV > 0) {
-    float m = -kInf;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) held[i] = load_raw<VEC>(x, (int64_t)(i * RT + t) * 8, a.vocab);
+    for (int i = 0; i < NV; ++i) held[i] = x.load(i * RT + t);
+    const int single = x.single(t);
+    const float one = single >= 0 ? (float)x.p[single] : -kInf;
+    float m = one;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) m = fmaxf(m, max8(widen(held[i])));
+    for (int i = 0; i < NV; ++i) m = fmaxf(m, largest(widen(held[i])));
     st.top = row_max<RT>(m, red);
     const float from = st.top == -kInf ? 0.f : st.top;
-    float s = 0.f;
+    float s = exp_from(one, from);
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const f32x8 v = widen(held[i]);
+      const auto v = widen(held[i]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) s += exp_from(v[e], from);
+      for (int e = 0; e < Row<T>::W; ++e) s += exp_from(v[e], from);
     }
     st.sum = row_total<RT>(s, red);
   } else {
-    st = row_stats<T, VEC, RT>(x, a.vocab, red);
+    st = row_stats<T, RT>(x, red);
   }
-  const double lp = label_logp(x, label, a.vocab, st);
+  const double lp = label_logp(x.p, label, a.vocab, st);
   const TokenLoss loss = token_loss(p, a, row, lp);
   if (t == 0) {
     p.logps[row] = (float)lp;
     p.terms[row * 2] = loss.loss;
     p.terms[row * 2 + 1] = loss.kl;
   }
-  if (!g) return;
+  if (!p.gx) return;
   const float c = (float)loss.slope, lse = (float)((double)st.top + log((double)st.sum));
-  if (c == 0.f) return write_zeros<T, VEC, RT>(g, a.vocab);
-  auto put = [&](f32x8 v, int64_t c0) {
-    f32x8 q;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) q[e] = exp_from(v[e], lse);
-    store8<VEC>(g, c0, a.vocab, row_gradient(q, c, c0, label));
-  };
+  if (c == 0.f) return write_zeros<T, RT>(g, x);
   if constexpr (NV > 0) {
+    single_gradient(x, g.g, t, lse, c, label);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) put(widen(held[i]), (int64_t)(i * RT + t) * 8);
+    for (int i = 0; i < NV; ++i)
+      if (i * RT + t < x.body) g.store(x.column(i * RT + t), row_gradient(widen(held[i]), lse, c, x.column(i * RT + t), label));
   } else {
-    constexpr int U = 4;
-    for (int64_t c0 = (int64_t)t * 8; c0 < a.vocab; c0 += RT * 8 * U) {
-      f32x8 v[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) v[u] = load8<VEC>(x, c0 + u * RT * 8, a.vocab);
-#pragma unroll
-      for (int u = 0; u < U; ++u) put(v[u], c0 + u * RT * 8);
-    }
+    write_gradient<T, RT>(x, g, lse, c, label);
   }
 }
 
 // sums[part] = the terms of a part of the rows; with one part, straight to the loss and the KL term
-__global__ void __launch_bounds__(256) sum_terms_kernel(const double* terms, int64_t rows, int64_t span, double* sums,
+__global__ void __launch_bounds__(1024) sum_terms_kernel(const double* terms, int64_t rows, int64_t span, double* sums,
                                                         float* loss, float* kl) {
-  __shared__ double red[4];
+  __shared__ double red[32];
   const int64_t beg = blockIdx.x * span, end = min(beg + span, rows);
   double l = 0.0, k = 0.0;
-  for (int64_t i = beg + threadIdx.x; i < end; i += 256) l += terms[i * 2], k += terms[i * 2 + 1];
-  l = block_sum(l, red);
-  k = block_sum(k, red);
+#pragma unroll 4
+  for (int64_t i = beg + threadIdx.x; i < end; i += 1024) l += terms[i * 2], k += terms[i * 2 + 1];
+  block_sums<1024>(l, k, red);
   if (threadIdx.x) return;
   if (loss) *loss = (float)l, *kl = (float)k;
   else sums[blockIdx.x * 2] = l, sums[blockIdx.x * 2 + 1] = k;
@@ -431,7 +495,12 @@ __global__ void __launch_bounds__(256) scale_by_kernel(T* x, int64_t n, const fl
 // ---- launches -------------------------------------------------------------------------------------------------------
 
 constexpr int64_t kLogitMaxRows = 1 << 28, kLogitMaxVocab = 1 << 28;
+constexpr int64_t kFewLabels = 1024;  // labels that each row's threads count for themselves, for a launch less
 constexpr int64_t kParts = 64;  // workgroups that count labels, or sum terms, at most
+// Logits of more than this are taken backwards in their second pass (the last cache holds 256 MB; rows that do not count are not in
+// it): preference loss and gradient of 16 x 512 x 32768 bfloat16 213 us forwards, 185 backwards, x 131072 834 and 794; of 6 x 301 x
+// 50021 float32, all of whose counted rows are still there, 138 and 143.
+constexpr int64_t kBackwardsBytes = 384 << 20;
 
 static int logits_check(const char* fn, const omt_logits* q) {
   if (!q) return fail(OMT_INVALID, "%s: null pointer", fn);
@@ -447,49 +516,46 @@ static LogitRows rows_of(const omt_logits* q) {
   return {q->x, q->labels, q->ignore_index, std::max<int64_t>(q->length, 1), q->vocab, q->sequence_stride, q->row_stride,
           q->sequences * q->length};
 }
-static bool vectors(const omt_logits* q, const void* gx) {
-  const int64_t per16 = q->dtype == OMT_DT_F32 ? 4 : 8;
-  return q->vocab % 8 == 0 && q->sequence_stride % per16 == 0 && q->row_stride % per16 == 0 && !((uintptr_t)q->x & 15) &&
-         !((uintptr_t)gx & 15);
-}
-// go(T, VEC): the type and whether rows are read by aligned vectors
+// go(T): the logits' type
 template <class Go>
-static void for_type(const omt_logits* q, const void* gx, Go go) {
-  const bool vec = vectors(q, gx);
-  if (q->dtype == OMT_DT_F32) vec ? go(0.f, std::true_type()) : go(0.f, std::false_type());
-  else vec ? go((__bf16)0.f, std::true_type()) : go((__bf16)0.f, std::false_type());
+static void for_type(const omt_logits* q, Go go) {
+  if (q->dtype == OMT_DT_F32) go(0.f);
+  else go((__bf16)0.f);
 }
+static int64_t row_bytes(const omt_logits* q) { return q->vocab * (q->dtype == OMT_DT_F32 ? 4 : 2); }
 // a workgroup or, at RT = 64, a wave to each row; a dimension of the grid holds fewer than 2^32 threads
 template <int RT, class Kernel, class... A>
 static void launch_rows(Kernel kernel, int64_t rows, hipStream_t s, A... args) {
   const int64_t groups = RT == 64 ? cdiv(rows, 4) : rows, along = std::min<int64_t>(groups, 1 << 20);
   hipLaunchKernelGGL(kernel, dim3((unsigned)along, (unsigned)cdiv(groups, along)), dim3(RT == 64 ? 256 : RT), 0, s, args...);
 }
-// go(RT): threads to a row that is read as it is used
+// go(RT): threads to a row that is read as it is used. Preference loss and gradient of 16 x 512 rows in bfloat16, us, by 64, 128, 256,
+// 512 and 1024 threads: 4 KB 24.1, 25.3, 32.5; 8 KB 35.1, 32.7, 36.9, 52.5; 16 KB 59, 52.8, 51.1, 62; 64 KB -, 202, 186, 181, 186;
+// 256 KB -, -, 878, 845, 794.
 template <class Go>
-static void for_row_threads(int64_t vocab, Go go) {
-  if (vocab <= 2048) go(std::integral_constant<int, 64>());
-  else if (vocab <= 32768) go(std::integral_constant<int, 256>());
+static void for_row_threads(int64_t bytes, Go go) {
+  if (bytes <= 6144) go(std::integral_constant<int, 64>());
+  else if (bytes <= 12288) go(std::integral_constant<int, 128>());
+  else if (bytes <= 32768) go(std::integral_constant<int, 256>());
+  else if (bytes <= 131072) go(std::integral_constant<int, 512>());
   else go(std::integral_constant<int, 1024>());
 }
 
 static int token_logps(const omt_logits* q, float* logps, float* lse, hipStream_t s) {
-  for_type(q, nullptr, [&](auto t, auto vec) {
-    typedef decltype(t) T;
-    for_row_threads(q->vocab, [&](auto rt) {
+  for_type(q, [&](auto t) {
+    for_row_threads(row_bytes(q), [&](auto rt) {
       constexpr int RT = decltype(rt)::value;
-      launch_rows<RT>(token_logps_kernel<T, decltype(vec)::value, RT>, q->sequences * q->length, s, rows_of(q), logps, lse);
+      launch_rows<RT>(token_logps_kernel<decltype(t), RT>, q->sequences * q->length, s, rows_of(q), logps, lse);
     });
   });
   return launch_check("token_logps_kernel");
 }
-static int logit_grad(const omt_logits* q, const float* lse, const float* coefs, int per_row, void* gx, hipStream_t s) {
-  for_type(q, gx, [&](auto t, auto vec) {
+static int logit_grad(const omt_logits* q, const GradArgs& a, void* gx, hipStream_t s) {
+  for_type(q, [&](auto t) {
     typedef decltype(t) T;
-    for_row_threads(q->vocab, [&](auto rt) {
+    for_row_threads(row_bytes(q), [&](auto rt) {
       constexpr int RT = decltype(rt)::value;
-      launch_rows<RT>(logit_grad_kernel<T, decltype(vec)::value, RT>, q->sequences * q->length, s, rows_of(q), lse, coefs,
-                      per_row, (T*)gx);
+      launch_rows<RT>(logit_grad_kernel<T, RT>, q->sequences * q->length, s, rows_of(q), a, (T*)gx);
     });
   });
   return launch_check("logit_grad_kernel");
@@ -515,32 +581,27 @@ struct PolicyPlan {
 static PolicyPlan policy_plan(int64_t sequences, int64_t length, bool by_sequence) {
   const int64_t rows = sequences * length;
   PolicyPlan p;
-  p.segments = by_sequence ? sequences : std::min(kParts, std::max<int64_t>(1, cdiv(rows, 4096)));
+  p.segments = by_sequence ? sequences : std::min(kParts, std::max<int64_t>(1, cdiv(rows, 256)));
   p.span = by_sequence ? length : cdiv(rows, p.segments);
-  p.parts = std::min(kParts, std::max<int64_t>(1, cdiv(rows, 16384)));
+  p.parts = std::min(kParts, std::max<int64_t>(1, cdiv(rows, 65536)));
   p.counts = up256((size_t)p.segments * 8), p.terms = up256((size_t)rows * 16), p.sums = up256((size_t)p.parts * 16);
   return p;
 }
 
-// go(RT, NV): a row of `vocab` logits of type T in the registers of RT threads, NV vectors each; NV = 0: it does not fit
-template <class T, class Go>
-static void for_held_row(int64_t vocab, Go go) {
-#define HELD(RT, NV) go(std::integral_constant<int, RT>(), std::integral_constant<int, NV>())
-  if (vocab <= 512) HELD(64, 1);
-  else if (vocab <= 1024) HELD(64, 2);
-  else if (vocab <= 2048) HELD(64, 4);
-  else if (vocab <= 4096) HELD(256, 2);
-  else if (vocab <= 8192) HELD(256, 4);
-  else if (vocab <= 16384) HELD(256, 8);
-  else if (vocab <= 32768) HELD(1024, 4);
-  else if (vocab <= 65536) HELD(1024, 8);
-  else if constexpr (sizeof(T) == 2) {
-    if (vocab <= 131072) HELD(1024, 16);
-    else HELD(1024, 0);
-  } else {
-    HELD(1024, 0);
-  }
+// go(RT, NV): a row of so many bytes in the registers of RT threads, NV vectors each; NV = 0: it does not fit
+template <class Go>
+static void for_held_row(int64_t bytes, Go go) {
+#define HELD(RT, NV) if (bytes <= RT * NV * 16) return go(std::integral_constant<int, RT>(), std::integral_constant<int, NV>())
+  HELD(64, 1);
+  HELD(64, 2);
+  HELD(64, 4);
+  HELD(64, 8);
+  HELD(256, 4);
+  HELD(256, 8);
+  HELD(256, 16);
+  HELD(512, 16);
 #undef HELD
+  go(std::integral_constant<int, 1024>(), std::integral_constant<int, 0>());
 }
 
 }  // namespace omt
@@ -558,7 +619,7 @@ OMT_EXPORT int omt_token_logps_bwd(const omt_logits* logits, const float* lse, c
   if (int e = logits_check("omt_token_logps_bwd", logits)) return e;
   if (logits->sequences * logits->length == 0) return OMT_OK;
   if (!lse || !g || !gx) return fail(OMT_INVALID, "omt_token_logps_bwd: null pointer");
-  return logit_grad(logits, lse, g, 1, gx, stream_of(stream));
+  return logit_grad(logits, {lse, g, 1, 0, nullptr, 0, nullptr}, gx, stream_of(stream));
 }
 
 OMT_EXPORT size_t omt_preference_workspace(int64_t sequences, int64_t length) {
@@ -585,15 +646,17 @@ OMT_EXPORT int omt_preference_loss(const omt_logits* logits, const float* refere
   double* losses = (double*)(at + p.logps + p.lse);
   float* coefs = (float*)(at + p.logps + p.lse + p.losses);
   hipStream_t s = stream_of(stream);
+  const int64_t pairs = n / 2;
   if (rows > 0)
     if (int e = token_logps(logits, logps, lse, s)) return e;
-  const PairArgs a{logits->labels, logps, reference, logits->ignore_index, logits->length, n / 2, kind, average, beta, smoothing,
+  const PairArgs a{logits->labels, logps, reference, logits->ignore_index, logits->length, pairs, kind, average, beta, smoothing,
                    rewards, coefs, losses};
-  hipLaunchKernelGGL(preference_pair_kernel, dim3((unsigned)(n / 2)), dim3(256), 0, s, a);
+  hipLaunchKernelGGL(preference_pair_kernel, dim3((unsigned)pairs), dim3(256), 0, s, a);
   if (int e = launch_check("preference_pair_kernel")) return e;
-  hipLaunchKernelGGL(mean_kernel, dim3(1), dim3(256), 0, s, losses, n / 2, 1.0 / (double)(n / 2), loss);
-  if (int e = launch_check("mean_kernel")) return e;
-  return gx && rows > 0 ? logit_grad(logits, lse, coefs, 0, gx, s) : OMT_OK;
+  if (gx && rows > 0)
+    return logit_grad(logits, {lse, coefs, 0, rows * row_bytes(logits) > kBackwardsBytes, losses, pairs, loss}, gx, s);
+  hipLaunchKernelGGL(mean_loss_kernel, dim3(1), dim3(64), 0, s, losses, pairs, loss);
+  return launch_check("mean_loss_kernel");
 }
 
 OMT_EXPORT size_t omt_policy_workspace(int64_t sequences, int64_t length, int by_sequence) {
@@ -618,26 +681,28 @@ OMT_EXPORT int omt_policy_loss(const omt_logits* logits, const float* old_logps,
   double *counts = (double*)at, *terms = (double*)(at + p.counts), *sums = (double*)(at + p.counts + p.terms);
   hipStream_t s = stream_of(stream);
   if (rows > 0) {
-    hipLaunchKernelGGL(count_labels_kernel, dim3((unsigned)p.segments), dim3(256), 0, s, logits->labels, rows, p.span,
-                       logits->ignore_index, counts);
-    if (int e = launch_check("count_labels_kernel")) return e;
-    const PolicyArgs a{old_logps, reference, advantages, advantage_sequence_stride, advantage_row_stride, counts, p.segments,
+    const bool few = (by_sequence ? logits->length : rows) <= kFewLabels;
+    if (!few) {
+      hipLaunchKernelGGL(count_labels_kernel, dim3((unsigned)p.segments), dim3(256), 0, s, logits->labels, rows, p.span,
+                         logits->ignore_index, counts);
+      if (int e = launch_check("count_labels_kernel")) return e;
+    }
+    const PolicyArgs a{old_logps, reference, advantages, advantage_sequence_stride, advantage_row_stride, few ? nullptr : counts, p.segments,
                        by_sequence, clip_low, clip_high, kl_weight, logps, terms, gx};
-    for_type(logits, gx, [&](auto t, auto vec) {
-      typedef decltype(t) T;
-      for_held_row<T>(logits->vocab, [&](auto rt, auto nv) {
+    for_type(logits, [&](auto t) {
+      for_held_row(row_bytes(logits), [&](auto rt, auto nv) {
         constexpr int RT = decltype(rt)::value;
-        launch_rows<RT>(policy_kernel<T, decltype(vec)::value, RT, decltype(nv)::value>, rows, s, rows_of(logits), a);
+        launch_rows<RT>(policy_kernel<decltype(t), RT, decltype(nv)::value>, rows, s, rows_of(logits), a);
       });
     });
     if (int e = launch_check("policy_kernel")) return e;
   }
   const bool two = p.parts > 1;
-  hipLaunchKernelGGL(sum_terms_kernel, dim3((unsigned)p.parts), dim3(256), 0, s, terms, rows, cdiv(rows, p.parts), sums,
+  hipLaunchKernelGGL(sum_terms_kernel, dim3((unsigned)p.parts), dim3(1024), 0, s, terms, rows, cdiv(rows, p.parts), sums,
                      two ? nullptr : loss, two ? nullptr : kl);
   if (int e = launch_check("sum_terms_kernel")) return e;
   if (!two) return OMT_OK;
-  hipLaunchKernelGGL(sum_terms_kernel, dim3(1), dim3(256), 0, s, sums, p.parts, p.parts, sums, loss, kl);
+  hipLaunchKernelGGL(sum_terms_kernel, dim3(1), dim3(1024), 0, s, sums, p.parts, p.parts, sums, loss, kl);
   return launch_check("sum_terms_kernel");
 }
 
