@@ -1,11 +1,13 @@
 // Embedding: y[i] = scale * weight[token_i], and its gradient gw[v] = scale * (sum over i with token_i = v of gy[i]), the
 // positions of a token in their order, so that the same inputs give the same bits: no atomics on values.
 //
-// The gradient sorts the positions by token (a stable sort by digits of up to 9 bits: a workgroup in LDS up to 8192
+// The gradient sorts the positions by token (a stable sort by digits of up to 9 bits: one workgroup in LDS up to 2048
 // positions; above, at most 64 workgroups, which count and then scatter each digit), cuts the sorted positions into runs of
 // equal length, whatever the tokens' frequencies, and sums each run's rows of gy in float32: what begins and ends within a run
 // is rounded and written at once, the sums of a token that reaches over runs are joined by a second launch. Rows that no
-// position holds are written as zeros by the workgroups behind the runs'. Bound by memory: gy is read once, gw written once.
+// position holds are written as zeros by further workgroups of the sort's launches, which it leaves most of the card to: at a
+// vocabulary that is large beside the positions the sort takes no time of its own. Bound by memory: gy is read once, gw
+// written once.
 //
 // Tokens outside the vocabulary: a row of NaN, and no part in the gradient; no memory is touched for them.
 #include <algorithm>
@@ -54,9 +56,9 @@ __global__ void __launch_bounds__(256) embedding_kernel(EmbedArgs a) {
 
 // ---- sorting positions by token -------------------------------------------------------------------------------------
 
-constexpr int kSortThreads = 1024, kSortWaves = kSortThreads / 64;
-constexpr int kDigitBits = 9, kBins = 1 << kDigitBits;
-constexpr int kSmallSort = 8192;  // positions that one workgroup sorts in LDS
+constexpr int kSortThreads = 512, kSortWaves = kSortThreads / 64;
+constexpr int kDigitBits = 9, kBins = 1 << kDigitBits;  // a thread to each bin
+constexpr int kSmallSort = 2048;  // positions that one workgroup sorts in LDS
 constexpr int kSortTiles = 64;    // workgroups of a larger sort at most: each adds up the counts of all
 
 // Tokens as keys: those that take part in the gradient, `vocab` for the others, which so come last.
@@ -106,7 +108,7 @@ __device__ __forceinline__ void place_digits(uint32_t* at, int64_t beg, int64_t 
     if (on) put(j, first + (uint32_t)__popcll(below));
   }
 }
-// Of kBins values, one to each of the first kBins threads, the sum of those before it; all threads call it.
+// Of kBins values, one to each thread, the sum of those before it.
 __device__ __forceinline__ uint32_t exclusive_scan(uint32_t v, uint32_t* sums) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   uint32_t run = v;
@@ -118,13 +120,52 @@ __device__ __forceinline__ uint32_t exclusive_scan(uint32_t v, uint32_t* sums) {
   __syncthreads();
   if (lane == 63) sums[wave] = run;
   __syncthreads();
-  for (int i = 0; i < wave; ++i) run += sums[i];
+#pragma unroll
+  for (int i = 0; i < kSortWaves; ++i) run += i < wave ? sums[i] : 0;
   return run - v;
+}
+static_assert(kSortThreads == kBins, "a thread to each bin");
+
+// Rows of the weight's gradient without positions, which workgroups beside a sort's write: those of [first, end), kZeroRows to
+// a workgroup.
+constexpr int kZeroRows = 64;
+struct ZeroRows {
+  void* gw;
+  int64_t first, end, dim;
+  int bytes;  // of an element
+  __device__ __forceinline__ int64_t begin(int64_t group) const { return first + group * kZeroRows; }
+};
+__device__ __forceinline__ void write_zero_rows(const ZeroRows& z, int64_t begin, const uint8_t* holds) {
+  const int rows = (int)min((int64_t)kZeroRows, z.end - begin), lane = threadIdx.x & 63;
+  const int64_t size = z.dim * z.bytes;
+  for (int r = threadIdx.x >> 6; r < rows; r += kSortWaves) {
+    if (holds[r]) continue;
+    char* row = (char*)z.gw + (begin + r) * size;
+    // (rows of any size and alignment: whole vectors on 16 bytes, and the elements before and behind them)
+    const int64_t head = min((int64_t)(0 - (uintptr_t)row & 15), size), body = (size - head) / 16, tail = head + body * 16;
+    if (lane * z.bytes < head)
+      z.bytes == 4 ? *(uint32_t*)(row + lane * 4) = 0 : *(uint16_t*)(row + lane * 2) = 0;
+    if (tail + lane * z.bytes < size)
+      z.bytes == 4 ? *(uint32_t*)(row + tail + lane * 4) = 0 : *(uint16_t*)(row + tail + lane * 2) = 0;
+    for (int64_t i = lane; i < body; i += 64) __builtin_nontemporal_store(omt_u32x4{}, (omt_u32x4*)(row + head) + i);
+  }
 }
 
 // Up to kSmallSort positions, all digits, in one workgroup.
 __global__ void __launch_bounds__(kSortThreads) sort_small_kernel(KeyOf key, int n, int bits, int passes, uint32_t* keys_out,
-                                                                  uint32_t* pos_out) {
+                                                                  uint32_t* pos_out, ZeroRows zeros) {
+  if (blockIdx.x > 0) {  // the positions are few: each workgroup looks through them
+    __shared__ uint8_t holds[kZeroRows];
+    const int64_t begin = zeros.begin(blockIdx.x - 1);
+    if (threadIdx.x < kZeroRows) holds[threadIdx.x] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kSortThreads) {
+      const int64_t r = (int64_t)key(i) - begin;
+      if ((uint64_t)r < kZeroRows) holds[r] = 1;
+    }
+    __syncthreads();
+    return write_zero_rows(zeros, begin, holds);
+  }
   __shared__ uint32_t keys[2][kSmallSort];
   __shared__ uint16_t pos[2][kSmallSort];
   __shared__ uint32_t counts[kSortWaves][kBins];
@@ -138,21 +179,22 @@ __global__ void __launch_bounds__(kSortThreads) sort_small_kernel(KeyOf key, int
     const uint16_t* from_pos = pos[p & 1];
     uint32_t* to = keys[~p & 1];
     uint16_t* to_pos = pos[~p & 1];
-    for (int i = threadIdx.x; i < kSortWaves * kBins; i += kSortThreads) counts[0][i] = 0;
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) counts[w][threadIdx.x] = 0;
     __syncthreads();
     auto at = [&](int64_t j) { return from[j]; };
     count_digits(counts[wave], beg, end, at, p * bits, bits);
     __syncthreads();
     uint32_t total = 0;
-    if (threadIdx.x < kBins)
-      for (int w = 0; w < kSortWaves; ++w) total += counts[w][threadIdx.x];
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) total += counts[w][threadIdx.x];
     uint32_t first = exclusive_scan(total, sums);
-    if (threadIdx.x < kBins)
-      for (int w = 0; w < kSortWaves; ++w) {
-        const uint32_t c = counts[w][threadIdx.x];
-        counts[w][threadIdx.x] = first;
-        first += c;
-      }
+#pragma unroll
+    for (int w = 0; w < kSortWaves; ++w) {
+      const uint32_t c = counts[w][threadIdx.x];
+      counts[w][threadIdx.x] = first;
+      first += c;
+    }
     __syncthreads();
     place_digits(counts[wave], beg, end, at, p * bits, bits, [&](int64_t j, uint32_t place) {
       to[place] = from[j];
@@ -163,7 +205,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_small_kernel(KeyOf key, int
   for (int i = threadIdx.x; i < n; i += kSortThreads) keys_out[i] = keys[passes & 1][i], pos_out[i] = pos[passes & 1][i];
 }
 
-// The keys and positions that a pass of a larger sort reads: the tokens themselves (keys null), or the pass before.
+// The keys and positions that a pass of a larger sort reads: the tokens themselves, or the pass before.
 struct SortFrom {
   KeyOf key;
   const uint32_t *keys, *pos;
@@ -172,52 +214,74 @@ struct SortArgs {
   SortFrom from;
   uint32_t *keys, *pos;  // what it writes
   uint32_t* counts;      // [workgroups][kBins]
-  int64_t n, tile;       // positions, and how many to a workgroup
+  // of each token that occurs, one of its positions, written by the first launch. The others' entries are whatever the memory
+  // held: an entry counts only if the token at that position is the row's, so nothing needs to be cleared first.
+  uint32_t* marks;
+  int64_t n, tile;  // positions, and how many to a workgroup
+  unsigned tiles;   // workgroups that sort; those behind them write zeros
   int shift, bits;
+  ZeroRows zeros;
 };
 
 template <bool FIRST>
 __device__ __forceinline__ uint32_t key_at(const SortFrom& f, int64_t j) {
   return FIRST ? f.key(j) : f.keys[j];
 }
+__device__ __forceinline__ void write_unmarked_rows(const SortArgs& a) {
+  __shared__ uint8_t holds[kZeroRows];
+  const int64_t begin = a.zeros.begin(blockIdx.x - a.tiles), row = begin + threadIdx.x;
+  if (threadIdx.x < kZeroRows && row < a.zeros.end) {
+    const uint32_t at = a.marks[row];
+    holds[threadIdx.x] = at < a.n && a.from.key(at) == (uint32_t)row;
+  }
+  __syncthreads();
+  write_zero_rows(a.zeros, begin, holds);
+}
 
 template <bool FIRST>
 __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortArgs a) {
+  if (blockIdx.x >= a.tiles) return write_unmarked_rows(a);
   __shared__ uint32_t counts[kBins];
-  if (threadIdx.x < kBins) counts[threadIdx.x] = 0;
+  counts[threadIdx.x] = 0;
   __syncthreads();
   const int64_t share = a.tile / kSortWaves;
   const int64_t beg = min(blockIdx.x * a.tile + (threadIdx.x >> 6) * share, a.n), end = min(beg + share, a.n);
-  count_digits(counts, beg, end, [&](int64_t j) { return key_at<FIRST>(a.from, j); }, a.shift, a.bits);
+  count_digits(counts, beg, end, [&](int64_t j) {
+    const uint32_t key = key_at<FIRST>(a.from, j);
+    if (FIRST && key != (uint32_t)a.from.key.vocab) a.marks[key] = (uint32_t)j;
+    return key;
+  }, a.shift, a.bits);
   __syncthreads();
-  if (threadIdx.x < kBins) a.counts[blockIdx.x * kBins + threadIdx.x] = counts[threadIdx.x];
+  a.counts[blockIdx.x * kBins + threadIdx.x] = counts[threadIdx.x];
 }
 
 template <bool FIRST>
 __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortArgs a) {
+  if (blockIdx.x >= a.tiles) return write_unmarked_rows(a);
   __shared__ uint32_t counts[kSortWaves][kBins];
   __shared__ uint32_t sums[kSortWaves];
   const int wave = threadIdx.x >> 6;
-  for (int i = threadIdx.x; i < kSortWaves * kBins; i += kSortThreads) counts[0][i] = 0;
+  uint32_t total = 0, before = 0;  // of this thread's digit, over all workgroups and over those before this one
+#pragma unroll 8
+  for (unsigned t = 0; t < a.tiles; ++t) {
+    const uint32_t c = a.counts[t * kBins + threadIdx.x];
+    total += c;
+    before += t < blockIdx.x ? c : 0;
+  }
+#pragma unroll
+  for (int w = 0; w < kSortWaves; ++w) counts[w][threadIdx.x] = 0;
   __syncthreads();
   const int64_t share = a.tile / kSortWaves;
   const int64_t beg = min(blockIdx.x * a.tile + wave * share, a.n), end = min(beg + share, a.n);
   auto key = [&](int64_t j) { return key_at<FIRST>(a.from, j); };
   count_digits(counts[wave], beg, end, key, a.shift, a.bits);
-  uint32_t total = 0, before = 0;  // of this thread's digit, over all workgroups and over those before this one
-  if (threadIdx.x < kBins)
-    for (unsigned t = 0; t < gridDim.x; ++t) {
-      const uint32_t c = a.counts[t * kBins + threadIdx.x];
-      total += c;
-      before += t < blockIdx.x ? c : 0;
-    }
   uint32_t first = exclusive_scan(total, sums) + before;  // (its barriers stand between the counts above and their use below)
-  if (threadIdx.x < kBins)
-    for (int w = 0; w < kSortWaves; ++w) {
-      const uint32_t c = counts[w][threadIdx.x];
-      counts[w][threadIdx.x] = first;
-      first += c;
-    }
+#pragma unroll
+  for (int w = 0; w < kSortWaves; ++w) {
+    const uint32_t c = counts[w][threadIdx.x];
+    counts[w][threadIdx.x] = first;
+    first += c;
+  }
   __syncthreads();
   place_digits(counts[wave], beg, end, key, a.shift, a.bits, [&](int64_t j, uint32_t place) {
     a.keys[place] = key(j);
@@ -233,12 +297,9 @@ struct SumArgs {
   float* parts;                // [runs][2][dim]: what a run holds of a token that began before it, and of one that goes on after
   void* gw;
   int64_t n, vocab, dim;
-  int64_t run, runs;   // positions to a run, and how many
-  int64_t sum_groups;  // workgroups that sum; those behind them write zeros
+  int64_t run, runs;  // positions to a run, and how many
   float scale;
 };
-
-constexpr int kZeroRows = 64;  // rows of the weight to a workgroup that writes zeros
 
 // the first place in the sorted keys from which on they are `key` or more
 __device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t n, uint32_t key) {
@@ -250,26 +311,9 @@ __device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t n, 
   return lo;
 }
 
-template <class T, bool VEC>
-__device__ __forceinline__ void write_zero_rows(const SumArgs& a, int64_t first) {
-  __shared__ uint8_t empty[kZeroRows];
-  const int rows = (int)min((int64_t)kZeroRows, a.vocab - first);
-  if ((int)threadIdx.x < rows) {
-    const uint32_t v = (uint32_t)(first + threadIdx.x);
-    const int64_t at = lower_bound(a.keys, a.n, v);
-    empty[threadIdx.x] = !(at < a.n && a.keys[at] == v);
-  }
-  __syncthreads();
-  const int lane = threadIdx.x & 63;
-  for (int r = threadIdx.x >> 6; r < rows; r += 4)
-    if (empty[r])
-      for (int64_t c = lane * 8; c < a.dim; c += 512) store8<VEC>((T*)a.gw + (first + r) * a.dim, c, a.dim, f32x8{});
-}
-
 // LANES threads to a run and 8 LANES columns
 template <class T, bool VEC, int LANES>
 __global__ void __launch_bounds__(256) embedding_sum_kernel(SumArgs a) {
-  if ((int64_t)blockIdx.x >= a.sum_groups) return write_zero_rows<T, VEC>(a, (blockIdx.x - a.sum_groups) * (int64_t)kZeroRows);
   const int64_t chunks = (a.dim + LANES * 8 - 1) / (LANES * 8);
   const int64_t unit = blockIdx.x * (int64_t)(256 / LANES) + threadIdx.x / LANES;
   const int64_t run = unit / chunks, c = (unit % chunks * LANES + threadIdx.x % LANES) * 8;
@@ -306,7 +350,7 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(SumArgs a) {
   put(end < a.n && a.keys[end] == key);
 }
 
-// gw of the tokens that began in run blockIdx.x and go on after it: the runs' sums, in order
+// gw of the tokens that began in run blockIdx.x and go on after it: the runs' sums, in order; 8 LANES columns to a workgroup
 template <class T, bool VEC, int LANES>
 __global__ void __launch_bounds__(256) embedding_join_kernel(SumArgs a) {
   __shared__ f32x8 sums[256];
@@ -319,24 +363,22 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(SumArgs a) {
   const int g = threadIdx.x / LANES;
   const int64_t count = last - run, share = (count + GROUPS - 1) / GROUPS;  // runs after this one, and to a group of threads
   const int64_t from = run + 1 + min(g * share, count), to = min(from + share, last + 1);
-  for (int64_t c0 = 0; c0 < a.dim; c0 += LANES * 8) {
-    const int64_t c = c0 + threadIdx.x % LANES * 8;
-    f32x8 sum = {};
-    if (g == 0) sum = load8<false>(a.parts + (run * 2 + 1) * a.dim, c, a.dim);
+  const int64_t c = ((int64_t)blockIdx.y * LANES + threadIdx.x % LANES) * 8;
+  f32x8 sum = {};
+  if (g == 0) sum = load8<false>(a.parts + (run * 2 + 1) * a.dim, c, a.dim);
 #pragma unroll 4
-    for (int64_t r = from; r < to; ++r) sum += load8<false>(a.parts + r * 2 * a.dim, c, a.dim);
-    sums[threadIdx.x] = sum;
-    __syncthreads();
-    if (g == 0) {
-      for (int i = 1; i < GROUPS; ++i) sum += sums[i * LANES + threadIdx.x];
-      store8<VEC>((T*)a.gw + key * a.dim, c, a.dim, sum * a.scale);
-    }
-    __syncthreads();
-  }
+  for (int64_t r = from; r < to; ++r) sum += load8<false>(a.parts + r * 2 * a.dim, c, a.dim);
+  sums[threadIdx.x] = sum;
+  __syncthreads();
+  if (g > 0) return;
+#pragma unroll
+  for (int i = 1; i < GROUPS; ++i) sum += sums[i * LANES + threadIdx.x];
+  store8<VEC>((T*)a.gw + key * a.dim, c, a.dim, sum * a.scale);
 }
 
-// Limits: positions are 32-bit, and a launch holds fewer than 2^24 workgroups of 256 threads along one dimension.
+// Limits: positions and keys are 32-bit, and a launch holds fewer than 2^24 workgroups of 256 threads along one dimension.
 constexpr int64_t kEmbedMaxTokens = 1 << 28, kEmbedMaxVocab = 1 << 28, kEmbedMaxDim = 1 << 16;
+constexpr int64_t kEmbedMaxGroups = (1 << 24) - 1;
 
 // ---- plans ----------------------------------------------------------------------------------------------------------
 
@@ -352,14 +394,15 @@ static int digits_of(int64_t vocab) {
 }
 struct EmbedPlan {
   int64_t run, runs;
-  size_t counts, sorted, parts;  // bytes: of one array each
-  size_t total() const { return counts + 4 * sorted + parts; }
+  size_t counts, marks, sorted, parts;  // bytes: of one array each
+  size_t total() const { return counts + marks + 4 * sorted + parts; }
 };
-static EmbedPlan embed_plan(int64_t n, int64_t dim) {
+static EmbedPlan embed_plan(int64_t n, int64_t vocab, int64_t dim) {
   EmbedPlan p;
   p.run = run_length(n, dim);
   p.runs = cdiv(n, p.run);
-  p.counts = (size_t)kSortTiles * kBins * 4;
+  p.counts = n > kSmallSort ? (size_t)kSortTiles * kBins * 4 : 0;
+  p.marks = n > kSmallSort ? (size_t)cdiv(vocab, 64) * 256 : 0;
   p.sorted = (size_t)cdiv(n, 64) * 256;
   p.parts = (size_t)p.runs * 2 * dim * 4;
   return p;
@@ -412,7 +455,7 @@ OMT_EXPORT int omt_embedding_fwd(int dtype, int token_dtype, int64_t n, int64_t 
 
 OMT_EXPORT size_t omt_embedding_bwd_workspace(int64_t n, int64_t vocab, int64_t dim) {
   if (n < 0 || n > kEmbedMaxTokens || vocab < 1 || dim < 1) return 0;
-  return embed_plan(n, dim).total();
+  return embed_plan(n, vocab, dim).total();
 }
 
 OMT_EXPORT int omt_embedding_bwd(int dtype, int token_dtype, int64_t n, int64_t vocab, int64_t dim, const void* gy,
@@ -420,17 +463,19 @@ OMT_EXPORT int omt_embedding_bwd(int dtype, int token_dtype, int64_t n, int64_t 
                                  size_t workspace_bytes, void* stream) {
   const char* fn = "omt_embedding_bwd";
   if (int e = embed_check(fn, dtype, token_dtype, n, vocab, dim)) return e;
-  if (n > kEmbedMaxTokens || vocab > kEmbedMaxVocab || dim > kEmbedMaxDim)
+  if (n > kEmbedMaxTokens || vocab > kEmbedMaxVocab || dim > kEmbedMaxDim || cdiv(n, run_length(n, dim)) * cdiv(dim, 64) > kEmbedMaxGroups)
     return fail(OMT_UNSUPPORTED, "%s: %lld tokens, weight %lld x %lld", fn, (long long)n, (long long)vocab, (long long)dim);
   if (!gweight || (n > 0 && (!gy || !tokens))) return fail(OMT_INVALID, "%s: null pointer", fn);
-  const EmbedPlan p = embed_plan(n, dim);
-  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.total())
+  const EmbedPlan p = embed_plan(n, vocab, dim);
+  if (p.total() > 0 && (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.total()))
     return fail(OMT_INVALID, "%s: workspace of %zu bytes at %p", fn, workspace_bytes, workspace);
   hipStream_t s = stream_of(stream);
   char* at = (char*)workspace;
   uint32_t* counts = (uint32_t*)at;
   uint32_t *keys[2], *pos[2];
   at += p.counts;
+  uint32_t* marks = (uint32_t*)at;
+  at += p.marks;
   for (int i = 0; i < 2; ++i) {
     keys[i] = (uint32_t*)at, at += p.sorted;
     pos[i] = (uint32_t*)at, at += p.sorted;
@@ -438,39 +483,47 @@ OMT_EXPORT int omt_embedding_bwd(int dtype, int token_dtype, int64_t n, int64_t 
   const KeyOf key{{tokens, token_dtype == OMT_DT_I64}, vocab, padding_idx};
   const int all = digits_of(vocab), passes = (all + kDigitBits - 1) / kDigitBits, bits = (all + passes - 1) / passes;
   int last = 0;
-  if (n > 0 && n <= kSmallSort) {
-    hipLaunchKernelGGL(sort_small_kernel, dim3(1), dim3(kSortThreads), 0, s, key, (int)n, bits, passes, keys[0], pos[0]);
+  const int64_t zero_groups = cdiv(vocab, kZeroRows);
+  const int bytes = dtype == OMT_DT_F32 ? 4 : 2;
+  if (n <= kSmallSort) {
+    hipLaunchKernelGGL(sort_small_kernel, dim3((unsigned)(1 + zero_groups)), dim3(kSortThreads), 0, s, key, (int)n, bits, passes,
+                       keys[0], pos[0], ZeroRows{gweight, 0, vocab, dim, bytes});
     if (int e = launch_check("sort_small_kernel")) return e;
-  } else if (n > 0) {
-    const int64_t tile = cdiv(std::max<int64_t>(4096, cdiv(n, kSortTiles)), kSortThreads) * kSortThreads;
+  } else {
+    const int64_t tile = cdiv(std::max<int64_t>(1024, cdiv(n, kSortTiles)), kSortThreads) * kSortThreads;
     const unsigned tiles = (unsigned)cdiv(n, tile);
-    for (int q = 0; q < passes; ++q) {
-      const SortArgs a{{key, keys[~q & 1], pos[~q & 1]}, keys[q & 1], pos[q & 1], counts, n, tile, q * bits, bits};
-      hipLaunchKernelGGL(q ? sort_count_kernel<false> : sort_count_kernel<true>, dim3(tiles), dim3(kSortThreads), 0, s, a);
-      if (int e = launch_check("sort_count_kernel")) return e;
-      hipLaunchKernelGGL(q ? sort_place_kernel<false> : sort_place_kernel<true>, dim3(tiles), dim3(kSortThreads), 0, s, a);
-      if (int e = launch_check("sort_place_kernel")) return e;
-      last = q & 1;
+    // the rows of zeros, in equal shares beside every launch but the first, which marks the others
+    const int64_t share = cdiv(zero_groups, 2 * passes - 1);
+    for (int q = 0; q < 2 * passes; ++q) {
+      const int64_t done = std::min(zero_groups, std::max(0, q - 1) * share), more = q ? std::min(share, zero_groups - done) : 0;
+      const int pass = q / 2;
+      const SortArgs a{{key, keys[~pass & 1], pos[~pass & 1]}, keys[pass & 1], pos[pass & 1], counts, marks, n, tile, tiles, pass * bits,
+                       bits, {gweight, done * kZeroRows, std::min(vocab, (done + more) * kZeroRows), dim, bytes}};
+      auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(tiles + (unsigned)more), dim3(kSortThreads), 0, s, a);
+      };
+      if (q % 2 == 0) pass ? go(sort_count_kernel<false>) : go(sort_count_kernel<true>);
+      else pass ? go(sort_place_kernel<false>) : go(sort_place_kernel<true>);
+      if (int e = launch_check(q % 2 ? "sort_place_kernel" : "sort_count_kernel")) return e;
+      last = pass & 1;
     }
   }
+  if (n == 0) return OMT_OK;
   const bool vec = dim % 8 == 0 && on16({gy, gweight});
   int status = OMT_OK;
   for_lanes(dim, [&](auto lanes) {
     constexpr int LANES = decltype(lanes)::value;
     const int64_t units = p.runs * cdiv(dim, LANES * 8), groups = cdiv(units, 256 / LANES);
-    const SumArgs a{gy, keys[last], pos[last], (float*)at, gweight, n, vocab, dim, p.run, p.runs, groups, scale};
-    auto go = [&](auto kernel, int64_t grid) { hipLaunchKernelGGL(kernel, dim3((unsigned)grid), dim3(256), 0, s, a); };
-    const int64_t grid = groups + cdiv(vocab, kZeroRows);
-    if (grid >= 1 << 24) {
-      status = fail(OMT_UNSUPPORTED, "%s: %lld tokens, weight %lld x %lld", fn, (long long)n, (long long)vocab, (long long)dim);
-      return;
-    }
+    const SumArgs a{gy, keys[last], pos[last], (float*)at, gweight, n, vocab, dim, p.run, p.runs, scale};
+    auto go = [&](auto kernel, dim3 grid) { hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, a); };
+    const dim3 grid((unsigned)groups);
     if (dtype == OMT_DT_F32) vec ? go(embedding_sum_kernel<float, true, LANES>, grid) : go(embedding_sum_kernel<float, false, LANES>, grid);
     else vec ? go(embedding_sum_kernel<__bf16, true, LANES>, grid) : go(embedding_sum_kernel<__bf16, false, LANES>, grid);
     status = launch_check("embedding_sum_kernel");
     if (status || p.runs < 2) return;
-    if (dtype == OMT_DT_F32) vec ? go(embedding_join_kernel<float, true, LANES>, p.runs) : go(embedding_join_kernel<float, false, LANES>, p.runs);
-    else vec ? go(embedding_join_kernel<__bf16, true, LANES>, p.runs) : go(embedding_join_kernel<__bf16, false, LANES>, p.runs);
+    const dim3 joins((unsigned)p.runs, (unsigned)cdiv(dim, LANES * 8));
+    if (dtype == OMT_DT_F32) vec ? go(embedding_join_kernel<float, true, LANES>, joins) : go(embedding_join_kernel<float, false, LANES>, joins);
+    else vec ? go(embedding_join_kernel<__bf16, true, LANES>, joins) : go(embedding_join_kernel<__bf16, false, LANES>, joins);
     status = launch_check("embedding_join_kernel");
   });
   return status;
