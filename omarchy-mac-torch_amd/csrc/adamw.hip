@@ -16,15 +16,16 @@
 // master copy. Sixteen lanes hold a block of 128, eight values each, and find its largest magnitude in their registers.
 // Every operation on the moments is rounded by itself (no contraction), so that what is stored in 8 bits does not depend on
 // how a compiler pairs them.
-#include <cmath>
-
 #include "block_fp8.h"
 
 namespace omt {
 
-constexpr int kAdamwSlots = 32;    // tensors to a launch: their table travels in the kernel's arguments
-constexpr int kAdamwChunk = 8192;  // elements to a workgroup of 256 threads: four vectors of eight to a thread
+constexpr int kAdamwSlots = 32;  // tensors to a launch: their table travels in the kernel's arguments
 constexpr int kAdamwThreads = 256;
+// Elements to a workgroup, eight to a thread: more of them one after another to a thread, with the next ones' loads ahead, cost more
+// in uneven ends than they saved in starts (8.8 million parameters float32 28.3 us with 8, 32.9 with 16, 35.2 with 32 and 41.1 with
+// 64; 470 million bfloat16 1401, 1407, 1439 and 1471).
+constexpr int kAdamwChunk = kAdamwThreads * 8;
 constexpr int64_t kAdamwMaxNumel = (int64_t)kAdamwChunk * ((1 << 24) - 1);  // a launch holds fewer than 2^32 threads
 constexpr float kFp8Smallest = 0x1p-9f;
 
@@ -60,6 +61,14 @@ struct AdamwScalars {
   float rate, root, decay, eps, grad;
 };
 
+// beta^t for the step count t, by squaring (within t's bits times 2^-52)
+__device__ __forceinline__ double power(double beta, double t) {
+  double p = 1.0;
+  for (uint32_t n = (uint32_t)t; n; n >>= 1, beta *= beta)
+    if (n & 1) p *= beta;
+  return p;
+}
+
 template <class P, bool FP8, bool MASTER>
 __global__ void __launch_bounds__(kAdamwThreads) adamw_kernel(const AdamwTable t, const AdamwHyper h) {
 #pragma clang fp contract(off)
@@ -69,57 +78,55 @@ __global__ void __launch_bounds__(kAdamwThreads) adamw_kernel(const AdamwTable t
   int si = 0;
   while (si + 1 < t.count && chunk >= t.first[si + 1]) ++si;
   const AdamwSlot& s = t.s[si];
+  const int64_t c = (int64_t)(chunk - t.first[si]) * kAdamwChunk + (int)threadIdx.x * 8, block = c / kFp8Block;
+  f32x8 p, g = load8<false>((const P*)s.g, c, s.n), m, v, root;  // on their way while the scalars are computed
+  float m_scale = 0.f, v_scale = 0.f;
+  if constexpr (MASTER) p = load8<false>(s.master, c, s.n);
+  else p = load8<false>((const P*)s.p, c, s.n);
+  if constexpr (FP8) {
+    m = load8<false>((const uint8_t*)s.m, c, s.n), v = load8<false>((const uint8_t*)s.v, c, s.n);
+    if (c < s.n) m_scale = s.m_scale[block], v_scale = s.v_scale[block];
+  } else {
+    m = load8<false>((const float*)s.m, c, s.n), v = load8<false>((const float*)s.v, c, s.n);
+  }
   if (threadIdx.x == 0) {
     const double step = (double)*s.step, lr = h.lr_dev ? (double)*h.lr_dev : h.lr;
     shared = {(float)h.beta1, (float)(1.0 - h.beta1), (float)h.beta2, (float)(1.0 - h.beta2),
-              (float)(lr / (1.0 - pow(h.beta1, step))), (float)sqrt(1.0 - pow(h.beta2, step)), (float)(lr * h.wd), h.eps,
+              (float)(lr / (1.0 - power(h.beta1, step))), (float)sqrt(1.0 - power(h.beta2, step)), (float)(lr * h.wd), h.eps,
               (h.maximize ? -1.f : 1.f) / (h.grad_scale ? *h.grad_scale : 1.f)};
   }
   __syncthreads();
   const AdamwScalars k = shared;
-  const int64_t beg = (int64_t)(chunk - t.first[si]) * kAdamwChunk;
+  if constexpr (FP8) {
+    m *= m_scale;
+    v *= v_scale;
+    v *= v;
+  }
 #pragma unroll
-  for (int i = 0; i < kAdamwChunk / (kAdamwThreads * 8); ++i) {
-    const int64_t c = beg + (i * kAdamwThreads + (int)threadIdx.x) * 8, block = c / kFp8Block;
-    f32x8 p, g = load8<false>((const P*)s.g, c, s.n), m, v;
-    if constexpr (MASTER) p = load8<false>(s.master, c, s.n);
-    else p = load8<false>((const P*)s.p, c, s.n);
-    if constexpr (FP8) {
-      m = load8<false>((const uint8_t*)s.m, c, s.n), v = load8<false>((const uint8_t*)s.v, c, s.n);
-      const float ms = c < s.n ? s.m_scale[block] : 0.f, vs = c < s.n ? s.v_scale[block] : 0.f;
-      m *= ms;
-      v *= vs;
-      v *= v;
-    } else {
-      m = load8<false>((const float*)s.m, c, s.n), v = load8<false>((const float*)s.v, c, s.n);
-    }
-    f32x8 root;
+  for (int e = 0; e < 8; ++e) {
+    const float ge = g[e] * k.grad;
+    m[e] = k.b1 * m[e] + k.c1 * ge;
+    v[e] = k.b2 * v[e] + k.c2 * ge * ge;
+    root[e] = sqrtf(v[e]);
+    p[e] -= k.decay * p[e];
+    p[e] -= k.rate * m[e] / (root[e] / k.root + k.eps);
+  }
+  if constexpr (MASTER) store8<false>(s.master, c, s.n, p);
+  store8<false>((P*)s.p, c, s.n, p);
+  if constexpr (FP8) {
+    const float ms = state_scale(row16_max(abs_bits8(m))), vs = state_scale(row16_max(abs_bits8(root)));
+    const float inv = 1.f / vs;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const float ge = g[e] * k.grad;
-      m[e] = k.b1 * m[e] + k.c1 * ge;
-      v[e] = k.b2 * v[e] + k.c2 * ge * ge;
-      root[e] = sqrtf(v[e]);
-      p[e] -= k.decay * p[e];
-      p[e] -= k.rate * m[e] / (root[e] / k.root + k.eps);
+      const float q = root[e] * inv;
+      root[e] = root[e] > 0.f && q < kFp8Smallest ? kFp8Smallest : q;
     }
-    if constexpr (MASTER) store8<false>(s.master, c, s.n, p);
-    store8<false>((P*)s.p, c, s.n, p);
-    if constexpr (FP8) {
-      const float ms = state_scale(row16_max(abs_bits8(m))), vs = state_scale(row16_max(abs_bits8(root)));
-      const float inv = 1.f / vs;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float q = root[e] * inv;
-        root[e] = root[e] > 0.f && q < kFp8Smallest ? kFp8Smallest : q;
-      }
-      store_fp8x8<false>((uint8_t*)s.m, c, s.n, pack_fp8x8(m, 1.f / ms));
-      store_fp8x8<false>((uint8_t*)s.v, c, s.n, pack_fp8x8(root, 1.f));
-      if ((threadIdx.x & 15) == 0 && c < s.n) s.m_scale[block] = ms, s.v_scale[block] = vs;
-    } else {
-      store8<false>((float*)s.m, c, s.n, m);
-      store8<false>((float*)s.v, c, s.n, v);
-    }
+    store_fp8x8<false>((uint8_t*)s.m, c, s.n, pack_fp8x8(m, 1.f / ms));
+    store_fp8x8<false>((uint8_t*)s.v, c, s.n, pack_fp8x8(root, 1.f));
+    if ((threadIdx.x & 15) == 0 && c < s.n) s.m_scale[block] = ms, s.v_scale[block] = vs;
+  } else {
+    store8<false>((float*)s.m, c, s.n, m);
+    store8<false>((float*)s.v, c, s.n, v);
   }
 }
 
@@ -146,7 +153,8 @@ OMT_EXPORT int omt_adamw(int dtype, int state_bits, const omt_adamw_params* hp, 
   const AdamwHyper h{hp->lr, hp->beta1, hp->beta2, hp->weight_decay, (float)hp->eps, hp->lr_dev, hp->grad_scale, hp->found_inf,
                      hp->maximize};
   for (int i = 0; i < n;) {
-    AdamwTable t{};
+    AdamwTable t;
+    t.count = 0;
     int64_t chunks = 0;
     for (; i < n && t.count < kAdamwSlots; ++i) {
       const omt_adamw_tensor& a = ts[i];
