@@ -301,16 +301,6 @@ struct SumArgs {
   float scale;
 };
 
-// the first place in the sorted keys from which on they are `key` or more
-__device__ __forceinline__ int64_t lower_bound(const uint32_t* keys, int64_t n, uint32_t key) {
-  int64_t lo = 0, hi = n;
-  while (lo < hi) {
-    const int64_t mid = (lo + hi) / 2;
-    if (keys[mid] < key) lo = mid + 1; else hi = mid;
-  }
-  return lo;
-}
-
 // LANES threads to a run and 8 LANES columns
 template <class T, bool VEC, int LANES>
 __global__ void __launch_bounds__(256) embedding_sum_kernel(SumArgs a) {
@@ -328,21 +318,28 @@ __global__ void __launch_bounds__(256) embedding_sum_kernel(SumArgs a) {
     if (began || goes_on) store8<false>(a.parts + (run * 2 + (began ? 0 : 1)) * a.dim, c, a.dim, sum);
     else store8<VEC>((T*)a.gw + key * a.dim, c, a.dim, sum * a.scale);
   };
-  constexpr int U = 4;
+  constexpr int U = 8;
+  uint32_t k[U], at[U];
+  auto look = [&](int64_t i) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) k[u] = i + u < end ? a.keys[i + u] : none, at[u] = i + u < end ? a.pos[i + u] : 0;
+  };
+  look(beg);
   for (int64_t i = beg; i < end; i += U) {
     f32x8 v[U];
-    uint32_t k[U];
+    uint32_t now[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      k[u] = i + u < end ? a.keys[i + u] : none;
-      v[u] = k[u] != none ? load8<VEC>((const T*)a.gy + (int64_t)a.pos[i + u] * a.dim, c, a.dim) : f32x8{};
+      now[u] = k[u];
+      v[u] = k[u] != none ? load8<VEC>((const T*)a.gy + (int64_t)at[u] * a.dim, c, a.dim) : f32x8{};
     }
+    if (i + U < end) look(i + U);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (i + u >= end) break;
-      if (k[u] != key) {
+      if (now[u] != key) {
         put(false);
-        key = k[u], began = false, sum = f32x8{};
+        key = now[u], began = false, sum = f32x8{};
       }
       sum += v[u];
     }
@@ -358,7 +355,14 @@ __global__ void __launch_bounds__(256) embedding_join_kernel(SumArgs a) {
   const uint32_t key = a.keys[end - 1];
   if (key == (uint32_t)a.vocab || end == a.n || a.keys[end] != key) return;  // (the same for the whole workgroup)
   if (beg > 0 && a.keys[beg - 1] == key) return;                            // began before
-  const int64_t last = (lower_bound(a.keys, a.n, key + 1) - 1) / a.run;      // the run where it ends
+  // the last run that begins with it: the wave's lanes cut what is left of the runs into 64 at a time
+  int64_t last = run, over = a.runs;  // it begins with the key (or holds the token's beginning); it does not
+  while (over - last > 1) {
+    const int64_t step = (over - last + 63) / 64, at = last + ((threadIdx.x & 63) + 1) * step;
+    const int64_t with = __popcll(__ballot(at < over && a.keys[at * a.run] == key));
+    over = min(over, last + (with + 1) * step);
+    last += with * step;
+  }
   constexpr int GROUPS = 256 / LANES;
   const int g = threadIdx.x / LANES;
   const int64_t count = last - run, share = (count + GROUPS - 1) / GROUPS;  // runs after this one, and to a group of threads
