@@ -193,21 +193,25 @@ __device__ __forceinline__ int64_t this_row(int64_t rows) {
 }
 
 template <class T, int RT>
-__global__ void __launch_bounds__(RT == 64 ? 256 : RT) token_logps_kernel(LogitRows a, float* logps, float* lse) {
+__global__ void __launch_bounds__(RT == 64 ? 256 : RT) token_logps_kernel(LogitRows a, float* logps, float* lse, RowStats* stats) {
   __shared__ float red[16];
   const int64_t row = this_row<RT>(a.rows);
   if (row < 0) return;
   const bool first = (RT == 64 ? threadIdx.x & 63 : threadIdx.x) == 0;
   const int64_t label = a.labels[row];
   if (label == a.ignore) {
-    if (first) logps[row] = 0.f, lse[row] = 0.f;
+    if (first) {
+      logps[row] = 0.f;
+      if (lse) lse[row] = 0.f;
+    }
     return;
   }
   const Row<T> x((const T*)a.x + a.offset(row), a.vocab);
   const RowStats st = row_stats<T, RT>(x, red);
   if (first) {
     logps[row] = (float)label_logp(x.p, label, a.vocab, st);
-    lse[row] = (float)((double)st.top + log((double)st.sum));
+    if (lse) lse[row] = (float)((double)st.top + log((double)st.sum));
+    if (stats) stats[row] = st;
   }
 }
 
@@ -221,45 +225,52 @@ __device__ __forceinline__ void write_zeros(const GradRow<T>& g, const Row<T>& x
   for (int j = t; j < x.body; j += RT) g.store(x.column(j), typename Row<T>::Wide{});
 }
 
-// c (onehot(label) - exp(x - lse)) of the columns from c0 on
+// c onehot(label) - scale exp(x - from), scale exp(-from) = c / sum exp x, of the columns from c0 on
+struct Slope {
+  float c, scale, from;
+  int64_t label;
+};
 template <class Wide>
-__device__ __forceinline__ Wide row_gradient(Wide v, float lse, float c, int c0, int64_t label) {
+__device__ __forceinline__ Wide row_gradient(Wide v, const Slope& s, int c0) {
   constexpr int W = sizeof(Wide) / 4;
   Wide g;
 #pragma unroll
-  for (int e = 0; e < W; ++e) g[e] = exp_from(v[e], lse) * -c;
-  if ((uint64_t)(label - c0) < W)
+  for (int e = 0; e < W; ++e) g[e] = exp_from(v[e], s.from) * -s.scale;
+  if ((uint64_t)(s.label - c0) < W)
 #pragma unroll
     for (int e = 0; e < W; ++e)
-      if (c0 + e == label) g[e] += c;
+      if (c0 + e == s.label) g[e] += s.c;
   return g;
 }
 // of the thread's single column
 template <class T>
-__device__ __forceinline__ void single_gradient(const Row<T>& x, T* g, int t, float lse, float c, int64_t label) {
+__device__ __forceinline__ void single_gradient(const Row<T>& x, T* g, int t, const Slope& s) {
   const int single = x.single(t);
-  if (single >= 0) g[single] = (T)(exp_from((float)x.p[single], lse) * -c + (single == label ? c : 0.f));
+  if (single >= 0) g[single] = (T)(exp_from((float)x.p[single], s.from) * -s.scale + (single == s.label ? s.c : 0.f));
 }
 // of a row of memory
 template <class T, int RT>
-__device__ __forceinline__ void write_gradient(const Row<T>& x, const GradRow<T>& g, float lse, float c, int64_t label) {
+__device__ __forceinline__ void write_gradient(const Row<T>& x, const GradRow<T>& g, const Slope& s) {
   constexpr int U = 4;
   const int t = RT == 64 ? threadIdx.x & 63 : threadIdx.x;
-  single_gradient(x, g.g, t, lse, c, label);
+  single_gradient(x, g.g, t, s);
   for (int j = t; j < x.body; j += RT * U) {
     typename Row<T>::Raw v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) v[u] = x.load(j + u * RT);
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (j + u * RT < x.body) g.store(x.column(j + u * RT), row_gradient(widen(v[u]), lse, c, x.column(j + u * RT), label));
+      if (j + u * RT < x.body) g.store(x.column(j + u * RT), row_gradient(widen(v[u]), s, x.column(j + u * RT)));
   }
 }
 
-// per_row: coefs holds one for each row, else one for each sequence. backwards: the last rows first, which a pass over all rows
+// Of each row, lse, or its RowStats, which spares lse's rounding. per_row: coefs holds one for each row, else one for each sequence.
+// backwards: the last rows first, which a pass over all rows
 // has left in the last cache. losses (or null): the mean of so many goes to loss, by the first workgroup.
 struct GradArgs {
-  const float *lse, *coefs;
+  const float* lse;
+  const RowStats* stats;
+  const float* coefs;
   int per_row, backwards;
   const double* losses;
   int64_t count;
@@ -282,7 +293,9 @@ __global__ void __launch_bounds__(RT == 64 ? 256 : RT) logit_grad_kernel(LogitRo
   const Row<T> x((const T*)a.x + a.offset(row), a.vocab);
   const GradRow<T> g(gx + row * a.vocab, x);
   if (label == a.ignore || coef == 0.f) return write_zeros<T, RT>(g, x);
-  write_gradient<T, RT>(x, g, q.lse[row], in_vocab(label, a.vocab) ? coef : __builtin_nanf(""), label);
+  const float c = in_vocab(label, a.vocab) ? coef : __builtin_nanf("");
+  const RowStats st = q.stats ? q.stats[row] : RowStats{q.lse[row], 1.f};
+  write_gradient<T, RT>(x, g, {c, c / st.sum, st.top, label});
 }
 __global__ void __launch_bounds__(64) mean_loss_kernel(const double* losses, int64_t count, float* loss) {
   mean_loss(losses, count, loss);
@@ -457,15 +470,16 @@ __global__ void __launch_bounds__(RT == 64 ? 256 : RT) policy_kernel(LogitRows a
     p.terms[row * 2 + 1] = loss.kl;
   }
   if (!p.gx) return;
-  const float c = (float)loss.slope, lse = (float)((double)st.top + log((double)st.sum));
+  const float c = (float)loss.slope;
   if (c == 0.f) return write_zeros<T, RT>(g, x);
+  const Slope slope{c, c / st.sum, st.top, label};
   if constexpr (NV > 0) {
-    single_gradient(x, g.g, t, lse, c, label);
+    single_gradient(x, g.g, t, slope);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      if (i * RT + t < x.body) g.store(x.column(i * RT + t), row_gradient(widen(held[i]), lse, c, x.column(i * RT + t), label));
+      if (i * RT + t < x.body) g.store(x.column(i * RT + t), row_gradient(widen(held[i]), slope, x.column(i * RT + t)));
   } else {
-    write_gradient<T, RT>(x, g, lse, c, label);
+    write_gradient<T, RT>(x, g, slope);
   }
 }
 
@@ -541,11 +555,11 @@ static void for_row_threads(int64_t bytes, Go go) {
   else go(std::integral_constant<int, 1024>());
 }
 
-static int token_logps(const omt_logits* q, float* logps, float* lse, hipStream_t s) {
+static int token_logps(const omt_logits* q, float* logps, float* lse, RowStats* stats, hipStream_t s) {
   for_type(q, [&](auto t) {
     for_row_threads(row_bytes(q), [&](auto rt) {
       constexpr int RT = decltype(rt)::value;
-      launch_rows<RT>(token_logps_kernel<decltype(t), RT>, q->sequences * q->length, s, rows_of(q), logps, lse);
+      launch_rows<RT>(token_logps_kernel<decltype(t), RT>, q->sequences * q->length, s, rows_of(q), logps, lse, stats);
     });
   });
   return launch_check("token_logps_kernel");
@@ -564,12 +578,12 @@ static int logit_grad(const omt_logits* q, const GradArgs& a, void* gx, hipStrea
 static size_t up256(size_t n) { return (n + 255) / 256 * 256; }
 
 struct PreferencePlan {
-  size_t logps, lse, losses, coefs;  // bytes
-  size_t total() const { return logps + lse + losses + coefs; }
+  size_t logps, stats, losses, coefs;  // bytes
+  size_t total() const { return logps + stats + losses + coefs; }
 };
 static PreferencePlan preference_plan(int64_t sequences, int64_t length) {
-  const size_t rows = up256((size_t)(sequences * length) * 4);
-  return {rows, rows, up256((size_t)sequences * 4), up256((size_t)sequences * 4)};
+  const size_t rows = (size_t)(sequences * length);
+  return {up256(rows * 4), up256(rows * sizeof(RowStats)), up256((size_t)sequences * 4), up256((size_t)sequences * 4)};
 }
 
 struct PolicyPlan {
@@ -612,14 +626,14 @@ OMT_EXPORT int omt_token_logps_fwd(const omt_logits* logits, float* logps, float
   if (int e = logits_check("omt_token_logps_fwd", logits)) return e;
   if (logits->sequences * logits->length == 0) return OMT_OK;
   if (!logps || !lse) return fail(OMT_INVALID, "omt_token_logps_fwd: null pointer");
-  return token_logps(logits, logps, lse, stream_of(stream));
+  return token_logps(logits, logps, lse, nullptr, stream_of(stream));
 }
 
 OMT_EXPORT int omt_token_logps_bwd(const omt_logits* logits, const float* lse, const float* g, void* gx, void* stream) {
   if (int e = logits_check("omt_token_logps_bwd", logits)) return e;
   if (logits->sequences * logits->length == 0) return OMT_OK;
   if (!lse || !g || !gx) return fail(OMT_INVALID, "omt_token_logps_bwd: null pointer");
-  return logit_grad(logits, {lse, g, 1, 0, nullptr, 0, nullptr}, gx, stream_of(stream));
+  return logit_grad(logits, {lse, nullptr, g, 1, 0, nullptr, 0, nullptr}, gx, stream_of(stream));
 }
 
 OMT_EXPORT size_t omt_preference_workspace(int64_t sequences, int64_t length) {
@@ -642,19 +656,20 @@ OMT_EXPORT int omt_preference_loss(const omt_logits* logits, const float* refere
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.total())
     return fail(OMT_INVALID, "%s: workspace of %zu bytes at %p", fn, workspace_bytes, workspace);
   char* at = (char*)workspace;
-  float *logps = (float*)at, *lse = (float*)(at + p.logps);
-  double* losses = (double*)(at + p.logps + p.lse);
-  float* coefs = (float*)(at + p.logps + p.lse + p.losses);
+  float* logps = (float*)at;
+  RowStats* stats = (RowStats*)(at + p.logps);
+  double* losses = (double*)(at + p.logps + p.stats);
+  float* coefs = (float*)(at + p.logps + p.stats + p.losses);
   hipStream_t s = stream_of(stream);
   const int64_t pairs = n / 2;
   if (rows > 0)
-    if (int e = token_logps(logits, logps, lse, s)) return e;
+    if (int e = token_logps(logits, logps, nullptr, gx ? stats : nullptr, s)) return e;
   const PairArgs a{logits->labels, logps, reference, logits->ignore_index, logits->length, pairs, kind, average, beta, smoothing,
                    rewards, coefs, losses};
   hipLaunchKernelGGL(preference_pair_kernel, dim3((unsigned)pairs), dim3(256), 0, s, a);
   if (int e = launch_check("preference_pair_kernel")) return e;
   if (gx && rows > 0)
-    return logit_grad(logits, {lse, coefs, 0, rows * row_bytes(logits) > kBackwardsBytes, losses, pairs, loss}, gx, s);
+    return logit_grad(logits, {nullptr, stats, coefs, 0, rows * row_bytes(logits) > kBackwardsBytes, losses, pairs, loss}, gx, s);
   hipLaunchKernelGGL(mean_loss_kernel, dim3(1), dim3(64), 0, s, losses, pairs, loss);
   return launch_check("mean_loss_kernel");
 }
