@@ -5,18 +5,20 @@
     preference_loss  training on pairs of sequences: one chosen, one rejected
     policy_loss      training on rewards: clipped probability ratios times advantages, with a KL term to a reference
 
-Differentiable functions over torch.ops.omt's operators. The two losses compute the logits' gradient with the loss, where
+Differentiable functions, and Embedding as a module, over torch.ops.omt's operators. The two losses compute the logits' gradient with the loss, where
 one can be asked for, and hand it on in the backward pass, which therefore runs once. optim.AdamW is the step at the end.
 
 No counterpart in the reference. hip_ops has the same operators as plain functions, for torch.cuda tensors too.
 """
 
 import torch
+from torch import nn
 from torch.autograd.function import once_differentiable
 
 from omarchy_mac_torch import hip_ops
+from omarchy_mac_torch.native import DEVICE
 
-__all__ = ["embedding", "policy_loss", "preference_loss", "token_logps"]
+__all__ = ["Embedding", "embedding", "policy_loss", "preference_loss", "token_logps"]
 
 
 class _Embedding(torch.autograd.Function):
@@ -80,6 +82,22 @@ def embedding(tokens, weight, scale=1.0, padding_idx=None):
     if padding_idx is not None and not -weight.shape[0] <= padding_idx < weight.shape[0]:
         raise ValueError(f"padding_idx: expected a row of {weight.shape[0]}, got {padding_idx}")
     return _Embedding.apply(tokens, weight, scale, padding_idx)
+
+
+class Embedding(nn.Embedding):
+    """nn.Embedding whose rows are multiplied by `scale`: embedding's forward and gradient on the HIP device; elsewhere torch's."""
+
+    def __init__(self, num_embeddings, embedding_dim, padding_idx=None, scale=1.0):
+        super().__init__(num_embeddings, embedding_dim, padding_idx)
+        self.scale = scale
+
+    def forward(self, tokens):
+        if self.weight.device.type not in (DEVICE, "cuda"):
+            return super().forward(tokens) * self.scale
+        return embedding(tokens, self.weight, self.scale, self.padding_idx)
+
+    def extra_repr(self):
+        return super().extra_repr() + f", scale={self.scale}"
 
 
 @torch.compiler.disable

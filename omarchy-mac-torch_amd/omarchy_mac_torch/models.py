@@ -142,12 +142,12 @@ class MlpLM(nn.Module):
     feed-forward sublayers."""
 
     def __init__(self, vocab, dim, hidden, depth, context=4, act="silu", checkpoint="fp8", embed_scale=1.0):
-        from omarchy_mac_torch import ffn  # the operators' library, which a user of the convnets' definitions need not have
+        from omarchy_mac_torch import ffn, lm  # the operators' library, which a user of the convnets' definitions need not have
         super().__init__()
         if dim % context:
             raise ValueError(f"dim {dim} is not a multiple of the context, {context}")
-        self.context, self.embed_scale = context, embed_scale
-        self.embed = nn.Embedding(vocab, dim // context)
+        self.context = context
+        self.embed = lm.Embedding(vocab, dim // context, scale=embed_scale)
         self.blocks = nn.ModuleList(ffn.FeedForward(dim, hidden, act, checkpoint) for _ in range(depth))
         self.norm = ffn.RMSNorm(dim)
         self.head = nn.Linear(dim, vocab, bias=False)
@@ -155,8 +155,7 @@ class MlpLM(nn.Module):
 
     def forward(self, tokens):
         """tokens [batch, length >= context] -> logits [batch, length - context + 1, vocab]"""
-        from omarchy_mac_torch import lm
-        e = lm.embedding(tokens, self.embed.weight, self.embed_scale)
+        e = self.embed(tokens)
         n = tokens.shape[1] - self.context + 1
         x, stream = torch.cat([e[:, i:i + n] for i in range(self.context)], -1), None
         for block in self.blocks:

@@ -34,6 +34,39 @@ def test_embedding_gradient(omt):
         assert lm.embedding(t.to(omt.DEVICE), dev).grad_fn is None
 
 
+def test_embedding_module(omt):
+    """The device's gradient is the host's; padding's row has none; the model's embedding is one."""
+    from omarchy_mac_torch import lm, models
+    host = lm.Embedding(30, 20, padding_idx=3, scale=2.5)
+    dev = lm.Embedding(30, 20, padding_idx=3, scale=2.5)
+    dev.load_state_dict(host.state_dict())
+    dev = dev.to(omt.DEVICE)
+    t = torch.randint(30, (4, 50))
+    a, b = host(t), dev(t.to(omt.DEVICE))
+    assert torch.equal(a.detach(), b.detach().cpu())
+    gy = torch.randn(4, 50, 20)
+    a.backward(gy)
+    b.backward(gy.to(omt.DEVICE))
+    assert rel(dev.weight.grad, host.weight.grad.double()) <= 2e-6 and not bool(dev.weight.grad.cpu()[3].any())
+    m = models.mlp_lm(16, 32, 48, 1, embed_scale=3.0)
+    assert isinstance(m.embed, lm.Embedding) and m.embed.scale == 3.0 and "scale=3.0" in repr(m)
+
+
+def test_a_compiled_model_keeps_the_embedding(omt):
+    from omarchy_mac_torch import models
+    torch.manual_seed(6)
+    m = models.mlp_lm(16, 32, 48, 1, checkpoint="full", embed_scale=3.0).to(omt.DEVICE)
+    t = torch.randint(16, (3, 9)).to(omt.DEVICE)
+    want = m(t)
+    want.sum().backward()
+    grads = [p.grad.cpu().clone() for p in m.parameters()]
+    m.zero_grad()
+    got = torch.compile(m, backend=omt.DEVICE)(t)
+    got.sum().backward()
+    assert rel(got, want.cpu()) <= 1e-5
+    assert all(rel(p.grad, g) <= 1e-5 for p, g in zip(m.parameters(), grads))
+
+
 @pytest.mark.parametrize("scale", [1.0, 3.0])
 def test_losses_hand_their_gradient_on(omt, scale):
     """Through what comes before them and with what comes after; against differences too."""
@@ -187,7 +220,7 @@ def test_language_model_is_tuned(omt, loss):
         opt.zero_grad()
         out.backward()
         if k == 0:
-            plain = plain_lm_scaled(ref, tokens[:, :-1])
+            plain = plain_lm(ref, tokens[:, :-1])
             lp = torch.log_softmax(plain, -1).gather(2, labels.clamp(min=0)[..., None])[..., 0] * (labels != -100)
             was = held.cpu().double()
             if loss == "preference":
@@ -207,20 +240,6 @@ def test_language_model_is_tuned(omt, loss):
         assert math.isfinite(float(out))
     assert all(bool(torch.isfinite(p.detach().cpu()).all()) for p in dev.parameters())
     assert not any(k.startswith("omt::") for k in omt.FALLBACKS)
-
-
-def plain_lm_scaled(m, tokens):
-    embed = m.embed
-
-    class Scaled(torch.nn.Module):
-        def forward(self, t):
-            return embed(t) * m.embed_scale
-
-    m.embed = Scaled()
-    try:
-        return plain_lm(m, tokens)
-    finally:
-        m.embed = embed
 
 
 def test_a_captured_training_step(omt):
