@@ -386,10 +386,10 @@ constexpr int64_t kEmbedMaxGroups = (1 << 24) - 1;
 
 // ---- few positions ---------------------------------------------------------------------------------------------------
 
-// Few positions in one launch instead of three: a workgroup to 64 rows of the weight and 8 LANES columns looks through all tokens,
-// sorts the positions of its rows by row in LDS, and sums them in runs as above, its groups of LANES threads a run each, joined
-// in LDS. Rows of zeros are among those of each workgroup.
-constexpr int kFewTokens = 1024, kFewRows = 64;
+// Few positions in one launch instead of three or more: a workgroup to ROWS rows of the weight and 8 LANES columns looks through all
+// tokens, sorts the positions of its rows by row in LDS, and sums them in runs as above, its groups of LANES threads a run each,
+// joined in LDS. Rows of zeros are among those of each workgroup.
+constexpr int kFewTokens = 2048;
 struct FewArgs {
   KeyOf key;
   const void* gy;
@@ -398,67 +398,80 @@ struct FewArgs {
   int64_t vocab, dim;
   float scale;
 };
-template <class T, bool VEC, int LANES>
+template <class T, bool VEC, int LANES, int ROWS>
 __global__ void __launch_bounds__(512) embedding_few_kernel(FewArgs a) {
-  constexpr int GROUPS = 512 / LANES, WAVES = 8;
-  __shared__ uint16_t at[kFewTokens];  // positions, by row and then in order
-  __shared__ uint8_t of[kFewTokens];   // their rows
-  __shared__ uint32_t counts[WAVES][kFewRows], starts[kFewRows + 1];
+  constexpr int GROUPS = 512 / LANES, WAVES = 8, BITS = ROWS == 64 ? 6 : 3, NONE = 255;
+  __shared__ uint8_t row_of[kFewTokens];  // of each token: the workgroup's row, or NONE
+  __shared__ uint16_t at[kFewTokens];     // positions, by row and then in order
+  __shared__ uint8_t of[kFewTokens];      // their rows
+  __shared__ uint32_t counts[WAVES][ROWS], starts[ROWS + 1];
   __shared__ f32x8 parts[2][512];  // of a run: what began before it, what goes on after
-  const int64_t begin = (int64_t)blockIdx.x * kFewRows;
+  const int64_t begin = (int64_t)blockIdx.x * ROWS;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const int share = (a.n + 511) / 512 * 64, beg = min(wave * share, a.n), end = min(beg + share, a.n);
-  ((uint32_t*)counts)[threadIdx.x] = 0;
+  if (threadIdx.x < WAVES * ROWS) ((uint32_t*)counts)[threadIdx.x] = 0;
   __syncthreads();
-  auto row_of = [&](int j) { return (int64_t)a.key(j) - begin; };
-  auto mine = [&](int64_t r) { return (uint64_t)r < kFewRows && begin + r < a.vocab; };
-  for (int i = beg; i < end; i += 64) {
-    const int64_t r = i + lane < end ? row_of(i + lane) : -1;
-    const uint64_t same = same_digit((uint32_t)r & 63, mine(r), 6);
-    if (mine(r) && !(same & lanes_below())) counts[wave][r] += (uint32_t)__popcll(same);
+  for (int i = beg; i < end; i += 256) {
+    int r[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = i + u * 64 + lane;
+      const int64_t row = j < end ? (int64_t)a.key(j) - begin : NONE;
+      r[u] = (uint64_t)row < ROWS && begin + row < a.vocab ? (int)row : NONE;
+      if (j < end) row_of[j] = (uint8_t)r[u];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint64_t same = same_digit((uint32_t)r[u], r[u] != NONE, BITS);
+      if (r[u] != NONE && !(same & lanes_below())) counts[wave][r[u]] += (uint32_t)__popcll(same);
+      __builtin_amdgcn_wave_barrier();
+    }
   }
   __syncthreads();
   if (wave == 0) {
     uint32_t total = 0;
+    if (lane < ROWS)
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) total += counts[w][lane];
+      for (int w = 0; w < WAVES; ++w) total += counts[w][lane];
     uint32_t run = total;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
       const uint32_t up = __shfl_up(run, d);
       if (lane >= d) run += up;
     }
-    if (lane == 63) starts[kFewRows] = run;
+    if (lane == 63) starts[ROWS] = run;
     run -= total;
-    starts[lane] = run;
+    if (lane < ROWS) {
+      starts[lane] = run;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
-      const uint32_t c = counts[w][lane];
-      counts[w][lane] = run;
-      run += c;
+      for (int w = 0; w < WAVES; ++w) {
+        const uint32_t c = counts[w][lane];
+        counts[w][lane] = run;
+        run += c;
+      }
     }
   }
   __syncthreads();
   for (int i = beg; i < end; i += 64) {
-    const int64_t r = i + lane < end ? row_of(i + lane) : -1;
-    const bool on = mine(r);
-    const uint64_t same = same_digit((uint32_t)r & 63, on, 6), below = same & lanes_below();
+    const int j = i + lane, r = j < end ? row_of[j] : NONE;
+    const bool on = r != NONE;
+    const uint64_t same = same_digit((uint32_t)r, on, BITS), below = same & lanes_below();
     const uint32_t first = on ? counts[wave][r] : 0;
     __builtin_amdgcn_wave_barrier();
     if (on) {
       const uint32_t place = first + (uint32_t)__popcll(below);
-      at[place] = (uint16_t)(i + lane);
+      at[place] = (uint16_t)j;
       of[place] = (uint8_t)r;
       if (!below) counts[wave][r] = first + (uint32_t)__popcll(same);
     }
     __builtin_amdgcn_wave_barrier();
   }
   __syncthreads();
-  const int m = (int)starts[kFewRows], run = (m + GROUPS - 1) / GROUPS, g = threadIdx.x / LANES;
+  const int m = (int)starts[ROWS], run = (m + GROUPS - 1) / GROUPS, g = threadIdx.x / LANES;
   const int from = min(g * run, m), to = min(from + run, m);
   const int64_t c = ((int64_t)blockIdx.y * LANES + threadIdx.x % LANES) * 8;
   auto put = [&](int row, f32x8 sum) { store8<VEC>((T*)a.gw + (begin + row) * a.dim, c, a.dim, sum * a.scale); };
-  for (int r = g; r < kFewRows && begin + r < a.vocab; r += GROUPS)
+  for (int r = g; r < ROWS && begin + r < a.vocab; r += GROUPS)
     if (starts[r] == starts[r + 1]) put(r, f32x8{});
   bool goes_on = false;
   if (from < to) {
@@ -496,13 +509,25 @@ __global__ void __launch_bounds__(512) embedding_few_kernel(FewArgs a) {
   for (int k = g + 1; k * run < m && of[k * run] == row; ++k) sum += parts[0][k * LANES + threadIdx.x % LANES];
   put(row, sum);
 }
-// Threads to a workgroup's columns, 0 where the sort's launches take less. Gradients of 20, 100, 300, 512 and 1024 skewed tokens, us,
-// in one launch and by the sort: 256 x 128 bfloat16 5.1, 6.6, 7.6, 9.1, 13.0 and 12.6, 15.1, 16.0, 16.0, 18.3; 64 x 4096 5.1, 7.0, 8.4, 10.4,
-// 16.0 and 14.6, 14.7, 14.7, 15.6, 16.7; 32768 x 512 8.9, 10.5, 14.5, 19.4, 29.8 and 16.4, 16.9, 18.2, 19.4, 21.4; 32768 x 4096 55, 54, 64, 76, 106 and
-// 60, 63, 61, 61, 63.
-static int few_lanes(int64_t n, int64_t vocab, int64_t dim) {
-  if (cdiv(vocab, kFewRows) * cdiv(dim, 512) < 512) return n <= kFewTokens ? 16 : 0;
-  return n <= 256 ? 64 : 0;
+// How a gradient of few positions is cut, by what it measured: lanes 0 where the sort's launches take less. Skewed tokens, us, with 8
+// rows to a workgroup, with 64, and by the sort:
+//   300 tokens     256 x 128 bfloat16  5.9,  8.0, 15.7   64 x 4096  6.3,  9.1, 14.6   1000 x 1000 float32  9.6,  7.1, 16.6
+//   1024                               8.3, 13.3, 18.0             13.0, 16.4, 16.2                       12.3, 12.2, 19.3
+//   2048                              11.9,    -, 21.1             20.9,    -, 23.1                       16.4,    -, 24.4
+//   4096                              20.2,    -, 22.7             37.5,    -, 28.6                       26.2,    -, 36.1
+// and, of many rows, at 100, 300 and 512 tokens with 64 rows and lanes: 32768 x 512 10.5, 14.5, 19.4 (sort 16.9, 18.2, 19.4), 32768 x 4096
+// 54, 64, 76 (63, 61, 61).
+struct FewPlan {
+  int lanes, rows;
+};
+static FewPlan few_plan(int64_t n, int64_t vocab, int64_t dim) {
+  const int64_t groups = cdiv(vocab, 8) * cdiv(dim, 128);  // workgroups of 8 rows
+  if (n <= 1024) {
+    if (groups <= 512) return {16, 8};
+    if (cdiv(vocab, 64) * cdiv(dim, 512) < 512) return {16, 64};
+    return n <= 256 ? FewPlan{64, 64} : FewPlan{0, 0};
+  }
+  return n <= kFewTokens && groups <= 2048 ? FewPlan{16, 8} : FewPlan{0, 0};
 }
 
 // ---- plans ----------------------------------------------------------------------------------------------------------
@@ -579,7 +604,7 @@ OMT_EXPORT int omt_embedding_fwd(int dtype, int token_dtype, int64_t n, int64_t 
 }
 
 OMT_EXPORT size_t omt_embedding_bwd_workspace(int64_t n, int64_t vocab, int64_t dim) {
-  if (n < 0 || n > kEmbedMaxTokens || vocab < 1 || dim < 1 || few_lanes(n, vocab, dim)) return 0;
+  if (n < 0 || n > kEmbedMaxTokens || vocab < 1 || dim < 1 || few_plan(n, vocab, dim).lanes) return 0;
   return embed_plan(n, vocab, dim).total();
 }
 
@@ -594,17 +619,18 @@ OMT_EXPORT int omt_embedding_bwd(int dtype, int token_dtype, int64_t n, int64_t 
   hipStream_t s = stream_of(stream);
   const KeyOf key{{tokens, token_dtype == OMT_DT_I64}, vocab, padding_idx};
   const bool vec = dim % 8 == 0 && on16({gy, gweight});
-  if (const int lanes = few_lanes(n, vocab, dim)) {
+  if (const FewPlan few = few_plan(n, vocab, dim); few.lanes) {
     const FewArgs a{key, gy, gweight, (int)n, vocab, dim, scale};
-    const dim3 grid((unsigned)cdiv(vocab, kFewRows), (unsigned)cdiv(dim, lanes * 8));
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(512), 0, s, a); };
-    if (lanes == 16) {
-      if (dtype == OMT_DT_F32) vec ? go(embedding_few_kernel<float, true, 16>) : go(embedding_few_kernel<float, false, 16>);
-      else vec ? go(embedding_few_kernel<__bf16, true, 16>) : go(embedding_few_kernel<__bf16, false, 16>);
-    } else {
-      if (dtype == OMT_DT_F32) vec ? go(embedding_few_kernel<float, true, 64>) : go(embedding_few_kernel<float, false, 64>);
-      else vec ? go(embedding_few_kernel<__bf16, true, 64>) : go(embedding_few_kernel<__bf16, false, 64>);
-    }
+    const dim3 grid((unsigned)cdiv(vocab, few.rows), (unsigned)cdiv(dim, few.lanes * 8));
+    auto go = [&](auto lanes, auto rows) {
+      constexpr int LANES = decltype(lanes)::value, ROWS = decltype(rows)::value;
+      auto with = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(512), 0, s, a); };
+      if (dtype == OMT_DT_F32) vec ? with(embedding_few_kernel<float, true, LANES, ROWS>) : with(embedding_few_kernel<float, false, LANES, ROWS>);
+      else vec ? with(embedding_few_kernel<__bf16, true, LANES, ROWS>) : with(embedding_few_kernel<__bf16, false, LANES, ROWS>);
+    };
+    if (few.lanes == 64) go(std::integral_constant<int, 64>(), std::integral_constant<int, 64>());
+    else if (few.rows == 64) go(std::integral_constant<int, 16>(), std::integral_constant<int, 64>());
+    else go(std::integral_constant<int, 16>(), std::integral_constant<int, 8>());
     return launch_check("embedding_few_kernel");
   }
   const EmbedPlan p = embed_plan(n, vocab, dim);

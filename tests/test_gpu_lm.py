@@ -95,10 +95,10 @@ def check_embedding_grad(ops, n, vocab, dim, dtype, tokens, scale=1.3, padding=N
 
 @pytest.mark.parametrize("how", ["one", "distinct", "skewed", "any"])
 @pytest.mark.parametrize("n,vocab", [(1, 1), (15, 2), (16, 16), (17, 511), (64, 512), (1000, 513), (1024, 65), (256, 40000),
-                                     (257, 40000), (1025, 300), (2048, 511), (2048, 40000), (2049, 512), (4097, 70000), (8192, 300),
+                                     (257, 40000), (1025, 300), (1024, 8000), (2048, 511), (1500, 30000), (2048, 40000), (2049, 512), (4097, 70000), (8192, 300),
                                      (8193, 300), (9000, 262143), (20000, 262144), (70001, 1000)])
 def test_embedding_grad_sorts_any_tokens(ops, cuda, n, vocab, how):
-    """In LDS (up to 1024 tokens, or 256 beside many rows), by one workgroup (2048) and by many, of one digit, two and three."""
+    """Few in LDS, by rows of 8 and 64; up to 2048 beside many rows by one workgroup; more by many, of one digit, two and three."""
     check_embedding_grad(ops, n, vocab, 8, F32, some_tokens(n, vocab, how, n))
 
 
@@ -110,6 +110,7 @@ def test_embedding_grad_of_any_width(ops, cuda, dtype, dim):
     check_embedding_grad(ops, 1333, 50, dim, dtype, some_tokens(1333, 50, "skewed", dim), padding=3)
     check_embedding_grad(ops, 2333, 70, dim, dtype, some_tokens(2333, 70, "skewed", dim))
     check_embedding_grad(ops, 150, 33000, dim, dtype, some_tokens(150, 33000, "skewed", dim))
+    check_embedding_grad(ops, 700, 6000, dim, dtype, some_tokens(700, 6000, "skewed", dim))
 
 
 @pytest.mark.parametrize("n", [100, 1500, 10000])
@@ -643,7 +644,7 @@ def every_operator(ops, seed, n=9000):
     return {"embedding": ([few, w], lambda t, w: [ops.embedding(t, w, 2.0)]),
             "embedding_backward": ([gy, tokens], lambda a, t: [ops.embedding_backward(a, t, 600)]),
             "embedding_backward_few": ([gy[:500].clone(), few], lambda a, t: [ops.embedding_backward(a, t, 600)]),
-            "embedding_backward_small": ([gy[:1500].clone(), tokens[:1500].clone()], lambda a, t: [ops.embedding_backward(a, t, 600)]),
+            "embedding_backward_small": ([gy[:1500].clone(), tokens[:1500].clone()], lambda a, t: [ops.embedding_backward(a, t, 30000)]),
             "token_logps": ([x, labels], lambda x, y: list(ops.token_logps(x, y))),
             "preference": ([x, labels, ref], lambda x, y, r: list(ops.preference_loss(x, y, r))),
             "policy": ([x, labels, old, ref], lambda x, y, o, a: list(ops.policy_loss(x, y, o, a, reference=o * 0.99, kl=0.1))),

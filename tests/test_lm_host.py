@@ -36,7 +36,7 @@ def test_embedding_statuses(lib):
     assert b(F32, I64, 4, (1 << 28) + 1, 16, p, p, -1, 1.0, p, p, 1 << 40, None) == no
     # sorted tokens and positions twice, each run's two sums
     assert ws(100000, 50000, 1024) >= 4 * 4 * 100000 and ws(-1, 8, 16) == 0
-    assert ws(100, 8, 16) == 0  # few positions are sorted in LDS
+    assert ws(100, 8, 16) == ws(2048, 256, 128) == 0 < ws(2049, 256, 128)  # few positions are sorted in LDS
 
 
 def logits(lib, sequences=2, length=3, vocab=10, dtype=F32, x=4096, labels=4096):
