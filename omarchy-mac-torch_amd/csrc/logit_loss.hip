@@ -329,8 +329,9 @@ struct PairArgs {
 __device__ __forceinline__ double softplus_neg(double z) { return (z < 0 ? -z : 0.0) + log1p(exp(z < 0 ? z : -z)); }
 __device__ __forceinline__ double sigmoid(double z) { return 1.0 / (1.0 + exp(-z)); }
 
-__global__ void __launch_bounds__(256) preference_pair_kernel(PairArgs a) {
-  __shared__ double red[8];
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) preference_pair_kernel(PairArgs a) {
+  __shared__ double red[THREADS / 32];
   const int64_t pair = blockIdx.x;
   double ratio[2], share[2];
 #pragma unroll
@@ -338,11 +339,11 @@ __global__ void __launch_bounds__(256) preference_pair_kernel(PairArgs a) {
     const int64_t seq = pair + k * a.pairs, base = seq * a.length;
     double sum = 0.0, count = 0.0;
 #pragma unroll 4
-    for (int64_t i = threadIdx.x; i < a.length; i += 256) {  // (logps of labels that do not count are 0)
+    for (int64_t i = threadIdx.x; i < a.length; i += THREADS) {  // (logps of labels that do not count are 0)
       sum += (double)a.logps[base + i];
       count += a.labels[base + i] != a.ignore ? 1.0 : 0.0;
     }
-    block_sums<256>(sum, count, red);
+    block_sums<THREADS>(sum, count, red);
     share[k] = a.average ? 1.0 / fmax(count, 1.0) : 1.0;
     ratio[k] = sum * share[k] - (double)a.reference[seq];
   }
@@ -370,15 +371,15 @@ __global__ void __launch_bounds__(256) preference_pair_kernel(PairArgs a) {
 // ---- policy ---------------------------------------------------------------------------------------------------------
 
 // counts[segment] = the labels of it that count: segments of `span` labels
-__global__ void __launch_bounds__(256) count_labels_kernel(const int64_t* labels, int64_t n, int64_t span, int64_t ignore,
+__global__ void __launch_bounds__(1024) count_labels_kernel(const int64_t* labels, int64_t n, int64_t span, int64_t ignore,
                                                            double* counts) {
-  __shared__ double red[8];
+  __shared__ double red[32];
   const int64_t beg = blockIdx.x * span, end = min(beg + span, n);
   int64_t c = 0;
 #pragma unroll 4
-  for (int64_t i = beg + threadIdx.x; i < end; i += 256) c += labels[i] != ignore;
+  for (int64_t i = beg + threadIdx.x; i < end; i += 1024) c += labels[i] != ignore;
   double all = (double)c, none = 0.0;
-  block_sums<256>(all, none, red);
+  block_sums<1024>(all, none, red);
   if (threadIdx.x == 0) counts[blockIdx.x] = all;
 }
 
@@ -595,7 +596,7 @@ struct PolicyPlan {
 static PolicyPlan policy_plan(int64_t sequences, int64_t length, bool by_sequence) {
   const int64_t rows = sequences * length;
   PolicyPlan p;
-  p.segments = by_sequence ? sequences : std::min(kParts, std::max<int64_t>(1, cdiv(rows, 256)));
+  p.segments = by_sequence ? sequences : std::min(kParts, std::max<int64_t>(1, cdiv(rows, 1024)));
   p.span = by_sequence ? length : cdiv(rows, p.segments);
   p.parts = std::min(kParts, std::max<int64_t>(1, cdiv(rows, 65536)));
   p.counts = up256((size_t)p.segments * 8), p.terms = up256((size_t)rows * 16), p.sums = up256((size_t)p.parts * 16);
@@ -650,7 +651,7 @@ OMT_EXPORT int omt_preference_loss(const omt_logits* logits, const float* refere
   if (n < 2 || n % 2) return fail(OMT_INVALID, "%s: %lld sequences: pairs are needed", fn, (long long)n);
   if (kind < OMT_PREFERENCE_SIGMOID || kind > OMT_PREFERENCE_IPO) return fail(OMT_INVALID, "%s: kind %d", fn, kind);
   if (!(beta > 0.0) || !(smoothing >= 0.0 && smoothing <= 1.0)) return fail(OMT_INVALID, "%s: beta %g, smoothing %g", fn, beta, smoothing);
-  if (n / 2 >= 1 << 24) return fail(OMT_UNSUPPORTED, "%s: %lld sequences", fn, (long long)n);
+  if (n / 2 >= 1 << 22) return fail(OMT_UNSUPPORTED, "%s: %lld sequences", fn, (long long)n);
   if (!reference || !loss || !rewards) return fail(OMT_INVALID, "%s: null pointer", fn);
   const PreferencePlan p = preference_plan(n, logits->length);
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.total())
@@ -666,7 +667,8 @@ OMT_EXPORT int omt_preference_loss(const omt_logits* logits, const float* refere
     if (int e = token_logps(logits, logps, nullptr, gx ? stats : nullptr, s)) return e;
   const PairArgs a{logits->labels, logps, reference, logits->ignore_index, logits->length, pairs, kind, average, beta, smoothing,
                    rewards, coefs, losses};
-  hipLaunchKernelGGL(preference_pair_kernel, dim3((unsigned)pairs), dim3(256), 0, s, a);
+  if (logits->length <= 2048) hipLaunchKernelGGL(preference_pair_kernel<256>, dim3((unsigned)pairs), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(preference_pair_kernel<1024>, dim3((unsigned)pairs), dim3(1024), 0, s, a);
   if (int e = launch_check("preference_pair_kernel")) return e;
   if (gx && rows > 0)
     return logit_grad(logits, {nullptr, stats, coefs, 0, rows * row_bytes(logits) > kBackwardsBytes, losses, pairs, loss}, gx, s);
@@ -687,7 +689,7 @@ OMT_EXPORT int omt_policy_loss(const omt_logits* logits, const float* old_logps,
   if (int e = logits_check(fn, logits)) return e;
   const int64_t rows = logits->sequences * logits->length;
   if (!(clip_low >= 0.0) || !(clip_high >= 0.0)) return fail(OMT_INVALID, "%s: clip %g, %g", fn, clip_low, clip_high);
-  if (by_sequence && logits->sequences >= 1 << 24) return fail(OMT_UNSUPPORTED, "%s: %lld sequences", fn, (long long)logits->sequences);
+  if (by_sequence && logits->sequences >= 1 << 22) return fail(OMT_UNSUPPORTED, "%s: %lld sequences", fn, (long long)logits->sequences);
   if (!loss || !kl || (rows > 0 && (!old_logps || !advantages || !logps))) return fail(OMT_INVALID, "%s: null pointer", fn);
   const PolicyPlan p = policy_plan(logits->sequences, logits->length, by_sequence != 0);
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.total())
@@ -698,7 +700,7 @@ OMT_EXPORT int omt_policy_loss(const omt_logits* logits, const float* old_logps,
   if (rows > 0) {
     const bool few = (by_sequence ? logits->length : rows) <= kFewLabels;
     if (!few) {
-      hipLaunchKernelGGL(count_labels_kernel, dim3((unsigned)p.segments), dim3(256), 0, s, logits->labels, rows, p.span,
+      hipLaunchKernelGGL(count_labels_kernel, dim3((unsigned)p.segments), dim3(1024), 0, s, logits->labels, rows, p.span,
                          logits->ignore_index, counts);
       if (int e = launch_check("count_labels_kernel")) return e;
     }

@@ -239,7 +239,7 @@ def test_preference_loss(ops, cuda, dtype, vocab):
 
 @pytest.mark.parametrize("kind,smoothing,average", [("sigmoid", 0.1, False), ("sigmoid", 1.0, True), ("hinge", 0.0, False),
                                                     ("hinge", 0.0, True), ("ipo", 0.0, False), ("ipo", 0.0, True)])
-@pytest.mark.parametrize("length", [1, 2, 300])
+@pytest.mark.parametrize("length", [1, 2, 300, 3001])
 def test_preference_kinds(ops, cuda, kind, smoothing, average, length):
     check_preference(ops, *some_logits(6, length, 33, F32, length), kind=kind, smoothing=smoothing, average=average)
 

@@ -66,6 +66,7 @@ def test_loss_statuses(lib):
     assert g(logits(lib), ref=None) == bad and g(logits(lib), loss=None) == bad and g(logits(lib), rewards=None) == bad
     assert g(logits(lib), ws=None) == bad and g(logits(lib), size=need - 1) == bad
     assert g(logits(lib), ws=ctypes.c_void_p(4104)) == bad
+    assert g(logits(lib, sequences=1 << 23, length=1), size=1 << 40) == no
     assert L.omt_preference_workspace(1 << 20, 1 << 20) == 0
 
     need = L.omt_policy_workspace(2, 3, 1)
@@ -75,7 +76,7 @@ def test_loss_statuses(lib):
     assert h(logits(lib), loss=None) == bad and h(logits(lib), kl=None) == bad
     assert h(logits(lib), lo=-0.1) == bad and h(logits(lib), hi=float("nan")) == bad
     assert h(logits(lib), ws=None) == bad and h(logits(lib), size=need - 1) == bad
-    assert h(logits(lib, length=1 << 28)) == no
+    assert h(logits(lib, length=1 << 28)) == no and h(logits(lib, sequences=1 << 22, length=1), size=1 << 40) == no
     assert L.omt_policy_workspace(-1, 3, 0) == 0
 
     s = L.omt_scale_by
