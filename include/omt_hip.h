@@ -702,9 +702,9 @@ int omt_embedding_bwd(int dtype, int token_dtype, int64_t n, int64_t vocab, int6
                       int64_t padding_idx, float scale, void* gweight, void* workspace, size_t workspace_bytes, void* stream);
 
 /* Logits x [sequences][length][vocab], each row dense, strides in elements, with labels [sequences][length] (dense). A row whose
- * label is ignore_index does not count and is not read; another label outside the vocabulary makes the loss and the row's gradient
- * NaN. Up to 2^28 rows and columns, and fewer than 2^22 pairs, or sequences where a mean is by sequence (OMT_UNSUPPORTED otherwise).
- * Gradients gx are dense, in x's type. */
+ * label is ignore_index does not count and is not read; another label outside the vocabulary makes the loss, and the gradient of its
+ * row (of its pair's rows), NaN. Gradients gx are dense, in x's type. Up to 2^28 rows and columns, and fewer than 2^22 pairs, or
+ * sequences where a mean is by sequence (OMT_UNSUPPORTED otherwise). */
 typedef struct omt_logits {
   const void* x;
   const int64_t* labels;

@@ -9,6 +9,10 @@
 // vocabulary that is large beside the positions the sort takes no time of its own. Bound by memory: gy is read once, gw
 // written once.
 //
+// bfloat16, tokens as text has them: 65536 rows of 2048 from 131072 82 us (0.36 GB at 4.3 TB/s; 0.45 GB pass the caches, since eight of
+// them read the frequent rows); the gradient of 32768 positions 148 us (0.67 GB at 4.5 TB/s), of which the sort with its rows of zeros
+// 98, the sums 31 and the joins 6. 8191 positions to 256 x 128 float32 22 us, four launches; few positions take one (below).
+//
 // Tokens outside the vocabulary: a row of NaN, and no part in the gradient; no memory is touched for them.
 #include <algorithm>
 

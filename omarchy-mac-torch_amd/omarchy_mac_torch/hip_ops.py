@@ -934,7 +934,7 @@ def embedding_backward(gy, tokens, vocab, scale=1.0, padding_idx=None):
 def token_logps(logits, labels, ignore_index=-100):
     """log softmax(logits)[label] of each label: logits [sequences, length, vocab] (rows dense, any other strides), labels int64
     [sequences, length]. Returns (logps, lse) in float32, lse each row's log sum exp; both 0 where the label is ignore_index, whose
-    rows are not read. A label outside the vocabulary gives NaN."""
+    rows are not read. A label outside the vocabulary gives NaN, here and in the losses below."""
     return _lm("token_logps", logits, labels, int(ignore_index))
 
 
