@@ -11,7 +11,7 @@
 //
 // bfloat16, tokens as text has them: 65536 rows of 2048 from 131072 82 us (0.36 GB at 4.3 TB/s; 0.45 GB pass the caches, since eight of
 // them read the frequent rows); the gradient of 32768 positions 148 us (0.67 GB at 4.5 TB/s), of which the sort with its rows of zeros
-// 98, the sums 31 and the joins 6. 8191 positions to 256 x 128 float32 22 us, four launches; few positions take one (below).
+// 98, the sums 31 and the joins 6. 8191 positions to 256 x 128 float32 20.5 us, three launches; few positions take one (below).
 //
 // Tokens outside the vocabulary: a row of NaN, and no part in the gradient; no memory is touched for them.
 #include <algorithm>
@@ -218,7 +218,8 @@ struct SortArgs {
   SortFrom from;
   uint32_t *keys, *pos;  // what it writes
   uint32_t* counts;      // [workgroups][kBins]
-  // of each token that occurs, one of its positions, written by the first launch. The others' entries are whatever the memory
+  uint32_t* starts;      // [kBins + 1], or null: where each digit begins
+  // (or null) of each token that occurs, one of its positions, written by the first launch. The others' entries are whatever the memory
   // held: an entry counts only if the token at that position is the row's, so nothing needs to be cleared first.
   uint32_t* marks;
   int64_t n, tile;  // positions, and how many to a workgroup
@@ -252,7 +253,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_count_kernel(SortArgs a) {
   const int64_t beg = min(blockIdx.x * a.tile + (threadIdx.x >> 6) * share, a.n), end = min(beg + share, a.n);
   count_digits(counts, beg, end, [&](int64_t j) {
     const uint32_t key = key_at<FIRST>(a.from, j);
-    if (FIRST && key != (uint32_t)a.from.key.vocab) a.marks[key] = (uint32_t)j;
+    if (FIRST && a.marks && key != (uint32_t)a.from.key.vocab) a.marks[key] = (uint32_t)j;
     return key;
   }, a.shift, a.bits);
   __syncthreads();
@@ -279,7 +280,12 @@ __global__ void __launch_bounds__(kSortThreads) sort_place_kernel(SortArgs a) {
   const int64_t beg = min(blockIdx.x * a.tile + wave * share, a.n), end = min(beg + share, a.n);
   auto key = [&](int64_t j) { return key_at<FIRST>(a.from, j); };
   count_digits(counts[wave], beg, end, key, a.shift, a.bits);
-  uint32_t first = exclusive_scan(total, sums) + before;  // (its barriers stand between the counts above and their use below)
+  uint32_t first = exclusive_scan(total, sums);
+  if (a.starts && blockIdx.x == 0) {
+    a.starts[threadIdx.x] = first;
+    if (threadIdx.x == kBins - 1) a.starts[kBins] = first + total;
+  }
+  first += before;  // (the scan's barriers stand between the counts above and their use below)
 #pragma unroll
   for (int w = 0; w < kSortWaves; ++w) {
     const uint32_t c = counts[w][threadIdx.x];
@@ -402,41 +408,34 @@ struct FewArgs {
   int64_t vocab, dim;
   float scale;
 };
-template <class T, bool VEC, int LANES, int ROWS>
-__global__ void __launch_bounds__(512) embedding_few_kernel(FewArgs a) {
-  constexpr int GROUPS = 512 / LANES, WAVES = 8, BITS = ROWS == 64 ? 6 : 3, NONE = 255;
-  __shared__ uint8_t row_of[kFewTokens];  // of each token: the workgroup's row, or NONE
-  __shared__ uint16_t at[kFewTokens];     // positions, by row and then in order
-  __shared__ uint8_t of[kFewTokens];      // their rows
-  __shared__ uint32_t counts[WAVES][ROWS], starts[ROWS + 1];
-  __shared__ f32x8 parts[2][512];  // of a run: what began before it, what goes on after
-  const int64_t begin = (int64_t)blockIdx.x * ROWS;
+// Entries 0..n by row, in LDS: first(j) is entry j's row, or -1, and again(j) the same when it is asked for once more; kept(j) is what
+// at[] gets for it. Entries of one row stay in order; starts[r] is where row r begins. All 512 threads call it.
+template <int ROWS, class First, class Again, class Kept>
+__device__ __forceinline__ void sort_rows(int n, First first, Again again, Kept kept, uint32_t (*counts)[ROWS], uint32_t* starts,
+                                          uint16_t* at, uint8_t* of) {
+  constexpr int WAVES = 8, BITS = ROWS == 256 ? 8 : ROWS == 64 ? 6 : 3, EACH = ROWS > 64 ? ROWS / 64 : 1;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int share = (a.n + 511) / 512 * 64, beg = min(wave * share, a.n), end = min(beg + share, a.n);
-  if (threadIdx.x < WAVES * ROWS) ((uint32_t*)counts)[threadIdx.x] = 0;
+  const int share = (n + 511) / 512 * 64, beg = min(wave * share, n), end = min(beg + share, n);
+  for (int i = threadIdx.x; i < WAVES * ROWS; i += 512) counts[0][i] = 0;
   __syncthreads();
   for (int i = beg; i < end; i += 256) {
     int r[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const int j = i + u * 64 + lane;
-      const int64_t row = j < end ? (int64_t)a.key(j) - begin : NONE;
-      r[u] = (uint64_t)row < ROWS && begin + row < a.vocab ? (int)row : NONE;
-      if (j < end) row_of[j] = (uint8_t)r[u];
-    }
+    for (int u = 0; u < 4; ++u) r[u] = i + u * 64 + lane < end ? first(i + u * 64 + lane) : -1;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const uint64_t same = same_digit((uint32_t)r[u], r[u] != NONE, BITS);
-      if (r[u] != NONE && !(same & lanes_below())) counts[wave][r[u]] += (uint32_t)__popcll(same);
+      const uint64_t same = same_digit((uint32_t)r[u], r[u] >= 0, BITS);
+      if (r[u] >= 0 && !(same & lanes_below())) counts[wave][r[u]] += (uint32_t)__popcll(same);
       __builtin_amdgcn_wave_barrier();
     }
   }
   __syncthreads();
   if (wave == 0) {
     uint32_t total = 0;
-    if (lane < ROWS)
+    if (lane * EACH < ROWS)
+      for (int k = 0; k < EACH; ++k)
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) total += counts[w][lane];
+        for (int w = 0; w < WAVES; ++w) total += counts[w][lane * EACH + k];
     uint32_t run = total;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -445,38 +444,41 @@ __global__ void __launch_bounds__(512) embedding_few_kernel(FewArgs a) {
     }
     if (lane == 63) starts[ROWS] = run;
     run -= total;
-    if (lane < ROWS) {
-      starts[lane] = run;
+    if (lane * EACH < ROWS)
+      for (int k = 0; k < EACH; ++k) {
+        starts[lane * EACH + k] = run;
 #pragma unroll
-      for (int w = 0; w < WAVES; ++w) {
-        const uint32_t c = counts[w][lane];
-        counts[w][lane] = run;
-        run += c;
+        for (int w = 0; w < WAVES; ++w) {
+          const uint32_t c = counts[w][lane * EACH + k];
+          counts[w][lane * EACH + k] = run;
+          run += c;
+        }
       }
-    }
   }
   __syncthreads();
   for (int i = beg; i < end; i += 64) {
-    const int j = i + lane, r = j < end ? row_of[j] : NONE;
-    const bool on = r != NONE;
+    const int j = i + lane, r = j < end ? again(j) : -1;
+    const bool on = r >= 0;
     const uint64_t same = same_digit((uint32_t)r, on, BITS), below = same & lanes_below();
-    const uint32_t first = on ? counts[wave][r] : 0;
+    const uint32_t next = on ? counts[wave][r] : 0;
     __builtin_amdgcn_wave_barrier();
     if (on) {
-      const uint32_t place = first + (uint32_t)__popcll(below);
-      at[place] = (uint16_t)j;
+      const uint32_t place = next + (uint32_t)__popcll(below);
+      at[place] = kept(j);
       of[place] = (uint8_t)r;
-      if (!below) counts[wave][r] = first + (uint32_t)__popcll(same);
+      if (!below) counts[wave][r] = next + (uint32_t)__popcll(same);
     }
     __builtin_amdgcn_wave_barrier();
   }
   __syncthreads();
-  const int m = (int)starts[ROWS], run = (m + GROUPS - 1) / GROUPS, g = threadIdx.x / LANES;
+}
+// put(row, sum) of each of the rows that the m sorted entries hold, by groups of LANES threads; all 512 threads call it
+template <class T, bool VEC, int LANES, class Put>
+__device__ __forceinline__ void sum_sorted(const uint16_t* at, const uint8_t* of, int m, f32x8 (*parts)[512], const T* gy, int64_t c,
+                                           int64_t dim, Put put) {
+  constexpr int GROUPS = 512 / LANES;
+  const int run = (m + GROUPS - 1) / GROUPS, g = threadIdx.x / LANES;
   const int from = min(g * run, m), to = min(from + run, m);
-  const int64_t c = ((int64_t)blockIdx.y * LANES + threadIdx.x % LANES) * 8;
-  auto put = [&](int row, f32x8 sum) { store8<VEC>((T*)a.gw + (begin + row) * a.dim, c, a.dim, sum * a.scale); };
-  for (int r = g; r < ROWS && begin + r < a.vocab; r += GROUPS)
-    if (starts[r] == starts[r + 1]) put(r, f32x8{});
   bool goes_on = false;
   if (from < to) {
     int row = of[from];
@@ -486,8 +488,7 @@ __global__ void __launch_bounds__(512) embedding_few_kernel(FewArgs a) {
     for (int i = from; i < to; i += U) {
       f32x8 v[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-        v[u] = i + u < to ? load8<VEC>((const T*)a.gy + (int64_t)at[i + u] * a.dim, c, a.dim) : f32x8{};
+      for (int u = 0; u < U; ++u) v[u] = i + u < to ? load8<VEC>(gy + (int64_t)at[i + u] * dim, c, dim) : f32x8{};
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         if (i + u >= to) break;
@@ -513,6 +514,64 @@ __global__ void __launch_bounds__(512) embedding_few_kernel(FewArgs a) {
   for (int k = g + 1; k * run < m && of[k * run] == row; ++k) sum += parts[0][k * LANES + threadIdx.x % LANES];
   put(row, sum);
 }
+
+template <class T, bool VEC, int LANES, int ROWS>
+__global__ void __launch_bounds__(512) embedding_few_kernel(FewArgs a) {
+  constexpr int NONE = 255;
+  __shared__ uint8_t row_of[kFewTokens];  // of each token: the workgroup's row, or NONE
+  __shared__ uint16_t at[kFewTokens];     // positions, by row and then in order
+  __shared__ uint8_t of[kFewTokens];      // their rows
+  __shared__ uint32_t counts[8][ROWS], starts[ROWS + 1];
+  __shared__ f32x8 parts[2][512];  // of a run: what began before it, what goes on after
+  const int64_t begin = (int64_t)blockIdx.x * ROWS;
+  sort_rows<ROWS>(
+      a.n,
+      [&](int j) {
+        const int64_t row = (int64_t)a.key(j) - begin;
+        const int r = (uint64_t)row < ROWS && begin + row < a.vocab ? (int)row : -1;
+        row_of[j] = (uint8_t)(r < 0 ? NONE : r);
+        return r;
+      },
+      [&](int j) { return row_of[j] == NONE ? -1 : (int)row_of[j]; }, [&](int j) { return (uint16_t)j; }, counts, starts, at, of);
+  const int64_t c = ((int64_t)blockIdx.y * LANES + threadIdx.x % LANES) * 8;
+  auto put = [&](int row, f32x8 sum) { store8<VEC>((T*)a.gw + (begin + row) * a.dim, c, a.dim, sum * a.scale); };
+  for (int r = threadIdx.x / LANES; r < ROWS && begin + r < a.vocab; r += 512 / LANES)
+    if (starts[r] == starts[r + 1]) put(r, f32x8{});
+  sum_sorted<T, VEC, LANES>(at, of, (int)starts[ROWS], parts, (const T*)a.gy, c, a.dim, put);
+}
+
+// A middling number of positions, which one pass of the sort has cut into bins by their tokens' low bits, so that neighbours among
+// the tokens, the frequent ones of a vocabulary, lie in different ones: a workgroup to a bin and 8 LANES columns does as above.
+constexpr int kBinTokens = 8192;
+struct BinArgs {
+  const uint32_t *keys, *pos, *starts;  // by bin; where each begins
+  const void* gy;
+  void* gw;
+  int64_t vocab, dim;
+  int bits;  // 2^bits bins
+  float scale;
+};
+template <class T, bool VEC, int LANES, int ROWS>
+__global__ void __launch_bounds__(512) embedding_bin_kernel(BinArgs a) {
+  __shared__ uint16_t at[kBinTokens];
+  __shared__ uint8_t of[kBinTokens];
+  __shared__ uint32_t counts[8][ROWS], starts[ROWS + 1];
+  __shared__ f32x8 parts[2][512];
+  const uint32_t bin = blockIdx.x, base = a.starts[bin], n = a.starts[bin + 1] - base;
+  auto row = [&](int j) {
+    const uint32_t key = a.keys[base + j];
+    return key < a.vocab ? (int)(key >> a.bits) : -1;
+  };
+  sort_rows<ROWS>((int)n, row, row, [&](int j) { return (uint16_t)a.pos[base + j]; }, counts, starts, at, of);
+  const int64_t c = ((int64_t)blockIdx.y * LANES + threadIdx.x % LANES) * 8;
+  auto put = [&](int r, f32x8 sum) {
+    store8<VEC>((T*)a.gw + (((int64_t)r << a.bits) + bin) * a.dim, c, a.dim, sum * a.scale);
+  };
+  for (int r = threadIdx.x / LANES; r < ROWS && ((int64_t)r << a.bits) + bin < a.vocab; r += 512 / LANES)
+    if (starts[r] == starts[r + 1]) put(r, f32x8{});
+  sum_sorted<T, VEC, LANES>(at, of, (int)starts[ROWS], parts, (const T*)a.gy, c, a.dim, put);
+}
+
 // How a gradient of few positions is cut, by what it measured: lanes 0 where the sort's launches take less. Skewed tokens, us, with 8
 // rows to a workgroup, with 64, and by the sort:
 //   300 tokens     256 x 128 bfloat16  5.9,  8.0, 15.7   64 x 4096  6.3,  9.1, 14.6   1000 x 1000 float32  9.6,  7.1, 16.6
@@ -534,6 +593,17 @@ static FewPlan few_plan(int64_t n, int64_t vocab, int64_t dim) {
   return n <= kFewTokens && groups <= 2048 ? FewPlan{16, 8} : FewPlan{0, 0};
 }
 
+// Threads to a bin's columns, 0 where the sort's launches take less: where the columns are few, so that a bin is sorted once. Skewed tokens,
+// us, in bins and by the sort, at 2049, 4096 and 8192 of them:
+//   16 lanes   256 x 128 bfloat16  18.7, 20.7, 24.1 and 22.2, 22.8, 22.7   16384 x 64 18.4, 19.7, 22.1 and 34.4, 35.6, 35.1
+//              50021 x 100 float32 23.9, 26.9, 30.1 and 40.5, 42.1, 41.1
+//   64 lanes   4096 x 512 bfloat16 18.7, 23.1, 33.4 and 32.3, 35.5, 34.4   32768 x 512 24.4, 29.9, 38.9 and 34.7, 36.0, 37.3
+//              131072 x 512 40.0, 46.3, 56.8 and 44.7, 46.0, 48.4          32768 x 4096 91, 110, 135 and 71.5, 73.2, 78.4
+static int bin_lanes(int64_t n, int64_t vocab, int64_t dim) {
+  if (vocab > (int64_t)256 << kDigitBits) return 0;
+  return dim <= 128 && n <= kBinTokens ? 16 : dim <= 512 && n <= kBinTokens / 2 ? 64 : 0;
+}
+
 // ---- plans ----------------------------------------------------------------------------------------------------------
 
 // Positions to a run: enough runs for the card's threads, no fewer positions than keep the joined sums few.
@@ -547,17 +617,25 @@ static int digits_of(int64_t vocab) {
   return bits;
 }
 struct EmbedPlan {
+  FewPlan few;  // one launch, or
+  int bins;     // sorted into bins, with so many lanes, or
   int64_t run, runs;
-  size_t counts, marks, sorted, parts;  // bytes: of one array each
-  size_t total() const { return counts + marks + 4 * sorted + parts; }
+  size_t starts, counts, marks, sorted, parts;  // bytes: of one array each
+  size_t total() const { return few.lanes ? 0 : starts + counts + marks + (bins ? 2 : 4) * sorted + parts; }
 };
 static EmbedPlan embed_plan(int64_t n, int64_t vocab, int64_t dim) {
-  EmbedPlan p;
+  EmbedPlan p{};
+  p.few = few_plan(n, vocab, dim);
+  p.bins = p.few.lanes ? 0 : bin_lanes(n, vocab, dim);
+  p.sorted = (size_t)cdiv(n, 64) * 256;
+  p.counts = n > kSmallSort || p.bins ? (size_t)kSortTiles * kBins * 4 : 0;
+  if (p.bins) {
+    p.starts = (size_t)(kBins + 64) * 4;
+    return p;
+  }
   p.run = run_length(n, dim);
   p.runs = cdiv(n, p.run);
-  p.counts = n > kSmallSort ? (size_t)kSortTiles * kBins * 4 : 0;
   p.marks = n > kSmallSort ? (size_t)cdiv(vocab, 64) * 256 : 0;
-  p.sorted = (size_t)cdiv(n, 64) * 256;
   p.parts = (size_t)p.runs * 2 * dim * 4;
   return p;
 }
@@ -608,7 +686,7 @@ OMT_EXPORT int omt_embedding_fwd(int dtype, int token_dtype, int64_t n, int64_t 
 }
 
 OMT_EXPORT size_t omt_embedding_bwd_workspace(int64_t n, int64_t vocab, int64_t dim) {
-  if (n < 0 || n > kEmbedMaxTokens || vocab < 1 || dim < 1 || few_plan(n, vocab, dim).lanes) return 0;
+  if (n < 0 || n > kEmbedMaxTokens || vocab < 1 || dim < 1) return 0;
   return embed_plan(n, vocab, dim).total();
 }
 
@@ -623,7 +701,8 @@ OMT_EXPORT int omt_embedding_bwd(int dtype, int token_dtype, int64_t n, int64_t 
   hipStream_t s = stream_of(stream);
   const KeyOf key{{tokens, token_dtype == OMT_DT_I64}, vocab, padding_idx};
   const bool vec = dim % 8 == 0 && on16({gy, gweight});
-  if (const FewPlan few = few_plan(n, vocab, dim); few.lanes) {
+  const EmbedPlan p = embed_plan(n, vocab, dim);
+  if (const FewPlan few = p.few; few.lanes) {
     const FewArgs a{key, gy, gweight, (int)n, vocab, dim, scale};
     const dim3 grid((unsigned)cdiv(vocab, few.rows), (unsigned)cdiv(dim, few.lanes * 8));
     auto go = [&](auto lanes, auto rows) {
@@ -637,18 +716,40 @@ OMT_EXPORT int omt_embedding_bwd(int dtype, int token_dtype, int64_t n, int64_t 
     else go(std::integral_constant<int, 16>(), std::integral_constant<int, 8>());
     return launch_check("embedding_few_kernel");
   }
-  const EmbedPlan p = embed_plan(n, vocab, dim);
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.total())
     return fail(OMT_INVALID, "%s: workspace of %zu bytes at %p", fn, workspace_bytes, workspace);
   char* at = (char*)workspace;
-  uint32_t* counts = (uint32_t*)at;
-  uint32_t *keys[2], *pos[2];
-  at += p.counts;
-  uint32_t* marks = (uint32_t*)at;
-  at += p.marks;
-  for (int i = 0; i < 2; ++i) {
-    keys[i] = (uint32_t*)at, at += p.sorted;
-    pos[i] = (uint32_t*)at, at += p.sorted;
+  auto array = [&](size_t size) {
+    uint32_t* a = (uint32_t*)at;
+    at += size;
+    return a;
+  };
+  uint32_t *starts = array(p.starts), *counts = array(p.counts), *marks = array(p.marks), *keys[2], *pos[2];
+  for (int i = 0; i < (p.bins ? 1 : 2); ++i) keys[i] = array(p.sorted), pos[i] = array(p.sorted);
+  const int64_t tile = cdiv(std::max<int64_t>(1024, cdiv(n, kSortTiles)), kSortThreads) * kSortThreads;
+  const unsigned tiles = (unsigned)cdiv(n, tile);
+  if (p.bins) {
+    const int bits = std::min(kDigitBits, digits_of(vocab));
+    const SortArgs q{{key, nullptr, nullptr}, keys[0], pos[0], counts, starts, nullptr, n, tile, tiles, 0, bits, {}};
+    hipLaunchKernelGGL(sort_count_kernel<true>, dim3(tiles), dim3(kSortThreads), 0, s, q);
+    if (int e = launch_check("sort_count_kernel")) return e;
+    hipLaunchKernelGGL(sort_place_kernel<true>, dim3(tiles), dim3(kSortThreads), 0, s, q);
+    if (int e = launch_check("sort_place_kernel")) return e;
+    const BinArgs a{keys[0], pos[0], starts, gy, gweight, vocab, dim, bits, scale};
+    auto go = [&](auto lanes, auto rows) {
+      constexpr int LANES = decltype(lanes)::value, ROWS = decltype(rows)::value;
+      const dim3 grid(1u << bits, (unsigned)cdiv(dim, LANES * 8));
+      auto with = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(512), 0, s, a); };
+      if (dtype == OMT_DT_F32) vec ? with(embedding_bin_kernel<float, true, LANES, ROWS>) : with(embedding_bin_kernel<float, false, LANES, ROWS>);
+      else vec ? with(embedding_bin_kernel<__bf16, true, LANES, ROWS>) : with(embedding_bin_kernel<__bf16, false, LANES, ROWS>);
+    };
+    auto by_rows = [&](auto lanes) {
+      if (cdiv(vocab, (int64_t)1 << bits) <= 64) go(lanes, std::integral_constant<int, 64>());
+      else go(lanes, std::integral_constant<int, 256>());
+    };
+    if (p.bins == 16) by_rows(std::integral_constant<int, 16>());
+    else by_rows(std::integral_constant<int, 64>());
+    return launch_check("embedding_bin_kernel");
   }
   const int all = digits_of(vocab), passes = (all + kDigitBits - 1) / kDigitBits, bits = (all + passes - 1) / passes;
   int last = 0;
@@ -659,14 +760,12 @@ OMT_EXPORT int omt_embedding_bwd(int dtype, int token_dtype, int64_t n, int64_t 
                        keys[0], pos[0], ZeroRows{gweight, 0, vocab, dim, bytes});
     if (int e = launch_check("sort_small_kernel")) return e;
   } else {
-    const int64_t tile = cdiv(std::max<int64_t>(1024, cdiv(n, kSortTiles)), kSortThreads) * kSortThreads;
-    const unsigned tiles = (unsigned)cdiv(n, tile);
     // the rows of zeros, in equal shares beside every launch but the first, which marks the others
     const int64_t share = cdiv(zero_groups, 2 * passes - 1);
     for (int q = 0; q < 2 * passes; ++q) {
       const int64_t done = std::min(zero_groups, std::max(0, q - 1) * share), more = q ? std::min(share, zero_groups - done) : 0;
       const int pass = q / 2;
-      const SortArgs a{{key, keys[~pass & 1], pos[~pass & 1]}, keys[pass & 1], pos[pass & 1], counts, marks, n, tile, tiles, pass * bits,
+      const SortArgs a{{key, keys[~pass & 1], pos[~pass & 1]}, keys[pass & 1], pos[pass & 1], counts, nullptr, marks, n, tile, tiles, pass * bits,
                        bits, {gweight, done * kZeroRows, std::min(vocab, (done + more) * kZeroRows), dim, bytes}};
       auto go = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(tiles + (unsigned)more), dim3(kSortThreads), 0, s, a);

@@ -98,8 +98,17 @@ def check_embedding_grad(ops, n, vocab, dim, dtype, tokens, scale=1.3, padding=N
                                      (257, 40000), (1025, 300), (1024, 8000), (2048, 511), (1500, 30000), (2048, 40000), (2049, 512), (4097, 70000), (8192, 300),
                                      (8193, 300), (9000, 262143), (20000, 262144), (70001, 1000)])
 def test_embedding_grad_sorts_any_tokens(ops, cuda, n, vocab, how):
-    """Few in LDS, by rows of 8 and 64; up to 2048 beside many rows by one workgroup; more by many, of one digit, two and three."""
+    """Few in LDS, by rows of 8 and 64; in bins; over 8192 by many workgroups, of one digit, two and three."""
     check_embedding_grad(ops, n, vocab, 8, F32, some_tokens(n, vocab, how, n))
+
+
+@pytest.mark.parametrize("how", ["one", "distinct", "skewed", "any"])
+@pytest.mark.parametrize("n,vocab,dim", [(300, 40000, 520), (2048, 40000, 520), (2049, 40000, 520), (5000, 3000, 1032), (1500, 200000, 8),
+                                         (3000, 200000, 8), (3000, 100, 512), (4096, 131072, 136), (8192, 131071, 9), (8192, 40000, 128),
+                                         (4097, 700, 200), (2049, 1, 16)])
+def test_embedding_grad_of_wide_rows_and_many(ops, cuda, n, vocab, dim, how):
+    """Up to 2048 by one workgroup, and by many, where bins are not taken; bins of one row, 64 and 256, of both widths."""
+    check_embedding_grad(ops, n, vocab, dim, BF16, some_tokens(n, vocab, how, n))
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -643,15 +652,16 @@ def every_operator(ops, seed, n=9000):
     pairs = [t for name in ("params", "grads", "m", "v", "ms", "vs", "masters") for t in getattr(c, name)]
     return {"embedding": ([few, w], lambda t, w: [ops.embedding(t, w, 2.0)]),
             "embedding_backward": ([gy, tokens], lambda a, t: [ops.embedding_backward(a, t, 600)]),
+            "embedding_backward_bins": ([gy[:5000].clone(), tokens[:5000].clone()], lambda a, t: [ops.embedding_backward(a, t, 6000)]),
             "embedding_backward_few": ([gy[:500].clone(), few], lambda a, t: [ops.embedding_backward(a, t, 600)]),
-            "embedding_backward_small": ([gy[:1500].clone(), tokens[:1500].clone()], lambda a, t: [ops.embedding_backward(a, t, 30000)]),
+            "embedding_backward_small": ([gy[:1500].clone(), tokens[:1500].clone()], lambda a, t: [ops.embedding_backward(a, t, 200000)]),
             "token_logps": ([x, labels], lambda x, y: list(ops.token_logps(x, y))),
             "preference": ([x, labels, ref], lambda x, y, r: list(ops.preference_loss(x, y, r))),
             "policy": ([x, labels, old, ref], lambda x, y, o, a: list(ops.policy_loss(x, y, o, a, reference=o * 0.99, kl=0.1))),
             "adamw": (pairs, adamw)}
 
 
-NAMES = ["embedding", "embedding_backward", "embedding_backward_few", "embedding_backward_small", "token_logps", "preference", "policy", "adamw"]
+NAMES = ["embedding", "embedding_backward", "embedding_backward_few", "embedding_backward_bins", "embedding_backward_small", "token_logps", "preference", "policy", "adamw"]
 
 
 @pytest.mark.parametrize("name", NAMES)
