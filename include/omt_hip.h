@@ -725,7 +725,8 @@ int omt_token_logps_bwd(const omt_logits* logits, const float* lse, const float*
  *   OMT_PREFERENCE_SIGMOID  -(1 - smoothing) log sigmoid(beta d) - smoothing log sigmoid(-beta d)
  *   OMT_PREFERENCE_HINGE    max(0, 1 - beta d)
  *   OMT_PREFERENCE_IPO      (d - 1 / (2 beta))^2
- * rewards[sequences] = beta (L - R). gx: the loss's gradient (null: not asked for). beta > 0, smoothing in [0, 1]. */
+ * rewards[sequences] = beta (L - R). gx: the loss's gradient (null: not asked for). beta > 0, smoothing in [0, 1] (0 but
+ * for OMT_PREFERENCE_SIGMOID). */
 enum { OMT_PREFERENCE_SIGMOID = 0, OMT_PREFERENCE_HINGE = 1, OMT_PREFERENCE_IPO = 2 };
 size_t omt_preference_workspace(int64_t sequences, int64_t length);
 int omt_preference_loss(const omt_logits* logits, const float* reference, int kind, double beta, double smoothing, int average,

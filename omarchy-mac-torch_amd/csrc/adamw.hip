@@ -18,7 +18,7 @@
 // how a compiler pairs them. The loads are on their way while one lane computes the step's scalars.
 //
 // In 8 bits, 470 million bfloat16 parameters with masters 1390 us (7.58 GB at 5.45 TB/s), without 840; 8.8 million float32 ones, 19 tensors,
-// 26 us (0.14 GB at 5.5 TB/s); 0.36 million bfloat16 ones 7 us, a launch and the scalars' latency.
+// 26 us (0.14 GB at 5.5 TB/s); 0.2 million bfloat16 ones 7 us, a launch and the scalars' latency.
 #include "block_fp8.h"
 
 namespace omt {

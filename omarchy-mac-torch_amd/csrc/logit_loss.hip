@@ -662,6 +662,7 @@ OMT_EXPORT int omt_preference_loss(const omt_logits* logits, const float* refere
   if (n < 2 || n % 2) return fail(OMT_INVALID, "%s: %lld sequences: pairs are needed", fn, (long long)n);
   if (kind < OMT_PREFERENCE_SIGMOID || kind > OMT_PREFERENCE_IPO) return fail(OMT_INVALID, "%s: kind %d", fn, kind);
   if (!(beta > 0.0) || !(smoothing >= 0.0 && smoothing <= 1.0)) return fail(OMT_INVALID, "%s: beta %g, smoothing %g", fn, beta, smoothing);
+  if (kind != OMT_PREFERENCE_SIGMOID && smoothing != 0.0) return fail(OMT_INVALID, "%s: smoothing %g of kind %d", fn, smoothing, kind);
   if (n / 2 >= 1 << 22) return fail(OMT_UNSUPPORTED, "%s: %lld sequences", fn, (long long)n);
   if (!reference || !loss || !rewards) return fail(OMT_INVALID, "%s: null pointer", fn);
   const PreferencePlan p = preference_plan(n, logits->length);

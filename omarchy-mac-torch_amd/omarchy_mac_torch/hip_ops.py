@@ -953,7 +953,8 @@ def preference_loss(logits, labels, reference, beta=0.1, kind="sigmoid", smoothi
         "hinge"    max(0, 1 - beta d)
         "ipo"      (d - 1 / (2 beta))^2
 
-    Returns (loss, rewards [sequences] = beta (L - R), the logits' gradient or, without grad, None)."""
+    (smoothing is the first one's alone). Returns (loss, rewards [sequences] = beta (L - R), the logits' gradient or, without grad,
+    None)."""
     return _lm("preference_loss", logits, labels, reference, float(beta), _choice("kind", kind, _PREFERENCES), float(smoothing),
                bool(average), int(ignore_index), bool(grad))
 

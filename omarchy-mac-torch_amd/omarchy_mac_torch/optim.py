@@ -100,12 +100,12 @@ class AdamW(torch.optim.Optimizer):
 
     @staticmethod
     def _new_state(p, group):
-        state = {"step": torch.zeros((), device=p.device)}
+        state = {"step": torch.zeros((), dtype=torch.float32, device=p.device)}
         held = torch.float8_e4m3fn if group["state_bits"] == 8 else torch.float32
         for name in ("exp_avg", "exp_avg_sq"):
             state[name] = torch.zeros_like(p, dtype=torch.float32).to(held)
             if group["state_bits"] == 8:
-                state[name + "_scale"] = torch.zeros(-(-p.numel() // 128), device=p.device)
+                state[name + "_scale"] = torch.zeros(-(-p.numel() // 128), dtype=torch.float32, device=p.device)
         if group["masters"] and p.dtype == torch.bfloat16:
             state["master"] = p.detach().float()
         return state

@@ -110,6 +110,7 @@ std::tuple<Tensor, Tensor, Tensor> preference_loss(const Tensor& logits, const T
   TORCH_CHECK_VALUE(l.q.sequences >= 2 && l.q.sequences % 2 == 0, "logits: expected pairs of sequences, got ", l.q.sequences);
   TORCH_CHECK_VALUE(beta > 0, "beta: expected over 0, got ", beta);
   TORCH_CHECK_VALUE(smoothing >= 0 && smoothing <= 1, "smoothing: expected from 0 to 1, got ", smoothing);
+  TORCH_CHECK_VALUE(kind == OMT_PREFERENCE_SIGMOID || smoothing == 0, "smoothing: of the sigmoid loss only, got ", smoothing);
   Tensor reference = take(reference_, "reference", at::kFloat, &l.x, IntArrayRef{l.q.sequences});
   Site at(l.x);
   Tensor loss = make(l.x, {}, at::kFloat), rewards = make(l.x, {l.q.sequences}, at::kFloat), gx = make_gradient(l, grad);

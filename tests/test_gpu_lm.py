@@ -613,6 +613,7 @@ def test_losses_refuse(ops, cuda):
                         (ValueError, lambda: ops.preference_loss(x, labels, ref[:2])),
                         (ValueError, lambda: ops.preference_loss(x, labels, ref, beta=0.0)),
                         (ValueError, lambda: ops.preference_loss(x, labels, ref, smoothing=2.0)),
+                        (ValueError, lambda: ops.preference_loss(x, labels, ref, kind="ipo", smoothing=0.1)),
                         (TypeError, lambda: ops.preference_loss(x.half(), labels, ref)),
                         (TypeError, lambda: ops.preference_loss(x, labels.int(), ref)),
                         (TypeError, lambda: ops.preference_loss(x, labels, ref.double())),

@@ -62,6 +62,7 @@ def test_loss_statuses(lib):
     assert g(logits(lib, sequences=3)) == bad and g(logits(lib, sequences=0)) == bad
     assert g(logits(lib), kind=3) == bad and g(logits(lib), kind=-1) == bad
     assert g(logits(lib), beta=0.0) == bad and g(logits(lib), beta=float("nan")) == bad
+    assert g(logits(lib), kind=1, smooth=0.1) == bad and g(logits(lib), kind=2, smooth=0.1) == bad
     assert g(logits(lib), smooth=-0.1) == bad and g(logits(lib), smooth=1.1) == bad
     assert g(logits(lib), ref=None) == bad and g(logits(lib), loss=None) == bad and g(logits(lib), rewards=None) == bad
     assert g(logits(lib), ws=None) == bad and g(logits(lib), size=need - 1) == bad
@@ -189,6 +190,20 @@ def test_optimizer_arguments():
     p[0].grad = torch.ones(3)
     with pytest.raises(TypeError, match="HIP device"):
         opt.step()
+
+
+def test_optimizer_states_are_float32_whatever_the_default(monkeypatch):
+    from omarchy_mac_torch import hip_ops, optim
+    monkeypatch.setattr(hip_ops, "adamw", lambda *args, **options: None)
+    p = torch.nn.Parameter(torch.ones(3))
+    p.grad = torch.ones(3)
+    opt = optim.AdamW([p])
+    torch.set_default_dtype(torch.float64)
+    try:
+        opt.step()
+    finally:
+        torch.set_default_dtype(torch.float32)
+    assert all(opt.state[p][name].dtype == torch.float32 for name in ("step", "exp_avg_scale", "exp_avg_sq_scale"))
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
