@@ -593,15 +593,18 @@ static FewPlan few_plan(int64_t n, int64_t vocab, int64_t dim) {
   return n <= kFewTokens && groups <= 2048 ? FewPlan{16, 8} : FewPlan{0, 0};
 }
 
-// Threads to a bin's columns, 0 where the sort's launches take less: where the columns are few, so that a bin is sorted once. Skewed tokens,
-// us, in bins and by the sort, at 2049, 4096 and 8192 of them:
+// Threads to a bin's columns, 0 where the sort's launches take less: where the columns are few, since each 8 lanes of them sort the bin
+// again. Skewed tokens, us, in bins and by the sort, at 2049, 4096 and 8192 of them:
 //   16 lanes   256 x 128 bfloat16  18.7, 20.7, 24.1 and 22.2, 22.8, 22.7   16384 x 64 18.4, 19.7, 22.1 and 34.4, 35.6, 35.1
 //              50021 x 100 float32 23.9, 26.9, 30.1 and 40.5, 42.1, 41.1
-//   64 lanes   4096 x 512 bfloat16 18.7, 23.1, 33.4 and 32.3, 35.5, 34.4   32768 x 512 24.4, 29.9, 38.9 and 34.7, 36.0, 37.3
-//              131072 x 512 40.0, 46.3, 56.8 and 44.7, 46.0, 48.4          32768 x 4096 91, 110, 135 and 71.5, 73.2, 78.4
+//   64 lanes   4096 x 512 bfloat16 18.5, 22.7, 33.4 and 32.3, 33.6, 34.4   131072 x 512 40.0, 46.3, 56.8 and 44.7, 46.0, 48.4
+//              300 x 512 20.1, 26.8 and 22.3, 22.3 (tokens of one digit)   16384 x 1024 24.7, 31.3 and 34.5, 37.6
+//              32768 x 1024 float32 44.2, 53.0 and 43.8, 45.4              16384 x 2048 50.9, 62.7 and 45.9, 48.1
 static int bin_lanes(int64_t n, int64_t vocab, int64_t dim) {
   if (vocab > (int64_t)256 << kDigitBits) return 0;
-  return dim <= 128 && n <= kBinTokens ? 16 : dim <= 512 && n <= kBinTokens / 2 ? 64 : 0;
+  if (dim <= 128) return n <= kBinTokens ? 16 : 0;
+  if (vocab < kBins || n > kBinTokens / 2 || dim > 1024) return 0;
+  return dim <= 512 || vocab * dim <= 1 << 24 ? 64 : 0;
 }
 
 // ---- plans ----------------------------------------------------------------------------------------------------------

@@ -105,6 +105,7 @@ def test_embedding_grad_sorts_any_tokens(ops, cuda, n, vocab, how):
 @pytest.mark.parametrize("how", ["one", "distinct", "skewed", "any"])
 @pytest.mark.parametrize("n,vocab,dim", [(300, 40000, 520), (2048, 40000, 520), (2049, 40000, 520), (5000, 3000, 1032), (1500, 200000, 8),
                                          (3000, 200000, 8), (3000, 100, 512), (4096, 131072, 136), (8192, 131071, 9), (8192, 40000, 128),
+                                         (4096, 16000, 1016), (3000, 512, 513), (3000, 511, 513),
                                          (4097, 700, 200), (2049, 1, 16)])
 def test_embedding_grad_of_wide_rows_and_many(ops, cuda, n, vocab, dim, how):
     """Up to 2048 by one workgroup, and by many, where bins are not taken; bins of one row, 64 and 256, of both widths."""
