@@ -593,8 +593,8 @@ static FewPlan few_plan(int64_t n, int64_t vocab, int64_t dim) {
   return n <= kFewTokens && groups <= 2048 ? FewPlan{16, 8} : FewPlan{0, 0};
 }
 
-// Threads to a bin's columns, 0 where the sort's launches take less: where the columns are few, since each 8 lanes of them sort the bin
-// again. Skewed tokens, us, in bins and by the sort, at 2049, 4096 and 8192 of them:
+// Threads to a bin's columns, 0 where the sort's launches take less: where the columns are few, since each workgroup's share of them sorts
+// the bin again. Skewed tokens, us, in bins and by the sort, at 2049, 4096 and 8192 of them:
 //   16 lanes   256 x 128 bfloat16  18.7, 20.7, 24.1 and 22.2, 22.8, 22.7   16384 x 64 18.4, 19.7, 22.1 and 34.4, 35.6, 35.1
 //              50021 x 100 float32 23.9, 26.9, 30.1 and 40.5, 42.1, 41.1
 //   64 lanes   4096 x 512 bfloat16 18.5, 22.7, 33.4 and 32.3, 33.6, 34.4   131072 x 512 40.0, 46.3, 56.8 and 44.7, 46.0, 48.4

@@ -136,6 +136,34 @@ def test_embedding_grad_leaves_out_padding_and_unknown_tokens(ops, cuda, n):
     assert gw.shape == (7, 8) and not bool(gw.any())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,vocab,dim", [(50, 30, 64), (1500, 40000, 520), (3000, 600, 64), (9000, 600, 64)])
+def test_embedding_at_any_alignment(ops, cuda, dtype, n, vocab, dim):
+    """The C entries on arrays that begin at their second element."""
+    import ctypes
+    from omarchy_mac_torch import _lib
+    kind = _lib.OMT_DT_F32 if dtype == F32 else _lib.OMT_DT_BF16
+    tokens = some_tokens(n, vocab, "skewed", 1).cuda()
+
+    def inside(t):
+        big = torch.zeros(t.numel() + 1, dtype=t.dtype, device="cuda")
+        big[1:] = t.flatten()
+        return big
+
+    w, gy = torch.randn(vocab, dim, generator=gen(2)).to(dtype).cuda(), torch.randn(n, dim, generator=gen(3)).to(dtype).cuda()
+    at = lambda t: ctypes.c_void_p(t.data_ptr() + t.element_size())  # noqa: E731
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    y, bw = inside(gy * 0), inside(w)
+    assert _lib.L.omt_embedding_fwd(kind, _lib.OMT_DT_I64, n, vocab, dim, ctypes.c_void_p(tokens.data_ptr()), at(bw), 2.0, at(y), stream) == 0
+    assert torch.equal(y[1:].view(n, dim), ops.embedding(tokens, w, 2.0))
+    gw, bgy = inside(w * math.nan), inside(gy)
+    need = _lib.L.omt_embedding_bwd_workspace(n, vocab, dim)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+    assert _lib.L.omt_embedding_bwd(kind, _lib.OMT_DT_I64, n, vocab, dim, at(bgy), ctypes.c_void_p(tokens.data_ptr()), -1, 2.0, at(gw),
+                                    ctypes.c_void_p(ws.data_ptr()), need, stream) == 0
+    assert torch.equal(gw[1:].view(vocab, dim), ops.embedding_backward(gy, tokens, vocab, 2.0)) and float(gw[0]) == 0
+
+
 def test_embedding_past_32_bit_offsets(ops, cuda):
     vocab, dim = 270000, 8192  # 2.2e9 elements
     w = torch.zeros(vocab, dim, device="cuda", dtype=BF16)
@@ -308,6 +336,22 @@ def test_policy_loss(ops, cuda, dtype, vocab):
 @pytest.mark.parametrize("length", [1, 300])
 def test_policy_kinds(ops, cuda, reduction, reference, kl, each, length):
     check_policy(ops, *some_logits(5, length, 33, F32, length), reduction=reduction, reference=reference, kl=kl, each=each)
+
+
+def test_empty_batches(ops, cuda):
+    x, labels = torch.zeros(4, 0, 7).cuda(), torch.zeros(4, 0, dtype=torch.int64).cuda()
+    none, ref = torch.zeros(4, 0).cuda(), torch.tensor([1.0, 2.0, 3.0, 4.0]).cuda()
+    loss, rewards, gx = ops.preference_loss(x, labels, ref, beta=0.5)
+    within(loss, torch.nn.functional.softplus(torch.tensor(-1.0).double()), 1e-7)
+    within(rewards, torch.tensor([-0.5, -1.0, -1.5, -2.0]), 0.0)
+    assert gx.shape == x.shape
+    for reduction in ("token", "sequence"):
+        loss, kl, logps, gx = ops.policy_loss(x, labels, none, ref, reduction=reduction)
+        assert float(loss) == float(kl) == 0 and logps.shape == (4, 0) and gx.shape == x.shape
+        loss, kl, logps, gx = ops.policy_loss(x.view(0, 4, 7), labels.view(0, 4), none.view(0, 4), ref[:0], reduction=reduction)
+        assert float(loss) == float(kl) == 0 and gx.shape == (0, 4, 7)
+    logps, lse = ops.token_logps(x, labels)
+    assert logps.shape == (4, 0) and ops.token_logps_backward(logps, x, labels, lse).shape == x.shape
 
 
 def test_policy_of_many_tokens(ops, cuda):
