@@ -6,12 +6,12 @@
 // equal length, whatever the tokens' frequencies, and sums each run's rows of gy in float32: what begins and ends within a run
 // is rounded and written at once, the sums of a token that reaches over runs are joined by a second launch. Rows that no
 // position holds are written as zeros by further workgroups of the sort's launches, which it leaves most of the card to: at a
-// vocabulary that is large beside the positions the sort takes no time of its own. Bound by memory: gy is read once, gw
-// written once.
+// vocabulary that is large beside the positions the sort takes no time of its own. Few positions, and a middling number of narrow
+// rows, have ways of fewer launches (below). Bound by memory: gy is read once, gw written once.
 //
 // bfloat16, tokens as text has them: 65536 rows of 2048 from 131072 82 us (0.36 GB at 4.3 TB/s; 0.45 GB pass the caches, since eight of
 // them read the frequent rows); the gradient of 32768 positions 148 us (0.67 GB at 4.5 TB/s), of which the sort with its rows of zeros
-// 98, the sums 31 and the joins 6. 8191 positions to 256 x 128 float32 20.5 us, three launches; few positions take one (below).
+// 98, the sums 31 and the joins 6. 8191 positions to 256 x 128 float32 20.5 us, three launches.
 //
 // Tokens outside the vocabulary: a row of NaN, and no part in the gradient; no memory is touched for them.
 #include <algorithm>

@@ -25,8 +25,7 @@
 //
 // 16 x 512 rows in bfloat16 of which 58% count: policy x 131072 685 us (3.40 GB that it cannot do without, 2.15 of them written), x 65536
 // 348, x 32768 167; preference x 32768 57 + 5 + 123 us for 0.85 GB; 6 x 301 x 50021 float32, rows on 4 bytes, 140 us for 0.58 GB. A large copy
-// reaches 4.74 TB/s on this card: the second pass finds part of its rows in the last cache. Small calls are launches: 4 x 63 x 256
-// float32 3.7 + 3.8 + 3.1 us on the GPU.
+// reaches 4.74 TB/s on this card: the second pass finds part of its rows in the last cache. Small calls are launches.
 #include <algorithm>
 
 #include "block_fp8.h"
@@ -223,6 +222,108 @@ __global__ void __launch_bounds__(RT == 64 ? 256 : RT) token_logps_kernel(LogitR
   }
 }
 
+// ---- pairs ----------------------------------------------------------------------------------------------------------
+
+// two sums over the workgroup's THREADS, in every one of them
+template <int THREADS>
+__device__ __forceinline__ void block_sums(double& u, double& v, double* red) {
+  u = wave_sum(u), v = wave_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[(threadIdx.x >> 6) * 2] = u, red[(threadIdx.x >> 6) * 2 + 1] = v;
+  __syncthreads();
+  u = v = 0.0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) u += red[w * 2], v += red[w * 2 + 1];
+}
+
+struct PairArgs {
+  const int64_t* labels;
+  const float *logps, *reference;
+  int64_t ignore, length, pairs;
+  int kind, average;
+  double beta, smoothing;
+  float *rewards, *coefs;
+  double* losses;
+};
+
+// log(1 + exp(-z)) without overflow
+__device__ __forceinline__ double softplus_neg(double z) { return (z < 0 ? -z : 0.0) + log1p(exp(z < 0 ? z : -z)); }
+__device__ __forceinline__ double sigmoid(double z) { return 1.0 / (1.0 + exp(-z)); }
+
+// The loss of a pair, and of each of its sequences the reward and the gradient of the mean loss by a log-probability
+struct PairLoss {
+  double loss;
+  float rewards[2], coefs[2];
+};
+__device__ __forceinline__ PairLoss pair_loss(const PairArgs& a, int64_t pair, const double (&sum)[2], const double (&count)[2]) {
+  double ratio[2], share[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    share[k] = a.average ? 1.0 / fmax(count[k], 1.0) : 1.0;
+    ratio[k] = sum[k] * share[k] - (double)a.reference[pair + k * a.pairs];
+  }
+  const double d = ratio[0] - ratio[1], z = a.beta * d;
+  double loss, slope;  // of the loss by d
+  if (a.kind == OMT_PREFERENCE_SIGMOID) {
+    // (a term of weight zero is left out: it may be infinite)
+    loss = (a.smoothing < 1.0 ? (1.0 - a.smoothing) * softplus_neg(z) : 0.0) + (a.smoothing > 0.0 ? a.smoothing * softplus_neg(-z) : 0.0);
+    slope = a.beta * (a.smoothing - sigmoid(-z));
+  } else if (a.kind == OMT_PREFERENCE_HINGE) {
+    loss = 1.0 - z < 0.0 ? 0.0 : 1.0 - z;  // (NaN stays NaN)
+    slope = 1.0 - z < 0.0 || z == 1.0 ? 0.0 : z < 1.0 ? -a.beta : z;
+  } else {
+    loss = (d - 0.5 / a.beta) * (d - 0.5 / a.beta);
+    slope = 2.0 * (d - 0.5 / a.beta);
+  }
+  PairLoss l;
+  l.loss = loss;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    l.rewards[k] = (float)(a.beta * ratio[k]);
+    l.coefs[k] = (float)((k ? -slope : slope) * share[k] / (double)a.pairs);
+  }
+  return l;
+}
+// log-probabilities of a sequence and how many count, every THREADS-th of them from `first` on (those that do not count are 0)
+template <int THREADS>
+__device__ __forceinline__ void sequence_share(const PairArgs& a, int64_t seq, int first, double& sum, double& count) {
+  const int64_t base = seq * a.length;
+  sum = count = 0.0;
+#pragma unroll 4
+  for (int64_t i = first; i < a.length; i += THREADS) {
+    sum += (double)a.logps[base + i];
+    count += a.labels[base + i] != a.ignore ? 1.0 : 0.0;
+  }
+}
+__device__ __forceinline__ PairLoss pair_by_wave(const PairArgs& a, int64_t pair) {
+  double sum[2], count[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) sequence_share<64>(a, pair + k * a.pairs, threadIdx.x & 63, sum[k], count[k]);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) sum[k] = wave_sum(sum[k]), count[k] = wave_sum(count[k]);
+  return pair_loss(a, pair, sum, count);
+}
+
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) preference_pair_kernel(PairArgs a) {
+  __shared__ double red[THREADS / 32];
+  const int64_t pair = blockIdx.x;
+  double sum[2], count[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    sequence_share<THREADS>(a, pair + k * a.pairs, threadIdx.x, sum[k], count[k]);
+    block_sums<THREADS>(sum[k], count[k], red);
+  }
+  if (threadIdx.x) return;
+  const PairLoss l = pair_loss(a, pair, sum, count);
+  a.losses[pair] = l.loss;
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    a.rewards[pair + k * a.pairs] = l.rewards[k];
+    a.coefs[pair + k * a.pairs] = l.coefs[k];
+  }
+}
+
 // ---- the gradient of rows -------------------------------------------------------------------------------------------
 
 template <class T, int RT>
@@ -305,75 +406,48 @@ __global__ void __launch_bounds__(RT == 64 ? 256 : RT) logit_grad_kernel(LogitRo
   const RowStats st = q.stats ? q.stats[row] : RowStats{q.lse[row], 1.f};
   write_gradient<T, RT>(x, g, {c, c / st.sum, st.top, label});
 }
+// Labels that each row's threads look through for themselves, for a launch less (policy, 8 x 61 x 256 float32: 11.0 us with that
+// launch, 9.3 without).
+constexpr int64_t kFewLabels = 1024;
+
+// The gradient of few short pairs, whose losses each row's threads compute for themselves, for a launch less (2 pairs x 63 x 256 float32 13.0
+// us with that launch, 10.7 without; 4 x 256 x 16384 bfloat16 32.5 and 29.5); the first workgroup adds them up.
+constexpr int64_t kFewPairs = 4;
+template <class T, int RT>
+__global__ void __launch_bounds__(RT == 64 ? 256 : RT) few_pairs_grad_kernel(LogitRows a, PairArgs q, const RowStats* stats, float* loss,
+                                                                             T* gx) {
+  __shared__ double losses[kFewPairs];
+  if (blockIdx.x == 0 && blockIdx.y == 0) {
+    constexpr int WAVES = (RT == 64 ? 256 : RT) / 64;
+    for (int p = threadIdx.x >> 6; p < q.pairs; p += WAVES) {
+      const PairLoss l = pair_by_wave(q, p);
+      if ((threadIdx.x & 63) == 0) {
+        losses[p] = l.loss;
+        q.rewards[p] = l.rewards[0], q.rewards[p + q.pairs] = l.rewards[1];
+      }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      double all = 0.0;
+      for (int p = 0; p < q.pairs; ++p) all += losses[p];
+      *loss = (float)(all / (double)q.pairs);
+    }
+  }
+  const int64_t row = this_row<RT>(a.rows);
+  if (row < 0) return;
+  const int64_t label = a.labels[row], seq = row / a.length;
+  const Row<T> x((const T*)a.x + a.offset(row), a.vocab);
+  const GradRow<T> g(gx + row * a.vocab, x);
+  if (label == a.ignore) return write_zeros<T, RT>(g, x);
+  const PairLoss l = pair_by_wave(q, seq % q.pairs);
+  const float coef = seq < q.pairs ? l.coefs[0] : l.coefs[1], c = in_vocab(label, a.vocab) ? coef : __builtin_nanf("");
+  if (c == 0.f) return write_zeros<T, RT>(g, x);
+  const RowStats st = stats[row];
+  write_gradient<T, RT>(x, g, {c, c / st.sum, st.top, label});
+}
+
 __global__ void __launch_bounds__(64) mean_loss_kernel(const double* losses, int64_t count, float* loss) {
   mean_loss(losses, count, loss);
-}
-
-// ---- pairs ----------------------------------------------------------------------------------------------------------
-
-// two sums over the workgroup's THREADS, in every one of them
-template <int THREADS>
-__device__ __forceinline__ void block_sums(double& u, double& v, double* red) {
-  u = wave_sum(u), v = wave_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[(threadIdx.x >> 6) * 2] = u, red[(threadIdx.x >> 6) * 2 + 1] = v;
-  __syncthreads();
-  u = v = 0.0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 64; ++w) u += red[w * 2], v += red[w * 2 + 1];
-}
-
-struct PairArgs {
-  const int64_t* labels;
-  const float *logps, *reference;
-  int64_t ignore, length, pairs;
-  int kind, average;
-  double beta, smoothing;
-  float *rewards, *coefs;
-  double* losses;
-};
-
-// log(1 + exp(-z)) without overflow
-__device__ __forceinline__ double softplus_neg(double z) { return (z < 0 ? -z : 0.0) + log1p(exp(z < 0 ? z : -z)); }
-__device__ __forceinline__ double sigmoid(double z) { return 1.0 / (1.0 + exp(-z)); }
-
-template <int THREADS>
-__global__ void __launch_bounds__(THREADS) preference_pair_kernel(PairArgs a) {
-  __shared__ double red[THREADS / 32];
-  const int64_t pair = blockIdx.x;
-  double ratio[2], share[2];
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int64_t seq = pair + k * a.pairs, base = seq * a.length;
-    double sum = 0.0, count = 0.0;
-#pragma unroll 4
-    for (int64_t i = threadIdx.x; i < a.length; i += THREADS) {  // (logps of labels that do not count are 0)
-      sum += (double)a.logps[base + i];
-      count += a.labels[base + i] != a.ignore ? 1.0 : 0.0;
-    }
-    block_sums<THREADS>(sum, count, red);
-    share[k] = a.average ? 1.0 / fmax(count, 1.0) : 1.0;
-    ratio[k] = sum * share[k] - (double)a.reference[seq];
-  }
-  if (threadIdx.x) return;
-  const double d = ratio[0] - ratio[1], z = a.beta * d;
-  double loss, slope;  // of the loss by d
-  if (a.kind == OMT_PREFERENCE_SIGMOID) {
-    loss = (1.0 - a.smoothing) * softplus_neg(z) + a.smoothing * softplus_neg(-z);
-    slope = a.beta * (a.smoothing - sigmoid(-z));
-  } else if (a.kind == OMT_PREFERENCE_HINGE) {
-    loss = 1.0 - z < 0.0 ? 0.0 : 1.0 - z;  // (NaN stays NaN)
-    slope = 1.0 - z < 0.0 || z == 1.0 ? 0.0 : z < 1.0 ? -a.beta : z;
-  } else {
-    loss = (d - 0.5 / a.beta) * (d - 0.5 / a.beta);
-    slope = 2.0 * (d - 0.5 / a.beta);
-  }
-  a.losses[pair] = loss;
-#pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    a.rewards[pair + k * a.pairs] = (float)(a.beta * ratio[k]);
-    a.coefs[pair + k * a.pairs] = (float)((k ? -slope : slope) * share[k] / (double)a.pairs);
-  }
 }
 
 // ---- policy ---------------------------------------------------------------------------------------------------------
@@ -518,8 +592,7 @@ __global__ void __launch_bounds__(256) scale_by_kernel(T* x, int64_t n, const fl
 // ---- launches -------------------------------------------------------------------------------------------------------
 
 constexpr int64_t kLogitMaxRows = 1 << 28, kLogitMaxVocab = 1 << 28;
-// Labels that each row's threads count for themselves, for a launch less (8 x 61 x 256 float32 11.0 us with that launch, 9.3 without).
-constexpr int64_t kFewLabels = 1024;
+constexpr int64_t kFewPairsLength = 256;
 constexpr int64_t kParts = 64;  // workgroups that count labels, or sum terms, at most
 // Logits of more than this are taken backwards in their second pass (the last cache holds 256 MB; rows that do not count are not in
 // it): preference loss and gradient of 16 x 512 x 32768 bfloat16 213 us forwards, 185 backwards, x 131072 834 and 794; of 6 x 301 x
@@ -679,6 +752,17 @@ OMT_EXPORT int omt_preference_loss(const omt_logits* logits, const float* refere
     if (int e = token_logps(logits, logps, nullptr, gx ? stats : nullptr, s)) return e;
   const PairArgs a{logits->labels, logps, reference, logits->ignore_index, logits->length, pairs, kind, average, beta, smoothing,
                    rewards, coefs, losses};
+  if (gx && rows > 0 && pairs <= kFewPairs && logits->length <= kFewPairsLength && row_bytes(logits) <= 32768) {
+    for_type(logits, [&](auto t) {
+      typedef decltype(t) T;
+      for_row_threads(row_bytes(logits), [&](auto rt) {
+        constexpr int RT = decltype(rt)::value;
+        if constexpr (RT <= 256)
+          launch_rows<RT>(few_pairs_grad_kernel<T, RT>, rows, s, rows_of(logits), a, (const RowStats*)stats, loss, (T*)gx);
+      });
+    });
+    return launch_check("few_pairs_grad_kernel");
+  }
   if (logits->length <= 2048) hipLaunchKernelGGL(preference_pair_kernel<256>, dim3((unsigned)pairs), dim3(256), 0, s, a);
   else hipLaunchKernelGGL(preference_pair_kernel<1024>, dim3((unsigned)pairs), dim3(1024), 0, s, a);
   if (int e = launch_check("preference_pair_kernel")) return e;

@@ -277,9 +277,21 @@ def test_preference_loss(ops, cuda, dtype, vocab):
 
 @pytest.mark.parametrize("kind,smoothing,average", [("sigmoid", 0.1, False), ("sigmoid", 1.0, True), ("hinge", 0.0, False),
                                                     ("hinge", 0.0, True), ("ipo", 0.0, False), ("ipo", 0.0, True)])
-@pytest.mark.parametrize("length", [1, 2, 300, 3001])
+@pytest.mark.parametrize("length", [1, 2, 200, 300, 3001])
 def test_preference_kinds(ops, cuda, kind, smoothing, average, length):
     check_preference(ops, *some_logits(6, length, 33, F32, length), kind=kind, smoothing=smoothing, average=average)
+
+
+def test_a_pair_that_is_told_apart_for_certain(ops, cuda):
+    """A rejected sequence that holds a banned token: no loss and no gradient without smoothing, in either way to a pair's loss."""
+    for pairs, length in ((1, 3), (5, 3)):
+        x, labels = some_logits(2 * pairs, length, 40, F32, 11, masked=0.0)
+        for b in range(pairs, 2 * pairs):
+            x[b, 1, labels[b, 1]] = -math.inf
+        loss, rewards, gx = ops.preference_loss(x.cuda(), labels.cuda(), torch.zeros(2 * pairs).cuda())
+        assert float(loss) == 0 and bool((rewards[pairs:] == -math.inf).all()) and not bool(gx.any())
+        loss, _, _ = ops.preference_loss(x.cuda(), labels.cuda(), torch.zeros(2 * pairs).cuda(), smoothing=0.1)
+        assert float(loss) == math.inf
 
 
 def check_policy(ops, x, labels, layout=lambda t: t, reduction="token", kl=0.05, reference=True, each=False, clip=(0.2, 0.3), fill=None,
