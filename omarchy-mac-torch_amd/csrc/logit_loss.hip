@@ -501,8 +501,10 @@ __device__ __forceinline__ TokenLoss token_loss(const PolicyArgs& p, const Logit
   if (p.reference) {
     const double more = (double)p.reference[row] - lp, e = exp(more);
     t.kl = e - more - 1.0;
-    t.loss += p.kl * t.kl;
-    t.slope += p.kl * (1.0 - e);
+    if (p.kl != 0.0) {  // (a term of weight zero is left out: it may be infinite)
+      t.loss += p.kl * t.kl;
+      t.slope += p.kl * (1.0 - e);
+    }
   }
   return {t.loss * share, t.kl * share, t.slope * share};
 }

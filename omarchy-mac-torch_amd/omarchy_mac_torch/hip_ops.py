@@ -964,8 +964,9 @@ def policy_loss(logits, labels, old_logps, advantages, reference=None, clip=(0.2
     """The clipped policy loss: logits and labels as token_logps', r = exp(logps - old_logps) against the probabilities that
     the tokens were sampled with, A = advantages ([sequences] or [sequences, length]); of each token
     -min(r A, clamp(r, 1 - clip[0], 1 + clip[1]) A) + kl k, k = exp(reference - logps) - (reference - logps) - 1 (0 without a
-    reference); old_logps and reference are float32 [sequences, length]. reduction: the mean over all "token"s that count, or over
-    "sequence"s of each one's mean. Returns (loss, k's mean, logps, the logits' gradient or, without grad, None)."""
+    reference; a k of weight 0, which may be infinite, takes no part); old_logps and reference are float32 [sequences, length].
+    reduction: the mean over all "token"s that count, or over "sequence"s of each one's mean. Returns (loss, k's mean, logps, the
+    logits' gradient or, without grad, None)."""
     by_sequence = _choice("reduction", reduction, {"token": False, "sequence": True})
     return _lm("policy_loss", logits, labels, old_logps, advantages, reference, float(clip[0]), float(clip[1]), float(kl),
                by_sequence, int(ignore_index), bool(grad))
