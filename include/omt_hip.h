@@ -733,10 +733,10 @@ int omt_preference_loss(const omt_logits* logits, const float* reference, int ki
                         float* loss, float* rewards, void* gx, void* workspace, size_t workspace_bytes, void* stream);
 
 /* r = exp(logps - old_logps); a token's loss is -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A) + kl_weight k with k =
- * exp(reference - logps) - (reference - logps) - 1 (0 where reference is null; a k of weight 0 takes no part); old_logps and reference [sequences][length], A =
- * advantages[sequence * advantage_sequence_stride + row * advantage_row_stride]. loss, and kl of k: the mean over all tokens
- * that count or, by_sequence, over sequences of each one's mean (0 of one where none counts). logps as omt_token_logps_fwd's. gx:
- * the loss's gradient (null: not asked for). */
+ * exp(reference - logps) - (reference - logps) - 1 (0 where reference is null; a k of weight 0 takes no part); old_logps and
+ * reference [sequences][length], A = advantages[sequence * advantage_sequence_stride + row * advantage_row_stride]. loss, and kl
+ * of k: the mean over all tokens that count or, by_sequence, over sequences of each one's mean (0 of one where none counts). logps
+ * as omt_token_logps_fwd's. gx: the loss's gradient (null: not asked for). */
 size_t omt_policy_workspace(int64_t sequences, int64_t length, int by_sequence);
 int omt_policy_loss(const omt_logits* logits, const float* old_logps, const float* reference, const float* advantages,
                     int64_t advantage_sequence_stride, int64_t advantage_row_stride, double clip_low, double clip_high,

@@ -499,11 +499,12 @@ __device__ __forceinline__ TokenLoss token_loss(const PolicyArgs& p, const Logit
   const double bounded = (r < 1.0 - p.lo ? 1.0 - p.lo : r > 1.0 + p.hi ? 1.0 + p.hi : r) * adv;
   TokenLoss t{bounded < ra ? -bounded : -ra, 0.0, bounded < ra ? 0.0 : -ra};
   if (p.reference) {
-    const double more = (double)p.reference[row] - lp, e = exp(more);
-    t.kl = e - more - 1.0;
+    // (exp(more) - 1 as one: beside the reference what is left of it, less than 1's last places, is the term)
+    const double more = (double)p.reference[row] - lp, grown = expm1(more);
+    t.kl = grown - more;
     if (p.kl != 0.0) {  // (a term of weight zero is left out: it may be infinite)
       t.loss += p.kl * t.kl;
-      t.slope += p.kl * (1.0 - e);
+      t.slope -= p.kl * grown;
     }
   }
   return {t.loss * share, t.kl * share, t.slope * share};

@@ -1,11 +1,12 @@
-"""Losses on logits where weights of zero decide, beside test_gpu_lm.py, whose inputs these use."""
+"""Losses on logits where rounding and weights of zero decide, beside test_gpu_lm.py, whose bounds and inputs these use. u = 2^-24, half a
+step of float32 relative to the value."""
 
 import math
 
 import pytest
 import torch
 
-from test_gpu_lm import F32, some_logits
+from test_gpu_lm import F32, U, gen, some_logits, within
 
 pytestmark = pytest.mark.gpu
 
@@ -14,6 +15,14 @@ pytestmark = pytest.mark.gpu
 def ops(cuda):
     from omarchy_mac_torch import hip_ops
     return hip_ops
+
+
+def level(sequences, length, vocab):
+    """Rows of equal logits, whose sums are exact: each log-probability is -log(vocab) to float64's last places."""
+    x = torch.full((sequences, length, vocab), 3.0)
+    labels = torch.randint(vocab, (sequences, length), generator=gen(vocab))
+    labels[:, 1::5] = -100
+    return x, labels
 
 
 # ---- the KL term ----------------------------------------------------------------------------------------------------
@@ -33,3 +42,22 @@ def test_a_kl_term_of_weight_zero_takes_no_part(ops, cuda, reduction, vocab):
     got = ops.policy_loss(*args, reference=ref.cuda(), kl=0.0, reduction=reduction)
     assert math.isfinite(float(loss)) and float(none) == 0 and not math.isfinite(float(got[1]))
     assert torch.equal(got[0], loss) and torch.equal(got[2], logps) and torch.equal(got[3], gx) and not bool(gx.isnan().any())
+
+
+@pytest.mark.parametrize("reduction", ["token", "sequence"])
+def test_the_kl_term_beside_the_reference(ops, cuda, reduction):
+    """k = exp(m) - m - 1 is m^2 / 2 at small m: known to float32's rounding, and m's own, of a log-probability off by 2^-52."""
+    x, labels = level(6, 7, 2)
+    lp = torch.tensor(2.0, dtype=torch.float64).log().neg()
+    ref = (lp + torch.linspace(-3e-6, 3e-6, 42, dtype=torch.float64).view(6, 7)).float()
+    m = ref.double() - lp
+    k, counted = m * m / 2 + m ** 3 / 6 + m ** 4 / 24, (labels != -100).double()
+    share = counted / counted.sum() if reduction == "token" else counted / counted.sum(1, keepdim=True) / 6
+    old, adv = lp.float().expand(6, 7), torch.zeros(6)
+    loss, mean_k, _, gx = ops.policy_loss(x.cuda(), labels.cuda(), old.cuda(), adv.cuda(), reference=ref.cuda(), kl=0.5, reduction=reduction)
+    want, off = (k * share).sum(), (m.abs() * share).sum() * 2.0 ** -51
+    within(mean_k, want, 2 * U * want + off)
+    within(loss, want / 2, 2 * U * want + off)
+    c = -0.5 * torch.expm1(m) * share
+    onehot = torch.zeros(6, 7, 2, dtype=torch.float64).scatter_(2, labels.clamp(min=0)[..., None], 1.0)
+    within(gx, c[..., None] * (onehot - 0.5), (c.abs() * 4 * U + share * 2.0 ** -51)[..., None].expand(6, 7, 2))
