@@ -148,6 +148,11 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> policy_loss(const Tensor& logits, con
   return {loss, kl, logps, gx};
 }
 
+// after an operator has written t in place: autograd then refuses what it saved of it before
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 void scale_by_(const Tensor& x, const Tensor& factor) {
   OMT_OP("scale_by_");
   real_type(x, "x");
@@ -156,6 +161,7 @@ void scale_by_(const Tensor& x, const Tensor& factor) {
   TORCH_CHECK_VALUE(f.numel() == 1, "factor: expected one element, got ", f.sizes());
   Site at(x);
   ok(omt_scale_by(dtype_of(x), x.numel(), raw(x), rawf(f), at.stream), "scale_by_");
+  written(x);
 }
 
 // whether two tensors' elements lie in the same order
@@ -185,9 +191,6 @@ const float* check_scalar(const OptTensor& t, const char* name, const Tensor& p)
                    t->scalar_type(), " on ", t->device());
   TORCH_CHECK_VALUE(t->numel() == 1, name, ": expected one element, got ", t->sizes());
   return rawf(*t);
-}
-void written(const Tensor& t) {
-  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 void adamw_(at::TensorList params, at::TensorList grads, at::TensorList exp_avgs, at::TensorList exp_avg_sqs,

@@ -61,3 +61,20 @@ def test_the_kl_term_beside_the_reference(ops, cuda, reduction):
     c = -0.5 * torch.expm1(m) * share
     onehot = torch.zeros(6, 7, 2, dtype=torch.float64).scatter_(2, labels.clamp(min=0)[..., None], 1.0)
     within(gx, c[..., None] * (onehot - 0.5), (c.abs() * 4 * U + share * 2.0 ** -51)[..., None].expand(6, 7, 2))
+
+
+# ---- tensors written in place ---------------------------------------------------------------------------------------
+
+def test_scale_by_is_seen_by_autograd(ops, cuda):
+    import omarchy_mac_torch as omt
+    for scale in (ops.scale_by_, torch.ops.omt.scale_by_):
+        for device in ("cuda", omt.DEVICE):
+            x, two = torch.ones(5, device=device), torch.full((), 2.0, device=device)
+            before = x._version
+            scale(x, two)
+            assert x._version == before + 1 and bool((x == 2).all())
+        w = torch.ones(5, device=device, requires_grad=True)
+        y = (w * x).sum()
+        scale(x, two)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
