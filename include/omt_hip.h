@@ -743,7 +743,7 @@ int omt_policy_loss(const omt_logits* logits, const float* old_logps, const floa
                     double kl_weight, int by_sequence, float* loss, float* kl, float* logps, void* gx, void* workspace,
                     size_t workspace_bytes, void* stream);
 
-/* x *= *factor (a float on the device), in place; nothing is read or written where it is 1. */
+/* x *= *factor (a float on the device, outside x), in place; nothing is read or written where it is 1. */
 int omt_scale_by(int dtype, int64_t n, void* x, const float* factor, void* stream);
 
 /* One parameter of an AdamW step: param and grad of the call's type, its step count (a float on the device, already incremented).

@@ -159,6 +159,8 @@ void scale_by_(const Tensor& x, const Tensor& factor) {
   TORCH_CHECK_VALUE(on_gpu(x) && x.is_contiguous(), "x: expected a contiguous tensor on the HIP device");
   Tensor f = take(factor, "factor", at::kFloat, &x);
   TORCH_CHECK_VALUE(f.numel() == 1, "factor: expected one element, got ", f.sizes());
+  const char *begin = (const char*)raw(x), *of = (const char*)raw(f);
+  if (of >= begin && of < begin + x.nbytes()) f = f.clone();  // an element of x: some threads would read it scaled
   Site at(x);
   ok(omt_scale_by(dtype_of(x), x.numel(), raw(x), rawf(f), at.stream), "scale_by_");
   written(x);

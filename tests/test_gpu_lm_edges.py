@@ -78,3 +78,10 @@ def test_scale_by_is_seen_by_autograd(ops, cuda):
         scale(x, two)
         with pytest.raises(RuntimeError, match="modified by an inplace operation"):
             y.backward()
+
+
+@pytest.mark.parametrize("at", [0, 1234567, -1])
+def test_scale_by_one_of_the_elements(ops, cuda, at):
+    x = torch.randn(5000001, generator=gen(3)).cuda()
+    want = x * x[at].clone()
+    assert torch.equal(ops.scale_by_(x, x[at]), want)
