@@ -199,8 +199,14 @@ __device__ __forceinline__ int64_t this_row(int64_t rows) {
   return row < rows ? row : -1;
 }
 
+// What is written of each row; null: not asked for. sums: lp in 64 bits, for those that are added up.
+struct RowOut {
+  float *logps, *lse;
+  double* sums;
+  RowStats* stats;
+};
 template <class T, int RT>
-__global__ void __launch_bounds__(RT == 64 ? 256 : RT) token_logps_kernel(LogitRows a, float* logps, float* lse, RowStats* stats) {
+__global__ void __launch_bounds__(RT == 64 ? 256 : RT) token_logps_kernel(LogitRows a, RowOut out) {
   __shared__ float red[16];
   const int64_t row = this_row<RT>(a.rows);
   if (row < 0) return;
@@ -208,17 +214,20 @@ __global__ void __launch_bounds__(RT == 64 ? 256 : RT) token_logps_kernel(LogitR
   const int64_t label = a.labels[row];
   if (label == a.ignore) {
     if (first) {
-      logps[row] = 0.f;
-      if (lse) lse[row] = 0.f;
+      if (out.logps) out.logps[row] = 0.f;
+      if (out.lse) out.lse[row] = 0.f;
+      if (out.sums) out.sums[row] = 0.0;
     }
     return;
   }
   const Row<T> x((const T*)a.x + a.offset(row), a.vocab);
   const RowStats st = row_stats<T, RT>(x, red);
   if (first) {
-    logps[row] = (float)label_logp(x.p, label, a.vocab, st);
-    if (lse) lse[row] = (float)((double)st.top + log((double)st.sum));
-    if (stats) stats[row] = st;
+    const double lp = label_logp(x.p, label, a.vocab, st);
+    if (out.logps) out.logps[row] = (float)lp;
+    if (out.lse) out.lse[row] = (float)((double)st.top + log((double)st.sum));
+    if (out.sums) out.sums[row] = lp;
+    if (out.stats) out.stats[row] = st;
   }
 }
 
@@ -238,7 +247,8 @@ __device__ __forceinline__ void block_sums(double& u, double& v, double* red) {
 
 struct PairArgs {
   const int64_t* labels;
-  const float *logps, *reference;
+  const double* logps;
+  const float* reference;
   int64_t ignore, length, pairs;
   int kind, average;
   double beta, smoothing;
@@ -291,7 +301,7 @@ __device__ __forceinline__ void sequence_share(const PairArgs& a, int64_t seq, i
   sum = count = 0.0;
 #pragma unroll 4
   for (int64_t i = first; i < a.length; i += THREADS) {
-    sum += (double)a.logps[base + i];
+    sum += a.logps[base + i];
     count += a.labels[base + i] != a.ignore ? 1.0 : 0.0;
   }
 }
@@ -641,11 +651,11 @@ static void for_row_threads(int64_t bytes, Go go) {
   else go(std::integral_constant<int, 1024>());
 }
 
-static int token_logps(const omt_logits* q, float* logps, float* lse, RowStats* stats, hipStream_t s) {
+static int token_logps(const omt_logits* q, const RowOut& out, hipStream_t s) {
   for_type(q, [&](auto t) {
     for_row_threads(row_bytes(q), [&](auto rt) {
       constexpr int RT = decltype(rt)::value;
-      launch_rows<RT>(token_logps_kernel<decltype(t), RT>, q->sequences * q->length, s, rows_of(q), logps, lse, stats);
+      launch_rows<RT>(token_logps_kernel<decltype(t), RT>, q->sequences * q->length, s, rows_of(q), out);
     });
   });
   return launch_check("token_logps_kernel");
@@ -669,7 +679,7 @@ struct PreferencePlan {
 };
 static PreferencePlan preference_plan(int64_t sequences, int64_t length) {
   const size_t rows = (size_t)(sequences * length);
-  return {up256(rows * 4), up256(rows * sizeof(RowStats)), up256((size_t)sequences * 4), up256((size_t)sequences * 4)};
+  return {up256(rows * 8), up256(rows * sizeof(RowStats)), up256((size_t)sequences * 4), up256((size_t)sequences * 4)};
 }
 
 struct PolicyPlan {
@@ -714,7 +724,7 @@ OMT_EXPORT int omt_token_logps_fwd(const omt_logits* logits, float* logps, float
   if (int e = logits_check("omt_token_logps_fwd", logits)) return e;
   if (logits->sequences * logits->length == 0) return OMT_OK;
   if (!logps || !lse) return fail(OMT_INVALID, "omt_token_logps_fwd: null pointer");
-  return token_logps(logits, logps, lse, nullptr, stream_of(stream));
+  return token_logps(logits, {logps, lse, nullptr, nullptr}, stream_of(stream));
 }
 
 OMT_EXPORT int omt_token_logps_bwd(const omt_logits* logits, const float* lse, const float* g, void* gx, void* stream) {
@@ -745,14 +755,14 @@ OMT_EXPORT int omt_preference_loss(const omt_logits* logits, const float* refere
   if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < p.total())
     return fail(OMT_INVALID, "%s: workspace of %zu bytes at %p", fn, workspace_bytes, workspace);
   char* at = (char*)workspace;
-  float* logps = (float*)at;
+  double* logps = (double*)at;
   RowStats* stats = (RowStats*)(at + p.logps);
   double* losses = (double*)(at + p.logps + p.stats);
   float* coefs = (float*)(at + p.logps + p.stats + p.losses);
   hipStream_t s = stream_of(stream);
   const int64_t pairs = n / 2;
   if (rows > 0)
-    if (int e = token_logps(logits, logps, nullptr, gx ? stats : nullptr, s)) return e;
+    if (int e = token_logps(logits, {nullptr, nullptr, logps, gx ? stats : nullptr}, s)) return e;
   const PairArgs a{logits->labels, logps, reference, logits->ignore_index, logits->length, pairs, kind, average, beta, smoothing,
                    rewards, coefs, losses};
   if (gx && rows > 0 && pairs <= kFewPairs && logits->length <= kFewPairsLength && row_bytes(logits) <= 32768) {

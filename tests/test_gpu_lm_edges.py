@@ -63,6 +63,22 @@ def test_the_kl_term_beside_the_reference(ops, cuda, reduction):
     within(gx, c[..., None] * (onehot - 0.5), (c.abs() * 4 * U + share * 2.0 ** -51)[..., None].expand(6, 7, 2))
 
 
+# ---- sums of log-probabilities --------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("average", [False, True])
+@pytest.mark.parametrize("vocab,length", [(2, 3), (2, 256), (2, 3001), (1000, 300), (40000, 40)])
+@pytest.mark.parametrize("pairs", [1, 5])
+def test_sequences_add_up_in_64_bits(ops, cuda, pairs, vocab, length, average):
+    """A sequence's log-probability beside its reference: off by float64's rounding of its sum, not by float32's of each."""
+    x, labels = level(2 * pairs, length, vocab)
+    count = (labels != -100).sum(1).double()
+    sums = -math.log(vocab) * (1 if average else count)
+    reference = (sums + torch.zeros(2 * pairs)).float()
+    _, rewards, _ = ops.preference_loss(x.cuda(), labels.cuda(), reference.cuda(), beta=1.0, average=average)
+    want = sums - reference.double()
+    within(rewards, want, 2 * U * want.abs() + (count + 4) * 2.0 ** -52 * reference.double().abs())
+
+
 # ---- tensors written in place ---------------------------------------------------------------------------------------
 
 def test_scale_by_is_seen_by_autograd(ops, cuda):
