@@ -715,9 +715,12 @@ typedef struct omt_logits {
 } omt_logits;
 
 /* logps = x[label] - lse, lse = log(sum exp x), each [sequences][length]; 0 in both where a row does not count. The backward:
- * gx = g (onehot(label) - exp(x - lse)), g the gradient of logps. */
+ * gx = g (onehot(label) - exp(x - lse)), g the gradient of logps. A gradient by lse in 32 bits has its rounding, 2^-24 |lse| of each
+ * exp(x - lse); the two ending in 64, which hold it in 64 bits, have none that grows with the logits. */
 int omt_token_logps_fwd(const omt_logits* logits, float* logps, float* lse, void* stream);
 int omt_token_logps_bwd(const omt_logits* logits, const float* lse, const float* g, void* gx, void* stream);
+int omt_token_logps_fwd64(const omt_logits* logits, float* logps, double* lse, void* stream);
+int omt_token_logps_bwd64(const omt_logits* logits, const double* lse, const float* g, void* gx, void* stream);
 
 /* Pairs of sequences, the chosen ones in the first half and the rejected ones, in the same order, in the second. L: the sum of a
  * sequence's logps, or with `average` their mean (0 where none counts); R: reference[sequences]; d = (L - R of the chosen) - (L - R

@@ -199,10 +199,10 @@ __device__ __forceinline__ int64_t this_row(int64_t rows) {
   return row < rows ? row : -1;
 }
 
-// What is written of each row; null: not asked for. sums: lp in 64 bits, for those that are added up.
+// What is written of each row; null: not asked for. sums: lp in 64 bits, for those that are added up; lse in 32 bits or in 64.
 struct RowOut {
   float *logps, *lse;
-  double* sums;
+  double *lse64, *sums;
   RowStats* stats;
 };
 template <class T, int RT>
@@ -216,6 +216,7 @@ __global__ void __launch_bounds__(RT == 64 ? 256 : RT) token_logps_kernel(LogitR
     if (first) {
       if (out.logps) out.logps[row] = 0.f;
       if (out.lse) out.lse[row] = 0.f;
+      if (out.lse64) out.lse64[row] = 0.0;
       if (out.sums) out.sums[row] = 0.0;
     }
     return;
@@ -225,7 +226,9 @@ __global__ void __launch_bounds__(RT == 64 ? 256 : RT) token_logps_kernel(LogitR
   if (first) {
     const double lp = label_logp(x.p, label, a.vocab, st);
     if (out.logps) out.logps[row] = (float)lp;
-    if (out.lse) out.lse[row] = (float)((double)st.top + log((double)st.sum));
+    const double lse = (double)st.top + log((double)st.sum);
+    if (out.lse) out.lse[row] = (float)lse;
+    if (out.lse64) out.lse64[row] = lse;
     if (out.sums) out.sums[row] = lp;
     if (out.stats) out.stats[row] = st;
   }
@@ -383,11 +386,12 @@ __device__ __forceinline__ void write_gradient(const Row<T>& x, const GradRow<T>
   }
 }
 
-// Of each row, lse, or its RowStats, which spares lse's rounding. per_row: coefs holds one for each row, else one for each sequence.
+// Of each row, lse in 32 bits, whose rounding makes exp(x - lse) off by 2^-24 |lse|, or in 64, or its RowStats. per_row: coefs holds one for each row, else one for each sequence.
 // backwards: the last rows first, which a pass over all rows has left in the last cache. losses (or null): the mean of so many
 // goes to loss, by the first workgroup.
 struct GradArgs {
   const float* lse;
+  const double* lse64;
   const RowStats* stats;
   const float* coefs;
   int per_row, backwards;
@@ -413,7 +417,16 @@ __global__ void __launch_bounds__(RT == 64 ? 256 : RT) logit_grad_kernel(LogitRo
   const GradRow<T> g(gx + row * a.vocab, x);
   if (label == a.ignore || coef == 0.f) return write_zeros<T, RT>(g, x);
   const float c = in_vocab(label, a.vocab) ? coef : __builtin_nanf("");
-  const RowStats st = q.stats ? q.stats[row] : RowStats{q.lse[row], 1.f};
+  RowStats st;
+  if (q.stats) {
+    st = q.stats[row];
+  } else if (q.lse64) {
+    const double lse = q.lse64[row];
+    st.top = (float)lse;
+    st.sum = exp_from((float)(lse - (double)st.top), 0.f);
+  } else {
+    st = {q.lse[row], 1.f};
+  }
   write_gradient<T, RT>(x, g, {c, c / st.sum, st.top, label});
 }
 // Labels that each row's threads look through for themselves, for a launch less (policy, 8 x 61 x 256 float32: 11.0 us with that
@@ -720,18 +733,31 @@ static void for_held_row(int64_t bytes, Go go) {
 
 using namespace omt;
 
-OMT_EXPORT int omt_token_logps_fwd(const omt_logits* logits, float* logps, float* lse, void* stream) {
-  if (int e = logits_check("omt_token_logps_fwd", logits)) return e;
+static int token_logps_fwd(const char* fn, const omt_logits* logits, float* logps, float* lse, double* lse64, void* stream) {
+  if (int e = logits_check(fn, logits)) return e;
   if (logits->sequences * logits->length == 0) return OMT_OK;
-  if (!logps || !lse) return fail(OMT_INVALID, "omt_token_logps_fwd: null pointer");
-  return token_logps(logits, {logps, lse, nullptr, nullptr}, stream_of(stream));
+  if (!logps || (!lse && !lse64)) return fail(OMT_INVALID, "%s: null pointer", fn);
+  return token_logps(logits, {logps, lse, lse64, nullptr, nullptr}, stream_of(stream));
+}
+OMT_EXPORT int omt_token_logps_fwd(const omt_logits* logits, float* logps, float* lse, void* stream) {
+  return token_logps_fwd("omt_token_logps_fwd", logits, logps, lse, nullptr, stream);
+}
+OMT_EXPORT int omt_token_logps_fwd64(const omt_logits* logits, float* logps, double* lse, void* stream) {
+  return token_logps_fwd("omt_token_logps_fwd64", logits, logps, nullptr, lse, stream);
 }
 
-OMT_EXPORT int omt_token_logps_bwd(const omt_logits* logits, const float* lse, const float* g, void* gx, void* stream) {
-  if (int e = logits_check("omt_token_logps_bwd", logits)) return e;
+static int token_logps_bwd(const char* fn, const omt_logits* logits, const float* lse, const double* lse64, const float* g, void* gx,
+                           void* stream) {
+  if (int e = logits_check(fn, logits)) return e;
   if (logits->sequences * logits->length == 0) return OMT_OK;
-  if (!lse || !g || !gx) return fail(OMT_INVALID, "omt_token_logps_bwd: null pointer");
-  return logit_grad(logits, {lse, nullptr, g, 1, 0, nullptr, 0, nullptr}, gx, stream_of(stream));
+  if ((!lse && !lse64) || !g || !gx) return fail(OMT_INVALID, "%s: null pointer", fn);
+  return logit_grad(logits, {lse, lse64, nullptr, g, 1, 0, nullptr, 0, nullptr}, gx, stream_of(stream));
+}
+OMT_EXPORT int omt_token_logps_bwd(const omt_logits* logits, const float* lse, const float* g, void* gx, void* stream) {
+  return token_logps_bwd("omt_token_logps_bwd", logits, lse, nullptr, g, gx, stream);
+}
+OMT_EXPORT int omt_token_logps_bwd64(const omt_logits* logits, const double* lse, const float* g, void* gx, void* stream) {
+  return token_logps_bwd("omt_token_logps_bwd64", logits, nullptr, lse, g, gx, stream);
 }
 
 OMT_EXPORT size_t omt_preference_workspace(int64_t sequences, int64_t length) {
@@ -762,7 +788,7 @@ OMT_EXPORT int omt_preference_loss(const omt_logits* logits, const float* refere
   hipStream_t s = stream_of(stream);
   const int64_t pairs = n / 2;
   if (rows > 0)
-    if (int e = token_logps(logits, {nullptr, nullptr, logps, gx ? stats : nullptr}, s)) return e;
+    if (int e = token_logps(logits, {nullptr, nullptr, nullptr, logps, gx ? stats : nullptr}, s)) return e;
   const PairArgs a{logits->labels, logps, reference, logits->ignore_index, logits->length, pairs, kind, average, beta, smoothing,
                    rewards, coefs, losses};
   if (gx && rows > 0 && pairs <= kFewPairs && logits->length <= kFewPairsLength && row_bytes(logits) <= 32768) {
@@ -780,7 +806,7 @@ OMT_EXPORT int omt_preference_loss(const omt_logits* logits, const float* refere
   else hipLaunchKernelGGL(preference_pair_kernel<1024>, dim3((unsigned)pairs), dim3(1024), 0, s, a);
   if (int e = launch_check("preference_pair_kernel")) return e;
   if (gx && rows > 0)
-    return logit_grad(logits, {nullptr, stats, coefs, 0, rows * row_bytes(logits) > kBackwardsBytes, losses, pairs, loss}, gx, s);
+    return logit_grad(logits, {nullptr, nullptr, stats, coefs, 0, rows * row_bytes(logits) > kBackwardsBytes, losses, pairs, loss}, gx, s);
   hipLaunchKernelGGL(mean_loss_kernel, dim3(1), dim3(64), 0, s, losses, pairs, loss);
   return launch_check("mean_loss_kernel");
 }

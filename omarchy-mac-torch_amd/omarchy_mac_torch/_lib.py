@@ -260,6 +260,8 @@ SIGNATURES = {
     "omt_embedding_bwd": (I32, [I32, I32, I64, I64, I64, VP, VP, I64, F32, VP, VP, SZ, VP]),
     "omt_token_logps_fwd": (I32, [LG, VP, VP, VP]),
     "omt_token_logps_bwd": (I32, [LG, VP, VP, VP, VP]),
+    "omt_token_logps_fwd64": (I32, [LG, VP, VP, VP]),
+    "omt_token_logps_bwd64": (I32, [LG, VP, VP, VP, VP]),
     "omt_preference_workspace": (SZ, [I64, I64]),
     "omt_preference_loss": (I32, [LG, VP, I32, F64, F64, I32, VP, VP, VP, VP, SZ, VP]),
     "omt_policy_workspace": (SZ, [I64, I64, I32]),

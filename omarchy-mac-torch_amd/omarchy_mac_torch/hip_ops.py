@@ -912,7 +912,7 @@ def _lm(name, *args):
 
 def _choice(name, value, choices):
     if value not in choices:
-        raise ValueError(f"{name}: expected one of {sorted(choices)}, got {value!r}")
+        raise ValueError(f"{name}: expected one of {sorted(choices, key=str)}, got {value!r}")
     return choices[value]
 
 
@@ -931,15 +931,17 @@ def embedding_backward(gy, tokens, vocab, scale=1.0, padding_idx=None):
     return _lm("embedding_backward", gy, tokens, int(vocab), float(scale), padding_idx)
 
 
-def token_logps(logits, labels, ignore_index=-100):
+def token_logps(logits, labels, ignore_index=-100, lse_dtype=torch.float32):
     """log softmax(logits)[label] of each label: logits [sequences, length, vocab] (rows dense, any other strides), labels int64
-    [sequences, length]. Returns (logps, lse) in float32, lse each row's log sum exp; both 0 where the label is ignore_index, whose
-    rows are not read. A label outside the vocabulary gives NaN, here and in the losses below."""
-    return _lm("token_logps", logits, labels, int(ignore_index))
+    [sequences, length]. Returns (logps, lse), logps in float32, lse each row's log sum exp in float32 or float64; both 0 where the
+    label is ignore_index, whose rows are not read. A label outside the vocabulary gives NaN, here and in the losses below."""
+    lse64 = _choice("lse_dtype", lse_dtype, {torch.float32: False, torch.float64: True})
+    return _lm("token_logps", logits, labels, int(ignore_index), lse64)
 
 
 def token_logps_backward(g, logits, labels, lse, ignore_index=-100):
-    """The gradient of token_logps' logits from g, the gradient of its logps, and its lse."""
+    """The gradient of token_logps' logits from g, the gradient of its logps, and its lse. By an lse in float32 each probability is off
+    by up to 2^-24 |lse| of itself; by one in float64 by nothing that grows with the logits."""
     return _lm("token_logps_backward", g, logits, labels, lse, int(ignore_index))
 
 

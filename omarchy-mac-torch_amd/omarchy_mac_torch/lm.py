@@ -38,7 +38,7 @@ class _Embedding(torch.autograd.Function):
 class _TokenLogps(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, labels, ignore_index):
-        logps, lse = hip_ops.token_logps(logits, labels, ignore_index)
+        logps, lse = hip_ops.token_logps(logits, labels, ignore_index, lse_dtype=torch.float64)
         ctx.save_for_backward(logits, labels, lse)
         ctx.ignore_index = ignore_index
         return logps

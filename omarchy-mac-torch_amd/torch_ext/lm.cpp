@@ -81,12 +81,14 @@ Logits take_logits(const Tensor& x_, const Tensor& labels_, int64_t ignore_index
 }
 Tensor make_gradient(const Logits& l, bool asked) { return asked ? make(l.x, l.x.sizes(), l.x.scalar_type()) : Tensor(); }
 
-std::tuple<Tensor, Tensor> token_logps(const Tensor& logits, const Tensor& labels, int64_t ignore_index) {
+std::tuple<Tensor, Tensor> token_logps(const Tensor& logits, const Tensor& labels, int64_t ignore_index, bool lse64) {
   OMT_OP("token_logps");
   const Logits l = take_logits(logits, labels, ignore_index);
   Site at(l.x);
-  Tensor logps = make(l.x, l.labels.sizes(), at::kFloat), lse = make(l.x, l.labels.sizes(), at::kFloat);
-  ok(omt_token_logps_fwd(&l.q, rawf(logps), rawf(lse), at.stream), "token_logps");
+  Tensor logps = make(l.x, l.labels.sizes(), at::kFloat), lse = make(l.x, l.labels.sizes(), lse64 ? at::kDouble : at::kFloat);
+  ok(lse64 ? omt_token_logps_fwd64(&l.q, rawf(logps), (double*)raw(lse), at.stream)
+           : omt_token_logps_fwd(&l.q, rawf(logps), rawf(lse), at.stream),
+     "token_logps");
   return {logps, lse};
 }
 
@@ -94,10 +96,14 @@ Tensor token_logps_backward(const Tensor& g_, const Tensor& logits, const Tensor
                             int64_t ignore_index) {
   OMT_OP("token_logps_backward");
   const Logits l = take_logits(logits, labels, ignore_index);
-  Tensor g = take(g_, "g", at::kFloat, &l.x, l.labels.sizes()), lse = take(lse_, "lse", at::kFloat, &l.x, l.labels.sizes());
+  const bool lse64 = lse_.defined() && lse_.scalar_type() == at::kDouble;
+  Tensor g = take(g_, "g", at::kFloat, &l.x, l.labels.sizes());
+  Tensor lse = take(lse_, "lse", lse64 ? at::kDouble : at::kFloat, &l.x, l.labels.sizes());
   Site at(l.x);
   Tensor gx = make_gradient(l, true);
-  ok(omt_token_logps_bwd(&l.q, rawf(lse), rawf(g), raw(gx), at.stream), "token_logps_backward");
+  ok(lse64 ? omt_token_logps_bwd64(&l.q, (const double*)raw(lse), rawf(g), raw(gx), at.stream)
+           : omt_token_logps_bwd(&l.q, rawf(lse), rawf(g), raw(gx), at.stream),
+     "token_logps_backward");
   return gx;
 }
 
@@ -278,7 +284,7 @@ void bind_lm(pybind11::module_& m) {
 TORCH_LIBRARY_FRAGMENT(omt, m) {
   m.def("embedding(Tensor tokens, Tensor weight, float scale) -> Tensor");
   m.def("embedding_backward(Tensor gy, Tensor tokens, int vocab, float scale, int padding_idx) -> Tensor");
-  m.def("token_logps(Tensor logits, Tensor labels, int ignore_index) -> (Tensor, Tensor)");
+  m.def("token_logps(Tensor logits, Tensor labels, int ignore_index, bool lse64=False) -> (Tensor, Tensor)");
   m.def("token_logps_backward(Tensor g, Tensor logits, Tensor labels, Tensor lse, int ignore_index) -> Tensor");
   m.def("preference_loss(Tensor logits, Tensor labels, Tensor reference, float beta, int kind, float smoothing, bool average, "
         "int ignore_index, bool grad) -> (Tensor, Tensor, Tensor)");

@@ -8,6 +8,7 @@ import torch
 import torch.nn.functional as F
 
 from test_gpu_ffn_device import plain_lm, rel
+from test_gpu_lm import U, log_probs, some_logits, within
 
 pytestmark = pytest.mark.gpu
 
@@ -303,3 +304,21 @@ def test_operators_of_the_dispatcher(omt):
     assert torch.equal(p.cpu(), q.cpu())
     with pytest.raises(ValueError):
         ops.embedding(t.to(d), w.cuda())
+
+
+def test_log_probabilities_gradient_far_from_zero(omt):
+    """Logits shifted by thousands: softmax does not change, and its gradient's error does not grow with the shift. p is off by the
+    sum's error, by 3 u |lp| + 2 u of the exponential, 3 u where the rounded part of log sum exp is put back and 1 u of a product."""
+    from omarchy_mac_torch import lm
+    for shift in (0.0, 1000.0, -16384.0):
+        x, labels = some_logits(3, 5, 2050, torch.float32, 7)
+        x += shift
+        _, lp, off = log_probs(x, labels)
+        dev = x.to(omt.DEVICE).requires_grad_(True)
+        g = torch.randn(3, 5, generator=torch.Generator().manual_seed(1))
+        lm.token_logps(dev, labels.to(omt.DEVICE)).backward(g.to(omt.DEVICE))
+        counted = (labels != -100)[..., None]
+        onehot, p = torch.zeros_like(lp).scatter_(2, labels.clamp(min=0)[..., None], 1.0), lp.exp()
+        want = torch.where(counted, g.double()[..., None] * (onehot - p), 0.0)
+        bound = g.double().abs()[..., None] * (p * (off + U * (3 * lp.abs() + 6)) + 3 * U * (p + onehot)) + 2.0 ** -126
+        within(dev.grad, want, torch.where(counted, bound, 0.0))

@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_lm import F32, U, gen, some_logits, within
+from test_gpu_lm import BF16, F32, U, gen, log_probs, rounding, some_logits, within
 
 pytestmark = pytest.mark.gpu
 
@@ -77,6 +77,37 @@ def test_sequences_add_up_in_64_bits(ops, cuda, pairs, vocab, length, average):
     _, rewards, _ = ops.preference_loss(x.cuda(), labels.cuda(), reference.cuda(), beta=1.0, average=average)
     want = sums - reference.double()
     within(rewards, want, 2 * U * want.abs() + (count + 4) * 2.0 ** -52 * reference.double().abs())
+
+
+# ---- the gradient of log-probabilities ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("vocab", [9, 2050, 33000, 70001])
+def test_log_probabilities_by_lse_in_64_bits(ops, cuda, dtype, vocab):
+    """The same log-probabilities; lse without float32's rounding, and a gradient without it: p is off by the sum's error, by
+    3 u |lp| + 2 u of the exponential, 3 u where the rounded part of lse is put back and 1 u of a product."""
+    x, labels = some_logits(2, 5, vocab, dtype, vocab)
+    x = x + 2048  # (in bfloat16, in steps of 16)
+    own, lp, off = log_probs(x, labels)
+    logps, lse = ops.token_logps(x.cuda(), labels.cuda(), lse_dtype=torch.float64)
+    short = ops.token_logps(x.cuda(), labels.cuda())
+    assert lse.dtype == torch.float64 and torch.equal(logps, short[0]) and torch.equal(lse.float(), short[1])
+    counted = labels != -100
+    within(lse, torch.where(counted, torch.logsumexp(x.double(), -1), 0.0), torch.where(counted, off, 0.0))
+    g = torch.randn(2, 5, generator=gen(1))
+    gx = ops.token_logps_backward(g.cuda(), x.cuda(), labels.cuda(), lse)
+    onehot, p = torch.zeros_like(lp).scatter_(2, labels.clamp(min=0)[..., None], 1.0), lp.exp()
+    want = torch.where(counted[..., None], g.double()[..., None] * (onehot - p), 0.0)
+    bound = g.double().abs()[..., None] * (p * (off + U * (3 * lp.abs() + 6)) + 3 * U * (p + onehot)) + 2.0 ** -126
+    within(gx, want, torch.where(counted[..., None], bound * (1 + 2.0 ** -8) + rounding(dtype) * want.abs(), 0.0))
+    with pytest.raises(ValueError):
+        ops.token_logps(x.cuda(), labels.cuda(), lse_dtype=dtype if dtype == BF16 else torch.float16)
+    with pytest.raises(TypeError):
+        ops.token_logps_backward(g.cuda(), x.cuda(), labels.cuda(), lse.half())
+    bad = labels.clone()
+    bad[1, 2] = vocab
+    gx = ops.token_logps_backward(g.cuda(), x.cuda(), bad.cuda(), lse)
+    assert bool(gx[1, 2].isnan().all()) and not bool(gx[0].isnan().any())
 
 
 # ---- tensors written in place ---------------------------------------------------------------------------------------

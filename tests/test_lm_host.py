@@ -232,3 +232,15 @@ def test_optimizer_states_keep_their_types_through_a_state_dict(monkeypatch, dty
     for name, t in state.items():
         mine = other.state[q][name]
         assert mine.dtype == t.dtype and torch.equal(mine.float(), t.float()) and mine.data_ptr() != t.data_ptr()
+
+
+def test_statuses_of_log_probabilities_in_64_bits(lib):
+    L, p, bad, no, ok = lib.L, ctypes.c_void_p(4096), lib.OMT_INVALID, lib.OMT_UNSUPPORTED, lib.OMT_OK
+    f, b = L.omt_token_logps_fwd64, L.omt_token_logps_bwd64
+    assert f(None, p, p, None) == bad and b(None, p, p, p, None) == bad
+    for wrong in (dict(dtype=I64), dict(sequences=-1), dict(vocab=0), dict(x=None), dict(labels=None)):
+        assert f(logits(lib, **wrong), p, p, None) == bad and b(logits(lib, **wrong), p, p, p, None) == bad
+    assert f(logits(lib, length=1 << 28), p, p, None) == no and b(logits(lib, vocab=(1 << 28) + 1), p, p, p, None) == no
+    assert f(logits(lib), None, p, None) == bad and f(logits(lib), p, None, None) == bad
+    assert b(logits(lib), None, p, p, None) == bad and b(logits(lib), p, None, p, None) == bad and b(logits(lib), p, p, None, None) == bad
+    assert f(logits(lib, length=0, x=None), None, None, None) == ok and b(logits(lib, length=0, x=None), None, None, None, None) == ok
