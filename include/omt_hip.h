@@ -753,7 +753,7 @@ int omt_scale_by(int dtype, int64_t n, void* x, const float* factor, void* strea
  * master (bfloat16 parameters; of all tensors of a call, or null in all): the float32 copy that is updated, param its rounding.
  * States of 32 bits: float32, no scales. Of 8 bits: e4m3 with a scale for each block of 128 consecutive elements
  * ([ceil(numel / 128)]), max(largest magnitude, 1e-30) / 448; exp_avg_sq then holds the second moment's square root, and what is
- * over 0 as e4m3's smallest value at least. */
+ * over 0 as e4m3's smallest value at least. Of all arrays of a call, none that is written may overlap another. */
 typedef struct omt_adamw_tensor {
   void* param;
   const void* grad;

@@ -9,7 +9,8 @@
 #include <pybind11/stl.h>
 #include <torch/extension.h>
 
-#include <unordered_set>
+#include <algorithm>
+#include <utility>
 
 #include "operands.h"
 
@@ -201,6 +202,24 @@ const float* check_scalar(const OptTensor& t, const char* name, const Tensor& p)
   return rawf(*t);
 }
 
+// The memory of one call's tensors: what one of them is written to, no other of them may hold.
+struct Ranges {
+  c10::SmallVector<std::pair<uintptr_t, uintptr_t>, 128> all;  // begin, and twice the end, odd where the memory is only read
+  void add(const void* p, int64_t bytes, bool read = false) {
+    if (p) all.emplace_back((uintptr_t)p, ((uintptr_t)p + bytes) << 1 | read);
+  }
+  bool overlap() {
+    std::sort(all.begin(), all.end(), [](const auto& a, const auto& b) { return a.first < b.first; });
+    uintptr_t any = 0, written = 0;  // where those before end
+    for (const auto& [begin, end] : all) {
+      if (begin < (end & 1 ? written : any)) return true;
+      any = std::max(any, end >> 1);
+      if (!(end & 1)) written = std::max(written, end >> 1);
+    }
+    return false;
+  }
+};
+
 void adamw_(at::TensorList params, at::TensorList grads, at::TensorList exp_avgs, at::TensorList exp_avg_sqs,
             at::TensorList steps, at::TensorList exp_avg_scales, at::TensorList exp_avg_sq_scales, at::TensorList masters,
             double lr, const OptTensor& lr_dev, double beta1, double beta2, double eps, double weight_decay,
@@ -219,14 +238,13 @@ void adamw_(at::TensorList params, at::TensorList grads, at::TensorList exp_avgs
   TORCH_CHECK_TYPE(on_gpu(first), "parameter 0: expected a tensor on the HIP device, got one on ", first.device());
   TORCH_CHECK_TYPE(masters.empty() || type == at::kBFloat16, "masters: of bfloat16 parameters only");
   std::vector<omt_adamw_tensor> ts(n);
-  std::unordered_set<const void*> seen;
+  Ranges memory;
   std::vector<Tensor> copies;  // gradients whose elements lie in another order
   for (size_t i = 0; i < n; ++i) {
     const Tensor& p = params[i];
     TORCH_CHECK_TYPE(p.scalar_type() == type && p.device() == first.device(), "parameter ", i, ": expected ", type, " on ",
                      first.device(), " as the first, got ", p.scalar_type(), " on ", p.device());
     TORCH_CHECK_VALUE(p.is_non_overlapping_and_dense(), "parameter ", i, ": expected dense, got strides ", p.strides());
-    TORCH_CHECK_VALUE(p.numel() == 0 || seen.insert(raw(p)).second, "parameter ", i, ": given twice");
     Tensor g = grads[i];
     TORCH_CHECK_TYPE(g.defined() && g.scalar_type() == type && g.device() == p.device() && g.layout() == at::kStrided, "gradient ", i,
                      ": expected dense ", type, " on ", p.device(), " as the parameter, got ", g.scalar_type(), " on ", g.device());
@@ -245,7 +263,19 @@ void adamw_(at::TensorList params, at::TensorList grads, at::TensorList exp_avgs
                              check_scalar(steps[i], "step", p),
                              p.numel()};
     TORCH_CHECK_VALUE(ts[i].step, "step ", i, ": expected a tensor");
+    const omt_adamw_tensor& t = ts[i];
+    if (t.numel == 0) continue;
+    const int64_t size = type == at::kFloat ? 4 : 2, held_size = fp8 ? 1 : 4, scales = (t.numel + kBlock - 1) / kBlock * 4;
+    memory.add(t.param, t.numel * size);
+    memory.add(t.master, t.numel * 4);
+    memory.add(t.exp_avg, t.numel * held_size);
+    memory.add(t.exp_avg_sq, t.numel * held_size);
+    memory.add(t.exp_avg_scale, scales);
+    memory.add(t.exp_avg_sq_scale, scales);
+    // (a parameter that is its own gradient: each element is read before it is written, by one thread)
+    if (t.grad != t.param) memory.add(t.grad, t.numel * size, true);
   }
+  TORCH_CHECK_VALUE(!memory.overlap(), "adamw: a parameter, a gradient or a state is given twice, or overlaps another");
   const omt_adamw_params hp{lr,
                             beta1,
                             beta2,

@@ -6,7 +6,7 @@ import math
 import pytest
 import torch
 
-from test_gpu_lm import BF16, F32, U, gen, log_probs, rounding, some_logits, within
+from test_gpu_lm import BF16, F32, U, Case, gen, log_probs, rounding, some_logits, within
 
 pytestmark = pytest.mark.gpu
 
@@ -132,3 +132,45 @@ def test_scale_by_one_of_the_elements(ops, cuda, at):
     x = torch.randn(5000001, generator=gen(3)).cuda()
     want = x * x[at].clone()
     assert torch.equal(ops.scale_by_(x, x[at]), want)
+
+
+@pytest.mark.parametrize("masters", [False, True])
+def test_adamw_refuses_shared_memory(ops, cuda, masters):
+    """Tensors that are written by one thread and held by another: given twice, or overlapping by an element."""
+    c = Case([(300,), (300,)], BF16, 8, masters)
+    step, names = torch.ones((), device="cuda"), ("params", "grads", "m", "v", "ms", "vs") + ("masters",) * masters
+    before = {name: [t.clone() for t in getattr(c, name)] for name in names}
+
+    def call(**other):
+        of = {name: other.get(name, getattr(c, name)) for name in names}
+        ops.adamw(of["params"], of["grads"], of["m"], of["v"], step, of["ms"], of["vs"], of.get("masters"))
+
+    def overlapping(like, apart):
+        big = torch.zeros(2 * len(like), device="cuda").to(like.dtype)
+        return [big[:len(like)], big[apart:apart + len(like)]]
+
+    for name in names:
+        t = getattr(c, name)
+        if name != "grads":
+            for wrong in ([t[0], t[0]], [t[1], t[1]], overlapping(t[0], 1), overlapping(t[0], len(t[0]) - 1), overlapping(t[0], 0)):
+                with pytest.raises(ValueError, match="overlaps"):
+                    call(**{name: wrong})
+    for other in (dict(m=c.m, v=c.m), dict(ms=c.ms, vs=c.ms), dict(m=c.m, v=c.m[::-1]), dict(grads=c.params[::-1])):
+        with pytest.raises(ValueError, match="overlaps"):
+            call(**other)
+    assert all(torch.equal(a.float(), b.float()) for name in names for a, b in zip(before[name], getattr(c, name)))
+
+
+def test_adamw_of_shared_gradients_and_neighbours(ops, cuda):
+    """One gradient of two parameters; parameters and states side by side in one buffer; a parameter that is its own gradient."""
+    c, d = (Case([(300,), (300,)], F32, 32, False) for _ in range(2))
+    step = torch.ones((), device="cuda")
+    ops.adamw(c.params, [c.grads[0]] * 2, c.m, c.v, step)
+    buffer = torch.cat(d.params + d.m + d.v)
+    p, q, *held = buffer.split(300)
+    ops.adamw([p, q], [d.grads[0].clone(), d.grads[0].clone()], held[:2], held[2:], step)
+    assert torch.equal(buffer, torch.cat(c.params + c.m + c.v))
+    c, d = (Case([(300,)], F32, 32, False) for _ in range(2))
+    ops.adamw(c.params, [c.params[0].clone()], c.m, c.v, step)
+    ops.adamw(d.params, d.params, d.m, d.v, step)
+    assert torch.equal(c.params[0], d.params[0]) and torch.equal(c.v[0], d.v[0])
