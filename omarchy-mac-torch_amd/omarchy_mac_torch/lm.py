@@ -85,16 +85,27 @@ def embedding(tokens, weight, scale=1.0, padding_idx=None):
 
 
 class Embedding(nn.Embedding):
-    """nn.Embedding whose rows are multiplied by `scale`: embedding's forward and gradient on the HIP device; elsewhere torch's."""
+    """nn.Embedding whose rows are multiplied by `scale`, with nn.Embedding's other arguments by keyword: embedding's forward and
+    gradient on the HIP device; elsewhere, in other types and with those options that embedding lacks (max_norm,
+    scale_grad_by_freq, sparse), torch's."""
 
-    def __init__(self, num_embeddings, embedding_dim, padding_idx=None, scale=1.0):
-        super().__init__(num_embeddings, embedding_dim, padding_idx)
+    def __init__(self, num_embeddings, embedding_dim, padding_idx=None, scale=1.0, **options):
+        super().__init__(num_embeddings, embedding_dim, padding_idx, **options)
         self.scale = scale
 
+    @classmethod
+    def from_pretrained(cls, *args, scale=1.0, **options):
+        """nn.Embedding.from_pretrained, with a scale."""
+        module = super().from_pretrained(*args, **options)
+        module.scale = scale
+        return module
+
     def forward(self, tokens):
-        if self.weight.device.type not in (DEVICE, "cuda"):
-            return super().forward(tokens) * self.scale
-        return embedding(tokens, self.weight, self.scale, self.padding_idx)
+        w = self.weight
+        if (w.device.type in (DEVICE, "cuda") and w.dtype in (torch.float32, torch.bfloat16) and self.max_norm is None
+                and not self.scale_grad_by_freq and not self.sparse):
+            return embedding(tokens, w, self.scale, self.padding_idx)
+        return super().forward(tokens) * self.scale
 
     def extra_repr(self):
         return super().extra_repr() + f", scale={self.scale}"

@@ -322,3 +322,20 @@ def test_log_probabilities_gradient_far_from_zero(omt):
         want = torch.where(counted, g.double()[..., None] * (onehot - p), 0.0)
         bound = g.double().abs()[..., None] * (p * (off + U * (3 * lp.abs() + 6)) + 3 * U * (p + onehot)) + 2.0 ** -126
         within(dev.grad, want, torch.where(counted, bound, 0.0))
+
+
+def test_embedding_module_takes_torchs_way(omt):
+    """With what the operators lack, on the device too: other types and options, with torch's results."""
+    from omarchy_mac_torch import lm
+    w, t = torch.randn(9, 8), torch.randint(9, (4, 5))
+    for dtype, options in ((torch.float64, {}), (torch.float16, {}), (torch.float32, dict(scale_grad_by_freq=True))):
+        host = torch.nn.Embedding.from_pretrained(w.to(dtype), freeze=False, **options)
+        dev = lm.Embedding.from_pretrained(w.to(dtype), freeze=False, scale=2.0, **options).to(omt.DEVICE)
+        y = dev(t.to(omt.DEVICE))
+        assert y.dtype == dtype and torch.equal(y.detach().cpu(), 2 * host(t).detach())
+        y.sum().backward()
+        (2 * host(t)).sum().backward()
+        assert rel(dev.weight.grad, host.weight.grad.double()) <= 2e-6  # sums of twos, by the frequency in float32
+    dev = lm.Embedding.from_pretrained(w, freeze=False, padding_idx=2, scale=2.0).to(omt.DEVICE)
+    y = dev(t.to(omt.DEVICE))
+    assert "_Embedding" in type(y.grad_fn).__name__ and torch.equal(y.detach().cpu(), 2 * w[t])

@@ -244,3 +244,25 @@ def test_statuses_of_log_probabilities_in_64_bits(lib):
     assert f(logits(lib), None, p, None) == bad and f(logits(lib), p, None, None) == bad
     assert b(logits(lib), None, p, p, None) == bad and b(logits(lib), p, None, p, None) == bad and b(logits(lib), p, p, None, None) == bad
     assert f(logits(lib, length=0, x=None), None, None, None) == ok and b(logits(lib, length=0, x=None), None, None, None, None) == ok
+
+
+def test_embedding_takes_what_torchs_does():
+    """from_pretrained, types, devices and options; on the host torch's results times the scale."""
+    from omarchy_mac_torch import lm
+    w, t = torch.randn(5, 4), torch.tensor([[0, 3], [4, 4]])
+    for args, options in (((w,), {}), ((w, False), {}), ((w,), dict(freeze=False, padding_idx=3)), ((w, True, 1), dict(max_norm=0.5)),
+                          ((w, False), dict(sparse=True)), ((w, False), dict(scale_grad_by_freq=True))):
+        m, plain = lm.Embedding.from_pretrained(*args, scale=2.0, **options), torch.nn.Embedding.from_pretrained(*args, **options)
+        assert isinstance(m, lm.Embedding) and m.scale == 2.0 and m.weight.requires_grad == plain.weight.requires_grad
+        assert m.padding_idx == plain.padding_idx and torch.equal(m(t), 2 * plain(t))
+        if m.weight.requires_grad:
+            m(t).sum().backward()
+            (2 * plain(t)).sum().backward()
+            assert m.weight.grad.is_sparse == plain.weight.grad.is_sparse
+            assert torch.equal(m.weight.grad.to_dense(), plain.weight.grad.to_dense())
+    assert lm.Embedding.from_pretrained(w).scale == 1.0
+    m = lm.Embedding(5, 4, dtype=torch.float64, device="cpu", scale=3.0)
+    assert m.weight.dtype == torch.float64 and torch.equal(m(t), 3 * m.weight[t])
+    assert lm.Embedding(5, 4, 2, 0.5).scale == 0.5 and lm.Embedding(5, 4, -1).padding_idx == 4
+    with pytest.raises(TypeError):
+        lm.Embedding(5, 4, other=1)
