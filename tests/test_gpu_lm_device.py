@@ -339,3 +339,26 @@ def test_embedding_module_takes_torchs_way(omt):
     dev = lm.Embedding.from_pretrained(w, freeze=False, padding_idx=2, scale=2.0).to(omt.DEVICE)
     y = dev(t.to(omt.DEVICE))
     assert "_Embedding" in type(y.grad_fn).__name__ and torch.equal(y.detach().cpu(), 2 * w[t])
+
+
+@pytest.mark.parametrize("padding_idx", [None, 3])
+def test_embeddings_second_derivative_and_forward_mode(omt, padding_idx):
+    """As nn.Embedding has them: the second derivative, and tangents, on the device against torch in float64 on the host."""
+    from torch.autograd import forward_ad
+    from omarchy_mac_torch import lm
+    g = torch.Generator().manual_seed(0)
+    w, v, t = torch.randn(20, 12, generator=g), torch.randn(20, 12, generator=g), torch.randint(20, (5, 9), generator=g)
+
+    def second(e, w, v):
+        w = w.detach().requires_grad_(True)
+        first, = torch.autograd.grad((e(w) ** 3).sum(), w, create_graph=True)
+        return torch.autograd.grad((first * v).sum(), w)[0]
+
+    mine = lambda w: lm.embedding(t.to(omt.DEVICE), w, 1.5, padding_idx)  # noqa: E731
+    want = second(lambda w: 1.5 * F.embedding(t, w, padding_idx), w.double(), v.double())
+    assert rel(second(mine, w.to(omt.DEVICE), v.to(omt.DEVICE)), want) <= 4e-6  # two float32 sums of a few terms, one after the other
+    with forward_ad.dual_level():
+        y = forward_ad.unpack_dual(mine(forward_ad.make_dual(w.to(omt.DEVICE), v.to(omt.DEVICE))))
+        assert torch.equal(y.primal.cpu(), 1.5 * w[t]) and torch.equal(y.tangent.cpu(), 1.5 * v[t])
+    got = torch.func.vmap(mine)(torch.stack([w, v]).to(omt.DEVICE))
+    assert torch.equal(got.cpu(), 1.5 * torch.stack([w[t], v[t]]))

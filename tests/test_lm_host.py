@@ -266,3 +266,60 @@ def test_embedding_takes_what_torchs_does():
     assert lm.Embedding(5, 4, 2, 0.5).scale == 0.5 and lm.Embedding(5, 4, -1).padding_idx == 4
     with pytest.raises(TypeError):
         lm.Embedding(5, 4, other=1)
+
+
+@pytest.fixture
+def plain_embedding(monkeypatch):
+    """hip_ops' embedding and its gradient in plain torch, without autograd, as the operators are."""
+    from omarchy_mac_torch import hip_ops
+
+    def embedding(tokens, weight, scale=1.0):
+        with torch.no_grad():
+            known = (tokens >= 0) & (tokens < len(weight))
+            return torch.where(known[..., None], weight[tokens.clamp(0, len(weight) - 1)] * scale, float("nan"))
+
+    def embedding_backward(gy, tokens, vocab, scale=1.0, padding_idx=None):
+        with torch.no_grad():
+            on = (tokens >= 0) & (tokens < vocab) & (tokens != (-1 if padding_idx is None else padding_idx % vocab))
+            return torch.zeros(vocab, gy.shape[-1], dtype=gy.dtype).index_add_(0, tokens[on], gy[on]) * scale
+
+    monkeypatch.setattr(hip_ops, "embedding", embedding)
+    monkeypatch.setattr(hip_ops, "embedding_backward", embedding_backward)
+
+
+@pytest.mark.parametrize("padding_idx", [None, 2, -1])
+def test_embeddings_derivatives_of_any_order(plain_embedding, padding_idx):
+    from torch.autograd import forward_ad
+    from torch.autograd.gradcheck import gradcheck, gradgradcheck
+    from omarchy_mac_torch import lm
+    g = torch.Generator().manual_seed(0)
+    w = torch.randn(5, 3, generator=g, dtype=torch.float64, requires_grad=True)
+    v = torch.randn(5, 3, generator=g, dtype=torch.float64)
+    t = torch.tensor([[0, 2, 2], [4, 1, 0]])
+    mine = lambda w: lm.embedding(t, w, 1.5, padding_idx)  # noqa: E731
+    plain = lambda w: 1.5 * torch.nn.functional.embedding(t, w, padding_idx)  # noqa: E731
+    if padding_idx is None:  # (the padding row has a value but by definition no gradient)
+        assert gradcheck(mine, w, check_forward_ad=True) and gradgradcheck(mine, w, check_fwd_over_rev=True)
+    for f in (lambda f: torch.autograd.functional.hvp(lambda w: f(w).pow(3).sum(), w, v)[1],
+              lambda f: torch.func.grad(lambda w: f(w).pow(3).sum())(w),
+              lambda f: torch.func.jvp(f, (w,), (v,))[1],
+              lambda f: torch.func.vmap(lambda a: f(w * a))(torch.arange(3.0, dtype=torch.float64)),
+              lambda f: torch.func.vmap(torch.func.grad(lambda w: f(w).pow(2).sum()))(torch.stack([w, v]))):
+        assert torch.allclose(f(mine), f(plain), rtol=1e-12, atol=0)
+    for f in (lm.embedding, lambda t, w, s, p: s * torch.nn.functional.embedding(t, w, p)):  # by samples of tokens
+        rows = torch.func.vmap(lambda row: f(row, w, 1.5, padding_idx))(t)
+        each = torch.func.vmap(torch.func.grad(lambda w, row: f(row, w, 1.5, padding_idx).pow(2).sum()), (None, 0))(w, t)
+        assert torch.equal(rows, 1.5 * w[t])
+        assert torch.allclose(each.sum(0), torch.func.grad(lambda w: plain(w).pow(2).sum())(w), rtol=1e-12, atol=0)
+    with forward_ad.dual_level():
+        y = forward_ad.unpack_dual(mine(forward_ad.make_dual(w.detach(), v)))
+        assert torch.equal(y.tangent, 1.5 * v[t])
+
+
+def test_tokens_outside_the_vocabulary_have_no_second_derivative(plain_embedding):
+    from omarchy_mac_torch import lm
+    w, t = torch.ones(4, 2, requires_grad=True), torch.tensor([1, 7, -1])
+    x = torch.ones(3, 2, requires_grad=True)
+    gw, = torch.autograd.grad(lm.embedding(t, w), w, x, create_graph=True)
+    gx, = torch.autograd.grad((gw * torch.tensor(3.0)).sum(), x)
+    assert gx.tolist() == [[3, 3], [0, 0], [0, 0]]
