@@ -22,6 +22,7 @@ __all__ = ["Embedding", "embedding", "policy_loss", "preference_loss", "token_lo
 
 _transforms_active = torch._C._are_functorch_transforms_active  # whether one of torch.func's is on
 
+
 def _each(apply, size, in_dims, args):
     """apply on each of `size` samples of those arguments that have a dimension of them, stacked."""
     return torch.stack([apply(*(a if d is None else a.select(d, i) for a, d in zip(args, in_dims))) for i in range(size)]), 0

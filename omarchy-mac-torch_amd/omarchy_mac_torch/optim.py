@@ -132,9 +132,13 @@ class AdamW(torch.optim.Optimizer):
 
                 steps = of("step")
                 torch._foreach_add_(steps, 1)
-                hip_ops.adamw(ps, [p.grad for p in ps], of("exp_avg"), of("exp_avg_sq"), steps, of("exp_avg_scale"),
-                              of("exp_avg_sq_scale"), of("master"), lr=group["lr"], betas=group["betas"], eps=group["eps"],
-                              weight_decay=group["weight_decay"], maximize=group["maximize"])
+                try:
+                    hip_ops.adamw(ps, [p.grad for p in ps], of("exp_avg"), of("exp_avg_sq"), steps, of("exp_avg_scale"),
+                                  of("exp_avg_sq_scale"), of("master"), lr=group["lr"], betas=group["betas"], eps=group["eps"],
+                                  weight_decay=group["weight_decay"], maximize=group["maximize"])
+                except Exception:  # refused: no step has been made
+                    torch._foreach_add_(steps, -1)
+                    raise
         return loss
 
     def load_state_dict(self, state_dict):

@@ -362,3 +362,22 @@ def test_embeddings_second_derivative_and_forward_mode(omt, padding_idx):
         assert torch.equal(y.primal.cpu(), 1.5 * w[t]) and torch.equal(y.tangent.cpu(), 1.5 * v[t])
     got = torch.func.vmap(mine)(torch.stack([w, v]).to(omt.DEVICE))
     assert torch.equal(got.cpu(), 1.5 * torch.stack([w[t], v[t]]))
+
+
+def test_a_refused_step_leaves_the_optimizer_as_it_was(omt):
+    """A rate on the host is refused; the same step with one on the device is the first."""
+    from omarchy_mac_torch import optim
+    start, grad = torch.randn(300), torch.randn(300)
+    ps = [torch.nn.Parameter(start.to(omt.DEVICE)) for _ in range(2)]
+    opts = [optim.AdamW([p], lr=torch.tensor(1e-2, device=device)) for p, device in zip(ps, ("cpu", omt.DEVICE))]
+    for p in ps:
+        p.grad = grad.to(omt.DEVICE)
+    with pytest.raises(TypeError, match="lr"):
+        opts[0].step()
+    assert torch.equal(ps[0].detach().cpu(), start)
+    opts[0].param_groups[0]["lr"] = opts[1].param_groups[0]["lr"]
+    for opt in opts:
+        opt.step()
+    assert torch.equal(ps[0].detach().cpu(), ps[1].detach().cpu()) and not torch.equal(ps[0].detach().cpu(), start)
+    for name, t in opts[0].state[ps[0]].items():
+        assert torch.equal(t.float().cpu(), opts[1].state[ps[1]][name].float().cpu()), name

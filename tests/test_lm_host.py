@@ -323,3 +323,14 @@ def test_tokens_outside_the_vocabulary_have_no_second_derivative(plain_embedding
     gw, = torch.autograd.grad(lm.embedding(t, w), w, x, create_graph=True)
     gx, = torch.autograd.grad((gw * torch.tensor(3.0)).sum(), x)
     assert gx.tolist() == [[3, 3], [0, 0], [0, 0]]
+
+
+def test_a_refused_step_is_not_counted():
+    from omarchy_mac_torch import optim
+    p = torch.nn.Parameter(torch.ones(3))
+    p.grad = torch.ones(3)
+    opt = optim.AdamW([p])
+    for _ in range(2):
+        with pytest.raises(TypeError, match="HIP device"):
+            opt.step()
+        assert float(opt.state[p]["step"]) == 0
