@@ -142,8 +142,18 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        super().load_state_dict(state_dict)
-        # (torch casts states to their parameter's type; these keep their own)
+        # (torch casts states to their parameter's type; these keep their own. Its hooks may put another dictionary in this one's place,
+        # and what they do to the states afterwards stays.)
+        taken = []
+        hooks = (self.register_load_state_dict_pre_hook(lambda _, d: taken.append(d)),
+                 self.register_load_state_dict_post_hook(lambda _: self._take_states(taken[-1]), prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for hook in hooks:
+                hook.remove()
+
+    def _take_states(self, state_dict):
         ids = itertools.chain.from_iterable(g["params"] for g in state_dict["param_groups"])
         params = itertools.chain.from_iterable(g["params"] for g in self.param_groups)
         for i, p in zip(ids, params):

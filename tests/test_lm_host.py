@@ -334,3 +334,32 @@ def test_a_refused_step_is_not_counted():
         with pytest.raises(TypeError, match="HIP device"):
             opt.step()
         assert float(opt.state[p]["step"]) == 0
+
+
+def test_optimizer_loads_what_its_hooks_give_it(monkeypatch):
+    """A hook before may replace the state dictionary, one after may change the states that were loaded."""
+    from omarchy_mac_torch import hip_ops, optim
+    monkeypatch.setattr(hip_ops, "adamw", lambda *args, **options: None)
+    p, q = (torch.nn.Parameter(torch.linspace(-1, 1, 130).bfloat16()) for _ in range(2))
+    p.grad = torch.ones_like(p)
+    opt, other = optim.AdamW([p]), optim.AdamW([q])
+    opt.step()
+    saved = opt.state_dict()
+
+    def before(_, d):
+        state = {k: v | {"master": v["master"] + 1e-5, "step": v["step"] + 4} for k, v in d["state"].items()}
+        return {"state": state, "param_groups": d["param_groups"]}
+
+    def after(o):
+        o.state[q]["step"] *= 2
+
+    other.register_load_state_dict_pre_hook(before)
+    other.register_load_state_dict_post_hook(after)
+    for _ in range(2):
+        other.load_state_dict(saved)
+        assert other.state[q]["master"].dtype == torch.float32 and float(other.state[q]["step"]) == 10
+        assert torch.equal(other.state[q]["master"], opt.state[p]["master"] + 1e-5)
+        assert other.state[q]["exp_avg"].dtype == torch.float8_e4m3fn
+    assert float(opt.state[p]["step"]) == 1
+    with pytest.raises(ValueError):
+        other.load_state_dict({"state": {}, "param_groups": []})
