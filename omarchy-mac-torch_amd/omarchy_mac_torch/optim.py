@@ -83,7 +83,10 @@ class AdamW(torch.optim.Optimizer):
     state_bits: 8 (e4m3 with a scale for each block of 128, two bytes and 1/16 a parameter; the second moment as its root) or 32
     (eight bytes). masters: bfloat16 parameters keep a float32 copy, which is what is updated; without one, an update below half a
     parameter's last place is lost. lr may be a one-element float32 tensor on the device. The step's counters are on the device,
-    so a step may be captured into a graph once it has run eagerly (which makes the states)."""
+    so a step may be captured into a graph once it has run eagerly (which makes the states).
+
+    load_state_dict takes torch.optim.AdamW's too: its states go on in 32 bits, those of further parameters are of this optimizer's
+    state_bits."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, *, state_bits=8, masters=True,
                  maximize=False):
@@ -125,7 +128,8 @@ class AdamW(torch.optim.Optimizer):
                     raise TypeError("AdamW: sparse gradients are not covered")
                 if not self.state[p]:
                     self.state[p] = self._new_state(p, group)
-                by_type.setdefault((p.dtype, p.device), []).append(p)
+                state = self.state[p]  # (in 8 bits or not, with a master copy or not, as it was made or loaded)
+                by_type.setdefault((p.dtype, p.device, "exp_avg_scale" in state, "master" in state), []).append(p)
             for ps in by_type.values():
                 def of(name):
                     return [self.state[p][name] for p in ps] if name in self.state[ps[0]] else None
@@ -141,11 +145,23 @@ class AdamW(torch.optim.Optimizer):
                     raise
         return loss
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        for group in self.param_groups:  # (loaded ones may be torch.optim.AdamW's, without this class's options)
+            for name, value in self.defaults.items():
+                group.setdefault(name, value)
+
     def load_state_dict(self, state_dict):
         # (torch casts states to their parameter's type; these keep their own. Its hooks may put another dictionary in this one's place,
         # and what they do to the states afterwards stays.)
         taken = []
-        hooks = (self.register_load_state_dict_pre_hook(lambda _, d: taken.append(d)),
+
+        def take(_, d):
+            if any(g.get("amsgrad") for g in d["param_groups"]):
+                raise ValueError("AdamW: amsgrad is not covered")
+            taken.append(d)
+
+        hooks = (self.register_load_state_dict_pre_hook(take),
                  self.register_load_state_dict_post_hook(lambda _: self._take_states(taken[-1]), prepend=True))
         try:
             super().load_state_dict(state_dict)
@@ -158,7 +174,8 @@ class AdamW(torch.optim.Optimizer):
         params = itertools.chain.from_iterable(g["params"] for g in self.param_groups)
         for i, p in zip(ids, params):
             for name, t in state_dict["state"].get(i, {}).items():
-                self.state[p][name] = t.detach().to(p.device, copy=True)
+                t = t.detach().to(p.device, copy=True)
+                self.state[p][name] = t if t.dtype in (torch.float32, torch.float8_e4m3fn) else t.float()
 
 
 if os.environ.get("OMARCHY_MAC_TORCH_FUSED_OPTIM", "1") != "0":

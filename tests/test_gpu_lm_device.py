@@ -381,3 +381,25 @@ def test_a_refused_step_leaves_the_optimizer_as_it_was(omt):
     assert torch.equal(ps[0].detach().cpu(), ps[1].detach().cpu()) and not torch.equal(ps[0].detach().cpu(), start)
     for name, t in opts[0].state[ps[0]].items():
         assert torch.equal(t.float().cpu(), opts[1].state[ps[1]][name].float().cpu()), name
+
+
+def test_optimizer_goes_on_where_torchs_stopped(omt):
+    """Two steps of torch.optim.AdamW, then one of each from the same state: the parameter's three roundings a side and 16 of an
+    update of up to 3 lr."""
+    from omarchy_mac_torch import optim
+    g = torch.Generator().manual_seed(6)
+    start, grads = torch.randn(1000, generator=g), [torch.randn(1000, generator=g) for _ in range(3)]
+    p, q = (torch.nn.Parameter(start.to(omt.DEVICE)) for _ in range(2))
+    theirs = torch.optim.AdamW([p], lr=1e-2, weight_decay=0.1)
+    ours = optim.AdamW([q], state_bits=32)
+    for k, grad in enumerate(grads):
+        p.grad, q.grad = grad.to(omt.DEVICE), grad.to(omt.DEVICE)
+        if k == 2:
+            with torch.no_grad():
+                q.copy_(p)
+            ours.load_state_dict(theirs.state_dict())
+            ours.step()
+        theirs.step()
+    got, want = q.detach().cpu().double(), p.detach().cpu().double()
+    assert bool(((got - want).abs() <= U * (6 * start.abs() + 6 * want.abs() + 32 * 3e-2)).all())
+    assert bool(((want - start.double()).abs().max() > 1e-2)) and float(ours.state[q]["step"]) == 3

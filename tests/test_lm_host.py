@@ -363,3 +363,31 @@ def test_optimizer_loads_what_its_hooks_give_it(monkeypatch):
     assert float(opt.state[p]["step"]) == 1
     with pytest.raises(ValueError):
         other.load_state_dict({"state": {}, "param_groups": []})
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_optimizer_goes_on_from_torchs_states(monkeypatch, dtype):
+    """torch's states stay in 32 bits; a parameter that had none gets this optimizer's; each kind is a call of its own."""
+    from omarchy_mac_torch import hip_ops, optim
+    calls = []
+    monkeypatch.setattr(hip_ops, "adamw", lambda *args, **options: calls.append((args, options)))
+    ps = [torch.nn.Parameter(torch.ones(3, dtype=dtype)) for _ in range(2)]
+    theirs = torch.optim.AdamW(ps, lr=0.5, betas=(0.5, 0.75), weight_decay=0.25, fused=False)
+    ps[0].grad = torch.full_like(ps[0], 0.5)
+    theirs.step()
+    opt = optim.AdamW(ps, state_bits=8)
+    opt.load_state_dict(theirs.state_dict())
+    ps[1].grad = torch.ones_like(ps[1])
+    opt.step()
+    assert len(calls) == 2
+    for (args, options), p, bits, step in zip(calls, ps, (32, 8), (2, 1)):
+        params, _, m, v, steps, ms, vs, masters = args
+        assert params[0] is p and float(steps[0]) == step and (options["lr"], options["betas"]) == (0.5, (0.5, 0.75))
+        held = torch.float32 if bits == 32 else torch.float8_e4m3fn
+        assert m[0].dtype == v[0].dtype == held and (ms is None) == (vs is None) == (bits == 32)
+        assert (masters is not None) == (bits == 8 and dtype == torch.bfloat16)
+    assert opt.state[ps[0]]["exp_avg"].tolist() == [0.25] * 3
+    theirs = torch.optim.AdamW(ps, amsgrad=True, fused=False)
+    with pytest.raises(ValueError, match="amsgrad"):
+        opt.load_state_dict(theirs.state_dict())
+    assert opt.param_groups[0]["lr"] == 0.5
