@@ -1,12 +1,12 @@
-"""Losses on logits where rounding and weights of zero decide, beside test_gpu_lm.py, whose bounds and inputs these use. u = 2^-24, half a
-step of float32 relative to the value."""
+"""Embedding, losses on logits and AdamW where rounding, weights of zero, shared memory and captured graphs decide, beside
+test_gpu_lm.py, whose bounds and inputs these use. u = 2^-24, half a step of float32 relative to the value."""
 
 import math
 
 import pytest
 import torch
 
-from test_gpu_lm import BF16, F32, U, Case, gen, log_probs, rounding, some_logits, within
+from test_gpu_lm import BF16, F32, U, Case, gen, log_probs, rounding, some_logits, some_tokens, within
 
 pytestmark = pytest.mark.gpu
 
@@ -174,3 +174,86 @@ def test_adamw_of_shared_gradients_and_neighbours(ops, cuda):
     ops.adamw(c.params, [c.params[0].clone()], c.m, c.v, step)
     ops.adamw(d.params, d.params, d.m, d.v, step)
     assert torch.equal(c.params[0], d.params[0]) and torch.equal(c.v[0], d.v[0])
+
+
+# ---- captured graphs ------------------------------------------------------------------------------------------------
+
+def way(name, ops, seed):
+    """(inputs, the call on them): an operator in one of the ways that its sizes lead to."""
+    g = gen(seed)
+    kind, *size = name.split()
+    size = [int(s) if s.isdigit() else s for s in size]
+    if kind == "embedding":
+        n, vocab, dim = size
+        return [some_tokens(n, vocab, "skewed", seed).cuda(), torch.randn(vocab, dim, generator=g).cuda()], \
+            lambda t, w: [ops.embedding(t, w, 2.0)]
+    if kind == "gradient":
+        n, vocab, dim = size
+        return [torch.randn(n, dim, generator=g).cuda(), some_tokens(n, vocab, "skewed", seed).cuda()], \
+            lambda a, t: [ops.embedding_backward(a, t, vocab, padding_idx=1)]
+    if kind == "adamw":
+        c = Case([(300,), (40, 50)], BF16 if size[0] == "bf16" else F32, size[1], size[2:] == ["masters"], seed)
+        names = [name for name in ("params", "grads", "m", "v", "ms", "vs", "masters") if getattr(c, name)]
+
+        def adamw(*ts):
+            of = {name: [ts[2 * i].clone(), ts[2 * i + 1].clone()] for i, name in enumerate(names)}
+            ops.adamw(of["params"], of["grads"], of["m"], of["v"], torch.full((), 3.0, device="cuda"), of.get("ms"), of.get("vs"),
+                      of.get("masters") if c.has_masters else None)
+            return [t.float() for name in names if name != "grads" for t in of[name]]
+
+        return [t for name in names for t in getattr(c, name)], adamw
+    n, length, vocab, *rest = size
+    x, labels = some_logits(n, length, vocab, BF16, seed)
+    x, labels, ref = x.cuda(), labels.cuda(), torch.randn(n, generator=g).cuda()
+    old = torch.randn(n, length, generator=g).cuda() - 7
+    if kind == "logps":
+        return [x, labels], lambda x, y: list(ops.token_logps(x, y))
+    if kind == "logps_gradient":
+        return [old, x, labels, (old + 9).to(torch.float64 if rest[0] == "f64" else F32)], \
+            lambda g, x, y, lse: [ops.token_logps_backward(g, x, y, lse)]
+    if kind == "preference":
+        return [x, labels, ref], lambda x, y, r: list(ops.preference_loss(x, y, r))
+    return [x, labels, old, ref], lambda x, y, o, a: list(ops.policy_loss(x, y, o, a, reference=o * 0.99, kl=0.1, reduction=rest[0]))
+
+
+WAYS = ["embedding 500 600 72", "gradient 500 600 72", "gradient 900 6000 200", "gradient 2000 600 72",
+        "gradient 200 40000 520",                                                                             # few positions, four plans
+        "gradient 1500 200000 16", "gradient 5000 6000 72", "gradient 3000 20000 520",                       # sorted by one workgroup; bins
+        "gradient 9000 300 72", "gradient 9000 600 72", "gradient 3000 300000 16",                            # the sort, of 1, 2 and 3 digits
+        "logps 4 50 700", "logps 2 3 70001", "logps_gradient 4 50 700 f32", "logps_gradient 4 50 700 f64", "preference 4 50 700", "preference 12 50 700",
+        "preference 4 2500 33", "policy 4 50 700 token", "policy 4 50 700 sequence", "policy 7 1500 33 token", "policy 7 1500 33 sequence",
+        "policy 30 3000 16 token", "policy 2 3 70001 token", "adamw f32 8", "adamw f32 32", "adamw bf16 8", "adamw bf16 32",
+        "adamw bf16 8 masters", "adamw bf16 32 masters"]
+
+
+@pytest.mark.parametrize("name", WAYS)
+def test_a_replay_gives_the_calls_values(ops, cuda, name):
+    """Two graphs of the same call, captured once, replayed in turn on new inputs with eager work between, each replay's values
+    against the eager call's, which differ from the last replay's."""
+    inputs, call = way(name, ops, 1)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call(*inputs)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs = []
+    for _ in range(2):
+        static = [t.clone() for t in inputs]
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = call(*static)
+        graphs.append((graph, static, out))
+    last = None
+    for seed in (2, 3, 4):
+        for k, (graph, static, out) in enumerate(graphs):
+            new, _ = way(name, ops, 10 * seed + k)
+            for a, b in zip(static, new):
+                a.copy_(b)
+            graph.replay()
+            torch.cuda.synchronize()
+            want = call(*new)
+            for a, b in zip(out, want):
+                assert a.dtype == b.dtype
+                torch.testing.assert_close(a, b, rtol=0, atol=0, equal_nan=True)
+            assert last is None or not any(torch.equal(a, b) for a, b in zip(want, last) if a.numel() > 1)
+            last = [t.clone() for t in want]
