@@ -8,7 +8,7 @@ import torch
 import torch.nn.functional as F
 
 from test_gpu_ffn_device import plain_lm, rel
-from test_gpu_lm import U, log_probs, some_logits, within
+from test_gpu_lm import U, check_held, log_probs, some_logits, values, within
 
 pytestmark = pytest.mark.gpu
 
@@ -403,3 +403,36 @@ def test_optimizer_goes_on_where_torchs_stopped(omt):
     got, want = q.detach().cpu().double(), p.detach().cpu().double()
     assert bool(((got - want).abs() <= U * (6 * start.abs() + 6 * want.abs() + 32 * 3e-2)).all())
     assert bool(((want - start.double()).abs().max() > 1e-2)) and float(ours.state[q]["step"]) == 3
+
+
+@pytest.mark.parametrize("dtype,masters", [(torch.float32, False), (torch.bfloat16, False), (torch.bfloat16, True)])
+def test_optimizer_in_8_bits_step_by_step(omt, dtype, masters):
+    """Each step against float64 from the states that were held before it, with the bounds of one step."""
+    from omarchy_mac_torch import optim
+    g = torch.Generator().manual_seed(5)
+    lr, (b1, b2), eps, decay = 1e-2, (0.9, 0.99), 1e-6, 0.05
+    params = [torch.nn.Parameter(torch.randn(s, generator=g).to(dtype).to(omt.DEVICE)) for s in [(33, 40), (7,), (256,)]]
+    opt = optim.AdamW(params, lr=lr, betas=(b1, b2), eps=eps, weight_decay=decay, state_bits=8, masters=masters)
+    half = 2.0 ** -8 if dtype == torch.bfloat16 else U
+    for k in range(1, 5):
+        before = []
+        for p in params:
+            s = opt.state[p]
+            m, root = (values(s[n], s[n + "_scale"]) if s else torch.zeros(p.shape, dtype=torch.float64) for n in ("exp_avg", "exp_avg_sq"))
+            before.append(((s["master"] if s and masters else p).detach().cpu().double(), m, root ** 2))
+            p.grad = torch.randn(p.shape, generator=g).to(dtype).to(omt.DEVICE)
+        opt.step()
+        for p, (old, m, v) in zip(params, before):
+            s, d = opt.state[p], p.grad.cpu().double()
+            size, m, v = b1 * m.abs() + (1 - b1) * d.abs(), b1 * m + (1 - b1) * d, b2 * v + (1 - b2) * d * d
+            over = lr / (1 - b1 ** k) / ((v / (1 - b2 ** k)).sqrt() + eps)
+            want, off = old - lr * decay * old - over * m, 16 * U * over * size + 3 * U * old.abs()
+            assert bool((over * m).abs().max() > 2e-3)  # what a step that did nothing would be off by
+            if masters:
+                within(s["master"], want, off)
+                assert torch.equal(p.detach().cpu(), s["master"].cpu().to(dtype))
+            else:
+                within(p, want, off + half * want.abs() * (1 + 1e-3))
+            check_held(s["exp_avg"], s["exp_avg_scale"], m)
+            check_held(s["exp_avg_sq"], s["exp_avg_sq_scale"], v.sqrt(), root=True)
+            assert float(s["step"]) == k
