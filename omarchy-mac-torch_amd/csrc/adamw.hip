@@ -64,7 +64,8 @@ struct AdamwScalars {
   float rate, root, over_root, decay, eps, grad;  // root: sqrt(1 - b2^t)
 };
 
-// beta^t for the step count t, by squaring (within t's bits times 2^-52)
+// beta^t for the step count t, by squaring, which doubles the relative error: within about t 2^-53, far below float32's rounding of 1 -
+// beta^t for every t at which beta^t is not far below that itself
 __device__ __forceinline__ double power(double beta, double t) {
   double p = 1.0;
   for (uint32_t n = (uint32_t)t; n; n >>= 1, beta *= beta)
@@ -75,6 +76,7 @@ __device__ __forceinline__ double power(double beta, double t) {
 template <class P, bool FP8, bool MASTER>
 __global__ void __launch_bounds__(kAdamwThreads) adamw_kernel(const AdamwTable t, const AdamwHyper h) {
 #pragma clang fp contract(off)
+  constexpr bool RECIPROCAL = FP8 && !MASTER;
   if (h.found_inf && *h.found_inf == 1.f) return;
   __shared__ AdamwScalars shared;
   const int chunk = (int)blockIdx.x;
@@ -96,7 +98,7 @@ __global__ void __launch_bounds__(kAdamwThreads) adamw_kernel(const AdamwTable t
     const double step = (double)*s.step, lr = h.lr_dev ? (double)*h.lr_dev : h.lr;
     const double root = sqrt(1.0 - power(h.beta2, step));
     shared = {(float)h.beta1, (float)(1.0 - h.beta1), (float)h.beta2, (float)(1.0 - h.beta2),
-              (float)(lr / (1.0 - power(h.beta1, step))), (float)root, (float)(1.0 / root), (float)(lr * h.wd), h.eps,
+              (float)(lr / (1.0 - power(h.beta1, step))), (float)root, RECIPROCAL ? (float)(1.0 / root) : 0.f, (float)(lr * h.wd), h.eps,
               (h.maximize ? -1.f : 1.f) / (h.grad_scale ? *h.grad_scale : 1.f)};
   }
   __syncthreads();
@@ -113,10 +115,11 @@ __global__ void __launch_bounds__(kAdamwThreads) adamw_kernel(const AdamwTable t
     v[e] = k.b2 * v[e] + k.c2 * ge * ge;
     root[e] = sqrtf(v[e]);
     p[e] -= k.decay * p[e];
-    // (The update's quotient to float32's last place or two is far below the parameter's. Without masters, where the bytes are few, by
-    // the reciprocal instruction: 470 million bfloat16 parameters 840 us for 992; with them it gained nothing, 1434 for 1397.)
-    if constexpr (MASTER) p[e] -= k.rate * m[e] / (root[e] / k.root + k.eps);
-    else p[e] -= k.rate * m[e] * __builtin_amdgcn_rcpf(root[e] * k.over_root + k.eps);
+    // (By the reciprocal instruction, to float32's last place or two, where bytes are so few that a division takes longer: in 8 bits without
+    // masters, 155 million bfloat16 parameters 289 us for 350, 8.8 million float32 ones 25.8 for 26.7; in 32 bits, 842 us for 839 of 155
+    // million float32 ones, and with masters, 1434 for 1397 of 470 million in 8 bits, it gained nothing.)
+    if constexpr (RECIPROCAL) p[e] -= k.rate * m[e] * __builtin_amdgcn_rcpf(root[e] * k.over_root + k.eps);
+    else p[e] -= k.rate * m[e] / (root[e] / k.root + k.eps);
   }
   if constexpr (MASTER) store8<false>(s.master, c, s.n, p);
   store8<false>((P*)s.p, c, s.n, p);

@@ -176,6 +176,30 @@ def test_adamw_of_shared_gradients_and_neighbours(ops, cuda):
     assert torch.equal(c.params[0], d.params[0]) and torch.equal(c.v[0], d.v[0])
 
 
+# ---- roundings ------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype,masters", [(F32, False), (BF16, False), (BF16, True)])
+def test_adamw_in_32_bits_rounds_as_its_formula(ops, cuda, dtype, masters):
+    """States of 32 bits: each operation of the formula rounded to float32 by itself, in its order, to the bit. (The root by way of
+    float64, whose rounding to float32 is the root's own; torch's float32 root on the host is not rounded to nearest.)"""
+    c = Case([(5000,), (33, 40)], dtype, 32, masters)
+    lr, (b1, b2), eps, decay = 0.0078125, (0.875, 0.984375), 2.0 ** -20, 0.125  # (which float32 holds, and their powers)
+    f = lambda v: torch.tensor(v, dtype=torch.float64).float()  # noqa: E731
+    for count in (1, 2, 5):
+        want = []
+        for p, g, m, v in zip(c.masters if masters else c.params, c.grads, c.m, c.v):
+            p, g, m, v = (t.cpu().float() for t in (p, g, m, v))
+            m = f(b1) * m + f(1 - b1) * g
+            v = f(b2) * v + f(1 - b2) * g * g
+            p = p - f(lr * decay) * p
+            want.append((p - f(lr / (1 - b1 ** count)) * m / (v.double().sqrt().float() / f((1 - b2 ** count) ** 0.5) + f(eps)), m, v))
+        ops.adamw(c.params, c.grads, c.m, c.v, torch.tensor(float(count)).cuda(), None, None, c.masters if masters else None, lr=lr,
+                  betas=(b1, b2), eps=eps, weight_decay=decay)
+        for i, (p, m, v) in enumerate(want):
+            assert torch.equal(c.m[i].cpu(), m) and torch.equal(c.v[i].cpu(), v)
+            assert torch.equal(c.params[i].cpu(), p.to(dtype)) and (not masters or torch.equal(c.masters[i].cpu(), p))
+
+
 # ---- captured graphs ------------------------------------------------------------------------------------------------
 
 def way(name, ops, seed):
