@@ -691,7 +691,7 @@ int omt_glu_fp8(int64_t m, int64_t k, int64_t f, int act, const void* x, const f
  * bytes, with rows of a multiple of eight elements, take the vector paths), workspaces 16 bytes. Every sum runs in a fixed order. */
 
 /* y[i] = scale * weight[tokens[i]], weight [vocab][dim], tokens of OMT_DT_I64 or OMT_DT_I32. A token outside the vocabulary gives
- * a row of NaN and touches no memory. */
+ * a row of NaN; nothing outside the arrays is read for it. */
 int omt_embedding_fwd(int dtype, int token_dtype, int64_t n, int64_t vocab, int64_t dim, const void* tokens, const void* weight,
                       float scale, void* y, void* stream);
 /* gweight[v] = scale * sum of gy[i] over the i with tokens[i] = v, in their order, float32 sums rounded once; zeros for v =

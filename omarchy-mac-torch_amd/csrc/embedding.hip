@@ -13,7 +13,7 @@
 // them read the frequent rows); the gradient of 32768 positions 148 us (0.67 GB at 4.5 TB/s), of which the sort with its rows of zeros
 // 98, the sums 31 and the joins 6. 8191 positions to 256 x 128 float32 20.5 us, three launches.
 //
-// Tokens outside the vocabulary: a row of NaN, and no part in the gradient; no memory is touched for them.
+// Tokens outside the vocabulary: a row of NaN (the first row is read in place of theirs, whatever it holds), and no part in the gradient.
 #include <algorithm>
 
 #include "block_fp8.h"
@@ -578,8 +578,9 @@ __global__ void __launch_bounds__(512) embedding_bin_kernel(BinArgs a) {
 //   1024                               8.3, 13.3, 18.0             13.0, 16.4, 16.2                       12.3, 12.2, 19.3
 //   2048                              11.9,    -, 21.1             20.9,    -, 23.1                       16.4,    -, 24.4
 //   4096                              20.2,    -, 22.7             37.5,    -, 28.6                       26.2,    -, 36.1
-// and, of many rows, at 100, 300 and 512 tokens with 64 rows and lanes: 32768 x 512 10.5, 14.5, 19.4 (sort 16.9, 18.2, 19.4), 32768 x 4096
-// 54, 64, 76 (63, 61, 61).
+// and, of many rows, with 64 rows and 64 lanes to a workgroup at 256, 300, 512 and 1024 tokens, bfloat16: 32768 x 512 13.4, 14.9, 18.2, 28.7
+// (in bins 17.6, 18.2, 18.9, 20.4), 131072 x 512 -, 22.3, -, 28.1 (-, 31.1, -, 33.0), 32768 x 4096 53.3, 59.6, 70.3, - (by the sort 61.4, 61.3,
+// 61.5). The rule's border of 256 keeps to where the widest of these rows gain; narrower ones would up to 512.
 struct FewPlan {
   int lanes, rows;
 };
@@ -595,11 +596,14 @@ static FewPlan few_plan(int64_t n, int64_t vocab, int64_t dim) {
 
 // Threads to a bin's columns, 0 where the sort's launches take less: where the columns are few, since each workgroup's share of them sorts
 // the bin again. Skewed tokens, us, in bins and by the sort, at 2049, 4096 and 8192 of them:
-//   16 lanes   256 x 128 bfloat16  18.7, 20.7, 24.1 and 22.2, 22.8, 22.7   16384 x 64 18.4, 19.7, 22.1 and 34.4, 35.6, 35.1
+//   16 lanes   256 x 128 bfloat16  18.7, 20.9, 24.6 and 22.3, 22.6, 22.7   16384 x 64 18.4, 19.7, 22.1 and 34.4, 35.6, 35.1
 //              50021 x 100 float32 23.9, 26.9, 30.1 and 40.5, 42.1, 41.1
 //   64 lanes   4096 x 512 bfloat16 18.5, 22.7, 33.4 and 32.3, 33.6, 34.4   131072 x 512 40.0, 46.3, 56.8 and 44.7, 46.0, 48.4
-//              300 x 512 20.1, 26.8 and 22.3, 22.3 (tokens of one digit)   16384 x 1024 24.7, 31.3 and 34.5, 37.6
+//              300 x 512 19.9, 26.2 and 21.3, 22.0 (tokens of one digit)   16384 x 1024 24.7, 31.3 and 34.5, 37.6
 //              32768 x 1024 float32 44.2, 53.0 and 43.8, 45.4              16384 x 2048 50.9, 62.7 and 45.9, 48.1
+// (256 rows of 128 at 8192 are 2 us over the sort: one rule for all that is narrow.) Fewer, where one launch is not taken either: 300 and 1024
+// to 32768 x 512 18.2, 20.4 and 18.7, 21.7, to 131072 x 512 31.1, 33.0 and 37.2, 38.0, to 16384 x 1024 20.2, 22.3 and 18.7, 21.4; 300 to 131072 x 128
+// 18.5 and 25.3.
 static int bin_lanes(int64_t n, int64_t vocab, int64_t dim) {
   if (vocab > (int64_t)256 << kDigitBits) return 0;
   if (dim <= 128) return n <= kBinTokens ? 16 : 0;

@@ -1,7 +1,7 @@
 // Losses on a language model's logits x [sequences][length][vocab] with labels, and their gradients. Of each row whose label
 // counts (it is not ignore_index): lse = log(sum exp x), lp = x[label] - lse, and d lp / d x = onehot(label) - exp(x - lse).
 //
-// token_logps: lp and lse of every row, and the gradient from one of lp.
+// token_logps: lp and lse of every row, and the gradient from one of lp, by lse in 32 bits or in 64.
 //
 // preference: sequences in pairs, the chosen ones in the first half. With L the sum (or mean) of a sequence's lp and R its
 //   reference, d = (L - R of the chosen) - (L - R of the rejected):
@@ -11,12 +11,12 @@
 //   and the mean over pairs. The gradient of every lp of a sequence is the same.
 //
 // policy: r = exp(lp - old), loss of a token -min(r A, clip(r, 1 - lo, 1 + hi) A) + kl (exp(ref - lp) - (ref - lp) - 1), and the mean
-//   over all tokens, or over sequences of each one's mean.
+//   over all tokens, or over sequences of each one's mean. k of weight 0 takes no part.
 //
 // Rows that do not count are not read, so that nothing in them matters, and get a gradient of zeros; so do rows whose lp has a
 // gradient of zero. A label outside the vocabulary makes the loss, and its row's gradient (its pair's), NaN. Exponentials and their sums over a
-// row are float32, what is computed of lp (sums over a sequence, ratios next to the clip's borders) is float64. No atomics: every
-// sum runs in a fixed order.
+// row are float32, what is computed of lp (sums over a sequence, ratios next to the clip's borders, the KL term) is float64. No atomics:
+// every sum runs in a fixed order.
 //
 // Bound by memory. The gradient needs a row's sum, so a row is read twice, or once where a workgroup holds it in registers
 // (policy); a pair's coefficient needs all rows of both sequences, so the preference loss reads its rows twice. A row takes a
@@ -24,7 +24,7 @@
 // one's reductions and exponentials pass under another's loads.
 //
 // 16 x 512 rows in bfloat16 of which 58% count: policy x 131072 685 us (3.40 GB that it cannot do without, 2.15 of them written), x 65536
-// 348, x 32768 167; preference x 32768 57 + 5 + 123 us for 0.85 GB; 6 x 301 x 50021 float32, rows on 4 bytes, 140 us for 0.58 GB. A large copy
+// 348, x 32768 167; preference x 32768 58 + 6 + 121 us for 0.85 GB; 6 x 301 x 50021 float32, rows on 4 bytes, 140 us for 0.58 GB. A large copy
 // reaches 4.74 TB/s on this card: the second pass finds part of its rows in the last cache. Small calls are launches.
 #include <algorithm>
 

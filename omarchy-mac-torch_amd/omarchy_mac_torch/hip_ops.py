@@ -979,9 +979,10 @@ def adamw(params, grads, exp_avgs, exp_avg_sqs, step, exp_avg_scales=None, exp_a
     """One AdamW step over lists of tensors, in place: parameters and gradients all of float32, or all of bfloat16, which may
     have `masters`, float32 copies that are updated in their place. States of float32; or, with lists of scales (float32, one for
     each block of 128 elements of a tensor in memory), of torch.float8_e4m3fn, exp_avg_sqs then holding the second moments' square
-    roots. step: a one-element float32 tensor already incremented for this step, or a list of them; lr may be one too.
-    grad_scale divides the gradients (which stay as they are); found_inf == 1 skips the step. No tensor that is written may share
-    memory with another (ValueError); gradients may with each other."""
+    roots; a gradient that is not finite then makes its whole block's states NaN. step: a one-element float32 tensor already
+    incremented for this step, or a list of them; lr may be one too. grad_scale divides the gradients (which stay as they are);
+    found_inf == 1 skips the step. No tensor that is written may share memory with another (ValueError); gradients may with each
+    other."""
     n = len(params)
     steps = [step] * n if isinstance(step, torch.Tensor) else step
     lr_dev = lr if isinstance(lr, torch.Tensor) else None

@@ -6,7 +6,8 @@
     policy_loss      training on rewards: clipped probability ratios times advantages, with a KL term to a reference
 
 Differentiable functions, and Embedding as a module, over torch.ops.omt's operators. The two losses compute the logits' gradient with the loss, where
-one can be asked for, and hand it on in the backward pass, which therefore runs once. optim.AdamW is the step at the end.
+one can be asked for, and hand it on in the backward pass, which therefore runs once; scaled by what arrives there, a gradient in
+bfloat16 is rounded a second time, unless that is a power of two. optim.AdamW is the step at the end.
 
 No counterpart in the reference. hip_ops has the same operators as plain functions, for torch.cuda tensors too.
 """

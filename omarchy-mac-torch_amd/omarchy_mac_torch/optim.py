@@ -126,9 +126,10 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 if p.grad.is_sparse:
                     raise TypeError("AdamW: sparse gradients are not covered")
-                if not self.state[p]:
-                    self.state[p] = self._new_state(p, group)
-                state = self.state[p]  # (in 8 bits or not, with a master copy or not, as it was made or loaded)
+                state = self.state[p]
+                if not state:
+                    state = self.state[p] = self._new_state(p, group)
+                # (a state is in 8 bits or not, and with a master copy or not, as it was made or loaded)
                 by_type.setdefault((p.dtype, p.device, "exp_avg_scale" in state, "master" in state), []).append(p)
             for ps in by_type.values():
                 def of(name):
