@@ -81,8 +81,8 @@ class AdamW(torch.optim.Optimizer):
     device (or on torch.cuda); gradients of their type.
 
     state_bits: 8 (e4m3 with a scale for each block of 128, two bytes and 1/16 a parameter; the second moment as its root) or 32
-    (eight bytes). masters: bfloat16 parameters keep a float32 copy, which is what is updated; without one, an update below half a
-    parameter's last place is lost. lr may be a one-element float32 tensor on the device. The step's counters are on the device,
+    (eight bytes). masters: bfloat16 parameters keep a float32 copy, which is what is updated (so what else is written to a parameter
+    after its first step is lost at the next); without one, an update below half a parameter's last place is lost. lr may be a one-element float32 tensor on the device. The step's counters are on the device,
     so a step may be captured into a graph once it has run eagerly (which makes the states).
 
     load_state_dict takes torch.optim.AdamW's too: its states go on in 32 bits, those of further parameters are of this optimizer's
@@ -90,16 +90,25 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01, *, state_bits=8, masters=True,
                  maximize=False):
-        if state_bits not in (8, 32):
-            raise ValueError(f"state_bits: expected 8 or 32, got {state_bits!r}")
-        if not isinstance(lr, torch.Tensor) and not lr >= 0:
-            raise ValueError(f"lr: expected at least 0, got {lr!r}")
-        if not all(0 <= b < 1 for b in betas):
-            raise ValueError(f"betas: expected from 0 to below 1, got {betas!r}")
-        if not eps >= 0 or not weight_decay >= 0:
-            raise ValueError(f"eps, weight_decay: expected at least 0, got {eps!r}, {weight_decay!r}")
-        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
-                                      masters=masters, maximize=maximize))
+        defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits, masters=masters,
+                        maximize=maximize)
+        self._check(defaults)
+        super().__init__(params, defaults)
+
+    @staticmethod
+    def _check(g):
+        if g["state_bits"] not in (8, 32):
+            raise ValueError(f"state_bits: expected 8 or 32, got {g['state_bits']!r}")
+        if not isinstance(g["lr"], torch.Tensor) and not g["lr"] >= 0:
+            raise ValueError(f"lr: expected at least 0, got {g['lr']!r}")
+        if not all(0 <= b < 1 for b in g["betas"]):
+            raise ValueError(f"betas: expected from 0 to below 1, got {g['betas']!r}")
+        if not g["eps"] >= 0 or not g["weight_decay"] >= 0:
+            raise ValueError(f"eps, weight_decay: expected at least 0, got {g['eps']!r}, {g['weight_decay']!r}")
+
+    def add_param_group(self, param_group):
+        self._check({**self.defaults, **param_group})
+        super().add_param_group(param_group)
 
     @staticmethod
     def _new_state(p, group):

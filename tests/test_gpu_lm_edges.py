@@ -92,6 +92,8 @@ def test_log_probabilities_by_lse_in_64_bits(ops, cuda, dtype, vocab):
     logps, lse = ops.token_logps(x.cuda(), labels.cuda(), lse_dtype=torch.float64)
     short = ops.token_logps(x.cuda(), labels.cuda())
     assert lse.dtype == torch.float64 and torch.equal(logps, short[0]) and torch.equal(lse.float(), short[1])
+    for got, want in zip(torch.ops.omt.token_logps(x.cuda(), labels.cuda(), -100), short):
+        assert torch.equal(got, want)
     counted = labels != -100
     within(lse, torch.where(counted, torch.logsumexp(x.double(), -1), 0.0), torch.where(counted, off, 0.0))
     g = torch.randn(2, 5, generator=gen(1))

@@ -391,3 +391,19 @@ def test_optimizer_goes_on_from_torchs_states(monkeypatch, dtype):
     with pytest.raises(ValueError, match="amsgrad"):
         opt.load_state_dict(theirs.state_dict())
     assert opt.param_groups[0]["lr"] == 0.5
+
+
+def test_optimizer_arguments_of_groups():
+    from omarchy_mac_torch import optim
+    p, q = (torch.nn.Parameter(torch.ones(3)) for _ in range(2))
+    opt = optim.AdamW([p])
+    for wrong in (dict(state_bits=16), dict(lr=-1.0), dict(betas=(0.9, 1.0)), dict(eps=-1.0), dict(weight_decay=-1.0)):
+        with pytest.raises(ValueError):
+            optim.AdamW([dict(params=[p], **wrong)])
+        with pytest.raises(ValueError):
+            opt.add_param_group(dict(params=[q], **wrong))
+        with pytest.raises(ValueError):
+            optim.AdamW([dict(params=[p], lr=1e-2, betas=(0.5, 0.5), eps=0.0, weight_decay=0.0, state_bits=8)], **wrong)
+        assert len(opt.param_groups) == 1
+    opt.add_param_group(dict(params=[q], state_bits=32, lr=0.5))
+    assert opt.param_groups[1]["state_bits"] == 32 and opt.param_groups[1]["betas"] == opt.defaults["betas"]
