@@ -43,7 +43,7 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     def backward(ctx, gy):
         tokens, = ctx.saved_tensors
-        gradient = _EmbeddingGradient.apply if torch.is_grad_enabled() else hip_ops.embedding_backward
+        gradient = _EmbeddingGradient.apply if torch.is_grad_enabled() or _transforms_active() else hip_ops.embedding_backward
         return None, gradient(gy, tokens, ctx.vocab, ctx.scale, ctx.padding_idx), None, None
 
     @staticmethod

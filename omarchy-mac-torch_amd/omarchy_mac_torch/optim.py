@@ -82,8 +82,9 @@ class AdamW(torch.optim.Optimizer):
 
     state_bits: 8 (e4m3 with a scale for each block of 128, two bytes and 1/16 a parameter; the second moment as its root) or 32
     (eight bytes). masters: bfloat16 parameters keep a float32 copy, which is what is updated (so what else is written to a parameter
-    after its first step is lost at the next); without one, an update below half a parameter's last place is lost. lr may be a one-element float32 tensor on the device. The step's counters are on the device,
-    so a step may be captured into a graph once it has run eagerly (which makes the states).
+    after its first step is lost at the next); without one, an update below half a parameter's last place is lost. lr may be a
+    one-element float32 tensor on the device. The step's counters are on the device, so a step may be captured into a graph once it
+    has run eagerly (which makes the states).
 
     load_state_dict takes torch.optim.AdamW's too: its states go on in 32 bits, those of further parameters are of this optimizer's
     state_bits."""

@@ -311,6 +311,10 @@ def test_embeddings_derivatives_of_any_order(plain_embedding, padding_idx):
         each = torch.func.vmap(torch.func.grad(lambda w, row: f(row, w, 1.5, padding_idx).pow(2).sum()), (None, 0))(w, t)
         assert torch.equal(rows, 1.5 * w[t])
         assert torch.allclose(each.sum(0), torch.func.grad(lambda w: plain(w).pow(2).sum())(w), rtol=1e-12, atol=0)
+    assert torch.equal(*(torch.autograd.functional.jacobian(f, w.detach()) for f in (mine, plain)))
+    vs = torch.randn(4, 2, 3, 3, generator=g, dtype=torch.float64)  # several of the result's gradients at once
+    mine_, plain_ = (torch.func.vmap(lambda v, y=f(w): torch.autograd.grad(y, w, v, retain_graph=True)[0])(vs) for f in (mine, plain))
+    assert torch.allclose(mine_, plain_, rtol=1e-12, atol=0)
     with forward_ad.dual_level():
         y = forward_ad.unpack_dual(mine(forward_ad.make_dual(w.detach(), v)))
         assert torch.equal(y.tangent, 1.5 * v[t])
