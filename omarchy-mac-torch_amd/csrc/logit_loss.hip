@@ -184,9 +184,8 @@ __device__ __forceinline__ RowStats row_stats(const Row<T>& x, float* red) {
 __device__ __forceinline__ bool in_vocab(int64_t label, int64_t vocab) { return (uint64_t)label < (uint64_t)vocab; }
 // lp of a label, NaN outside the vocabulary; a row of minus infinities has top - top = NaN in it, as the definition has
 template <class T>
-__device__ __forceinline__ double label_logp(const T* x, int64_t label, int64_t vocab, RowStats st) {
-  if (!in_vocab(label, vocab)) return (double)__builtin_nanf("");
-  return ((double)(float)x[label] - (double)st.top) - log((double)st.sum);
+__device__ __forceinline__ double label_logp(const T* x, int64_t label, int64_t vocab, float top, double log_sum) {
+  return in_vocab(label, vocab) ? ((double)(float)x[label] - (double)top) - log_sum : (double)__builtin_nanf("");
 }
 
 // ---- statistics of rows ---------------------------------------------------------------------------------------------
@@ -224,9 +223,8 @@ __global__ void __launch_bounds__(RT == 64 ? 256 : RT) token_logps_kernel(LogitR
   const Row<T> x((const T*)a.x + a.offset(row), a.vocab);
   const RowStats st = row_stats<T, RT>(x, red);
   if (first) {
-    const double lp = label_logp(x.p, label, a.vocab, st);
+    const double log_sum = log((double)st.sum), lp = label_logp(x.p, label, a.vocab, st.top, log_sum), lse = (double)st.top + log_sum;
     if (out.logps) out.logps[row] = (float)lp;
-    const double lse = (double)st.top + log((double)st.sum);
     if (out.lse) out.lse[row] = (float)lse;
     if (out.lse64) out.lse64[row] = lse;
     if (out.sums) out.sums[row] = lp;
@@ -571,7 +569,7 @@ __global__ void __launch_bounds__(RT == 64 ? 256 : RT) policy_kernel(LogitRows a
   } else {
     st = row_stats<T, RT>(x, red);
   }
-  const double lp = label_logp(x.p, label, a.vocab, st);
+  const double lp = label_logp(x.p, label, a.vocab, st.top, log((double)st.sum));
   const TokenLoss loss = token_loss(p, a, row, lp);
   if (t == 0) {
     p.logps[row] = (float)lp;
