@@ -24,7 +24,7 @@
 // one's reductions and exponentials pass under another's loads.
 //
 // 16 x 512 rows in bfloat16 of which 58% count: policy x 131072 685 us (3.40 GB that it cannot do without, 2.15 of them written), x 65536
-// 348, x 32768 167; preference x 32768 58 + 6 + 121 us for 0.85 GB; 6 x 301 x 50021 float32, rows on 4 bytes, 140 us for 0.58 GB. A large copy
+// 348, x 32768 167; preference x 32768 56 + 6 + 122 us for 0.85 GB; 6 x 301 x 50021 float32, rows on 4 bytes, 140 us for 0.58 GB. A large copy
 // reaches 4.74 TB/s on this card: the second pass finds part of its rows in the last cache. Small calls are launches.
 #include <algorithm>
 
